@@ -25,8 +25,16 @@ class QwenCfg(C.Structure):
         ("rope_freq_base", C.c_float), ("rms_eps", C.c_float)]
 
 
+class Kv(C.Structure):
+    """brrr_kv: a KV cache that the caller owns."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int32), ("n_seq", C.c_int32), ("n_head_kv", C.c_int32),
+                ("head_dim", C.c_int32), ("cap", C.c_int32), ("head_stride", C.c_int64), ("seq_stride", C.c_int64),
+                ("weight", C.c_void_p), ("pos", C.c_void_p), ("err", C.c_void_p)]
+
+
 _P = C.c_void_p
 _I = C.c_int
+_F = C.c_float
 # name -> (restype, argtypes); the authoritative list of exported entry points
 SIGNATURES = {
     "brrr_strerror": (C.c_char_p, [_I]),
@@ -95,6 +103,13 @@ SIGNATURES = {
     "brrr_qwen_generate": (_I, [_P, _P, _P, C.c_size_t, C.c_uint32, _P, _P, _P, C.c_size_t, _P]),
     "brrr_qwen_serve_parse": (_I, [C.c_char_p, C.POINTER(C.c_uint32), C.c_char_p, C.c_size_t]),
     "brrr_qwen_cli_main": (_I, [_I, _P]),
+    "brrr_kv_append": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, C.c_int64, _I, _P, _I, _P, _P]),
+    "brrr_attn_tree": (_I, [_P, _I, _I, _P, _P, _P, _P, _I, _P, _I, _F, _I, _P, _P, _P, _P]),
+    "brrr_kv_commit": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "brrr_kv_weigh": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _I, _F, _I, _P, _P]),
+    "brrr_kv_evict": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P]),
+    "brrr_kv_means": (_I, [_P, _I, _P, _P, _P, _I, _I, _P, _P]),
+    "brrr_attn_blocks": (_I, [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P, _I, _F, _P, _P, _P, _P, _P]),
     "brrr_quant_q8": (_I, [_P, _I, _P, _P, _P]),
     "brrr_quant_q8k": (_I, [_P, _I, _P, _P, _P, _P]),
     "brrr_q4k_matvec": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P]),

@@ -92,6 +92,21 @@ cudaError_t launch_router_rows(const float *xn, int d, const float *Wt, const fl
                                unsigned int *counter, DevState *state, bool pdl, cudaStream_t st);
 char *host_err_buf();   // thread-local text behind brrr_last_cuda_error (512 bytes)
 
+// ---- KV caches of the caller (kernels_kv.cu, kernels_kvattn.cu); KvDev and TreeArgs are declared in brrr_kv.cuh, the arguments described in the public header
+struct KvDev;
+struct TreeArgs;
+cudaError_t launch_kv_append(const KvDev &kv, int n, int rows, const int32_t *seq, const int32_t *len, const int32_t *count, const int32_t *at, const float *qkv,
+                             long long ld, int nh, const float *rope, int n_rope, float *q, cudaStream_t st);
+cudaError_t launch_kv_commit(const KvDev &kv, int n, int rows, const int32_t *seq, const int32_t *len, const int32_t *path, const int32_t *npath, int32_t *new_len,
+                             cudaStream_t st);
+cudaError_t launch_kv_evict(const KvDev &kv, const KvDev *dst, int n, const int32_t *seq, const int32_t *len, int keep, int first, int recent, const int32_t *end,
+                            int32_t *map, int32_t *new_len, int len_hint, cudaStream_t st);
+cudaError_t launch_kv_means(const KvDev &kv, int n, const int32_t *seq, const int32_t *since, const int32_t *len, int block, int len_hint, float *means, cudaStream_t st);
+cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st);
+cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st);
+cudaError_t launch_attn_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,
+                               int len_hint, const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *out, float *lse, cudaStream_t st);
+
 // ---- Q8 matrices (kernels_q8.cu)
 void launch_q8_pack(const uint16_t *w_bf16, int rows_src, int row0_dst, Q8Dev m, cudaStream_t st);
 void launch_q8_export(Q8Dev m, int8_t *q, float *s, cudaStream_t st);

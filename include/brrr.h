@@ -293,6 +293,90 @@ int brrr_qwen_serve_parse(const char *line, uint32_t *ngen, char *prompt, size_t
  * (src/bin/engine_qwen2.rs:486-489, 622-683). */
 int brrr_qwen_cli_main(int argc, char **argv);
 
+/* ---------------------------------------------------------------- KV caches: draft trees, eviction, chosen blocks
+ * Operators beside brrr_attn_decode for what a long cache and a draft need.  They work on caches that the caller owns, described by a
+ * brrr_kv; everything is enqueued on `stream` of the current device (to which every pointer belongs), nothing is allocated or kept
+ * between calls, and every call may be captured into a CUDA graph.  Arithmetic is single precision or better whatever the cache's type,
+ * in a fixed order: equal inputs give equal bits.
+ *
+ * Lengths, sequences, counts, paths and positions are device arrays.  What the host cannot see is checked by the kernels: an entry of a
+ * list whose sequence, length or count does not fit the cache, or that names a sequence which an earlier entry of a writing call (append,
+ * commit, weigh, evict, means) has named already, is left out, its outputs stay as they were, and *err (if given) becomes 1.
+ * d_seq [n] names the sequences of a call; NULL: entry b is sequence b.  len_hint: about the largest length among the entries (0: unknown);
+ * it steers how work is split, never what is computed.
+ * A slot that a row does not see may hold anything, infinities and NaN included; a row that sees such a value has no defined result. */
+enum { BRRR_KV_F32 = 0, BRRR_KV_BF16 = 1 };
+#define BRRR_TREE_MAX 64     /* rows per sequence of brrr_attn_tree, brrr_kv_commit and brrr_kv_weigh */
+#define BRRR_KV_CAP_MAX (1 << 19)     /* largest capacity */
+typedef struct brrr_kv {
+    void *k, *v;                      /* [n_seq][n_head_kv][cap][head_dim] values of `type`, keys rotated; 16-byte aligned */
+    int32_t type;                     /* BRRR_KV_F32 (the engines' caches) or BRRR_KV_BF16 */
+    int32_t n_seq, n_head_kv;
+    int32_t head_dim;                 /* 64 or 128 */
+    int32_t cap;                      /* slots per head */
+    int64_t head_stride, seq_stride;  /* values from one head to the next and from one sequence to the next, multiples of 8; 0: dense */
+    float *weight;                    /* [n_seq][n_head_kv][cap] book of attention weights, or NULL */
+    int32_t *pos;                     /* [n_seq][n_head_kv][cap] position that a slot's entry has in its sequence, or NULL */
+    int32_t *err;                     /* device word set to 1 by a kernel that left an entry out, or NULL */
+} brrr_kv;
+
+/* Row i < count[b] (d_count NULL: rows) of entry b goes to slot len[b] + i: keys rotated and values, converted to the cache's type; the
+ * slot's weight becomes 0 and its position at[b][i] (d_at NULL: the slot's number).  A row of d_qkv is q (n_head heads, may be 0) | k | v,
+ * ld floats from the next (0: dense), 16-byte aligned, ld % 4 == 0.  d_rope [n_rope][head_dim / 2][2] cosines and sines as brrr_rope_table makes them, pairs
+ * (j, j + head_dim / 2); NULL: k and q are taken as they are.  d_q (nullable, no overlap with d_qkv): the rotated q [n][rows][n_head * head_dim].
+ * A row whose position the table does not have is left out.  rows <= cap.  Replaces the rotation and the cache write of
+ * src/bin/engine_gpt2.rs:575-587, 783-800 for rows of many sequences. */
+int brrr_kv_append(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, const int32_t *d_len, const int32_t *d_count, const int32_t *d_at,
+                   const float *d_qkv, int64_t ld, int n_head, const float *d_rope, int n_rope, float *d_q, void *stream);
+
+/* Attention of `rows` (1..BRRR_TREE_MAX) drafted tokens per entry over the entry's cache: row i's key and value stand in slot len[b] + i.
+ * Row i sees the cached slots t < len[b] and of the drafted ones j < count[b] those whose bit j of mask[b][i] is set: the row itself and its
+ * ancestors (d_mask NULL: every j <= i, a chain).  window > 0: with depth(i) the number of rows that i sees other than itself, only slots
+ * t >= len[b] + depth(i) + 1 - window and rows with depth(i) - depth(j) < window are seen.  d_q [n][rows][n_head * head_dim], rotated; n_head a
+ * multiple of n_head_kv, at most 16 times it.  d_sinks [n_head] (nullable): a logit per head that takes weight and adds nothing.
+ *   d_out [n][rows][n_head * head_dim] = sum over seen t of exp(scale q.k_t - lse) v_t;  d_lse [n][rows][n_head] (nullable) = log of the sum of exponentials,
+ * the sink's included.  A row that sees nothing: zeros, and lse the sink or -infinity.  Rows >= count[b] stay as they were.
+ * Generalises the attention stage src/bin/engine_gpt2.rs:800-837 from one token to a tree. */
+int brrr_attn_tree(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, const int32_t *d_len, const int32_t *d_count, const uint64_t *d_mask,
+                   int len_hint, const float *d_q, int n_head, float scale, int window, const float *d_sinks, float *d_out, float *d_lse, void *stream);
+
+/* The accepted rows path[b][0 .. npath[b]) of a tree whose rows stand in slots len[b] .. len[b] + rows - 1 (d_path [n][rows], entries 0..rows-1)
+ * move to slots len[b], len[b] + 1, ... with their weights and positions.  d_new_len (nullable, not d_len) [n] = len[b] + npath[b], len[b] for an
+ * entry that is left out. */
+int brrr_kv_commit(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, const int32_t *d_len, const int32_t *d_path, const int32_t *d_npath,
+                   int32_t *d_new_len, void *stream);
+
+/* Attention weights into the book: weight[seq][kv head][t] += sum over the rows i and the query heads h of that kv head of
+ * exp(scale q.k_t - lse[b][i][h]) for every slot t that row i sees (as in brrr_attn_tree, with its d_lse).  d_rows [n] (nullable: all): bit i
+ * says whether row i counts, so that only the accepted rows of a tree do.  The view needs a weight book. */
+int brrr_kv_weigh(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, const int32_t *d_len, const int32_t *d_count, const uint64_t *d_mask,
+                  const uint64_t *d_rows, int len_hint, const float *d_q, int n_head, float scale, int window, const float *d_lse, void *stream);
+
+/* Of the len[b] entries of each kv head keep m = min(len[b], keep): those with a position < first or >= end[b] - recent (end[b]: positions the
+ * sequence has had; d_end may be NULL where recent is 0) before the others, then the larger weight (NaN below all), then the lower slot.
+ * Kept entries in slots below m stay there; the slots below m that are freed take, in ascending order, the kept entries from the slots behind, in
+ * ascending order, with their weights and positions: attention does not ask for an order, so no more than that moves.  d_map [n][n_head_kv][keep]: the
+ * slot that each entry came from, -1 from m on.  dst NULL: in place (what lies behind m is then nobody's); else all kept entries are written to the same sequence of
+ * dst, another view of the same type, heads and dimension with cap >= keep whose memory does not overlap.  d_new_len (nullable, not d_len) [n] = m.
+ * first + recent <= keep.  Views need both books. */
+int brrr_kv_evict(const brrr_kv *kv, const brrr_kv *dst, int n, const int32_t *d_seq, const int32_t *d_len, int keep, int first, int recent,
+                  const int32_t *d_end, int32_t *d_map, int32_t *d_new_len, int len_hint, void *stream);
+
+/* Means of the keys of every whole block of `block` (16, 32, 64 or 128) slots that ends behind since[b] (NULL: 0) and not behind len[b]:
+ * d_means [n_seq][n_head_kv][cap / block][head_dim], summed in double precision.  Other means stay as they were.  len_hint: about the largest
+ * len - since. */
+int brrr_kv_means(const brrr_kv *kv, int n, const int32_t *d_seq, const int32_t *d_since, const int32_t *d_len, int block, int len_hint, float *d_means,
+                  void *stream);
+
+/* Attention of independent rows over chosen blocks.  Row r sees slots t < len[r] of sequence seq[r] (NULL: r).  Of its ceil(len / block) blocks each
+ * kv head takes the `first` first, the `local` (>= 1) last and those of the others with the largest score, nsel (<= 256) in all: the score of a block is the largest
+ * q_h . mean over the query heads h of the kv head, in double precision, rounded to single; NaN below all, the lower block first among equals.
+ * d_sel [rows][n_head_kv][nsel]: the blocks in ascending order, -1 behind the last.  d_out and d_lse (nullable) as in brrr_attn_tree over the
+ * slots of those blocks.  cap / block <= 16384, first + local <= nsel, d_q [rows][n_head * head_dim].  Any rows, for prompts a row per position. */
+int brrr_attn_blocks(const brrr_kv *kv, int rows, const int32_t *d_seq, const int32_t *d_len, int block, const float *d_means, int nsel, int first,
+                     int local, int len_hint, const float *d_q, int n_head, float scale, const float *d_sinks, int32_t *d_sel, float *d_out, float *d_lse,
+                     void *stream);
+
 /* ---------------------------------------------------------------- stage-level entry points
  * Device pointers in, device pointers out.  They launch the same kernels the forward pass uses. */
 
