@@ -1,98 +1,610 @@
 // Attention over KV caches that the caller owns: trees of drafted tokens, chosen blocks, and the book of attention weights.
+//
+// Rows are (drafted token, query head of one kv head) pairs, 16 to a tile of mma.sync (m16n8k8, tf32 operands, f32 sums); a warp holds one tile of
+// rows and walks slots in steps of 16.  Results are single precision: an f32 operand x is split into hi = x rounded to tf32's 11 bits and the
+// rest lo = x - hi, exact, of which tf32 takes 11 bits again; hi hi + hi lo + lo hi leaves out 2^-22 of a product at most.  bf16 values are tf32
+// values: for such a cache two products are enough.  The tensor cores' adders truncate, so no long sum is left to them: a step's scores take
+// head_dim / 8 additions, a step's share of the output starts at zero and joins the running output by one fused multiply-add that also
+// rescales it to the new running maximum.
+//
+// Operand B comes from global memory straight into registers.  Its k index may be any order of the dimensions (keys) that operand A
+// has too, so a lane's k = t, t + 4 of consecutive products are the consecutive values of one 16-byte load; the accumulator of the scores, with keys 2t and
+// 2t + 1 in a lane, is operand A of the second product as it stands.  Queries are split once and wait in shared memory in fragment order.
+//
+// The slots of an entry are split over the warps of a CTA and the CTAs of a cluster, each with its own maximum and sum; partial results meet
+// in shared memory, those of the cluster through distributed shared memory, in a fixed order: one launch, no workspace, no atomics.
 #include "brrr_kernels.h"
 #include "brrr_block.cuh"
 #include "brrr_kv.cuh"
 
+#include <cooperative_groups.h>
+
 namespace brrr {
 
-__device__ __forceinline__ float kv_load(const void *p, int type, long long at) {
-    return type ? brrr_bf16_to_f32(((const uint16_t *)p)[at]) : ((const float *)p)[at];
+namespace cg = cooperative_groups;
+
+constexpr int AW = 8;                       // warps of an attention CTA
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const float4 &a, float b0, float b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(a.z)), "r"(__float_as_uint(a.w)), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
 
-// One query head's attention by one warp, four (two) dimensions per lane, over the slots that `next` names (-1: none left).
-template <class Next>
-__device__ __forceinline__ void warp_attend(const KvDev &kv, long long head, const float *q, float scale, const float *sink, float *out, float *lse, Next next) {
-    const int lane = threadIdx.x & 31, per = kv.hd / 32;
-    float qr[4], acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int d = 0; d < per; d++) qr[d] = q[d * 32 + lane];
-    float top = sink ? *sink : -INFINITY, sum = sink ? 1.0f : 0.0f;
-    for (int t = next(); t >= 0; t = next()) {
-        const long long at = head + (long long)t * kv.hd;
-        float s = 0.0f;
-        for (int d = 0; d < per; d++) s = __fmaf_rn(qr[d], kv_load(kv.k, kv.type, at + d * 32 + lane), s);
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= scale;
-        const float m = fmaxf(top, s), keep = top == m ? 1.0f : expf(top - m), p = expf(s - m);
-        sum = __fmaf_rn(sum, keep, p);
-        for (int d = 0; d < per; d++) acc[d] = __fmaf_rn(acc[d], keep, p * kv_load(kv.v, kv.type, at + d * 32 + lane));
-        top = m;
+// The two cache types: values per 16-byte load, and a load's values as floats.
+struct KvF32 {
+    static constexpr int V = 4;
+    static constexpr bool SPLIT = true;
+    typedef float Val;
+    static __device__ __forceinline__ void get(const uint4 &u, float (&x)[4]) {
+        x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
     }
-    for (int d = 0; d < per; d++) out[d * 32 + lane] = sum > 0.0f ? acc[d] / sum : acc[d] + sum;
-    if (lse && lane == 0) *lse = top + logf(sum);
+};
+struct KvBf16 {
+    static constexpr int V = 8;
+    static constexpr bool SPLIT = false;
+    typedef uint16_t Val;
+    static __device__ __forceinline__ void get(const uint4 &u, float (&x)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    }
+};
+
+__device__ __forceinline__ uint4 ldg_stream(const void *p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint4 ldg_shared(const void *p) {
+    uint4 r;
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
 }
 
-__global__ void __launch_bounds__(128) tree_kernel(KvDev kv, TreeArgs a) {
-    __shared__ uint64_t mask[KV_TREE_MAX];
+// What a lane keeps of a step of 8 NK slots.  Keys: of slot 8 j + lane / 4 the values 4V c + V (lane % 4) ...  Values: of slots 8 j + 2 (lane % 4) and the next
+// the values 8V c + V (lane / 4) ...
+template <class T, int HD, int NK>
+struct KvStep {
+    static constexpr int NC = HD / (4 * T::V), NVC = HD / (8 * T::V);
+    uint4 k[NK][NC], v[NK][2][NVC];
+    // slots base .. base + 8 NK - 1, those from end on left out (zeros)
+    template <bool STREAM>
+    __device__ __forceinline__ void load_k(const typename T::Val *kc, int base, int end) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int j = 0; j < NK; j++) {
+            const int t = base + 8 * j + (lane >> 2);
+            const typename T::Val *p = kc + (long long)t * HD + T::V * (lane & 3);
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                k[j][c] = t < end ? (STREAM ? ldg_stream(p + 4 * T::V * c) : ldg_shared(p + 4 * T::V * c)) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    template <bool STREAM>
+    __device__ __forceinline__ void load_v(const typename T::Val *vc, int base, int end) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int j = 0; j < NK; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int t = base + 8 * j + 2 * (lane & 3) + h;
+                const typename T::Val *p = vc + (long long)t * HD + T::V * (lane >> 2);
+#pragma unroll
+                for (int c = 0; c < NVC; c++)
+                    v[j][h][c] = t < end ? (STREAM ? ldg_stream(p + 8 * T::V * c) : ldg_shared(p + 8 * T::V * c)) : make_uint4(0, 0, 0, 0);
+            }
+    }
+};
+
+// Queries of `tiles` tiles of 16 rows in fragment order, hi and lo parts: per product (8 dimensions) and lane 16 bytes each.  row(r): the row's
+// values, or null for a row of padding (zeros).
+template <class T, int HD, class Row>
+__device__ __forceinline__ void stage_queries(float4 *frag, int tiles, Row row) {
+    constexpr int W = 4 * T::V;                 // dimensions that one load of the four lanes of a slot covers
+    float *f = reinterpret_cast<float *>(frag);
+    for (int u = threadIdx.x; u < tiles * 16 * (HD / 4); u += AW * 32) {
+        const int r = u / (HD / 4), d0 = u % (HD / 4) * 4;
+        const float *p = row(r);
+        const float4 x4 = p ? *reinterpret_cast<const float4 *>(p + d0) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = d0 + i, t = d % W / T::V, step = d / W * (T::V / 2) + d % T::V / 2, odd = d & 1;
+            const int at = ((((r / 16) * (HD / 8) + step) * 2) * 32 + (r % 8) * 4 + t) * 4 + (r % 16) / 8 + 2 * odd;
+            const float hi = tf32_hi(x[i]);
+            f[at] = hi;
+            f[at + 32 * 4] = x[i] - hi;
+        }
+    }
+}
+
+// Scores of a tile of rows against a step's slots: s[j] as the accumulator of slots 8 j .. 8 j + 7.
+template <class T, int HD, int NK>
+__device__ __forceinline__ void step_scores(const KvStep<T, HD, NK> &st, const float4 *frag, float (&s)[NK][4]) {
+    constexpr int P = T::V / 2;                 // products per load
+    const int lane = threadIdx.x & 31;
+    float lo1[NK][4], lo2[NK][4];
+#pragma unroll
+    for (int j = 0; j < NK; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[j][e] = lo1[j][e] = lo2[j][e] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < st.NC; c++) {
+        float x[NK][T::V];
+#pragma unroll
+        for (int j = 0; j < NK; j++) T::get(st.k[j][c], x[j]);
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            const float4 ah = frag[(c * P + p) * 64 + lane], al = frag[(c * P + p) * 64 + 32 + lane];
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+                const float b0 = x[j][2 * p], b1 = x[j][2 * p + 1];
+                if (T::SPLIT) {
+                    const float h0 = tf32_hi(b0), h1 = tf32_hi(b1);
+                    mma_tf32(s[j], ah, h0, h1);
+                    mma_tf32(lo1[j], ah, b0 - h0, b1 - h1);
+                    mma_tf32(lo2[j], al, h0, h1);
+                } else {
+                    mma_tf32(s[j], ah, b0, b1);
+                    mma_tf32(lo1[j], al, b0, b1);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NK; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[j][e] += T::SPLIT ? lo1[j][e] + lo2[j][e] : lo1[j][e];
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
+
+// A warp's running attention of 16 rows: maxima and sums in powers of two of rows lane / 4 and lane / 4 + 8 (the sum: this lane's slots only), and
+// the outputs, o[8 c' + V..]: see finish.
+template <class T, int HD, int NK>
+struct Running {
+    static constexpr int NN = HD / 8;           // 8 values wide products of the output
+    float m[2], l[2], o[NN][4];
+    __device__ __forceinline__ void clear() {
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NN; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[n][e] = 0.0f;
+    }
+    // s: scaled scores in powers of two, -infinity where a row does not see the slot.  partial: some row may not see some slot, whose values may be anything: a
+    // value that is no number goes into the sum of the rows that see it, and no further.
+    __device__ __forceinline__ void add(KvStep<T, HD, NK> &st, float (&s)[NK][4], bool partial) {
+        float top[2] = {m[0], m[1]};
+#pragma unroll
+        for (int j = 0; j < NK; j++) {
+            top[0] = fmaxf(top[0], fmaxf(s[j][0], s[j][1]));
+            top[1] = fmaxf(top[1], fmaxf(s[j][2], s[j][3]));
+        }
+        float corr[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+            const float safe = top[h] == -INFINITY ? 0.0f : top[h];
+            corr[h] = exp2_approx(m[h] - safe);
+            m[h] = top[h];
+            top[h] = safe;
+            l[h] *= corr[h];
+        }
+        float4 ph[NK], pl[NK];
+#pragma unroll
+        for (int j = 0; j < NK; j++) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[e] = exp2_approx(s[j][e] - top[e >> 1]);
+            if (partial) {
+                bool bad[2] = {false, false};
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int c = 0; c < st.NVC; c++) {
+                        float x[T::V];
+                        T::get(st.v[j][h][c], x);
+                        bool any = false;
+#pragma unroll
+                        for (int i = 0; i < T::V; i++) any |= not_finite(x[i]);
+                        bad[h] |= any;
+                        if (any) st.v[j][h][c] = make_uint4(0, 0, 0, 0);
+                    }
+                const uint32_t mine = 0x11111111u << (threadIdx.x & 3);
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (__ballot_sync(0xffffffffu, bad[h]) & mine) {
+                        if (s[j][h] != -INFINITY) p[h] = NAN;
+                        if (s[j][2 + h] != -INFINITY) p[2 + h] = NAN;
+                    }
+            }
+            l[0] += p[0] + p[1];
+            l[1] += p[2] + p[3];
+            // operand A: k = t is slot 2t, k = t + 4 slot 2t + 1
+            ph[j] = make_float4(tf32_hi(p[0]), tf32_hi(p[2]), tf32_hi(p[1]), tf32_hi(p[3]));
+            pl[j] = make_float4(p[0] - ph[j].x, p[2] - ph[j].y, p[1] - ph[j].z, p[3] - ph[j].w);
+        }
+#pragma unroll
+        for (int c = 0; c < st.NVC; c++) {
+            float d[T::V][4];
+#pragma unroll
+            for (int i = 0; i < T::V; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) d[i][e] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+                float x0[T::V], x1[T::V];
+                T::get(st.v[j][0][c], x0);
+                T::get(st.v[j][1][c], x1);
+#pragma unroll
+                for (int i = 0; i < T::V; i++) {
+                    if (T::SPLIT) {
+                        const float h0 = tf32_hi(x0[i]), h1 = tf32_hi(x1[i]);
+                        mma_tf32(d[i], ph[j], x0[i] - h0, x1[i] - h1);
+                        mma_tf32(d[i], pl[j], h0, h1);
+                        mma_tf32(d[i], ph[j], h0, h1);
+                    } else {
+                        mma_tf32(d[i], pl[j], x0[i], x1[i]);
+                        mma_tf32(d[i], ph[j], x0[i], x1[i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < T::V; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[c * T::V + i][e] = __fmaf_rn(o[c * T::V + i][e], corr[e >> 1], d[i][e]);
+        }
+    }
+    // Into shared memory: out [16][HD] (rows of this tile), ml [16][2].
+    __device__ __forceinline__ void store(float *out, float2 *ml) {
+        const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            const int r = (lane >> 2) + 8 * h;
+            if (t == 0) ml[r] = make_float2(m[h], l[h]);
+#pragma unroll
+            for (int c = 0; c < HD / (8 * T::V); c++)
+#pragma unroll
+                for (int n = 0; n < 2; n++)      // column 2t + n of products c V .. c V + V - 1: values 8V c + V (2t + n) ...
+#pragma unroll
+                    for (int i = 0; i < T::V; i += 4)
+                        *reinterpret_cast<float4 *>(out + r * HD + 8 * T::V * c + T::V * (2 * t + n) + i) =
+                            make_float4(o[c * T::V + i][2 * h + n], o[c * T::V + i + 1][2 * h + n], o[c * T::V + i + 2][2 * h + n], o[c * T::V + i + 3][2 * h + n]);
+        }
+    }
+};
+
+// Joins the parts of a CTA's WK groups of warps (part p: rows p * R ... of out and ml) into part 0.  All threads call it, after a barrier.
+template <int HD>
+__device__ __forceinline__ void join_warps(float *out, float2 *ml, int R, int parts) {
+    if (parts > 1) {
+        for (int u = threadIdx.x; u < R * (HD / 4); u += AW * 32) {
+            const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+            float m = -INFINITY;
+            for (int p = 0; p < parts; p++) m = fmaxf(m, ml[p * R + r].x);
+            const float safe = m == -INFINITY ? 0.0f : m;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int p = 0; p < parts; p++) {
+                const float w = exp2_approx(ml[p * R + r].x - safe);
+                const float4 y = *reinterpret_cast<const float4 *>(out + (p * R + r) * HD + d);
+                x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
+            }
+            *reinterpret_cast<float4 *>(out + r * HD + d) = x;
+        }
+        __syncthreads();
+        for (int r = threadIdx.x; r < R; r += AW * 32) {
+            float m = -INFINITY, l = 0.0f;
+            for (int p = 0; p < parts; p++) m = fmaxf(m, ml[p * R + r].x);
+            const float safe = m == -INFINITY ? 0.0f : m;
+            for (int p = 0; p < parts; p++) l = __fmaf_rn(exp2_approx(ml[p * R + r].x - safe), ml[p * R + r].y, l);
+            ml[r] = make_float2(m, l);
+        }
+    }
+}
+
+// Joins the CTAs of the cluster and writes the rows: CTA c takes its share of the values.  dst(r): the row's place in the output (< 0: padding), sink(r): its
+// sink in powers of two or -infinity.
+template <int HD, class Dst, class Sink>
+__device__ __forceinline__ void join_cluster(float *out, float2 *ml, int R, float *o, float *lse, Dst dst, Sink sink) {
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
+    cl.sync();
+    for (int u = c * AW * 32 + threadIdx.x; u < R * (HD / 4); u += C * AW * 32) {
+        const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+        const long long to = dst(r);
+        if (to < 0) continue;
+        const float sk = sink(r);
+        float m = sk;
+        for (int p = 0; p < C; p++) m = fmaxf(m, cl.map_shared_rank(ml, p)[r].x);
+        const float safe = m == -INFINITY ? 0.0f : m;
+        float l = exp2_approx(sk - safe);
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p = 0; p < C; p++) {
+            const float2 part = cl.map_shared_rank(ml, p)[r];
+            const float w = exp2_approx(part.x - safe);
+            const float4 y = *reinterpret_cast<const float4 *>(cl.map_shared_rank(out, p) + r * HD + d);
+            l = __fmaf_rn(w, part.y, l);
+            x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
+        }
+        const float den = l == 0.0f ? 1.0f : l;
+        *reinterpret_cast<float4 *>(o + to * HD + d) = make_float4(__fdividef(x.x, den), __fdividef(x.y, den), __fdividef(x.z, den), __fdividef(x.w, den));
+        if (lse && d == 0) lse[to] = (m + log2f(l)) * LN2;
+    }
+    cl.sync();
+}
+
+// ---------------------------------------------------------------- trees
+// What the rows of an entry see: cached slots from lo on, drafted rows by mask (windows applied, rows behind the count cut off).
+struct TreeRows {
+    uint64_t mask[KV_TREE_MAX];
+    int lo[KV_TREE_MAX];
+    int first, full;                        // smallest lo, largest lo: from there to len every row sees every slot
+};
+// All threads call it; ends with a barrier.
+__device__ __forceinline__ void tree_rows(const TreeArgs &a, int b, const KvEntry &e, TreeRows &w) {
     __shared__ int depth[KV_TREE_MAX];
-    const int b = blockIdx.y;
+    if (threadIdx.x == 0) { w.first = e.len; w.full = 0; }
+    tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
+    __syncthreads();
+    uint64_t m = 0;
+    int lo = 0;
+    const int i = threadIdx.x;
+    if (i < e.count) {
+        m = w.mask[i];
+        if (a.window > 0) {
+            lo = max(0, min(e.len, e.len + depth[i] + 1 - a.window));
+            uint64_t in = 0;
+            for (int j = 0; j < e.count; j++) in |= (uint64_t)(depth[i] - depth[j] < a.window) << j;
+            m &= in;
+        }
+    }
+    __syncthreads();
+    if (i < e.count) {
+        w.mask[i] = m;
+        w.lo[i] = lo;
+        atomicMin(&w.first, lo);
+        atomicMax(&w.full, lo);
+    }
+    __syncthreads();
+}
+
+// grid (C, kv heads x blocks of 16 WM rows, entries), clusters of C
+template <class T, int HD, int NK, int WM>
+__global__ void __launch_bounds__(AW * 32) tree_kernel(KvDev kv, TreeArgs a) {
+    constexpr int WK = AW / WM, R = 16 * WM, STEP = 8 * NK;
+    extern __shared__ __align__(16) float4 frag[];          // the queries, then the parts: out [WK][R][HD], ml [WK][R]
+    __shared__ TreeRows see;
+    const int per = a.nh / kv.nkv, blocks = (a.rows * per + R - 1) / R;
+    const int kvh = blockIdx.y / blocks, row0 = blockIdx.y % blocks * R, b = blockIdx.z;
     const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
-    if (!e.ok) {
-        if (threadIdx.x == 0) kv_error(kv);
+    if (!e.ok || row0 >= e.count * per) {
+        if (!e.ok && threadIdx.x == 0) kv_error(kv);
         return;
     }
-    tree_masks(a.mask, b, a.rows, e.count, mask, depth);
+    tree_rows(a, b, e, see);
+    stage_queries<T, HD>(frag, WM, [&](int r) -> const float * {
+        const int i = (row0 + r) / per;
+        return i < e.count ? a.q + (((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per) * HD : nullptr;
+    });
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp % WM, wk = warp / WM, end = e.len + e.count;
+    // this lane's two rows
+    uint64_t mask[2];
+    int lo[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int i = (row0 + wm * 16 + (lane >> 2) + 8 * h) / per;
+        mask[h] = i < e.count ? see.mask[i] : 0;
+        lo[h] = i < e.count ? see.lo[i] : 0x7fffffff;
+    }
     __syncthreads();
-    const int u = blockIdx.x * 4 + (threadIdx.x >> 5), i = u / a.nh, h = u % a.nh;
-    if (i >= e.count) return;
-    const long long row = ((long long)b * a.rows + i) * a.nh + h;
-    int t = -1;
-    auto next = [&]() {
-        for (t++; t < e.len + e.count; t++)
-            if (tree_sees(mask, depth, e.len, a.window, i, t)) return t;
-        return -1;
-    };
-    warp_attend(kv, kv.head(e.seq, h / (a.nh / kv.nkv)), a.q + row * kv.hd, a.scale, a.sinks ? a.sinks + h : nullptr, a.out + row * kv.hd, a.lse ? a.lse + row : nullptr, next);
+    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh), *vc = (const typename T::Val *)kv.v + kv.head(e.seq, kvh);
+    const float c = a.scale * LOG2E;
+    // the CTA's steps, the warp's among them
+    const int s0 = see.first / STEP, steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
+    const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps);
+    Running<T, HD, NK> run;
+    run.clear();
+    KvStep<T, HD, NK> st;
+    int s = from + wk;
+    if (s < to) {
+        st.template load_k<WM == 1>(kc, s * STEP, end);
+        st.template load_v<WM == 1>(vc, s * STEP, end);
+    }
+    for (; s < to; s += WK) {
+        const int base = s * STEP;
+        float x[NK][4];
+        step_scores<T, HD, NK>(st, frag + wm * (HD / 8) * 64, x);
+        if (s + WK < to) st.template load_k<WM == 1>(kc, (s + WK) * STEP, end);
+        const bool partial = base < see.full || base + STEP > e.len;
+#pragma unroll
+        for (int j = 0; j < NK; j++)
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                x[j][f] *= c;
+                if (partial) {
+                    const int t = base + 8 * j + 2 * (lane & 3) + (f & 1), h = f >> 1;
+                    const bool sees = t < e.len ? t >= lo[h] : t < end && (mask[h] >> (t - e.len) & 1);
+                    if (!sees) x[j][f] = -INFINITY;
+                }
+            }
+        run.add(st, x, partial);
+        if (s + WK < to) st.template load_v<WM == 1>(vc, (s + WK) * STEP, end);
+    }
+    __syncthreads();                 // the queries have been read
+    float *out = reinterpret_cast<float *>(frag);
+    float2 *ml = reinterpret_cast<float2 *>(out + WK * R * HD);
+    run.store(out + (wk * R + wm * 16) * HD, ml + wk * R + wm * 16);
+    __syncthreads();
+    join_warps<HD>(out, ml, R, WK);
+    join_cluster<HD>(out, ml, R, a.out, a.lse,
+                     [&](int r) -> long long {
+                         const int i = (row0 + r) / per;
+                         return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
+                     },
+                     [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
+}
+
+template <class Kernel, class... Args>
+cudaError_t launch_cluster(Kernel k, dim3 grid, int cluster, size_t smem, cudaStream_t st, Args... args) {
+    cudaError_t e = cudaSuccess;
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(AW * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
+// bytes of a CTA's shared memory: the queries, later the parts
+static size_t attn_smem(int hd, int wm) {
+    const size_t parts = (size_t)AW * 16 * (hd * 4 + 8), queries = (size_t)wm * hd * 128;
+    return parts > queries ? parts : queries;
+}
+
+// CTAs that share an entry's slots: as many as fill the GPU twice, while each has at least four steps
+static int cluster_size(long long ctas, int steps) {
+    int c = 1;
+    while (c < 16 && ctas * c * 2 <= 2 * 148 && steps / (2 * c) >= 4) c *= 2;
+    return c;
+}
+
+template <class T, int HD, int NK>
+static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
+    const int per = a.nh / kv.nkv, tiles = (a.rows * per + 15) / 16, wm = tiles > 4 ? 8 : tiles > 2 ? 4 : tiles, blocks = (tiles + wm - 1) / wm;
+    int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
+    if (a.window > 0) slots = min(slots, a.window + a.rows);
+    const int c = cluster_size((long long)a.n * kv.nkv * blocks, slots / (8 * NK));
+    const dim3 grid(c, kv.nkv * blocks, a.n);
+    const size_t smem = attn_smem(HD, wm);
+    switch (wm) {
+        case 1: return launch_cluster(tree_kernel<T, HD, NK, 1>, grid, c, smem, st, kv, a);
+        case 2: return launch_cluster(tree_kernel<T, HD, NK, 2>, grid, c, smem, st, kv, a);
+        case 4: return launch_cluster(tree_kernel<T, HD, NK, 4>, grid, c, smem, st, kv, a);
+        default: return launch_cluster(tree_kernel<T, HD, NK, 8>, grid, c, smem, st, kv, a);
+    }
 }
 
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
-    tree_kernel<<<dim3((a.rows * a.nh + 3) / 4, a.n), 128, 0, st>>>(kv, a);
-    return cudaGetLastError();
+    if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2>(kv, a, len_hint, st) : launch_tree<KvBf16, 128, 2>(kv, a, len_hint, st);
+    return kv.hd == 64 ? launch_tree<KvF32, 64, 2>(kv, a, len_hint, st) : launch_tree<KvF32, 128, 1>(kv, a, len_hint, st);
 }
 
 // ---------------------------------------------------------------- book of weights
-// A thread per slot: its key against every row's query.
-__global__ void __launch_bounds__(128) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked) {
-    __shared__ uint64_t mask[KV_TREE_MAX];
-    __shared__ int depth[KV_TREE_MAX];
-    const int kvh = blockIdx.y, b = blockIdx.z, per = a.nh / kv.nkv;
+// A CTA per run of slots, kv head and entry; a warp owns a step of slots and takes the rows 16 WT at a time, whose queries wait in shared memory: every
+// slot's weight is formed and added by one warp in the order of the rows.
+template <class T, int HD, int NK, int WT>
+__global__ void __launch_bounds__(AW * 32) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked) {
+    constexpr int R = 16 * WT, STEP = 8 * NK;
+    extern __shared__ __align__(16) float4 frag[];
+    __shared__ TreeRows see;
+    __shared__ float lse[R];
+    const int kvh = blockIdx.y, b = blockIdx.z, per = a.nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
     if (kv_named_before(a.seq, b) || !e.ok) {
         if (threadIdx.x == 0) kv_error(kv);
         return;
     }
-    tree_masks(a.mask, b, a.rows, e.count, mask, depth);
-    __syncthreads();
+    tree_rows(a, b, e, see);
     const uint64_t rows = picked ? picked[b] : ~0ull;
-    for (int t = blockIdx.x * 128 + threadIdx.x; t < e.len + e.count; t += gridDim.x * 128) {
-        const long long at = kv.head(e.seq, kvh) + (long long)t * kv.hd;
-        float sum = 0.0f;
-        for (int i = 0; i < e.count; i++) {
-            if (!(rows >> i & 1) || !tree_sees(mask, depth, e.len, a.window, i, t)) continue;
-            for (int g = 0; g < per; g++) {
-                const long long row = ((long long)b * a.rows + i) * a.nh + kvh * per + g;
-                float s = 0.0f;
-                for (int d = 0; d < kv.hd; d++) s = __fmaf_rn(a.q[row * kv.hd + d], kv_load(kv.k, kv.type, at + d), s);
-                sum += expf(__fmaf_rn(s, a.scale, -a.lse[row]));
+    const int end = e.len + e.count, steps = (end + STEP - 1) / STEP, s0 = see.first / STEP;
+    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh);
+    float *weight = kv.weight + kv.book(e.seq, kvh);
+    const float c = a.scale * LOG2E;
+    for (int row0 = 0; row0 < e.count * per; row0 += R) {
+        const int tiles = min(WT, (e.count * per - row0 + 15) / 16);
+        __syncthreads();
+        stage_queries<T, HD>(frag, tiles, [&](int r) -> const float * {
+            const int i = (row0 + r) / per;
+            return i < e.count ? a.q + (((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per) * HD : nullptr;
+        });
+        for (int r = threadIdx.x; r < R; r += AW * 32) {
+            const int i = (row0 + r) / per;
+            // a row that does not count has an infinite sum: weights of zero
+            lse[r] = i < e.count && (rows >> i & 1) ? a.lse[((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per] * LOG2E : INFINITY;
+        }
+        __syncthreads();
+        for (int s = s0 + blockIdx.x * AW + warp; s < steps; s += gridDim.x * AW) {
+            const int base = s * STEP;
+            KvStep<T, HD, NK> st;
+            st.template load_k<WT == 1>(kc, base, end);
+            const bool partial = base < see.full || base + STEP > e.len;
+            float sum[NK][2];
+#pragma unroll
+            for (int j = 0; j < NK; j++) sum[j][0] = sum[j][1] = 0.0f;
+            for (int w = 0; w < tiles; w++) {
+                float x[NK][4];
+                step_scores<T, HD, NK>(st, frag + w * (HD / 8) * 64, x);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int r = w * 16 + (lane >> 2) + 8 * h, i = (row0 + r) / per;
+                    const float z = lse[r];
+                    const uint64_t mask = partial && i < e.count ? see.mask[i] : 0;
+                    const int lo = i < e.count ? see.lo[i] : 0x7fffffff;
+#pragma unroll
+                    for (int j = 0; j < NK; j++)
+#pragma unroll
+                        for (int f = 0; f < 2; f++) {
+                            float p = exp2_approx(__fmaf_rn(x[j][2 * h + f], c, -z));
+                            if (partial) {
+                                const int t = base + 8 * j + 2 * (lane & 3) + f;
+                                if (!(t < e.len ? t >= lo : t < end && (mask >> (t - e.len) & 1))) p = 0.0f;
+                            }
+                            sum[j][f] += z == INFINITY ? 0.0f : p;
+                        }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+#pragma unroll
+                for (int f = 0; f < 2; f++)
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) sum[j][f] += __shfl_xor_sync(0xffffffffu, sum[j][f], o);
+                const int t = base + 8 * j + 2 * lane;
+                if (lane < 4) {
+                    if (t < end) weight[t] += sum[j][0];
+                    if (t + 1 < end) weight[t + 1] += sum[j][1];
+                }
             }
         }
-        kv.weight[kv.book(e.seq, kvh) + t] += sum;
     }
 }
 
+template <class T, int HD, int NK>
+static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
+    const int per = a.nh / kv.nkv, tiles = (a.rows * per + 15) / 16;
+    int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
+    const int ctas = (slots / (8 * NK) + AW) / AW;
+    const dim3 grid(max(1, min(ctas, 4096)), kv.nkv, a.n);
+    if (tiles == 1) return launch_cluster(weigh_kernel<T, HD, NK, 1>, grid, 1, (size_t)HD * 128, st, kv, a, picked);
+    if (tiles <= 4) return launch_cluster(weigh_kernel<T, HD, NK, 4>, grid, 1, (size_t)4 * HD * 128, st, kv, a, picked);
+    return launch_cluster(weigh_kernel<T, HD, NK, 8>, grid, 1, (size_t)8 * HD * 128, st, kv, a, picked);
+}
+
 cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
-    const int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
-    weigh_kernel<<<dim3((slots + 127) / 128, kv.nkv, a.n), 128, 0, st>>>(kv, a, picked);
-    return cudaGetLastError();
+    if (kv.type) return kv.hd == 64 ? launch_weigh<KvBf16, 64, 2>(kv, a, picked, len_hint, st) : launch_weigh<KvBf16, 128, 2>(kv, a, picked, len_hint, st);
+    return kv.hd == 64 ? launch_weigh<KvF32, 64, 2>(kv, a, picked, len_hint, st) : launch_weigh<KvF32, 128, 2>(kv, a, picked, len_hint, st);
 }
 
 // ---------------------------------------------------------------- chosen blocks
@@ -152,21 +664,61 @@ __global__ void __launch_bounds__(CB_THREADS) choose_blocks_kernel(KvDev kv, con
         }
 }
 
-__global__ void __launch_bounds__(128) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, int nsel, const int32_t *sel, const float *q, int nh,
-                                                     float scale, const float *sinks, float *out, float *lse) {
-    const int r = blockIdx.y, h = blockIdx.x * 4 + (threadIdx.x >> 5);
+// A cluster per (kv head, row): the chosen blocks' slots in steps, over the warps and the CTAs.
+template <class T, int HD, int NK>
+__global__ void __launch_bounds__(AW * 32) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, int nsel, const int32_t *sel, const float *q, int nh,
+                                                         float scale, const float *sinks, float *o, float *lse) {
+    constexpr int R = 16, STEP = 8 * NK;
+    extern __shared__ __align__(16) float4 frag[];
+    __shared__ int32_t chosen[256];
+    const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int s = seq ? seq[r] : r, n = len[r];
-    if (h >= nh || (unsigned)s >= (unsigned)kv.n_seq || (unsigned)n > (unsigned)kv.cap) return;
-    const int kvh = h / (nh / kv.nkv);
-    const int32_t *mine = sel + ((long long)r * kv.nkv + kvh) * nsel;
-    const long long row = (long long)r * nh + h;
-    int c = 0, o = -1;
-    auto next = [&]() {
-        if (++o == block) { o = 0; c++; }
-        const int t = c < nsel && mine[c] >= 0 ? mine[c] * block + o : n;
-        return t < n ? t : -1;
-    };
-    warp_attend(kv, kv.head(s, kvh), q + row * kv.hd, scale, sinks ? sinks + h : nullptr, out + row * kv.hd, lse ? lse + row : nullptr, next);
+    if ((unsigned)s >= (unsigned)kv.n_seq || (unsigned)n > (unsigned)kv.cap) return;
+    const long long row = (long long)r * nh + kvh * per;
+    for (int i = threadIdx.x; i < nsel; i += AW * 32) chosen[i] = sel[((long long)r * kv.nkv + kvh) * nsel + i];
+    stage_queries<T, HD>(frag, 1, [&](int i) -> const float * { return i < per ? q + (row + i) * HD : nullptr; });
+    __syncthreads();
+    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(s, kvh), *vc = (const typename T::Val *)kv.v + kv.head(s, kvh);
+    const float c = scale * LOG2E;
+    const int each = block / STEP, steps = min(nsel, (n + block - 1) / block) * each;
+    Running<T, HD, NK> run;
+    run.clear();
+    KvStep<T, HD, NK> st;
+    const int hop = gridDim.x * AW;
+    int i = blockIdx.x * AW + warp;
+    auto slot = [&](int i) { return chosen[i / each] * block + i % each * STEP; };
+    if (i < steps) {
+        st.template load_k<true>(kc, slot(i), n);
+        st.template load_v<true>(vc, slot(i), n);
+    }
+    for (; i < steps; i += hop) {
+        const int base = slot(i);
+        float x[NK][4];
+        step_scores<T, HD, NK>(st, frag, x);
+        if (i + hop < steps) st.template load_k<true>(kc, slot(i + hop), n);
+#pragma unroll
+        for (int j = 0; j < NK; j++)
+#pragma unroll
+            for (int f = 0; f < 4; f++) x[j][f] = base + 8 * j + 2 * (lane & 3) + (f & 1) < n ? x[j][f] * c : -INFINITY;
+        run.add(st, x, false);
+        if (i + hop < steps) st.template load_v<true>(vc, slot(i + hop), n);
+    }
+    __syncthreads();
+    float *out = reinterpret_cast<float *>(frag);
+    float2 *ml = reinterpret_cast<float2 *>(out + AW * R * HD);
+    run.store(out + warp * R * HD, ml + warp * R);
+    __syncthreads();
+    join_warps<HD>(out, ml, R, AW);
+    join_cluster<HD>(out, ml, R, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
+                     [&](int i) { return sinks ? sinks[kvh * per + i] * LOG2E : -INFINITY; });
+}
+
+template <class T, int HD, int NK>
+static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, int nsel, int len_hint, const float *q, int nh, float scale,
+                                 const float *sinks, const int32_t *sel, float *out, float *lse, cudaStream_t st) {
+    const int slots = min(nsel * block, len_hint > 0 ? min(len_hint, kv.cap) : kv.cap);
+    const int c = cluster_size((long long)rows * kv.nkv, slots / (8 * NK));
+    return launch_cluster(blocks_kernel<T, HD, NK>, dim3(c, rows, kv.nkv), c, attn_smem(HD, 1), st, kv, seq, len, block, nsel, sel, q, nh, scale, sinks, out, lse);
 }
 
 cudaError_t launch_attn_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,
@@ -177,8 +729,10 @@ cudaError_t launch_attn_blocks(const KvDev &kv, int rows, const int32_t *seq, co
     choose_blocks_kernel<<<dim3(rows, kv.nkv), CB_THREADS, smem, st>>>(kv, seq, len, block, means, nsel, first, local, q, nh, sel);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    blocks_kernel<<<dim3((nh + 3) / 4, rows), 128, 0, st>>>(kv, seq, len, block, nsel, sel, q, nh, scale, sinks, out, lse);
-    return cudaGetLastError();
+    if (kv.type) return kv.hd == 64 ? launch_blocks<KvBf16, 64, 2>(kv, rows, seq, len, block, nsel, len_hint, q, nh, scale, sinks, sel, out, lse, st)
+                                    : launch_blocks<KvBf16, 128, 2>(kv, rows, seq, len, block, nsel, len_hint, q, nh, scale, sinks, sel, out, lse, st);
+    return kv.hd == 64 ? launch_blocks<KvF32, 64, 2>(kv, rows, seq, len, block, nsel, len_hint, q, nh, scale, sinks, sel, out, lse, st)
+                       : launch_blocks<KvF32, 128, 1>(kv, rows, seq, len, block, nsel, len_hint, q, nh, scale, sinks, sel, out, lse, st);
 }
 
 }  // namespace brrr
