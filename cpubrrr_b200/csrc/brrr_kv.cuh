@@ -70,4 +70,54 @@ __device__ __forceinline__ bool tree_sees(const uint64_t *m, const int *depth, i
     return (m[i] >> j & 1) && (window <= 0 || depth[i] - depth[j] < window);
 }
 
+// Work space of block_kth in shared memory.
+struct KthSpace {
+    uint32_t hist[2048], found[2], sums[32];
+};
+// The key of the k-th largest (1 <= k <= n) of key(0) .. key(n - 1), and how many of the keys that equal it are among the k largest: eleven bits at a time
+// (the first hold sign, exponent and two more: fewer counts meet in one word than with eight).  All threads call it; it ends with a barrier.
+template <class Key>
+__device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpace &w, uint32_t *ties) {
+    uint32_t prefix = 0, known = 0;
+    const int each = 2048 / blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digit = pass == 2 ? 1023u : 2047u;
+        for (int i = threadIdx.x; i < 2048; i += blockDim.x) w.hist[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += blockDim.x) {
+            const uint32_t x = key(i);
+            if ((x & known) == prefix) atomicAdd(&w.hist[x >> shift & digit], 1u);
+        }
+        __syncthreads();
+        // thread i: `each` digits, the largest first
+        const int top = 2047 - threadIdx.x * each;
+        uint32_t sum = 0;
+        for (int j = 0; j < each; j++) sum += w.hist[top - j];
+        uint32_t upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane == 31) w.sums[warp] = upto;
+        __syncthreads();
+        for (int i = 0; i < warp; i++) upto += w.sums[i];
+        uint32_t above = upto - sum;
+        if (above < k && k <= upto)
+            for (int j = 0; j < each; j++) {
+                const uint32_t c = w.hist[top - j];
+                if (above < k && k <= above + c) { w.found[0] = top - j; w.found[1] = k - above; }
+                above += c;
+            }
+        __syncthreads();
+        prefix |= w.found[0] << shift;
+        known |= digit << shift;
+        k = w.found[1];
+        __syncthreads();
+    }
+    *ties = k;
+    return prefix;
+}
+
 }  // namespace brrr

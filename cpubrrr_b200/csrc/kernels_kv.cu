@@ -2,6 +2,7 @@
 #include "brrr_kernels.h"
 #include "brrr_block.cuh"
 #include "brrr_kv.cuh"
+#include "brrr_tma.cuh"
 
 #include <cuda_bf16.h>
 
@@ -23,7 +24,7 @@ __device__ __forceinline__ void kv_store4(void *p, int type, long long at, float
 // A CTA per row.  A thread turns four pairs (j, j + hd / 2): products and sums rounded one by one, as the engines rotate.
 __global__ void kv_append_kernel(KvDev kv, int rows, const int32_t *seq, const int32_t *len, const int32_t *count, const int32_t *at,
                                  const float *__restrict__ qkv, long long ld, int nh, const float *__restrict__ rope, int n_rope, float *__restrict__ q) {
-    const int i = blockIdx.x, b = blockIdx.y;
+    const int i = blockIdx.x, b = blockIdx.y, half = kv.hd / 2, per = half / 4;
     const KvEntry e = kv_entry(kv, b, rows, seq, len, count);
     if (kv_named_before(seq, b) || !e.ok) {
         if (threadIdx.x == 0) kv_error(kv);
@@ -35,9 +36,9 @@ __global__ void kv_append_kernel(KvDev kv, int rows, const int32_t *seq, const i
         if (threadIdx.x == 0) kv_error(kv);
         return;
     }
-    const int half = kv.hd / 2, per = half / 4;
     const float *x = qkv + ((long long)b * rows + i) * ld;
     float *qo = q ? q + ((long long)b * rows + i) * nh * kv.hd : nullptr;
+#pragma unroll 2
     for (int u = threadIdx.x + (q ? 0 : nh * per); u < (nh + 2 * kv.nkv) * per; u += blockDim.x) {
         const int head = u / per, j = u % per * 4;
         float4 lo = *reinterpret_cast<const float4 *>(x + head * kv.hd + j), hi = *reinterpret_cast<const float4 *>(x + head * kv.hd + half + j);
@@ -69,7 +70,7 @@ __global__ void kv_append_kernel(KvDev kv, int rows, const int32_t *seq, const i
 
 cudaError_t launch_kv_append(const KvDev &kv, int n, int rows, const int32_t *seq, const int32_t *len, const int32_t *count, const int32_t *at, const float *qkv,
                              long long ld, int nh, const float *rope, int n_rope, float *q, cudaStream_t st) {
-    kv_append_kernel<<<dim3(rows, n), 256, 0, st>>>(kv, rows, seq, len, count, at, qkv, ld, nh, rope, n_rope, q);
+    kv_append_kernel<<<dim3(rows, n), 512, 0, st>>>(kv, rows, seq, len, count, at, qkv, ld, nh, rope, n_rope, q);
     return cudaGetLastError();
 }
 
@@ -127,9 +128,9 @@ cudaError_t launch_kv_commit(const KvDev &kv, int n, int rows, const int32_t *se
 }
 
 // ---------------------------------------------------------------- eviction
-// Which entries stay: a CTA per (kv head, entry) finds the key of the last one kept digit by digit (four counts of 256 digits), then turns the
-// keys into one bit per slot, and pairs the freed slots below m with the kept entries behind.  Bits and running counts per 32 slots stand
-// in shared memory.
+// Which entries stay: a CTA per (kv head, entry) finds the key of the last one kept digit by digit, then turns the keys into one bit per slot, and pairs the
+// freed slots below m with the kept entries behind.  Bits and running counts per 32 slots stand in shared memory, and the keys where there is
+// room for a cache's (46,000 slots; above, they are formed from the books again at every pass).
 constexpr int EV_THREADS = 1024;
 
 // protected entries above all weights, NaN below all, -0 as +0
@@ -167,52 +168,12 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t *v, int n, uint32_t *war
     return carry;
 }
 
-// The key of the k-th largest (1 <= k <= n) of key(0) .. key(n - 1), and how many of the keys that equal it are among the k largest.
-template <class Key>
-__device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, uint32_t *hist, uint32_t *found, uint32_t *ties) {
-    uint32_t prefix = 0, known = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += blockDim.x) {
-            const uint32_t x = key(i);
-            if ((x & known) == prefix) atomicAdd(&hist[x >> shift & 255], 1u);
-        }
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            // lane l: digits 255 - 8 l .. 248 - 8 l, from the largest
-            uint32_t c[8], sum = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) { c[j] = hist[255 - 8 * threadIdx.x - j]; sum += c[j]; }
-            uint32_t upto = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-                if ((int)threadIdx.x >= o) upto += y;
-            }
-            uint32_t above = upto - sum;
-            if (above < k && k <= upto) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (above < k && k <= above + c[j]) { found[0] = 255 - 8 * threadIdx.x - j; found[1] = k - above; }
-                    above += c[j];
-                }
-            }
-        }
-        __syncthreads();
-        prefix |= found[0] << shift;
-        known |= 255u << shift;
-        k = found[1];
-        __syncthreads();
-    }
-    *ties = k;
-    return prefix;
-}
-
-__global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev dst, int rows, const int32_t *seq, const int32_t *len, int keep, int first, int recent,
+template <bool KEEP_KEYS>
+__global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev dst, const int32_t *seq, const int32_t *len, int keep, int first, int recent,
                                                               const int32_t *end, int32_t *map, int32_t *new_len) {
     extern __shared__ uint32_t sm[];
-    __shared__ uint32_t hist[256], found[2], sums[32];
+    __shared__ KthSpace kth;
+    pdl_trigger();
     const int kvh = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = EV_THREADS / 32;
     const KvEntry e = kv_entry(kv, b, 0, seq, len, nullptr);
     const bool bad = kv_named_before(seq, b) || !e.ok || e.seq >= dst.n_seq;
@@ -234,11 +195,17 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     const float *w = kv.weight + kv.book(e.seq, kvh);
     const int32_t *pos = kv.pos + kv.book(e.seq, kvh);
     const long long from = recent > 0 ? (long long)end[b] - recent : 1ll << 31;
-    auto key = [&](int t) { return evict_key(w[t], pos[t], first, from); };
-    uint32_t ties;
-    const uint32_t last = block_kth(e.len, m, key, hist, found, &ties);
     const int words = (e.len + 31) / 32, mw = m / 32;
-    uint32_t *kept = sm, *run = sm + words;      // bits of 32 slots each; running counts [words + 1]
+    uint32_t *kept = sm, *run = sm + words, *keys = run + words + 1;
+    if (KEEP_KEYS) {
+#pragma unroll 4
+        for (int t = threadIdx.x; t < e.len; t += EV_THREADS) keys[t] = evict_key(w[t], pos[t], first, from);
+        __syncthreads();
+    }
+    auto key = [&](int t) { return KEEP_KEYS ? keys[t] : evict_key(w[t], pos[t], first, from); };
+    uint32_t ties;
+    const uint32_t last = block_kth(e.len, m, key, kth, &ties);
+    // kept: bits of 32 slots each; run: running counts [words + 1]
     for (int i = warp; i < words; i += nwarp) {
         const int t = i * 32 + lane;
         const uint32_t x = t < e.len ? key(t) : 0;
@@ -246,7 +213,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
         if (lane == 0) { kept[i] = over; run[i] = __popc(same); }
     }
     __syncthreads();
-    block_scan(run, words, sums);
+    block_scan(run, words, kth.sums);
     for (int i = warp; i < words; i += nwarp) {
         const int t = i * 32 + lane;
         const bool same = t < e.len && key(t) == last;
@@ -263,8 +230,8 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
         else run[i] = __popc(i - 1 == mw ? kept[i - 1] & ~low : kept[i - 1]);
     }
     __syncthreads();
-    block_scan(run, mw + 1, sums);
-    block_scan(run + mw + 1, words - mw, sums);
+    block_scan(run, mw + 1, kth.sums);
+    block_scan(run + mw + 1, words - mw, kth.sums);
     for (int i = warp; i < words; i += nwarp) {
         const int t = i * 32 + lane;
         if (!(kept[i] >> lane & 1)) continue;
@@ -282,42 +249,59 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     }
 }
 
-// 16 bytes per thread and step; entry rows of K and V, the books with the first unit
+// A thread moves 16 bytes of up to MV_BATCH entries' keys and values, all read before the first is written; the books go with an entry's first bytes.
+constexpr int MV_BATCH = 4;
 __global__ void __launch_bounds__(256) kv_move_kernel(KvDev kv, KvDev dst, bool inplace, const int32_t *seq, int keep, const int32_t *map) {
-    const int kvh = blockIdx.y, b = blockIdx.z, per = kv.hd * kv.size() / 16;
+    const int kvh = blockIdx.y, b = blockIdx.z, per = kv.hd * kv.size() / 16;       // a power of two
     const int s = seq ? seq[b] : b;
+    if ((unsigned)s >= (unsigned)kv.n_seq || s >= dst.n_seq) return;
     const int32_t *from = map + ((long long)b * kv.nkv + kvh) * keep;
-    if (from[0] < 0 || (unsigned)s >= (unsigned)kv.n_seq || s >= dst.n_seq) return;       // an entry that was left out, or an empty one
     const uint4 *k = reinterpret_cast<const uint4 *>((const char *)kv.k + kv.head(s, kvh) * kv.size()), *v = reinterpret_cast<const uint4 *>((const char *)kv.v + kv.head(s, kvh) * kv.size());
     uint4 *k2 = reinterpret_cast<uint4 *>((char *)dst.k + dst.head(s, kvh) * dst.size()), *v2 = reinterpret_cast<uint4 *>((char *)dst.v + dst.head(s, kvh) * dst.size());
     const long long book = kv.book(s, kvh), book2 = dst.book(s, kvh);
-    for (long long u = blockIdx.x * 256ll + threadIdx.x; u < (long long)keep * per; u += gridDim.x * 256ll) {
-        const int d = (int)(u / per), c = (int)(u % per), t = from[d];
-        if (t < 0 || (inplace && t == d)) continue;
-        k2[(long long)d * per + c] = k[(long long)t * per + c];
-        v2[(long long)d * per + c] = v[(long long)t * per + c];
-        if (c == 0) { dst.weight[book2 + d] = kv.weight[book + t]; dst.pos[book2 + d] = kv.pos[book + t]; }
+    const int c = threadIdx.x % per, rows = 256 / per, d0 = blockIdx.x * rows * MV_BATCH + threadIdx.x / per;
+    pdl_wait();
+    int t[MV_BATCH];
+    uint4 x[MV_BATCH], y[MV_BATCH];
+#pragma unroll
+    for (int i = 0; i < MV_BATCH; i++) {
+        const int d = d0 + i * rows;
+        t[i] = d < keep ? from[d] : -1;           // -1 throughout for an entry that was left out
+        if (inplace && t[i] == d) t[i] = -1;
+    }
+#pragma unroll
+    for (int i = 0; i < MV_BATCH; i++)
+        if (t[i] >= 0) { x[i] = k[(long long)t[i] * per + c]; y[i] = v[(long long)t[i] * per + c]; }
+#pragma unroll
+    for (int i = 0; i < MV_BATCH; i++) {
+        const int d = d0 + i * rows;
+        if (t[i] < 0) continue;
+        k2[(long long)d * per + c] = x[i];
+        v2[(long long)d * per + c] = y[i];
+        if (c == 0) { dst.weight[book2 + d] = kv.weight[book + t[i]]; dst.pos[book2 + d] = kv.pos[book + t[i]]; }
     }
 }
 
 cudaError_t launch_kv_evict(const KvDev &kv, const KvDev *dst, int n, const int32_t *seq, const int32_t *len, int keep, int first, int recent, const int32_t *end,
                             int32_t *map, int32_t *new_len, int len_hint, cudaStream_t st) {
     const KvDev &to = dst ? *dst : kv;
-    const size_t smem = ((size_t)(kv.cap + 31) / 32 * 2 + 1) * 4;
-    cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(kv_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+    const size_t bits = ((size_t)(kv.cap + 31) / 32 * 2 + 1) * 4, all = bits + (size_t)kv.cap * 4, most = 200 * 1024;
+    const bool keys = all <= most;
+    const size_t smem = keys ? all : bits;
+    auto kern = keys ? kv_evict_kernel<true> : kv_evict_kernel<false>;
+    cudaError_t e = smem > 36 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) : cudaSuccess;
     if (e != cudaSuccess) return e;
-    kv_evict_kernel<<<dim3(kv.nkv, n), EV_THREADS, smem, st>>>(kv, to, 0, seq, len, keep, first, recent, end, map, new_len);
+    kern<<<dim3(kv.nkv, n), EV_THREADS, smem, st>>>(kv, to, seq, len, keep, first, recent, end, map, new_len);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const long long units = (long long)keep * (kv.hd * kv.size() / 16);
-    const int chunks = (int)min(max(units / 1024, 1ll), 1024ll);
-    kv_move_kernel<<<dim3(chunks, kv.nkv, n), 256, 0, st>>>(kv, to, dst == nullptr, seq, keep, map);
-    return cudaGetLastError();
+    const int rows = 256 / (kv.hd * kv.size() / 16) * MV_BATCH;
+    return launch_k(kv_move_kernel, dim3((keep + rows - 1) / rows, kv.nkv, n), dim3(256), 0, st, true, kv, to, dst == nullptr, seq, keep, (const int32_t *)map);
 }
 
 // ---------------------------------------------------------------- block means
-// A thread sums one dimension of a block in double precision.
-__global__ void kv_means_kernel(KvDev kv, const int32_t *seq, const int32_t *since, const int32_t *len, int block, float *__restrict__ means) {
+// A CTA per block: a thread adds four dimensions of every 16th (8th) row in double precision, then the groups of rows are added.
+__global__ void __launch_bounds__(256) kv_means_kernel(KvDev kv, const int32_t *seq, const int32_t *since, const int32_t *len, int block, float *__restrict__ means) {
+    __shared__ double part[256 * 4];
     const int kvh = blockIdx.y, b = blockIdx.z;
     const KvEntry e = kv_entry(kv, b, 0, seq, len, nullptr);
     const int s0 = since ? since[b] : 0;
@@ -325,22 +309,38 @@ __global__ void kv_means_kernel(KvDev kv, const int32_t *seq, const int32_t *sin
         if (threadIdx.x == 0) kv_error(kv);
         return;
     }
-    const int d = threadIdx.x;
+    const int quads = kv.hd / 4, groups = 256 / quads, d = threadIdx.x % quads * 4, g = threadIdx.x / quads;
     const long long head = kv.head(e.seq, kvh);
     float *out = means + ((long long)e.seq * kv.nkv + kvh) * (kv.cap / block) * kv.hd;
     for (int j = s0 / block + blockIdx.x; j < e.len / block; j += gridDim.x) {
-        double sum = 0.0;
-        for (int t = 0; t < block; t++) {
+        double sum[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 8
+        for (int t = g; t < block; t += groups) {
             const long long at = head + (long long)(j * block + t) * kv.hd + d;
-            sum += kv.type ? (double)brrr_bf16_to_f32(((const uint16_t *)kv.k)[at]) : (double)((const float *)kv.k)[at];
+            float4 x;
+            if (kv.type) {
+                const ushort4 u = *reinterpret_cast<const ushort4 *>((const uint16_t *)kv.k + at);
+                x = make_float4(brrr_bf16_to_f32(u.x), brrr_bf16_to_f32(u.y), brrr_bf16_to_f32(u.z), brrr_bf16_to_f32(u.w));
+            } else {
+                x = *reinterpret_cast<const float4 *>((const float *)kv.k + at);
+            }
+            sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
         }
-        out[(long long)j * kv.hd + d] = (float)(sum / block);
+#pragma unroll
+        for (int i = 0; i < 4; i++) part[i * 256 + threadIdx.x] = sum[i];
+        __syncthreads();
+        for (int x = threadIdx.x; x < kv.hd; x += 256) {
+            double all = 0.0;
+            for (int i = 0; i < groups; i++) all += part[(x & 3) * 256 + i * quads + (x >> 2)];
+            out[(long long)j * kv.hd + x] = (float)(all / block);
+        }
+        __syncthreads();
     }
 }
 
 cudaError_t launch_kv_means(const KvDev &kv, int n, const int32_t *seq, const int32_t *since, const int32_t *len, int block, int len_hint, float *means, cudaStream_t st) {
-    const int blocks = max(1, min((len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) / block + 1, 4096));
-    kv_means_kernel<<<dim3(blocks, kv.nkv, n), kv.hd, 0, st>>>(kv, seq, since, len, block, means);
+    const int blocks = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) / block + 1;
+    kv_means_kernel<<<dim3(min(blocks, 4096), kv.nkv, n), 256, 0, st>>>(kv, seq, since, len, block, means);
     return cudaGetLastError();
 }
 

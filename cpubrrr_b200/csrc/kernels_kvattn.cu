@@ -17,6 +17,7 @@
 #include "brrr_block.cuh"
 #include "brrr_kv.cuh"
 
+#include <atomic>
 #include <cooperative_groups.h>
 
 namespace brrr {
@@ -287,55 +288,51 @@ struct Running {
     }
 };
 
-// Joins the parts of a CTA's WK groups of warps (part p: rows p * R ... of out and ml) into part 0.  All threads call it, after a barrier.
-template <int HD>
-__device__ __forceinline__ void join_warps(float *out, float2 *ml, int R, int parts) {
-    if (parts > 1) {
+// Joins the parts of rows in shared memory (out [part][R][HD], ml [part][R]: maximum and sum) and, in a cluster, the CTAs, and writes the
+// rows.  dst(r): the row's place in the output (< 0: padding), sink(r): its sink in powers of two or -infinity.  All threads call it, after a barrier.
+template <int HD, class Dst, class Sink>
+__device__ __forceinline__ void join_parts(float *out, float2 *ml, int R, int parts, float *o, float *lse, Dst dst, Sink sink) {
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
+    if (C > 1 && parts > 1) {
+        // this CTA's parts into part 0
         for (int u = threadIdx.x; u < R * (HD / 4); u += AW * 32) {
             const int r = u / (HD / 4), d = u % (HD / 4) * 4;
-            float m = -INFINITY;
+            float m = -INFINITY, l = 0.0f;
             for (int p = 0; p < parts; p++) m = fmaxf(m, ml[p * R + r].x);
             const float safe = m == -INFINITY ? 0.0f : m;
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (int p = 0; p < parts; p++) {
-                const float w = exp2_approx(ml[p * R + r].x - safe);
+                const float2 part = ml[p * R + r];
+                const float w = exp2_approx(part.x - safe);
                 const float4 y = *reinterpret_cast<const float4 *>(out + (p * R + r) * HD + d);
+                l = __fmaf_rn(w, part.y, l);
                 x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
             }
             *reinterpret_cast<float4 *>(out + r * HD + d) = x;
+            if (d == 0) ml[parts * R + r] = make_float2(m, l);        // a place of its own: the parts' are still being read
         }
-        __syncthreads();
-        for (int r = threadIdx.x; r < R; r += AW * 32) {
-            float m = -INFINITY, l = 0.0f;
-            for (int p = 0; p < parts; p++) m = fmaxf(m, ml[p * R + r].x);
-            const float safe = m == -INFINITY ? 0.0f : m;
-            for (int p = 0; p < parts; p++) l = __fmaf_rn(exp2_approx(ml[p * R + r].x - safe), ml[p * R + r].y, l);
-            ml[r] = make_float2(m, l);
-        }
+        ml += parts * R;
+        parts = 1;
     }
-}
-
-// Joins the CTAs of the cluster and writes the rows: CTA c takes its share of the values.  dst(r): the row's place in the output (< 0: padding), sink(r): its
-// sink in powers of two or -infinity.
-template <int HD, class Dst, class Sink>
-__device__ __forceinline__ void join_cluster(float *out, float2 *ml, int R, float *o, float *lse, Dst dst, Sink sink) {
-    cg::cluster_group cl = cg::this_cluster();
-    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
-    cl.sync();
+    if (C > 1) cl.sync();
+    const int n = C > 1 ? C : parts;
     for (int u = c * AW * 32 + threadIdx.x; u < R * (HD / 4); u += C * AW * 32) {
         const int r = u / (HD / 4), d = u % (HD / 4) * 4;
         const long long to = dst(r);
         if (to < 0) continue;
+        auto mlp = [&](int p) { return C > 1 ? cl.map_shared_rank(ml, p)[r] : ml[p * R + r]; };
+        auto outp = [&](int p) { return *reinterpret_cast<const float4 *>(C > 1 ? cl.map_shared_rank(out, p) + r * HD + d : out + (p * R + r) * HD + d); };
         const float sk = sink(r);
         float m = sk;
-        for (int p = 0; p < C; p++) m = fmaxf(m, cl.map_shared_rank(ml, p)[r].x);
+        for (int p = 0; p < n; p++) m = fmaxf(m, mlp(p).x);
         const float safe = m == -INFINITY ? 0.0f : m;
         float l = exp2_approx(sk - safe);
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int p = 0; p < C; p++) {
-            const float2 part = cl.map_shared_rank(ml, p)[r];
+        for (int p = 0; p < n; p++) {
+            const float2 part = mlp(p);
             const float w = exp2_approx(part.x - safe);
-            const float4 y = *reinterpret_cast<const float4 *>(cl.map_shared_rank(out, p) + r * HD + d);
+            const float4 y = outp(p);
             l = __fmaf_rn(w, part.y, l);
             x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
         }
@@ -343,7 +340,7 @@ __device__ __forceinline__ void join_cluster(float *out, float2 *ml, int R, floa
         *reinterpret_cast<float4 *>(o + to * HD + d) = make_float4(__fdividef(x.x, den), __fdividef(x.y, den), __fdividef(x.z, den), __fdividef(x.w, den));
         if (lse && d == 0) lse[to] = (m + log2f(l)) * LN2;
     }
-    cl.sync();
+    if (C > 1) cl.sync();          // nobody leaves while its memory is read
 }
 
 // ---------------------------------------------------------------- trees
@@ -353,37 +350,33 @@ struct TreeRows {
     int lo[KV_TREE_MAX];
     int first, full;                        // smallest lo, largest lo: from there to len every row sees every slot
 };
-// All threads call it; ends with a barrier.
+// All threads call it; complete for them after the next barrier.
 __device__ __forceinline__ void tree_rows(const TreeArgs &a, int b, const KvEntry &e, TreeRows &w) {
     __shared__ int depth[KV_TREE_MAX];
-    if (threadIdx.x == 0) { w.first = e.len; w.full = 0; }
+    const int i = threadIdx.x;
+    if (a.window <= 0) {
+        tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
+        if (i < e.count) w.lo[i] = 0;
+        if (i == 0) w.first = w.full = 0;
+        return;
+    }
+    if (i == 0) { w.first = e.len; w.full = 0; }
     tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
     __syncthreads();
-    uint64_t m = 0;
-    int lo = 0;
-    const int i = threadIdx.x;
     if (i < e.count) {
-        m = w.mask[i];
-        if (a.window > 0) {
-            lo = max(0, min(e.len, e.len + depth[i] + 1 - a.window));
-            uint64_t in = 0;
-            for (int j = 0; j < e.count; j++) in |= (uint64_t)(depth[i] - depth[j] < a.window) << j;
-            m &= in;
-        }
-    }
-    __syncthreads();
-    if (i < e.count) {
-        w.mask[i] = m;
+        uint64_t in = 0;
+        for (int j = 0; j < e.count; j++) in |= (uint64_t)(depth[i] - depth[j] < a.window) << j;
+        const int lo = max(0, min(e.len, e.len + depth[i] + 1 - a.window));
+        w.mask[i] &= in;
         w.lo[i] = lo;
         atomicMin(&w.first, lo);
         atomicMax(&w.full, lo);
     }
-    __syncthreads();
 }
 
 // grid (C, kv heads x blocks of 16 WM rows, entries), clusters of C
 template <class T, int HD, int NK, int WM>
-__global__ void __launch_bounds__(AW * 32) tree_kernel(KvDev kv, TreeArgs a) {
+__global__ void __launch_bounds__(AW * 32, WM == 1 && HD == 64 ? 2 : 1) tree_kernel(KvDev kv, TreeArgs a) {
     constexpr int WK = AW / WM, R = 16 * WM, STEP = 8 * NK;
     extern __shared__ __align__(16) float4 frag[];          // the queries, then the parts: out [WK][R][HD], ml [WK][R]
     __shared__ TreeRows see;
@@ -394,12 +387,29 @@ __global__ void __launch_bounds__(AW * 32) tree_kernel(KvDev kv, TreeArgs a) {
         if (!e.ok && threadIdx.x == 0) kv_error(kv);
         return;
     }
-    tree_rows(a, b, e, see);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp % WM, wk = warp / WM, end = e.len + e.count;
+    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh), *vc = (const typename T::Val *)kv.v + kv.head(e.seq, kvh);
+    int s0 = 0;
+    if (a.window > 0) {
+        tree_rows(a, b, e, see);
+        __syncthreads();
+        s0 = see.first / STEP;
+    }
+    // the CTA's steps, the warp's among them; the first is on its way while masks and queries are prepared
+    const int steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
+    const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps);
+    int s = from + wk;
+    KvStep<T, HD, NK> st;
+    if (s < to) {
+        st.template load_k<WM == 1>(kc, s * STEP, end);
+        st.template load_v<WM == 1>(vc, s * STEP, end);
+    }
+    if (a.window <= 0) tree_rows(a, b, e, see);
     stage_queries<T, HD>(frag, WM, [&](int r) -> const float * {
         const int i = (row0 + r) / per;
         return i < e.count ? a.q + (((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per) * HD : nullptr;
     });
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp % WM, wk = warp / WM, end = e.len + e.count;
+    __syncthreads();
     // this lane's two rows
     uint64_t mask[2];
     int lo[2];
@@ -409,20 +419,9 @@ __global__ void __launch_bounds__(AW * 32) tree_kernel(KvDev kv, TreeArgs a) {
         mask[h] = i < e.count ? see.mask[i] : 0;
         lo[h] = i < e.count ? see.lo[i] : 0x7fffffff;
     }
-    __syncthreads();
-    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh), *vc = (const typename T::Val *)kv.v + kv.head(e.seq, kvh);
     const float c = a.scale * LOG2E;
-    // the CTA's steps, the warp's among them
-    const int s0 = see.first / STEP, steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
-    const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps);
     Running<T, HD, NK> run;
     run.clear();
-    KvStep<T, HD, NK> st;
-    int s = from + wk;
-    if (s < to) {
-        st.template load_k<WM == 1>(kc, s * STEP, end);
-        st.template load_v<WM == 1>(vc, s * STEP, end);
-    }
     for (; s < to; s += WK) {
         const int base = s * STEP;
         float x[NK][4];
@@ -448,8 +447,7 @@ __global__ void __launch_bounds__(AW * 32) tree_kernel(KvDev kv, TreeArgs a) {
     float2 *ml = reinterpret_cast<float2 *>(out + WK * R * HD);
     run.store(out + (wk * R + wm * 16) * HD, ml + wk * R + wm * 16);
     __syncthreads();
-    join_warps<HD>(out, ml, R, WK);
-    join_cluster<HD>(out, ml, R, a.out, a.lse,
+    join_parts<HD>(out, ml, R, WK, a.out, a.lse,
                      [&](int r) -> long long {
                          const int i = (row0 + r) / per;
                          return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
@@ -457,11 +455,23 @@ __global__ void __launch_bounds__(AW * 32) tree_kernel(KvDev kv, TreeArgs a) {
                      [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
 }
 
-template <class Kernel, class... Args>
-cudaError_t launch_cluster(Kernel k, dim3 grid, int cluster, size_t smem, cudaStream_t st, Args... args) {
-    cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+// Once per kernel and device: the shared memory it may ask for, clusters of up to 16.
+template <auto K>
+static cudaError_t allow(size_t smem) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+    return e;
+}
+
+// most: the largest shared memory this kernel is ever launched with
+template <auto K, class... Args>
+static cudaError_t launch_cluster(dim3 grid, int cluster, size_t smem, size_t most, cudaStream_t st, Args... args) {
+    cudaError_t e = allow<K>(most);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
@@ -473,21 +483,28 @@ cudaError_t launch_cluster(Kernel k, dim3 grid, int cluster, size_t smem, cudaSt
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k, args...);
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, K, args...);
 }
 
 // bytes of a CTA's shared memory: the queries, later the parts
-static size_t attn_smem(int hd, int wm) {
-    const size_t parts = (size_t)AW * 16 * (hd * 4 + 8), queries = (size_t)wm * hd * 128;
+__host__ __device__ constexpr size_t attn_smem(int hd, int wm) {
+    const size_t parts = (size_t)AW * 16 * (hd * 4 + 8) + 16 * wm * 8, queries = (size_t)wm * hd * 128;
     return parts > queries ? parts : queries;
 }
 
-// CTAs that share an entry's slots: as many as fill the GPU twice, while each has at least four steps
-static int cluster_size(long long ctas, int steps) {
-    int c = 1;
-    while (c < 16 && ctas * c * 2 <= 2 * 148 && steps / (2 * c) >= 4) c *= 2;
-    return c;
+// CTAs (1..16) that share the steps of one of `jobs` pieces of work, `lanes` warps of a CTA taking a step each at a time and `slots` CTAs resident on the GPU: the
+// least time of all waves, where a CTA's start and end cost about as much as four steps of a warp.
+static int cluster_size(long long jobs, int steps, int lanes, int slots) {
+    int best = 1;
+    double least = 0.0;
+    for (int c = 1; c <= 16; c++) {
+        const int turns = (steps + c * lanes - 1) / (c * lanes);
+        const double t = (double)((jobs * c + slots - 1) / slots) * (turns + 4);
+        if (c == 1 || t < least) { best = c; least = t; }
+        if (turns <= 1) break;
+    }
+    return best;
 }
 
 template <class T, int HD, int NK>
@@ -495,20 +512,20 @@ static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int len_hint,
     const int per = a.nh / kv.nkv, tiles = (a.rows * per + 15) / 16, wm = tiles > 4 ? 8 : tiles > 2 ? 4 : tiles, blocks = (tiles + wm - 1) / wm;
     int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
     if (a.window > 0) slots = min(slots, a.window + a.rows);
-    const int c = cluster_size((long long)a.n * kv.nkv * blocks, slots / (8 * NK));
+    const int c = cluster_size((long long)a.n * kv.nkv * blocks, (slots + 8 * NK - 1) / (8 * NK), AW / wm, wm == 1 && HD == 64 ? 296 : 148);
     const dim3 grid(c, kv.nkv * blocks, a.n);
-    const size_t smem = attn_smem(HD, wm);
+    constexpr size_t s1 = attn_smem(HD, 1), s2 = attn_smem(HD, 2), s4 = attn_smem(HD, 4), s8 = attn_smem(HD, 8);
     switch (wm) {
-        case 1: return launch_cluster(tree_kernel<T, HD, NK, 1>, grid, c, smem, st, kv, a);
-        case 2: return launch_cluster(tree_kernel<T, HD, NK, 2>, grid, c, smem, st, kv, a);
-        case 4: return launch_cluster(tree_kernel<T, HD, NK, 4>, grid, c, smem, st, kv, a);
-        default: return launch_cluster(tree_kernel<T, HD, NK, 8>, grid, c, smem, st, kv, a);
+        case 1: return launch_cluster<tree_kernel<T, HD, NK, 1>>(grid, c, s1, s1, st, kv, a);
+        case 2: return launch_cluster<tree_kernel<T, HD, NK, 2>>(grid, c, s2, s2, st, kv, a);
+        case 4: return launch_cluster<tree_kernel<T, HD, NK, 4>>(grid, c, s4, s4, st, kv, a);
+        default: return launch_cluster<tree_kernel<T, HD, NK, 8>>(grid, c, s8, s8, st, kv, a);
     }
 }
 
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
     if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2>(kv, a, len_hint, st) : launch_tree<KvBf16, 128, 2>(kv, a, len_hint, st);
-    return kv.hd == 64 ? launch_tree<KvF32, 64, 2>(kv, a, len_hint, st) : launch_tree<KvF32, 128, 1>(kv, a, len_hint, st);
+    return kv.hd == 64 ? launch_tree<KvF32, 64, 1>(kv, a, len_hint, st) : launch_tree<KvF32, 128, 1>(kv, a, len_hint, st);
 }
 
 // ---------------------------------------------------------------- book of weights
@@ -527,6 +544,7 @@ __global__ void __launch_bounds__(AW * 32) weigh_kernel(KvDev kv, TreeArgs a, co
         return;
     }
     tree_rows(a, b, e, see);
+    __syncthreads();
     const uint64_t rows = picked ? picked[b] : ~0ull;
     const int end = e.len + e.count, steps = (end + STEP - 1) / STEP, s0 = see.first / STEP;
     const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh);
@@ -545,10 +563,12 @@ __global__ void __launch_bounds__(AW * 32) weigh_kernel(KvDev kv, TreeArgs a, co
             lse[r] = i < e.count && (rows >> i & 1) ? a.lse[((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per] * LOG2E : INFINITY;
         }
         __syncthreads();
-        for (int s = s0 + blockIdx.x * AW + warp; s < steps; s += gridDim.x * AW) {
+        const int hop = gridDim.x * AW;
+        int s = s0 + blockIdx.x * AW + warp;
+        KvStep<T, HD, NK> st;
+        if (s < steps) st.template load_k<WT == 1>(kc, s * STEP, end);
+        for (; s < steps; s += hop) {
             const int base = s * STEP;
-            KvStep<T, HD, NK> st;
-            st.template load_k<WT == 1>(kc, base, end);
             const bool partial = base < see.full || base + STEP > e.len;
             float sum[NK][2];
 #pragma unroll
@@ -556,6 +576,7 @@ __global__ void __launch_bounds__(AW * 32) weigh_kernel(KvDev kv, TreeArgs a, co
             for (int w = 0; w < tiles; w++) {
                 float x[NK][4];
                 step_scores<T, HD, NK>(st, frag + w * (HD / 8) * 64, x);
+                if (w == tiles - 1 && s + hop < steps) st.template load_k<WT == 1>(kc, (s + hop) * STEP, end);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const int r = w * 16 + (lane >> 2) + 8 * h, i = (row0 + r) / per;
@@ -595,11 +616,14 @@ template <class T, int HD, int NK>
 static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
     const int per = a.nh / kv.nkv, tiles = (a.rows * per + 15) / 16;
     int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
-    const int ctas = (slots / (8 * NK) + AW) / AW;
-    const dim3 grid(max(1, min(ctas, 4096)), kv.nkv, a.n);
-    if (tiles == 1) return launch_cluster(weigh_kernel<T, HD, NK, 1>, grid, 1, (size_t)HD * 128, st, kv, a, picked);
-    if (tiles <= 4) return launch_cluster(weigh_kernel<T, HD, NK, 4>, grid, 1, (size_t)4 * HD * 128, st, kv, a, picked);
-    return launch_cluster(weigh_kernel<T, HD, NK, 8>, grid, 1, (size_t)8 * HD * 128, st, kv, a, picked);
+    if (a.window > 0) slots = min(slots, a.window + a.rows);
+    const int steps = (slots + 8 * NK - 1) / (8 * NK), jobs = kv.nkv * a.n;
+    // two CTAs on an SM, a few times over so that the last ones are short; no more than there are steps
+    const dim3 grid(max(1, min((steps + AW - 1) / AW, (3 * 296 + jobs - 1) / jobs)), kv.nkv, a.n);
+    constexpr size_t q = (size_t)HD * 128;
+    if (tiles == 1) return launch_cluster<weigh_kernel<T, HD, NK, 1>>(grid, 1, q, q, st, kv, a, picked);
+    if (tiles <= 4) return launch_cluster<weigh_kernel<T, HD, NK, 4>>(grid, 1, 4 * q, 4 * q, st, kv, a, picked);
+    return launch_cluster<weigh_kernel<T, HD, NK, 8>>(grid, 1, 8 * q, 8 * q, st, kv, a, picked);
 }
 
 cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
@@ -608,83 +632,127 @@ cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *
 }
 
 // ---------------------------------------------------------------- chosen blocks
-constexpr int CB_THREADS = 256;
+// A cluster per (kv head, row).  Its CTAs share the blocks' scores: products of f64 (mma m8n8k4, 8 heads by 8 blocks), whose largest over the heads every CTA
+// gets as a 32-bit key in the order of the values.  Then each CTA finds the nsel largest keys and takes its share of the chosen blocks' steps.
+__device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
+    asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
+}
 
-// A CTA per (kv head, row): scores of the blocks between the first and the local ones, then the nsel largest in ascending order of blocks.
-__global__ void __launch_bounds__(CB_THREADS) choose_blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel,
-                                                                   int first, int local, const float *__restrict__ q, int nh, int32_t *sel) {
-    extern __shared__ uint32_t keys[];
-    __shared__ float qs[16 * 128];
-    const int kvh = blockIdx.y, r = blockIdx.x, per = nh / kv.nkv;
+// Keys of blocks j0 .. j0 + 7 by one warp: lane 4 g + t has those of blocks 2t and 2t + 1 (the same for every g).
+template <int HD>
+__device__ __forceinline__ void block_keys(const float *__restrict__ q, int per, const float *__restrict__ mean, int j0, int nb, uint32_t (&key)[2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const float *m = mean + (long long)min(j0 + g, nb - 1) * HD + 4 * t;
+    float4 x[HD / 16];
+#pragma unroll
+    for (int c = 0; c < HD / 16; c++) x[c] = *reinterpret_cast<const float4 *>(m + 16 * c);
+    key[0] = key[1] = 0;
+    for (int h0 = 0; h0 < per; h0 += 8) {
+        double even[2] = {0.0, 0.0}, odd[2] = {0.0, 0.0};
+        const float *p = q + (h0 + g) * HD + 4 * t;
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) {
+            const float4 a = h0 + g < per ? *reinterpret_cast<const float4 *>(p + 16 * c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            mma_f64(even, a.x, x[c].x);
+            mma_f64(odd, a.y, x[c].y);
+            mma_f64(even, a.z, x[c].z);
+            mma_f64(odd, a.w, x[c].w);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            // the rounding keeps the order, so the largest may be taken afterwards; what is no number wins here and loses in the end
+            const float f = (float)(even[i] + odd[i]);
+            uint32_t k = f != f ? 0xFFFFFFFFu : float_orderable(f == 0.0f ? 0.0f : f);
+            if (h0 + g >= per) k = 0;
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+            key[i] = max(key[i], k);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (key[i] == 0xFFFFFFFFu) key[i] = 0;
+}
+
+template <class T, int HD, int NK>
+__global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel, int first, int local,
+                                                         const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *o, float *lse) {
+    constexpr int R = 16, STEP = 8 * NK;
+    extern __shared__ __align__(16) float4 frag[];
+    uint32_t *keys = reinterpret_cast<uint32_t *>(frag) + attn_smem(HD, 1) / 4;      // [cap / block + 1]
+    __shared__ int32_t chosen[256];
+    __shared__ float qs[16 * HD];
+    __shared__ KthSpace kth;
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks();
+    const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int s = seq ? seq[r] : r, n = len[r];
     if ((unsigned)s >= (unsigned)kv.n_seq || (unsigned)n > (unsigned)kv.cap) {
         if (threadIdx.x == 0) kv_error(kv);
         return;
     }
-    const int nb = (n + block - 1) / block;
-    int32_t *out = sel + ((long long)r * kv.nkv + kvh) * nsel;
-    for (int j = nb + threadIdx.x; j < nsel; j += CB_THREADS) out[j] = -1;
-    if (nb <= nsel) {
-        for (int j = threadIdx.x; j < nb; j += CB_THREADS) out[j] = j;
-        return;
-    }
-    for (int i = threadIdx.x; i < per * kv.hd; i += CB_THREADS) qs[i] = q[((long long)r * nh + kvh * per) * kv.hd + i];
-    __syncthreads();
-    const float *mean = means + ((long long)s * kv.nkv + kvh) * (kv.cap / block) * kv.hd;
-    for (int j = threadIdx.x; j < nb; j += CB_THREADS) {
-        uint32_t key = 0xFFFFFFFFu;
-        if (j >= first && j < nb - local) {
-            double top = -INFINITY;
-            bool nan = false;
-            for (int g = 0; g < per; g++) {
-                double x = 0.0;
-                for (int d = 0; d < kv.hd; d++) x += (double)qs[g * kv.hd + d] * (double)mean[(long long)j * kv.hd + d];
-                nan |= x != x;
-                top = fmax(top, x);
-            }
-            const float f = (float)top;
-            key = nan ? 0u : f == 0.0f ? 0x80000000u : float_orderable(f);
-        }
-        keys[j] = key;
-    }
-    __syncthreads();
-    // rank of a block: those that come before it
-    for (int j = threadIdx.x; j < nb; j += CB_THREADS) {
-        int rank = 0;
-        for (int i = 0; i < nb; i++) rank += keys[i] > keys[j] || (keys[i] == keys[j] && i < j);
-        if (rank < nsel) out[rank] = j;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0)
-        for (int i = 1; i < nsel; i++) {
-            const int x = out[i];
-            int at = i;
-            for (; at > 0 && out[at - 1] > x; at--) out[at] = out[at - 1];
-            out[at] = x;
-        }
-}
-
-// A cluster per (kv head, row): the chosen blocks' slots in steps, over the warps and the CTAs.
-template <class T, int HD, int NK>
-__global__ void __launch_bounds__(AW * 32) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, int nsel, const int32_t *sel, const float *q, int nh,
-                                                         float scale, const float *sinks, float *o, float *lse) {
-    constexpr int R = 16, STEP = 8 * NK;
-    extern __shared__ __align__(16) float4 frag[];
-    __shared__ int32_t chosen[256];
-    const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int s = seq ? seq[r] : r, n = len[r];
-    if ((unsigned)s >= (unsigned)kv.n_seq || (unsigned)n > (unsigned)kv.cap) return;
     const long long row = (long long)r * nh + kvh * per;
-    for (int i = threadIdx.x; i < nsel; i += AW * 32) chosen[i] = sel[((long long)r * kv.nkv + kvh) * nsel + i];
-    stage_queries<T, HD>(frag, 1, [&](int i) -> const float * { return i < per ? q + (row + i) * HD : nullptr; });
+    const int nb = (n + block - 1) / block, taken = min(nb, nsel);
+    for (int i = threadIdx.x; i < per * (HD / 4); i += AW * 32) reinterpret_cast<float4 *>(qs)[i] = reinterpret_cast<const float4 *>(q + row * HD)[i];
     __syncthreads();
+    if (nb <= nsel) {
+        for (int j = threadIdx.x; j < nb; j += AW * 32) chosen[j] = j;
+    } else {
+        // scores of the blocks that are not taken anyhow
+        const float *mean = means + ((long long)s * kv.nkv + kvh) * (kv.cap / block) * HD;
+        const int hi = nb - local, tiles = (hi - first + 7) / 8;
+        if (C > 1) cl.sync();          // every CTA is there: its memory may be written
+        for (int i = blockIdx.x * AW + warp; i < tiles; i += C * AW) {
+            uint32_t key[2];
+            const int j0 = first + 8 * i, j = j0 + 2 * (lane & 3);
+            block_keys<HD>(qs, per, mean, j0, hi, key);
+            for (int p = lane >> 2; p < C; p += 8) {
+                uint32_t *there = C > 1 ? cl.map_shared_rank(keys, p) : keys;
+                if (j < hi) there[j] = key[0];
+                if (j + 1 < hi) there[j + 1] = key[1];
+            }
+        }
+        if (C > 1) cl.sync();
+        else __syncthreads();
+        uint32_t ties;
+        const int want = nsel - first - local;
+        const uint32_t last = want > 0 ? block_kth(hi - first, want, [&](int i) { return keys[first + i]; }, kth, &ties) : 0xFFFFFFFFu;
+        if (want <= 0) ties = 0;
+        // the places of the chosen ones, in ascending order of blocks
+        uint32_t before = 0, same_before = 0;
+        for (int at = 0; at < nb; at += AW * 32) {
+            const int j = at + threadIdx.x;
+            const bool must = j < nb && (j < first || j >= hi), free = j >= first && j < hi;
+            const uint32_t k = free ? keys[j] : 0;
+            const bool over = must || (free && k > last), same = free && k == last && want > 0;
+            // counts of both kinds in one word: block <= 256 of each
+            const uint32_t b_over = __ballot_sync(0xffffffffu, over), b_same = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1;
+            if (lane == 0) kth.sums[warp] = __popc(b_over) | __popc(b_same) << 16;
+            __syncthreads();
+            uint32_t mine = __popc(b_over & below) | __popc(b_same & below) << 16, all = 0;
+            for (int w = 0; w < AW; w++) {
+                if (w < warp) mine += kth.sums[w];
+                all += kth.sums[w];
+            }
+            __syncthreads();
+            const uint32_t o_rank = before + (mine & 0xFFFF), s_rank = same_before + (mine >> 16);
+            if (over) chosen[o_rank + min(s_rank, ties)] = j;
+            else if (same && s_rank < ties) chosen[o_rank + s_rank] = j;
+            before += all & 0xFFFF;
+            same_before += all >> 16;
+        }
+    }
+    stage_queries<T, HD>(frag, 1, [&](int i) -> const float * { return i < per ? qs + i * HD : nullptr; });
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < nsel; i += AW * 32) sel[((long long)r * kv.nkv + kvh) * nsel + i] = i < taken ? chosen[i] : -1;
     const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(s, kvh), *vc = (const typename T::Val *)kv.v + kv.head(s, kvh);
     const float c = scale * LOG2E;
-    const int each = block / STEP, steps = min(nsel, (n + block - 1) / block) * each;
+    const int each = block / STEP, steps = taken * each;
     Running<T, HD, NK> run;
     run.clear();
     KvStep<T, HD, NK> st;
-    const int hop = gridDim.x * AW;
+    const int hop = C * AW;
     int i = blockIdx.x * AW + warp;
     auto slot = [&](int i) { return chosen[i / each] * block + i % each * STEP; };
     if (i < steps) {
@@ -708,31 +776,26 @@ __global__ void __launch_bounds__(AW * 32) blocks_kernel(KvDev kv, const int32_t
     float2 *ml = reinterpret_cast<float2 *>(out + AW * R * HD);
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
-    join_warps<HD>(out, ml, R, AW);
-    join_cluster<HD>(out, ml, R, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
-                     [&](int i) { return sinks ? sinks[kvh * per + i] * LOG2E : -INFINITY; });
+    join_parts<HD>(out, ml, R, AW, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
+                   [&](int i) { return sinks ? sinks[kvh * per + i] * LOG2E : -INFINITY; });
 }
 
 template <class T, int HD, int NK>
-static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, int nsel, int len_hint, const float *q, int nh, float scale,
-                                 const float *sinks, const int32_t *sel, float *out, float *lse, cudaStream_t st) {
-    const int slots = min(nsel * block, len_hint > 0 ? min(len_hint, kv.cap) : kv.cap);
-    const int c = cluster_size((long long)rows * kv.nkv, slots / (8 * NK));
-    return launch_cluster(blocks_kernel<T, HD, NK>, dim3(c, rows, kv.nkv), c, attn_smem(HD, 1), st, kv, seq, len, block, nsel, sel, q, nh, scale, sinks, out, lse);
+static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,
+                                 int len_hint, const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *out, float *lse, cudaStream_t st) {
+    const int longest = len_hint > 0 ? min(len_hint, kv.cap) : kv.cap, nb = longest / block, each = block / (8 * NK);
+    // a tile of eight blocks' scores costs about as much as a step
+    const int steps = min(nsel, nb + 1) * each + (nb > nsel ? nb / 8 : 0);
+    const int c = cluster_size((long long)rows * kv.nkv, steps, AW, HD == 64 ? 296 : 148);
+    const size_t smem = attn_smem(HD, 1) + (size_t)(kv.cap / block + 1) * 4;
+    return launch_cluster<blocks_kernel<T, HD, NK>>(dim3(c, rows, kv.nkv), c, smem, attn_smem(HD, 1) + 16385 * 4, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
+                                                    sinks, sel, out, lse);
 }
 
 cudaError_t launch_attn_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,
                                int len_hint, const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *out, float *lse, cudaStream_t st) {
-    const size_t smem = (size_t)(kv.cap / block + 1) * 4;
-    cudaError_t e = smem > 32 * 1024 ? cudaFuncSetAttribute(choose_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
-    if (e != cudaSuccess) return e;
-    choose_blocks_kernel<<<dim3(rows, kv.nkv), CB_THREADS, smem, st>>>(kv, seq, len, block, means, nsel, first, local, q, nh, sel);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    if (kv.type) return kv.hd == 64 ? launch_blocks<KvBf16, 64, 2>(kv, rows, seq, len, block, nsel, len_hint, q, nh, scale, sinks, sel, out, lse, st)
-                                    : launch_blocks<KvBf16, 128, 2>(kv, rows, seq, len, block, nsel, len_hint, q, nh, scale, sinks, sel, out, lse, st);
-    return kv.hd == 64 ? launch_blocks<KvF32, 64, 2>(kv, rows, seq, len, block, nsel, len_hint, q, nh, scale, sinks, sel, out, lse, st)
-                       : launch_blocks<KvF32, 128, 1>(kv, rows, seq, len, block, nsel, len_hint, q, nh, scale, sinks, sel, out, lse, st);
+    auto go = kv.type ? (kv.hd == 64 ? launch_blocks<KvBf16, 64, 2> : launch_blocks<KvBf16, 128, 2>) : (kv.hd == 64 ? launch_blocks<KvF32, 64, 1> : launch_blocks<KvF32, 128, 1>);
+    return go(kv, rows, seq, len, block, means, nsel, first, local, len_hint, q, nh, scale, sinks, sel, out, lse, st);
 }
 
 }  // namespace brrr
