@@ -27,7 +27,7 @@ EXE = os.path.join(HERE, "brrr_engine")
 EXE_QWEN = os.path.join(HERE, "brrr_engine_qwen")
 
 SOURCES = ["kernels_small.cu", "kernels_q8.cu", "kernels_mx.cu", "kernels_router.cu", "kernels_attn.cu", "kernels_ep.cu", "kernels_tile.cu", "kernels_rows.cu", "kernels_mxt.cu", "kernels_kq.cu", "kernels_qwen.cu", "kernels_kqt.cu", "kernels_qwrows.cu", "qwen_model.cu",
-           "model.cu", "kernels_kv.cu", "kernels_kvattn.cu", "capi_kv.cu", "capi_stage.cu", "capi_noalloc.cu", "host_text.cpp"]
+           "model.cu", "kernels_kv.cu", "kernels_kvattn.cu", "kernels_kvtc.cu", "capi_kv.cu", "capi_stage.cu", "capi_noalloc.cu", "host_text.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

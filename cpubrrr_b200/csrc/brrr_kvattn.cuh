@@ -1,0 +1,208 @@
+// What the attention kernels over the caller's caches share: cache types, what a tree's rows see, the join of partial results, cluster launches.
+#pragma once
+#include "brrr_block.cuh"
+#include "brrr_kv.cuh"
+
+#include <atomic>
+#include <cooperative_groups.h>
+
+namespace brrr {
+
+namespace cg = cooperative_groups;
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The two cache types: values per 16-byte load, and a load's values as floats.
+struct KvF32 {
+    static constexpr int V = 4;
+    static constexpr bool SPLIT = true;
+    typedef float Val;
+    static __device__ __forceinline__ void get(const uint4 &u, float (&x)[4]) {
+        x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
+    }
+};
+struct KvBf16 {
+    static constexpr int V = 8;
+    static constexpr bool SPLIT = false;
+    typedef uint16_t Val;
+    static __device__ __forceinline__ void get(const uint4 &u, float (&x)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    }
+};
+
+__device__ __forceinline__ uint4 ldg_stream(const void *p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint4 ldg_shared(const void *p) {
+    uint4 r;
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
+
+// Joins the parts of rows in shared memory (out [part][R][STRIDE], ml [part][R]: maximum in powers of two and sum) and, in a cluster, the CTAs, and writes the
+// rows.  dst(r): the row's place in the output (< 0: padding), sink(r): its sink in powers of two or -infinity.  All threads call it, after a barrier.
+template <int HD, int STRIDE, class Dst, class Sink>
+__device__ __forceinline__ void join_parts(float *out, float2 *ml, int R, int parts, float *o, float *lse, Dst dst, Sink sink) {
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
+    if (C > 1 && parts > 1) {
+        // this CTA's parts into part 0
+        for (int u = threadIdx.x; u < R * (HD / 4); u += (int)blockDim.x) {
+            const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+            float m = -INFINITY, l = 0.0f;
+            for (int p = 0; p < parts; p++) m = fmaxf(m, ml[p * R + r].x);
+            const float safe = m == -INFINITY ? 0.0f : m;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int p = 0; p < parts; p++) {
+                const float2 part = ml[p * R + r];
+                const float w = exp2_approx(part.x - safe);
+                const float4 y = *reinterpret_cast<const float4 *>(out + (p * R + r) * STRIDE + d);
+                l = __fmaf_rn(w, part.y, l);
+                x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
+            }
+            *reinterpret_cast<float4 *>(out + r * STRIDE + d) = x;
+            if (d == 0) ml[parts * R + r] = make_float2(m, l);        // a place of its own: the parts' are still being read
+        }
+        ml += parts * R;
+        parts = 1;
+    }
+    if (C > 1) cl.sync();
+    const int n = C > 1 ? C : parts;
+    for (int u = c * (int)blockDim.x + threadIdx.x; u < R * (HD / 4); u += C * (int)blockDim.x) {
+        const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+        const long long to = dst(r);
+        if (to < 0) continue;
+        auto mlp = [&](int p) { return C > 1 ? cl.map_shared_rank(ml, p)[r] : ml[p * R + r]; };
+        auto outp = [&](int p) { return *reinterpret_cast<const float4 *>(C > 1 ? cl.map_shared_rank(out, p) + r * STRIDE + d : out + (p * R + r) * STRIDE + d); };
+        const float sk = sink(r);
+        float m = sk;
+        for (int p = 0; p < n; p++) m = fmaxf(m, mlp(p).x);
+        const float safe = m == -INFINITY ? 0.0f : m;
+        float l = exp2_approx(sk - safe);
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p = 0; p < n; p++) {
+            const float2 part = mlp(p);
+            const float w = exp2_approx(part.x - safe);
+            const float4 y = outp(p);
+            l = __fmaf_rn(w, part.y, l);
+            x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
+        }
+        const float den = l == 0.0f ? 1.0f : l;
+        *reinterpret_cast<float4 *>(o + to * HD + d) = make_float4(__fdividef(x.x, den), __fdividef(x.y, den), __fdividef(x.z, den), __fdividef(x.w, den));
+        if (lse && d == 0) lse[to] = (m + log2f(l)) * LN2;
+    }
+    if (C > 1) cl.sync();          // nobody leaves while its memory is read
+}
+
+// ---------------------------------------------------------------- trees
+// What the rows of an entry see: cached slots from lo on, drafted rows by mask (windows applied, rows behind the count cut off).
+struct TreeRows {
+    uint64_t mask[KV_TREE_MAX];
+    int lo[KV_TREE_MAX];
+    int first, full;                        // smallest lo, largest lo: from there to len every row sees every slot
+};
+// All threads call it; complete for them after the next barrier.
+__device__ __forceinline__ void tree_rows(const TreeArgs &a, int b, const KvEntry &e, TreeRows &w) {
+    __shared__ int depth[KV_TREE_MAX];
+    const int i = threadIdx.x;
+    if (a.window <= 0) {
+        tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
+        if (i < e.count) w.lo[i] = 0;
+        if (i == 0) w.first = w.full = 0;
+        return;
+    }
+    if (i == 0) { w.first = e.len; w.full = 0; }
+    tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
+    __syncthreads();
+    if (i < e.count) {
+        uint64_t in = 0;
+        for (int j = 0; j < e.count; j++) in |= (uint64_t)(depth[i] - depth[j] < a.window) << j;
+        const int lo = max(0, min(e.len, e.len + depth[i] + 1 - a.window));
+        w.mask[i] &= in;
+        w.lo[i] = lo;
+        atomicMin(&w.first, lo);
+        atomicMax(&w.full, lo);
+    }
+}
+
+// Once per kernel and device: the shared memory it may ask for, clusters of up to 16.
+template <auto K>
+static cudaError_t allow(size_t smem) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+    return e;
+}
+
+// most: the largest shared memory this kernel is ever launched with
+template <auto K, class... Args>
+static cudaError_t launch_cluster(dim3 grid, int threads, int cluster, size_t smem, size_t most, cudaStream_t st, Args... args) {
+    cudaError_t e = allow<K>(most);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, K, args...);
+}
+
+// CTAs (1..16) that share the steps of one of `jobs` pieces of work, `lanes` steps of a CTA going on at a time: the least time of all waves, where a
+// CTA's start and end cost about as much as `fixed` steps.  How many clusters of a size the GPU holds at once is asked for once per kernel, size and device.
+template <auto K>
+static int cluster_size(long long jobs, int steps, int lanes, int fixed, int threads, size_t smem, size_t most, cudaError_t *err) {
+    static std::atomic<int> room[64][17];
+    int dev = 0;
+    *err = cudaGetDevice(&dev);
+    if (*err == cudaSuccess) *err = allow<K>(most);
+    if (*err != cudaSuccess) return 1;
+    int best = 1;
+    double least = 0.0;
+    for (int c = 1; c <= 16; c++) {
+        int held = dev < 64 ? room[dev][c].load() : 0;
+        if (!held) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(c);
+            cfg.blockDim = dim3(threads);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = c;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&held, K, &cfg) != cudaSuccess) { (void)cudaGetLastError(); held = 0; }
+            held = held > 0 ? held : -1;
+            if (dev < 64) room[dev][c].store(held);
+        }
+        if (held < 0) continue;
+        const int turns = (steps + c * lanes - 1) / (c * lanes);
+        const double t = (double)((jobs + held - 1) / held) * (turns + fixed);
+        if (c == 1 || t < least) { best = c; least = t; }
+        if (turns <= 1) break;
+    }
+    return best;
+}
+
+}  // namespace brrr

@@ -15,60 +15,19 @@
 // in shared memory, those of the cluster through distributed shared memory, in a fixed order: one launch, no workspace, no atomics.
 #include "brrr_kernels.h"
 #include "brrr_block.cuh"
-#include "brrr_kv.cuh"
-
-#include <atomic>
-#include <cooperative_groups.h>
+#include "brrr_kvattn.cuh"
 
 namespace brrr {
 
-namespace cg = cooperative_groups;
-
 constexpr int AW = 8;                       // warps of an attention CTA
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u); }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const float4 &a, float b0, float b1) {
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(a.z)), "r"(__float_as_uint(a.w)), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
 
-// The two cache types: values per 16-byte load, and a load's values as floats.
-struct KvF32 {
-    static constexpr int V = 4;
-    static constexpr bool SPLIT = true;
-    typedef float Val;
-    static __device__ __forceinline__ void get(const uint4 &u, float (&x)[4]) {
-        x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
-    }
-};
-struct KvBf16 {
-    static constexpr int V = 8;
-    static constexpr bool SPLIT = false;
-    typedef uint16_t Val;
-    static __device__ __forceinline__ void get(const uint4 &u, float (&x)[8]) {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-    }
-};
-
-__device__ __forceinline__ uint4 ldg_stream(const void *p) {
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-    return r;
-}
-__device__ __forceinline__ uint4 ldg_shared(const void *p) {
-    uint4 r;
-    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-    return r;
-}
 
 // What a lane keeps of a step of 8 NK slots.  Keys: of slot 8 j + lane / 4 the values 4V c + V (lane % 4) ...  Values: of slots 8 j + 2 (lane % 4) and the next
 // the values 8V c + V (lane / 4) ...
@@ -165,8 +124,6 @@ __device__ __forceinline__ void step_scores(const KvStep<T, HD, NK> &st, const f
 #pragma unroll
         for (int e = 0; e < 4; e++) s[j][e] += T::SPLIT ? lo1[j][e] + lo2[j][e] : lo1[j][e];
 }
-
-__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
 // A warp's running attention of 16 rows: maxima and sums in powers of two of rows lane / 4 and lane / 4 + 8 (the sum: this lane's slots only), and
 // the outputs, o[8 c' + V..]: see finish.
@@ -288,92 +245,6 @@ struct Running {
     }
 };
 
-// Joins the parts of rows in shared memory (out [part][R][HD], ml [part][R]: maximum and sum) and, in a cluster, the CTAs, and writes the
-// rows.  dst(r): the row's place in the output (< 0: padding), sink(r): its sink in powers of two or -infinity.  All threads call it, after a barrier.
-template <int HD, class Dst, class Sink>
-__device__ __forceinline__ void join_parts(float *out, float2 *ml, int R, int parts, float *o, float *lse, Dst dst, Sink sink) {
-    cg::cluster_group cl = cg::this_cluster();
-    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
-    if (C > 1 && parts > 1) {
-        // this CTA's parts into part 0
-        for (int u = threadIdx.x; u < R * (HD / 4); u += AW * 32) {
-            const int r = u / (HD / 4), d = u % (HD / 4) * 4;
-            float m = -INFINITY, l = 0.0f;
-            for (int p = 0; p < parts; p++) m = fmaxf(m, ml[p * R + r].x);
-            const float safe = m == -INFINITY ? 0.0f : m;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int p = 0; p < parts; p++) {
-                const float2 part = ml[p * R + r];
-                const float w = exp2_approx(part.x - safe);
-                const float4 y = *reinterpret_cast<const float4 *>(out + (p * R + r) * HD + d);
-                l = __fmaf_rn(w, part.y, l);
-                x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
-            }
-            *reinterpret_cast<float4 *>(out + r * HD + d) = x;
-            if (d == 0) ml[parts * R + r] = make_float2(m, l);        // a place of its own: the parts' are still being read
-        }
-        ml += parts * R;
-        parts = 1;
-    }
-    if (C > 1) cl.sync();
-    const int n = C > 1 ? C : parts;
-    for (int u = c * AW * 32 + threadIdx.x; u < R * (HD / 4); u += C * AW * 32) {
-        const int r = u / (HD / 4), d = u % (HD / 4) * 4;
-        const long long to = dst(r);
-        if (to < 0) continue;
-        auto mlp = [&](int p) { return C > 1 ? cl.map_shared_rank(ml, p)[r] : ml[p * R + r]; };
-        auto outp = [&](int p) { return *reinterpret_cast<const float4 *>(C > 1 ? cl.map_shared_rank(out, p) + r * HD + d : out + (p * R + r) * HD + d); };
-        const float sk = sink(r);
-        float m = sk;
-        for (int p = 0; p < n; p++) m = fmaxf(m, mlp(p).x);
-        const float safe = m == -INFINITY ? 0.0f : m;
-        float l = exp2_approx(sk - safe);
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int p = 0; p < n; p++) {
-            const float2 part = mlp(p);
-            const float w = exp2_approx(part.x - safe);
-            const float4 y = outp(p);
-            l = __fmaf_rn(w, part.y, l);
-            x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
-        }
-        const float den = l == 0.0f ? 1.0f : l;
-        *reinterpret_cast<float4 *>(o + to * HD + d) = make_float4(__fdividef(x.x, den), __fdividef(x.y, den), __fdividef(x.z, den), __fdividef(x.w, den));
-        if (lse && d == 0) lse[to] = (m + log2f(l)) * LN2;
-    }
-    if (C > 1) cl.sync();          // nobody leaves while its memory is read
-}
-
-// ---------------------------------------------------------------- trees
-// What the rows of an entry see: cached slots from lo on, drafted rows by mask (windows applied, rows behind the count cut off).
-struct TreeRows {
-    uint64_t mask[KV_TREE_MAX];
-    int lo[KV_TREE_MAX];
-    int first, full;                        // smallest lo, largest lo: from there to len every row sees every slot
-};
-// All threads call it; complete for them after the next barrier.
-__device__ __forceinline__ void tree_rows(const TreeArgs &a, int b, const KvEntry &e, TreeRows &w) {
-    __shared__ int depth[KV_TREE_MAX];
-    const int i = threadIdx.x;
-    if (a.window <= 0) {
-        tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
-        if (i < e.count) w.lo[i] = 0;
-        if (i == 0) w.first = w.full = 0;
-        return;
-    }
-    if (i == 0) { w.first = e.len; w.full = 0; }
-    tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
-    __syncthreads();
-    if (i < e.count) {
-        uint64_t in = 0;
-        for (int j = 0; j < e.count; j++) in |= (uint64_t)(depth[i] - depth[j] < a.window) << j;
-        const int lo = max(0, min(e.len, e.len + depth[i] + 1 - a.window));
-        w.mask[i] &= in;
-        w.lo[i] = lo;
-        atomicMin(&w.first, lo);
-        atomicMax(&w.full, lo);
-    }
-}
-
 // grid (C, kv heads x blocks of 16 WM rows, entries), clusters of C
 template <class T, int HD, int NK, int WM>
 __global__ void __launch_bounds__(AW * 32, WM == 1 && HD == 64 ? 2 : 1) tree_kernel(KvDev kv, TreeArgs a) {
@@ -447,44 +318,12 @@ __global__ void __launch_bounds__(AW * 32, WM == 1 && HD == 64 ? 2 : 1) tree_ker
     float2 *ml = reinterpret_cast<float2 *>(out + WK * R * HD);
     run.store(out + (wk * R + wm * 16) * HD, ml + wk * R + wm * 16);
     __syncthreads();
-    join_parts<HD>(out, ml, R, WK, a.out, a.lse,
+    join_parts<HD, HD>(out, ml, R, WK, a.out, a.lse,
                      [&](int r) -> long long {
                          const int i = (row0 + r) / per;
                          return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
                      },
                      [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
-}
-
-// Once per kernel and device: the shared memory it may ask for, clusters of up to 16.
-template <auto K>
-static cudaError_t allow(size_t smem) {
-    static std::atomic<unsigned long long> done{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev < 64 && done.load() >> dev & 1)) return e;
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
-    return e;
-}
-
-// most: the largest shared memory this kernel is ever launched with
-template <auto K, class... Args>
-static cudaError_t launch_cluster(dim3 grid, int cluster, size_t smem, size_t most, cudaStream_t st, Args... args) {
-    cudaError_t e = allow<K>(most);
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(AW * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, K, args...);
 }
 
 // bytes of a CTA's shared memory: the queries, later the parts
@@ -493,39 +332,23 @@ __host__ __device__ constexpr size_t attn_smem(int hd, int wm) {
     return parts > queries ? parts : queries;
 }
 
-// CTAs (1..16) that share the steps of one of `jobs` pieces of work, `lanes` warps of a CTA taking a step each at a time and `slots` CTAs resident on the GPU: the
-// least time of all waves, where a CTA's start and end cost about as much as four steps of a warp.
-static int cluster_size(long long jobs, int steps, int lanes, int slots) {
-    int best = 1;
-    double least = 0.0;
-    for (int c = 1; c <= 16; c++) {
-        const int turns = (steps + c * lanes - 1) / (c * lanes);
-        const double t = (double)((jobs * c + slots - 1) / slots) * (turns + 4);
-        if (c == 1 || t < least) { best = c; least = t; }
-        if (turns <= 1) break;
-    }
-    return best;
-}
-
-template <class T, int HD, int NK>
-static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
-    const int per = a.nh / kv.nkv, tiles = (a.rows * per + 15) / 16, wm = tiles > 4 ? 8 : tiles > 2 ? 4 : tiles, blocks = (tiles + wm - 1) / wm;
-    int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
-    if (a.window > 0) slots = min(slots, a.window + a.rows);
-    const int c = cluster_size((long long)a.n * kv.nkv * blocks, (slots + 8 * NK - 1) / (8 * NK), AW / wm, wm == 1 && HD == 64 ? 296 : 148);
-    const dim3 grid(c, kv.nkv * blocks, a.n);
-    constexpr size_t s1 = attn_smem(HD, 1), s2 = attn_smem(HD, 2), s4 = attn_smem(HD, 4), s8 = attn_smem(HD, 8);
-    switch (wm) {
-        case 1: return launch_cluster<tree_kernel<T, HD, NK, 1>>(grid, c, s1, s1, st, kv, a);
-        case 2: return launch_cluster<tree_kernel<T, HD, NK, 2>>(grid, c, s2, s2, st, kv, a);
-        case 4: return launch_cluster<tree_kernel<T, HD, NK, 4>>(grid, c, s4, s4, st, kv, a);
-        default: return launch_cluster<tree_kernel<T, HD, NK, 8>>(grid, c, s8, s8, st, kv, a);
-    }
+template <class T, int HD, int NK, int WM>
+static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
+    const int per = a.nh / kv.nkv, blocks = (a.rows * per + 16 * WM - 1) / (16 * WM);
+    constexpr size_t smem = attn_smem(HD, WM);
+    constexpr auto K = tree_kernel<T, HD, NK, WM>;
+    cudaError_t e = cudaSuccess;
+    const int c = cluster_size<K>((long long)a.n * kv.nkv * blocks, (slots + 8 * NK - 1) / (8 * NK), AW / WM, 4, AW * 32, smem, smem, &e);
+    if (e != cudaSuccess) return e;
+    return launch_cluster<K>(dim3(c, kv.nkv * blocks, a.n), AW * 32, c, smem, smem, st, kv, a);
 }
 
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
-    if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2>(kv, a, len_hint, st) : launch_tree<KvBf16, 128, 2>(kv, a, len_hint, st);
-    return kv.hd == 64 ? launch_tree<KvF32, 64, 1>(kv, a, len_hint, st) : launch_tree<KvF32, 128, 1>(kv, a, len_hint, st);
+    int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
+    if (a.window > 0) slots = min(slots, a.window + a.rows);
+    if (a.rows * (a.nh / kv.nkv) > 16) return launch_tree_tc(kv, a, slots, st);
+    if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2, 1>(kv, a, slots, st) : launch_tree<KvBf16, 128, 2, 1>(kv, a, slots, st);
+    return kv.hd == 64 ? launch_tree<KvF32, 64, 1, 1>(kv, a, slots, st) : launch_tree<KvF32, 128, 1, 1>(kv, a, slots, st);
 }
 
 // ---------------------------------------------------------------- book of weights
@@ -621,9 +444,9 @@ static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64
     // two CTAs on an SM, a few times over so that the last ones are short; no more than there are steps
     const dim3 grid(max(1, min((steps + AW - 1) / AW, (3 * 296 + jobs - 1) / jobs)), kv.nkv, a.n);
     constexpr size_t q = (size_t)HD * 128;
-    if (tiles == 1) return launch_cluster<weigh_kernel<T, HD, NK, 1>>(grid, 1, q, q, st, kv, a, picked);
-    if (tiles <= 4) return launch_cluster<weigh_kernel<T, HD, NK, 4>>(grid, 1, 4 * q, 4 * q, st, kv, a, picked);
-    return launch_cluster<weigh_kernel<T, HD, NK, 8>>(grid, 1, 8 * q, 8 * q, st, kv, a, picked);
+    if (tiles == 1) return launch_cluster<weigh_kernel<T, HD, NK, 1>>(grid, AW * 32, 1, q, q, st, kv, a, picked);
+    if (tiles <= 4) return launch_cluster<weigh_kernel<T, HD, NK, 4>>(grid, AW * 32, 1, 4 * q, 4 * q, st, kv, a, picked);
+    return launch_cluster<weigh_kernel<T, HD, NK, 8>>(grid, AW * 32, 1, 8 * q, 8 * q, st, kv, a, picked);
 }
 
 cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
@@ -776,7 +599,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
     float2 *ml = reinterpret_cast<float2 *>(out + AW * R * HD);
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
-    join_parts<HD>(out, ml, R, AW, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
+    join_parts<HD, HD>(out, ml, R, AW, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
                    [&](int i) { return sinks ? sinks[kvh * per + i] * LOG2E : -INFINITY; });
 }
 
@@ -786,9 +609,11 @@ static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, 
     const int longest = len_hint > 0 ? min(len_hint, kv.cap) : kv.cap, nb = longest / block, each = block / (8 * NK);
     // a tile of eight blocks' scores costs about as much as a step
     const int steps = min(nsel, nb + 1) * each + (nb > nsel ? nb / 8 : 0);
-    const int c = cluster_size((long long)rows * kv.nkv, steps, AW, HD == 64 ? 296 : 148);
-    const size_t smem = attn_smem(HD, 1) + (size_t)(kv.cap / block + 1) * 4;
-    return launch_cluster<blocks_kernel<T, HD, NK>>(dim3(c, rows, kv.nkv), c, smem, attn_smem(HD, 1) + 16385 * 4, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
+    const size_t smem = attn_smem(HD, 1) + (size_t)(kv.cap / block + 1) * 4, most = attn_smem(HD, 1) + 16385 * 4;
+    cudaError_t e = cudaSuccess;
+    const int c = cluster_size<blocks_kernel<T, HD, NK>>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, attn_smem(HD, 1), most, &e);
+    if (e != cudaSuccess) return e;
+    return launch_cluster<blocks_kernel<T, HD, NK>>(dim3(c, rows, kv.nkv), AW * 32, c, smem, most, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
                                                     sinks, sel, out, lse);
 }
 
