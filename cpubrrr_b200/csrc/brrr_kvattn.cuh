@@ -50,57 +50,86 @@ __device__ __forceinline__ uint4 ldg_shared(const void *p) {
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
-// Joins the parts of rows in shared memory (out [part][R][STRIDE], ml [part][R]: maximum in powers of two and sum) and, in a cluster, the CTAs, and writes the
-// rows.  dst(r): the row's place in the output (< 0: padding), sink(r): its sink in powers of two or -infinity.  All threads call it, after a barrier.
-template <int HD, int STRIDE, class Dst, class Sink>
-__device__ __forceinline__ void join_parts(float *out, float2 *ml, int R, int parts, float *o, float *lse, Dst dst, Sink sink) {
+// Joins the parts of R rows in shared memory (out [part][R][STRIDE], ml [part][R]: maximum in powers of two and sum) and, in a cluster, the CTAs, and
+// writes the rows, each CTA its share.  dst(r): the row's place in the output (< 0: padding), sink(r): its sink in powers of two or -infinity.  First the rows'
+// factors, then the values.  All threads call it, after a barrier; ml has room for R more.
+template <int HD, int STRIDE, int R, class Dst, class Sink>
+__device__ __forceinline__ void join_parts(float *out, float2 *ml, int parts, float *o, float *lse, Dst dst, Sink sink) {
+    __shared__ float weight[16][R], scale[R];
+    __shared__ long long place[R];
     cg::cluster_group cl = cg::this_cluster();
-    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
+    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank(), threads = (int)blockDim.x;
     if (C > 1 && parts > 1) {
         // this CTA's parts into part 0
-        for (int u = threadIdx.x; u < R * (HD / 4); u += (int)blockDim.x) {
-            const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+        for (int r = threadIdx.x; r < R; r += threads) {
             float m = -INFINITY, l = 0.0f;
             for (int p = 0; p < parts; p++) m = fmaxf(m, ml[p * R + r].x);
             const float safe = m == -INFINITY ? 0.0f : m;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (int p = 0; p < parts; p++) {
                 const float2 part = ml[p * R + r];
                 const float w = exp2_approx(part.x - safe);
-                const float4 y = *reinterpret_cast<const float4 *>(out + (p * R + r) * STRIDE + d);
+                weight[p][r] = w;
                 l = __fmaf_rn(w, part.y, l);
+            }
+            ml[parts * R + r] = make_float2(m, l);
+        }
+        __syncthreads();
+        for (int u = threadIdx.x; u < R * (HD / 4); u += threads) {
+            const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+            for (int p = 0; p < parts; p++) {
+                const float w = weight[p][r];
+                const float4 y = *reinterpret_cast<const float4 *>(out + (p * R + r) * STRIDE + d);
                 x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
             }
             *reinterpret_cast<float4 *>(out + r * STRIDE + d) = x;
-            if (d == 0) ml[parts * R + r] = make_float2(m, l);        // a place of its own: the parts' are still being read
         }
         ml += parts * R;
         parts = 1;
     }
     if (C > 1) cl.sync();
-    const int n = C > 1 ? C : parts;
-    for (int u = c * (int)blockDim.x + threadIdx.x; u < R * (HD / 4); u += C * (int)blockDim.x) {
-        const int r = u / (HD / 4), d = u % (HD / 4) * 4;
-        const long long to = dst(r);
-        if (to < 0) continue;
-        auto mlp = [&](int p) { return C > 1 ? cl.map_shared_rank(ml, p)[r] : ml[p * R + r]; };
-        auto outp = [&](int p) { return *reinterpret_cast<const float4 *>(C > 1 ? cl.map_shared_rank(out, p) + r * STRIDE + d : out + (p * R + r) * STRIDE + d); };
+    // this CTA's rows: r0 .. r0 + rows - 1
+    const int n = C > 1 ? C : parts, each = (R + C - 1) / C, r0 = c * each, rows = max(0, min(each, R - r0));
+    for (int i = threadIdx.x; i < rows; i += threads) {
+        const int r = r0 + i;
+        place[i] = dst(r);
+        if (place[i] < 0) continue;
         const float sk = sink(r);
+        float2 part[16];
         float m = sk;
-        for (int p = 0; p < n; p++) m = fmaxf(m, mlp(p).x);
+#pragma unroll
+        for (int p = 0; p < 16; p++)
+            if (p < n) part[p] = C > 1 ? cl.map_shared_rank(ml, p)[r] : ml[p * R + r];
+#pragma unroll
+        for (int p = 0; p < 16; p++)
+            if (p < n) m = fmaxf(m, part[p].x);
         const float safe = m == -INFINITY ? 0.0f : m;
         float l = exp2_approx(sk - safe);
+#pragma unroll
+        for (int p = 0; p < 16; p++)
+            if (p < n) {
+                const float w = exp2_approx(part[p].x - safe);
+                weight[p][i] = w;
+                l = __fmaf_rn(w, part[p].y, l);
+            }
+        scale[i] = __fdividef(1.0f, l == 0.0f ? 1.0f : l);
+        if (lse) lse[place[i]] = (m + log2f(l)) * LN2;
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < rows * (HD / 4); u += threads) {
+        const int i = u / (HD / 4), d = u % (HD / 4) * 4, at = (r0 + i) * STRIDE + d;
+        const long long to = place[i];
+        if (to < 0) continue;
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
         for (int p = 0; p < n; p++) {
-            const float2 part = mlp(p);
-            const float w = exp2_approx(part.x - safe);
-            const float4 y = outp(p);
-            l = __fmaf_rn(w, part.y, l);
+            const float w = weight[p][i];
+            const float4 y = *reinterpret_cast<const float4 *>(C > 1 ? cl.map_shared_rank(out, p) + at : out + p * R * STRIDE + at);
             x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
         }
-        const float den = l == 0.0f ? 1.0f : l;
-        *reinterpret_cast<float4 *>(o + to * HD + d) = make_float4(__fdividef(x.x, den), __fdividef(x.y, den), __fdividef(x.z, den), __fdividef(x.w, den));
-        if (lse && d == 0) lse[to] = (m + log2f(l)) * LN2;
+        const float k = scale[i];
+        *reinterpret_cast<float4 *>(o + to * HD + d) = make_float4(x.x * k, x.y * k, x.z * k, x.w * k);
     }
     if (C > 1) cl.sync();          // nobody leaves while its memory is read
 }

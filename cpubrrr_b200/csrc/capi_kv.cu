@@ -19,14 +19,13 @@ bool view(const brrr_kv *c, KvDev *out) {
     const int64_t head = (int64_t)c->cap * c->head_dim;
     if (c->head_stride < 0 || c->seq_stride < 0 || c->head_stride % 8 || c->seq_stride % 8) return false;
     KvDev d;
-    d.hs = c->head_stride ? c->head_stride : head;
     // heads inside a sequence or sequences inside a head: either way no two rows share memory
-    d.ss = c->seq_stride ? c->seq_stride : d.hs * c->n_head_kv;
+    d.hs = c->head_stride && c->n_head_kv > 1 ? c->head_stride : head;
+    d.ss = c->seq_stride && c->n_seq > 1 ? c->seq_stride : d.hs * c->n_head_kv;
     const int64_t lo = d.hs < d.ss ? d.hs : d.ss, hi = d.hs < d.ss ? d.ss : d.hs;
     const int64_t inner = d.hs < d.ss ? c->n_head_kv : c->n_seq, outer = d.hs < d.ss ? c->n_seq : c->n_head_kv;
-    if (hi > (int64_t)1 << 50) return false;
     const __int128 span = (__int128)lo * (inner - 1) + head;         // values of one outer step
-    if ((inner > 1 && lo < head) || (outer > 1 && hi < span) || (__int128)hi * (outer - 1) + span > (__int128)1 << 55) return false;
+    if ((inner > 1 && lo < head) || (outer > 1 && hi < span) || (__int128)hi * (outer - 1) + span > (__int128)1 << 38) return false;      // more than any GPU's memory
     d.k = c->k; d.v = c->v; d.weight = c->weight; d.pos = c->pos; d.err = c->err;
     d.type = c->type; d.n_seq = c->n_seq; d.nkv = c->n_head_kv; d.hd = c->head_dim; d.cap = c->cap;
     *out = d;

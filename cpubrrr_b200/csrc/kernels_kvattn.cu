@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(AW * 32, WM == 1 && HD == 64 ? 2 : 1) tree_ker
     float2 *ml = reinterpret_cast<float2 *>(out + WK * R * HD);
     run.store(out + (wk * R + wm * 16) * HD, ml + wk * R + wm * 16);
     __syncthreads();
-    join_parts<HD, HD>(out, ml, R, WK, a.out, a.lse,
+    join_parts<HD, HD, R>(out, ml, WK, a.out, a.lse,
                      [&](int r) -> long long {
                          const int i = (row0 + r) / per;
                          return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
     float2 *ml = reinterpret_cast<float2 *>(out + AW * R * HD);
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
-    join_parts<HD, HD>(out, ml, R, AW, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
+    join_parts<HD, HD, R>(out, ml, AW, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
                    [&](int i) { return sinks ? sinks[kvh * per + i] * LOG2E : -INFINITY; });
 }
 

@@ -6,34 +6,41 @@
 // three: the six products down to 2^-16 are formed, what is left out is 2^-22 of the product.  The small ones come first in the accumulator, so that few
 // of its (truncating) additions carry weight; an output tile starts at zero and joins the running output in registers, scaled to the new maximum.
 //
-// Warp roles: 0-7 softmax and output (thread = row and half of a tile's slots, then half of the dimensions), 8-11 keys and values from global memory
-// through registers into operand order (cut into pieces on the way), 12 issues.  Scores of two tiles alternate in tensor memory; the pieces of a tile's
-// weights take the place of its scores as operand A.  While the softmax warps work on tile i + 1 the tensor cores do the values of tile i and the
-// scores of tile i + 2.
+// Warp roles: 0-7 softmax and output (thread = row and half of a tile's slots, then half of the dimensions); 13 brings keys and values (bf16: tensor copies
+// in operand order, swizzled; f32: bulk copies of raw rows into a ring, which warps 8-11 cut into pieces in operand order); 8-11 look at the values of
+// tiles that not every row sees whole; 12 issues.  Queries are operand A in tensor memory (64 dimensions: the two upper pieces, there is no room for the third,
+// which stays in shared memory).  Scores of two tiles alternate in tensor memory; the pieces of a tile's weights take the place of its scores as operand A.
+// While the softmax warps work on tile i + 1 the tensor cores do the values of tile i and the scores of tile i + 2.
 //
-// Operands without swizzle: core matrices of 8 rows x 16 bytes, [slot / 8][dim / 8] of them.  As operand B of the scores (N = slots, K = dims) that is
-// K-major, as operand B of the outputs (N = dims, K = slots) MN-major: neither keys nor values are transposed.
+// Keys are operand B of the scores (N = slots, K = dims), K-major, values that of the outputs (N = dims, K = slots), MN-major: neither is transposed.  What is
+// not swizzled stands in core matrices of 8 rows x 16 bytes, keys [dim / 8][slot / 8], values [slot / 8][dim / 8].
 #include "brrr_kernels.h"
 #include "brrr_kvattn.cuh"
 #include "brrr_tc.cuh"
+#include "brrr_tmap.h"
 
 namespace brrr {
 
 namespace {
 
-constexpr int TC_SOFT = 8, TC_LOAD = 4, TC_THREADS = (TC_SOFT + TC_LOAD + 1) * 32, TC_M = 128;
+constexpr int TC_SOFT = 8, TC_LOAD = 4, TC_ISSUE = TC_SOFT + TC_LOAD, TC_BULK = TC_ISSUE + 1, TC_THREADS = (TC_BULK + 1) * 32, TC_M = 128;
 
-template <class T, int HD, int N>
+template <class T, int HD>
 struct Tc {
+    static constexpr int N = HD == 64 ? 128 : 64;                      // slots of a tile: 8192 values of keys and of values each
     static constexpr int PL = T::SPLIT ? 3 : 1;                       // pieces of a cached value
-    static constexpr int KST = T::SPLIT ? 1 : 2, VST = T::SPLIT || HD == 128 ? 1 : 2;      // stages
+    static constexpr int ST = T::SPLIT ? 1 : 4;                        // stages of operands
     static constexpr int NC = HD / 8;                                  // 16-byte pieces of a row
-    static constexpr int PLANE = N * HD * 2, QPLANE = TC_M * HD * 2;
-    static constexpr int Q = 0, K = 3 * QPLANE, V = K + KST * PL * PLANE, BYTES = V + VST * PL * PLANE;
+    static constexpr int PLANE = N * HD * 2, STAGE = PL * PLANE;
+    static constexpr int QT = HD == 64 ? 2 : 3;                        // pieces of the queries in tensor memory
+    static constexpr int UNITS = T::SPLIT ? 6 : 0, UROWS = N / 2, UNIT = UROWS * HD * 4;      // ring of raw f32 rows: half a tile each
+    static constexpr int Q2 = 0, K = QT == 2 ? TC_M * HD * 2 : 0, V = K + ST * STAGE, RAW = V + ST * STAGE, BYTES = RAW + UNITS * UNIT;
     // above half of an SM's shared memory: one CTA per SM, since each takes all of tensor memory
     static constexpr size_t SMEM = BYTES > 118784 ? BYTES : 118784;
-    static constexpr uint32_t BUF = N + N / 2, D = 2 * BUF;            // columns: scores, then pieces hi | mid by halves, and lo behind; the output tile
-    static_assert(D + HD <= 512 && SMEM <= 229376 && TC_M * (HD + 4) * 4 + TC_M * 16 <= K, "");
+    // columns: twice scores, which become the pieces hi | mid by halves, and the pieces lo behind; the output tile; the queries
+    static constexpr uint32_t BUF = N + N / 2, D = 2 * BUF, Q = D + HD;
+    static constexpr int OUT = HD + 4;                                 // floats from row to row of the result in shared memory
+    static_assert(Q + QT * HD / 2 <= 512 && SMEM + 1024 <= 227 * 1024 - 4608 && TC_M * OUT * 4 + TC_M * 16 <= 2 * ST * STAGE, "");
 };
 
 __device__ __forceinline__ void tc_mma_ss(uint32_t issue, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -64,28 +71,24 @@ __device__ __forceinline__ void tc_st16(uint32_t t, const uint32_t *v) {
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
+__device__ __forceinline__ f32x2 pack2(float a, float b) { return tl_pack2(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ f32x2 upper2(f32x2 x) { return x & 0xFFFF0000FFFF0000ull; }
+__device__ __forceinline__ f32x2 sub2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t uppers(f32x2 x) { return __byte_perm((uint32_t)x, (uint32_t)(x >> 32), 0x7632); }
 // the three pieces of two values, first value in the lower half
-__device__ __forceinline__ void cut2(float a, float b, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
-    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-    hi = __byte_perm(ua, ub, 0x7632);
-    const float ra = a - __uint_as_float(ua & 0xFFFF0000u), rb = b - __uint_as_float(ub & 0xFFFF0000u);
-    const uint32_t va = __float_as_uint(ra), vb = __float_as_uint(rb);
-    mid = __byte_perm(va, vb, 0x7632);
-    const float sa = ra - __uint_as_float(va & 0xFFFF0000u), sb = rb - __uint_as_float(vb & 0xFFFF0000u);
-    lo = __byte_perm(__float_as_uint(sa), __float_as_uint(sb), 0x7632);
+__device__ __forceinline__ void cut2(f32x2 x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+    hi = uppers(x);
+    const f32x2 r = sub2(x, upper2(x));
+    mid = uppers(r);
+    lo = uppers(sub2(r, upper2(r)));
 }
 __device__ __forceinline__ void st_shared16(uint32_t at, const uint32_t (&v)[4]) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
-// eight f32 values as 16 bytes in each of three planes
-__device__ __forceinline__ void store_pieces(uint32_t at, int plane, const float (&x)[8]) {
-    uint32_t p[3][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) cut2(x[2 * i], x[2 * i + 1], p[0][i], p[1][i], p[2][i]);
-#pragma unroll
-    for (int i = 0; i < 3; i++) st_shared16(at + i * plane, p[i]);
-}
-
 // products in the order in which they are formed: the piece of A and of B, four bits each
 template <int PL>
 struct Products {
@@ -95,34 +98,81 @@ struct Products {
     static __device__ __forceinline__ constexpr int b(int p) { return B >> (4 * p) & 15; }
 };
 
+// The order in which halves of operands are made: keys of tiles 0 and 1, then values of tile i and keys of tile i + 2 in turn (the scores of tile i + 2 follow the
+// outputs of tile i, before the values of tile i + 1 have room).
+struct Half {
+    int tile, second;
+    bool val;
+};
+__device__ __forceinline__ Half half_of(int u, int tiles) {
+    const int op = u >> 1, keys = min(op, (op + 2) >> 1);       // K0 K1 V0 K2 V1 K3 ...: operands 0, 1, 3, 5 ... are keys while there are any
+    Half h;
+    h.second = u & 1;
+    if (op < 2) {
+        h.val = tiles == 1 && op == 1;
+        h.tile = h.val ? 0 : op;
+    } else if (op < 2 * tiles - 1) {
+        h.val = !(op & 1);
+        h.tile = h.val ? (op - 2) >> 1 : keys;
+    } else {
+        h.val = true;
+        h.tile = tiles - 1;
+    }
+    return h;
+}
+// K and V of a bf16 cache as tensors [sequence][kv head][slot][dim], boxes of 64 dims x a tile's slots in rows of 128 swizzled bytes
+struct alignas(64) KvMaps {
+    CUtensorMap k, v;
+};
+__device__ __forceinline__ void tensor_rows(uint32_t dst, const CUtensorMap *map, int x, int slot, int kvh, int seq, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(slot),
+                 "r"(kvh), "r"(seq), "r"(smem_u32(bar))
+                 : "memory");
+}
+// descriptor of rows of 128 swizzled bytes: groups of eight rows 1024 bytes apart, blocks of 64 values `lbo` bytes apart (MN-major)
+__device__ __forceinline__ uint64_t desc_rows128(uint32_t at, uint32_t lbo) {
+    return (uint64_t)((at >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 | (uint64_t)64 << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
 // grid (C, kv heads x blocks of 128 rows, entries), clusters of C
-template <class T, int HD, int N>
-__global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeArgs a) {
-    typedef Tc<T, HD, N> S;
+template <class T, int HD>
+__global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeArgs a, const __grid_constant__ KvMaps maps) {
+    typedef Tc<T, HD> S;
     typedef Products<S::PL> Pr;
-    extern __shared__ __align__(128) unsigned char tsm[];
-    __shared__ __align__(8) uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready, dfull, qfull;
+    constexpr int N = S::N;
+    extern __shared__ unsigned char tsm_[];
+    unsigned char *tsm = tsm_ + ((1024u - (smem_u32(tsm_) & 1023u)) & 1023u);          // swizzled rows want 1024-byte alignment
+    __shared__ __align__(8) uint64_t kfull[S::ST], kempty[S::ST], vfull[S::ST], vempty[S::ST], vraw[S::ST], sfull[2], pready, dfull, qfull, rfull[S::UNITS + 1], rempty[S::UNITS + 1];
     __shared__ TreeRows see;
     __shared__ float part_max[2][2][TC_M];
-    __shared__ uint32_t bad[N / 32];           // slots of a tile whose values are no numbers (tiles that not every row sees whole)
+    __shared__ uint32_t bad[S::ST][N / 32];           // slots of a tile whose values are no numbers (tiles that not every row sees whole)
     __shared__ uint32_t tmem_sh;
     const int per = a.nh / kv.nkv, blocks = (a.rows * per + TC_M - 1) / TC_M;
     const int kvh = blockIdx.y / blocks, row0 = blockIdx.y % blocks * TC_M, b = blockIdx.z;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    // this thread's half of its row of queries and the row's sink, on their way before anything else is known
+    const int quarter = warp & 3, half = warp >> 2 & 1, r = quarter * 32 + lane, node = (row0 + r) / per, head = kvh * per + (row0 + r) % per;
+    const long long place = ((long long)b * a.rows + node) * a.nh + head;
+    float4 qx[HD / 8];
+    float sink = -INFINITY;
+    if (warp < TC_SOFT) {
+        const float4 *p = reinterpret_cast<const float4 *>(a.q + place * HD + half * (HD / 2));
+#pragma unroll
+        for (int i = 0; i < HD / 8; i++) qx[i] = node < a.rows ? p[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (a.sinks) sink = a.sinks[head] * LOG2E;
+    }
     const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
     if (!e.ok || row0 >= e.count * per) {
         if (!e.ok && threadIdx.x == 0) kv_error(kv);
         return;
     }
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&kfull[i], TC_LOAD); mbar_init(&vfull[i], TC_LOAD);
-            mbar_init(&kempty[i], 1); mbar_init(&vempty[i], 1); mbar_init(&sfull[i], 1);
-        }
-        mbar_init(&pready, TC_SOFT); mbar_init(&dfull, 1); mbar_init(&qfull, TC_SOFT);
+        for (int i = 0; i < S::ST; i++) { mbar_init(&kfull[i], T::SPLIT ? TC_LOAD : 1); mbar_init(&vfull[i], TC_LOAD); mbar_init(&vraw[i], 1); mbar_init(&kempty[i], 1); mbar_init(&vempty[i], 1); }
+        for (int i = 0; i < S::UNITS; i++) { mbar_init(&rfull[i], 1); mbar_init(&rempty[i], TC_LOAD); }
+        mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1); mbar_init(&pready, TC_SOFT); mbar_init(&dfull, 1); mbar_init(&qfull, TC_SOFT);
         mbar_fence_init();
     }
-    if (warp == TC_SOFT + TC_LOAD) {
+    if (warp == TC_ISSUE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -135,50 +185,72 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
     const int from = s0 + blockIdx.x * chunk, tiles = max(0, min(chunk, s0 + all - from));
     auto partial = [&](int i) { return (from + i) * N < see.full || (from + i + 1) * N > e.len; };
     TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
-    float *out = reinterpret_cast<float *>(tsm);
-    float2 *ml = reinterpret_cast<float2 *>(out + TC_M * (HD + 4));
+    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh), *vc = (const typename T::Val *)kv.v + kv.head(e.seq, kvh);
+    float *out = reinterpret_cast<float *>(tsm + S::K);
+    float2 *ml = reinterpret_cast<float2 *>(out + TC_M * S::OUT);
 
     if (warp < TC_SOFT) {
         // ---------------- queries, softmax, output
-        for (int u = tid; u < TC_M * S::NC; u += TC_SOFT * 32) {
-            const int r = (u & 7) + u / (8 * S::NC) * 8, c = u / 8 % S::NC, i = (row0 + r) / per;       // eight neighbours write one core matrix
-            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            if (i < e.count) {
-                const float4 *p = reinterpret_cast<const float4 *>(a.q + (((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per) * HD + c * 8);
-                const float4 y = p[0], z = p[1];
-                x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; x[4] = z.x; x[5] = z.y; x[6] = z.z; x[7] = z.w;
-                if (a.scale < 0.0f)
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] = -x[k];
+        for (int i = 0; i < HD / 8; i += 8) {
+            uint32_t p[3][16];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                cut2(pack2(qx[i + j].x, qx[i + j].y), p[0][2 * j], p[1][2 * j], p[2][2 * j]);
+                cut2(pack2(qx[i + j].z, qx[i + j].w), p[0][2 * j + 1], p[1][2 * j + 1], p[2][2 * j + 1]);
             }
-            store_pieces(base0 + S::Q + ((r >> 3) * S::NC + c) * 128 + (r & 7) * 16, S::QPLANE, x);
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) p[k][j] ^= flip;
+                if (k < S::QT) tc_st16(lanes + S::Q + k * (HD / 2) + half * (HD / 4) + i * 2, p[k]);
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t v[4] = {p[k][4 * j], p[k][4 * j + 1], p[k][4 * j + 2], p[k][4 * j + 3]};
+                        st_shared16(base0 + S::Q2 + ((half * (S::NC / 2) + i / 2 + j) * (TC_M / 8) + (r >> 3)) * 128 + (r & 7) * 16, v);
+                    }
+            }
         }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         fence_proxy_async();
+        tl_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&qfull);
-        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane, node = (row0 + r) / per;
         const uint64_t mask = node < e.count ? see.mask[node] : 0;
         const int lo = node < e.count ? see.lo[node] : 0x7fffffff;
         const bool idle = row0 + quarter * 32 >= e.count * per;         // a warp of padding
-        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        // which of the slots t0 .. t0 + 63 this row sees
+        auto sees = [&](int t0) {
+            auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+            const int d = e.len - t0;                                    // where the drafted ones begin
+            return (below(d) & ~below(lo - t0)) | (d >= 64 || d <= -64 ? 0ull : d >= 0 ? mask << d : mask >> -d);
+        };
         const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);           // above zero: -infinity stays what it is
-        float m = -INFINITY, l = 0.0f, f = 1.0f, o[HD / 2];
+        const f32x2 cc = pack2(c, c);
+        float m = -INFINITY, l = 0.0f, f = 1.0f;
+        f32x2 o[HD / 4];
 #pragma unroll
-        for (int d = 0; d < HD / 2; d++) o[d] = 0.0f;
+        for (int d = 0; d < HD / 4; d++) o[d] = 0ull;
         auto join_output = [&](int i) {
             wait(&dfull, i & 1);
             if (idle) return;
             tl_fence_after();
+            const f32x2 ff = pack2(f, f);
 #pragma unroll
             for (int d = 0; d < HD / 2; d += 32) {
                 float x[32];
                 tc_ld32(lanes + S::D + half * (HD / 2) + d, x);
 #pragma unroll
-                for (int k = 0; k < 32; k++) o[d + k] = __fmaf_rn(o[d + k], f, x[k]);
+                for (int k = 0; k < 16; k++) o[d / 2 + k] = tl_fma2(o[d / 2 + k], ff, pack2(x[2 * k], x[2 * k + 1]));
             }
         };
         for (int i = 0; i < tiles; i++) {
             const uint32_t buf = lanes + (i & 1) * S::BUF, mine = buf + half * (N / 2);
+            const bool part = partial(i);
+            const int t0 = (from + i) * N + half * (N / 2);
             wait(&sfull[i & 1], (i >> 1) & 1);
             float fn = 1.0f;
             if (!idle) {
@@ -186,26 +258,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
                 float s[N / 2];
 #pragma unroll
                 for (int k = 0; k < N / 2; k += 32) tc_ld32(mine + k, s + k);
-                uint32_t gone[N / 64];                                   // slots of this half that are no numbers
-#pragma unroll
-                for (int w = 0; w < N / 64; w++) gone[w] = 0;
-                const bool part = partial(i);
                 if (part) {
-                    const int t0 = (from + i) * N + half * (N / 2);
-                    wait(&vfull[i % S::VST], (i / S::VST) & 1);          // the loading warps have looked at the values
+                    const uint64_t seen = sees(t0);
 #pragma unroll
-                    for (int w = 0; w < N / 64; w++) gone[w] = bad[half * (N / 64) + w];
-#pragma unroll
-                    for (int k = 0; k < N / 2; k++) {
-                        const int t = t0 + k;
-                        const bool sees = t < e.len ? t >= lo : t < end && (mask >> (t - e.len) & 1);
-                        if (!sees) s[k] = -INFINITY;
-                        else if (gone[k >> 5] >> (k & 31) & 1) s[k] = NAN;
-                    }
+                    for (int k = 0; k < N / 2; k++)
+                        if (!((uint32_t)(seen >> (k & 32)) >> (k & 31) & 1)) s[k] = -INFINITY;
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < N / 2; k++) top[k & 3] = fmaxf(top[k & 3], s[k]);
+                for (int k = 0; k < N / 2; k += 8)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) top[j] = fmaxf(fmaxf(top[j], s[k + j]), s[k + 4 + j]);
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 part_max[i & 1][half][r] = mx;
                 asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
@@ -213,25 +276,34 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
                 const float safe = mn == -INFINITY ? 0.0f : mn * c;
                 fn = exp2_approx((m == -INFINITY ? m : m * c) - safe);
                 m = mn;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const f32x2 neg = pack2(-safe, -safe);
+                f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
                 for (int k = 0; k < N / 2; k += 32) {
                     uint32_t p0[16], p1[16], p2[16];
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
-                        const float x = exp2_approx(__fmaf_rn(s[k + 2 * j], c, -safe)), y = exp2_approx(__fmaf_rn(s[k + 2 * j + 1], c, -safe));
-                        sum[2 * (j & 1)] += x;
-                        sum[2 * (j & 1) + 1] += y;
-                        cut2(x, y, p0[j], p1[j], p2[j]);
+                        float x, y;
+                        tl_unpack2(tl_fma2(pack2(s[k + 2 * j], s[k + 2 * j + 1]), cc, neg), x, y);
+                        const f32x2 p = pack2(exp2_approx(x), exp2_approx(y));
+                        sum[j & 1] = tl_add2(sum[j & 1], p);
+                        cut2(p, p0[j], p1[j], p2[j]);
                     }
                     tc_st16(mine + k / 2, p0);
                     tc_st16(mine + N / 4 + k / 2, p1);
                     tc_st16(buf + N + half * (N / 4) + k / 2, p2);
                 }
-                l = __fmaf_rn(l, fn, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                float x, y;
+                tl_unpack2(tl_add2(sum[0], sum[1]), x, y);
+                l = __fmaf_rn(l, fn, x + y);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            } else if (partial(i)) {
-                wait(&vfull[i % S::VST], (i / S::VST) & 1);
+            }
+            if (part) {
+                // values that are no numbers stand as zeros in the operand; a row that sees one of them gets no result
+                wait(&vfull[i % S::ST], (i / S::ST) & 1);
+                const uint32_t *g = &bad[i % S::ST][half * (N / 64)];
+                const uint64_t gone = N == 64 ? g[0] : g[0] | (uint64_t)g[N / 64 - 1] << 32;
+                if (gone & sees(t0)) l = NAN;
             }
             if (i > 0) join_output(i - 1);
             f = fn;
@@ -240,109 +312,168 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
             if (lane == 0) mbar_arrive(&pready);
         }
         if (tiles > 0) join_output(tiles - 1);
-        // the queries are done with: their place takes the rows
         part_max[0][half][r] = l;
         asm volatile("bar.sync %0, 256;" ::"r"(9) : "memory");
-        if (half == 0) ml[r] = make_float2(m == -INFINITY ? m : m * c, l + part_max[0][1][r]);
+        l += part_max[0][half ^ 1][r];
+        const float m2 = m == -INFINITY ? m : m * c;
+        if (gridDim.x > 1) {
+            // keys and values are done with: their place takes the rows
+            if (half == 0) ml[r] = make_float2(m2, l);
 #pragma unroll
-        for (int d = 0; d < HD / 2; d += 4)
-            *reinterpret_cast<float4 *>(out + r * (HD + 4) + half * (HD / 2) + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-    } else if (warp < TC_SOFT + TC_LOAD) {
-        // ---------------- keys and values into operand order
-        constexpr int LPI = T::SPLIT ? 2 : 1, BI = 4 / LPI;             // 16-byte loads per item; items per batch
-        constexpr int ITEMS = N / 8 * (HD / 32) / TC_LOAD, NB = ITEMS / BI, RING = 4;
-        static_assert(ITEMS % BI == 0 && (2 * NB) % RING == 0, "");
-        const typename T::Val *src[2] = {(const typename T::Val *)kv.k + kv.head(e.seq, kvh), (const typename T::Val *)kv.v + kv.head(e.seq, kvh)};
-        const int lw = warp - TC_SOFT, row = lane & 7, sub = lane >> 3;
-        uint4 ring[RING][4];
-        // batch bt of tile i: items of the keys, then of the values
-        auto fetch = [&](int i, int bt, uint4 (&x)[4]) {
+            for (int d = 0; d < HD / 4; d += 2) *reinterpret_cast<ulonglong2 *>(out + r * S::OUT + half * (HD / 2) + 2 * d) = make_ulonglong2(o[d], o[d + 1]);
+        } else if (node < e.count) {
+            const float top = fmaxf(m2, sink), safe = top == -INFINITY ? 0.0f : top, w = exp2_approx(m2 - safe);
+            l = __fmaf_rn(l, w, exp2_approx(sink - safe));
+            const float k = w * __fdividef(1.0f, l == 0.0f ? 1.0f : l);
+            const f32x2 kk = pack2(k, k);
+            ulonglong2 *to = reinterpret_cast<ulonglong2 *>(a.out + place * HD + half * (HD / 2));
 #pragma unroll
-            for (int k = 0; k < BI; k++) {
-                const int it = ((bt % NB) * BI + k) * TC_LOAD + lw, t = (from + i) * N + it / (HD / 32) * 8 + row, chunk = it % (HD / 32) * 4 + sub;
-                const typename T::Val *p = src[bt / NB] + (long long)t * HD + chunk * 8;
-#pragma unroll
-                for (int j = 0; j < LPI; j++) x[k * LPI + j] = t < end ? ldg_shared(p + j * T::V) : make_uint4(0, 0, 0, 0);
-            }
+            for (int d = 0; d < HD / 4; d += 2) to[d / 2] = make_ulonglong2(tl_mul2(o[d], kk), tl_mul2(o[d + 1], kk));
+            if (a.lse && half == 0) a.lse[place] = (top + log2f(l)) * LN2;
+        }
+    } else if (warp < TC_ISSUE) {
+        const int lw = warp - TC_SOFT, lt = tid - TC_SOFT * 32;
+        auto arrive = [&](uint64_t *bar) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
         };
-        if (tiles > 0)
-#pragma unroll
-            for (int k = 0; k < RING - 1; k++) fetch(0, k, ring[k]);
-        for (int i = 0; i < tiles; i++) {
-            const bool part = partial(i);
-#pragma unroll
-            for (int bt = 0; bt < 2 * NB; bt++) {
-                const int nx = bt + RING - 1;
-                if (nx < 2 * NB) fetch(i, nx, ring[nx % RING]);
-                else if (i + 1 < tiles) fetch(i + 1, nx - 2 * NB, ring[nx % RING]);
-                const int st = bt < NB ? i % S::KST : i % S::VST;
-                if (bt == 0 && i >= S::KST) wait(&kempty[st], ((i / S::KST) & 1) ^ 1);
-                if (bt == NB) {
-                    if (i >= S::VST) wait(&vempty[st], ((i / S::VST) & 1) ^ 1);
-                    if (part) {
-                        // with two stages the tile before may be read still
-                        if (S::VST > 1 && i > 0) wait(&vempty[(i - 1) % S::VST], ((i - 1) / S::VST) & 1);
-                        if (lw == 0 && lane < N / 32) bad[lane] = 0;
-                        asm volatile("bar.sync %0, 128;" ::"r"(10) : "memory");
-                    }
-                }
-                const uint32_t dst = base0 + (bt < NB ? S::K : S::V) + st * S::PL * S::PLANE;
-#pragma unroll
-                for (int k = 0; k < BI; k++) {
-                    const int it = ((bt % NB) * BI + k) * TC_LOAD + lw, rg = it / (HD / 32), chunk = it % (HD / 32) * 4 + sub;
-                    const uint32_t at = dst + (rg * S::NC + chunk) * 128 + row * 16;
-                    uint4 (&x)[4] = ring[bt % RING];
-                    if (bt >= NB && part) {
+        // a clean slate for the slots of a tile that turn out to be no numbers
+        auto clean = [&](int st) {
+            if (lt < N / 32) bad[st][lt] = 0;
+            asm volatile("bar.sync %0, 128;" ::"r"(10) : "memory");
+        };
+        if constexpr (!T::SPLIT) {
+            // ---------------- bf16: values have come; where a row may not see all of them, those that are no numbers become zeros
+            for (int i = 0; i < tiles; i++) {
+                const int st = i % S::ST;
+                wait(&vraw[st], (i / S::ST) & 1);
+                if (partial(i)) {
+                    clean(st);
+                    for (int u = lt; u < N * S::NC; u += TC_LOAD * 32) {
+                        const int row = u / S::NC, c = u % S::NC;
+                        const uint32_t at = base0 + S::V + st * S::STAGE + (c >> 3) * (N * 128) + row * 128 + ((c & 7) ^ (row & 7)) * 16;
+                        float x[8];
+                        T::get(lds128(at), x);
                         bool any = false;
 #pragma unroll
-                        for (int j = 0; j < LPI; j++) {
-                            float y[T::V];
-                            T::get(x[k * LPI + j], y);
-#pragma unroll
-                            for (int d = 0; d < T::V; d++) any |= not_finite(y[d]);
-                        }
+                        for (int d = 0; d < 8; d++) any |= not_finite(x[d]);
                         if (any) {
-                            const int t = rg * 8 + row;
-                            atomicOr(&bad[t >> 5], 1u << (t & 31));
-#pragma unroll
-                            for (int j = 0; j < LPI; j++) x[k * LPI + j] = make_uint4(0, 0, 0, 0);
+                            const uint32_t zero[4] = {0, 0, 0, 0};
+                            st_shared16(at, zero);
+                            atomicOr(&bad[st][row >> 5], 1u << (row & 31));
                         }
-                    }
-                    if (T::SPLIT) {
-                        const uint4 y = x[k * LPI], z = x[k * LPI + LPI - 1];
-                        const float v[8] = {__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w),
-                                            __uint_as_float(z.x), __uint_as_float(z.y), __uint_as_float(z.z), __uint_as_float(z.w)};
-                        store_pieces(at, S::PLANE, v);
-                    } else {
-                        const uint32_t v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-                        st_shared16(at, v);
                     }
                 }
-                if (bt == NB - 1 || bt == 2 * NB - 1) {
-                    fence_proxy_async();
+                arrive(&vfull[st]);
+            }
+        } else {
+            // ---------------- f32: rows out of the ring, cut into pieces.  A thread walks along a row of its own, its neighbours' rows one piece (and by fours
+            // half a piece) ahead: reads and writes meet no bank conflicts
+            const int row = lane & 7, first = row >> 2 & 1;
+            for (int u = 0; u < 4 * tiles; u++) {                       // halves of operands in the ring's order
+                const Half x = half_of(u, tiles);
+                const bool val = x.val, part = partial(x.tile);
+                const int i = x.tile, h = x.second;
+                if (!h && i > 0) wait(val ? &vempty[0] : &kempty[0], (i - 1) & 1);
+                if (!h && val && part) clean(0);
+                {
+                    const int slot = u % S::UNITS;
+                    wait(&rfull[slot], (u / S::UNITS) & 1);
+                    const uint32_t raw = base0 + S::RAW + slot * S::UNIT, dst = base0 + (val ? S::V : S::K);
+                    constexpr int ITEMS = S::UROWS * S::NC / (TC_LOAD * 32);      // pieces of a thread
+#pragma unroll
+                    for (int k = 0; k < ITEMS; k++) {
+                        // a warp: four groups of eight rows at a time (128 dimensions: each warp one group of the unit's four, by its lanes a quarter of the pieces)
+                        int rg, c;
+                        if (S::UROWS == 64) {
+                            rg = (lw & 1) * 4 + (lane >> 3);
+                            c = ((lw >> 1) * (S::NC / 2) + k + row) & (S::NC - 1);
+                        } else {
+                            rg = lane >> 3;
+                            c = (lw * (S::NC / 4) + k + row) & (S::NC - 1);
+                        }
+                        const int rr = rg * 8 + row, t = (from + i) * N + h * S::UROWS + rr;
+                        const uint32_t src = raw + (rr * HD + c * 8) * 4;
+                        const uint4 y = lds128(src + first * 16), z = lds128(src + (first ^ 1) * 16);
+                        const bool there = t < end;
+                        f32x2 x[4];
+                        x[0] = tl_pack2(first ? z.x : y.x, first ? z.y : y.y); x[1] = tl_pack2(first ? z.z : y.z, first ? z.w : y.w);
+                        x[2] = tl_pack2(first ? y.x : z.x, first ? y.y : z.y); x[3] = tl_pack2(first ? y.z : z.z, first ? y.w : z.w);
+                        if (!there) x[0] = x[1] = x[2] = x[3] = 0ull;
+                        if (val && part) {
+                            bool any = false;
+#pragma unroll
+                            for (int d = 0; d < 4; d++) any |= not_finite(__uint_as_float((uint32_t)x[d])) || not_finite(__uint_as_float((uint32_t)(x[d] >> 32)));
+                            if (any) {
+                                x[0] = x[1] = x[2] = x[3] = 0ull;
+                                const int tr = h * S::UROWS + rr;
+                                atomicOr(&bad[0][tr >> 5], 1u << (tr & 31));
+                            }
+                        }
+                        uint32_t p[3][4];
+#pragma unroll
+                        for (int d = 0; d < 4; d++) cut2(x[d], p[0][d], p[1][d], p[2][d]);
+                        const int g8 = h * (S::UROWS / 8) + rg;
+                        const uint32_t at = dst + (val ? g8 * S::NC + c : c * (N / 8) + g8) * 128 + row * 16;
+#pragma unroll
+                        for (int d = 0; d < 3; d++) st_shared16(at + d * S::PLANE, p[d]);
+                    }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bt < NB ? &kfull[st] : &vfull[st]);
+                    if (lane == 0) mbar_arrive(&rempty[slot]);
+                    if (h) arrive(val ? &vfull[0] : &kfull[0]);
                 }
             }
         }
+    } else if (warp == TC_BULK) {
+        if (T::SPLIT && lane == 0) {
+            // ---------------- f32: the ring, half a tile's rows to a copy (rows behind the end are not read)
+            for (int u = 0; u < 4 * tiles; u++) {
+                const Half x = half_of(u, tiles);
+                const int slot = u % max(S::UNITS, 1), t = (from + x.tile) * N + x.second * S::UROWS, rows = max(0, min(S::UROWS, end - t));
+                if (u >= S::UNITS) wait(&rempty[slot], ((u / max(S::UNITS, 1)) & 1) ^ 1);
+                if (rows) {
+                    mbar_expect_tx(&rfull[slot], rows * HD * 4);
+                    bulk_g2s(tsm + S::RAW + slot * S::UNIT, (x.val ? vc : kc) + (long long)t * HD, rows * HD * 4, &rfull[slot]);
+                } else {
+                    mbar_arrive(&rfull[slot]);
+                }
+            }
+        } else if (!T::SPLIT && lane == 0) {
+            // ---------------- bf16: a tile's keys and values (slots behind the end come along: nobody sees them)
+            for (int i = 0; i < tiles; i++) {
+                const int st = i % S::ST, t = (from + i) * N;
+                if (i >= S::ST) wait(&kempty[st], (i / S::ST - 1) & 1);
+                mbar_expect_tx(&kfull[st], S::PLANE);
+                for (int x = 0; x < HD; x += 64) tensor_rows(base0 + S::K + st * S::STAGE + x * N * 2, &maps.k, x, t, kvh, e.seq, &kfull[st]);
+                if (i >= S::ST) wait(&vempty[st], (i / S::ST - 1) & 1);
+                mbar_expect_tx(&vraw[st], S::PLANE);
+                for (int x = 0; x < HD; x += 64) tensor_rows(base0 + S::V + st * S::STAGE + x * N * 2, &maps.v, x, t, kvh, e.seq, &vraw[st]);
+            }
+        }
+        __syncwarp();
     } else {
         // ---------------- products (the whole warp walks the loop, an elected lane issues)
         const uint32_t issue = elect_one() ? 1u : 0u;
         constexpr uint32_t types = (1u << 4) | (1u << 7) | (1u << 10) | ((TC_M >> 4) << 24);       // f32 += bf16 x bf16
         constexpr uint32_t id_s = types | ((uint32_t)(N >> 3) << 17), id_o = types | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-        const uint64_t dq = tl_smem_desc(tsm + S::Q, 128, S::NC * 128), dk = tl_smem_desc(tsm + S::K, 128, S::NC * 128), dv = tl_smem_desc(tsm + S::V, S::NC * 128, 128);
+        const uint64_t dq = tl_smem_desc(tsm + S::Q2, TC_M * 16, 128), dk = T::SPLIT ? tl_smem_desc(tsm + S::K, N * 16, 128) : desc_rows128(base0 + S::K, 16),
+                       dv = T::SPLIT ? tl_smem_desc(tsm + S::V, S::NC * 128, 128) : desc_rows128(base0 + S::V, N * 128);
         wait(&qfull, 0);
         auto scores = [&](int i) {
-            const int st = i % S::KST;
-            wait(&kfull[st], (i / S::KST) & 1);
+            const int st = i % S::ST;
+            wait(&kfull[st], (i / S::ST) & 1);
             tl_fence_after();
             const uint32_t d = tmem + (i & 1) * S::BUF;
-            const uint64_t k0 = dk + (uint64_t)(st * S::PL * S::PLANE / 16);
+            const uint64_t k0 = dk + (uint64_t)(st * S::STAGE / 16);
 #pragma unroll
             for (int p = 0; p < Pr::N; p++)
 #pragma unroll
-                for (int s = 0; s < HD / 16; s++)
-                    tc_mma_ss(issue, d, dq + (uint64_t)((Pr::a(p) * S::QPLANE + s * 256) / 16), k0 + (uint64_t)((Pr::b(p) * S::PLANE + s * 256) / 16), id_s, p > 0 || s > 0);
+                for (int s = 0; s < HD / 16; s++) {
+                    const uint64_t db = k0 + (uint64_t)((T::SPLIT ? Pr::b(p) * S::PLANE + s * 2 * N * 16 : s / 4 * N * 128 + s % 4 * 32) / 16);
+                    if (Pr::a(p) < S::QT) tc_mma_ts(issue, d, tmem + S::Q + Pr::a(p) * (HD / 2) + s * 8, db, id_s, p > 0 || s > 0);
+                    else tc_mma_ss(issue, d, dq + (uint64_t)(s * 2 * TC_M * 16 / 16), db, id_s, p > 0 || s > 0);
+                }
             tl_commit_if(issue, &sfull[i & 1]);
             tl_commit_if(issue, &kempty[st]);
             __syncwarp();
@@ -350,12 +481,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
         if (tiles > 0) scores(0);
         if (tiles > 1) scores(1);
         for (int i = 0; i < tiles; i++) {
-            const int st = i % S::VST;
-            wait(&vfull[st], (i / S::VST) & 1);
+            const int st = i % S::ST;
+            wait(&vfull[st], (i / S::ST) & 1);
             wait(&pready, i & 1);
             tl_fence_after();
             const uint32_t p0 = tmem + (i & 1) * S::BUF;
-            const uint64_t v0 = dv + (uint64_t)(st * S::PL * S::PLANE / 16);
+            const uint64_t v0 = dv + (uint64_t)(st * S::STAGE / 16);
 #pragma unroll
             for (int p = 0; p < Pr::N; p++)
 #pragma unroll
@@ -363,7 +494,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
                     constexpr int per_half = N / 32;
                     const int h = s / per_half, k = s % per_half;
                     const uint32_t at = p0 + (Pr::a(p) < 2 ? h * (N / 2) + Pr::a(p) * (N / 4) : N + h * (N / 4)) + k * 8;
-                    tc_mma_ts(issue, tmem + S::D, at, v0 + (uint64_t)((Pr::b(p) * S::PLANE + s * 2 * S::NC * 128) / 16), id_o, p > 0 || s > 0);
+                    tc_mma_ts(issue, tmem + S::D, at, v0 + (uint64_t)((T::SPLIT ? Pr::b(p) * S::PLANE + s * 2 * S::NC * 128 : s * 2048) / 16), id_o, p > 0 || s > 0);
                 }
             tl_commit_if(issue, &dfull);
             tl_commit_if(issue, &vempty[st]);
@@ -376,8 +507,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
     }
     tl_fence_before();
     __syncthreads();
-    if (warp == TC_SOFT + TC_LOAD) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    join_parts<HD, HD + 4>(out, ml, TC_M, 1, a.out, a.lse,
+    if (warp == TC_ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (gridDim.x == 1) return;
+    join_parts<HD, S::OUT, TC_M>(out, ml, 1, a.out, a.lse,
                            [&](int r) -> long long {
                                const int i = (row0 + r) / per;
                                return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
@@ -385,22 +517,35 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
                            [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
 }
 
-template <class T, int HD, int N>
+template <class T, int HD>
 cudaError_t launch_tree_tc_as(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
-    typedef Tc<T, HD, N> S;
+    typedef Tc<T, HD> S;
     const int blocks = (a.rows * (a.nh / kv.nkv) + TC_M - 1) / TC_M;
-    constexpr auto K = tree_tc_kernel<T, HD, N>;
+    KvMaps maps{};
+    if (!T::SPLIT) {
+        const tmap_encode_t encode = tmap_encode();
+        if (!encode) return cudaErrorNotSupported;
+        const cuuint64_t dims[4] = {(cuuint64_t)HD, (cuuint64_t)kv.cap, (cuuint64_t)kv.nkv, (cuuint64_t)kv.n_seq};
+        const cuuint64_t strides[3] = {HD * 2, (cuuint64_t)kv.hs * 2, (cuuint64_t)kv.ss * 2};
+        const cuuint32_t box[4] = {64, S::N, 1, 1}, ones[4] = {1, 1, 1, 1};
+        for (int i = 0; i < 2; i++)
+            if (encode(i ? &maps.v : &maps.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? kv.v : kv.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+                return cudaErrorInvalidValue;
+    }
+    constexpr auto K = tree_tc_kernel<T, HD>;
+    constexpr size_t smem = S::SMEM + 1024;
     cudaError_t e = cudaSuccess;
-    const int c = cluster_size<K>((long long)a.n * kv.nkv * blocks, (slots + N - 1) / N, 1, 3, TC_THREADS, S::SMEM, S::SMEM, &e);
+    const int c = cluster_size<K>((long long)a.n * kv.nkv * blocks, (slots + S::N - 1) / S::N, 1, 4, TC_THREADS, smem, smem, &e);
     if (e != cudaSuccess) return e;
-    return launch_cluster<K>(dim3(c, kv.nkv * blocks, a.n), TC_THREADS, c, S::SMEM, S::SMEM, st, kv, a);
+    return launch_cluster<K>(dim3(c, kv.nkv * blocks, a.n), TC_THREADS, c, smem, smem, st, kv, a, maps);
 }
 
 }  // namespace
 
 cudaError_t launch_tree_tc(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
-    if (kv.type) return kv.hd == 64 ? launch_tree_tc_as<KvBf16, 64, 128>(kv, a, slots, st) : launch_tree_tc_as<KvBf16, 128, 128>(kv, a, slots, st);
-    return kv.hd == 64 ? launch_tree_tc_as<KvF32, 64, 128>(kv, a, slots, st) : launch_tree_tc_as<KvF32, 128, 64>(kv, a, slots, st);
+    if (kv.type) return kv.hd == 64 ? launch_tree_tc_as<KvBf16, 64>(kv, a, slots, st) : launch_tree_tc_as<KvBf16, 128>(kv, a, slots, st);
+    return kv.hd == 64 ? launch_tree_tc_as<KvF32, 64>(kv, a, slots, st) : launch_tree_tc_as<KvF32, 128>(kv, a, slots, st);
 }
 
 }  // namespace brrr
