@@ -54,22 +54,6 @@ struct TreeArgs {
     const float *sinks;
     float *out, *lse;
 };
-// Masks (rows behind count cut off) and depths of an entry's rows, in shared memory; all threads call it, a barrier follows.
-__device__ __forceinline__ void tree_masks(const uint64_t *mask, int b, int rows, int count, uint64_t *m, int *depth) {
-    for (int i = threadIdx.x; i < count; i += blockDim.x) {
-        const uint64_t upto = i == 63 ? ~0ull : (1ull << (i + 1)) - 1, live = count == 64 ? ~0ull : (1ull << count) - 1;
-        const uint64_t x = (mask ? mask[(long long)b * rows + i] : upto) & live;
-        m[i] = x;
-        depth[i] = __popcll(x & ~(1ull << i));
-    }
-}
-// Whether row i sees slot t < len + count.
-__device__ __forceinline__ bool tree_sees(const uint64_t *m, const int *depth, int len, int window, int i, int t) {
-    if (t < len) return window <= 0 || t >= len + depth[i] + 1 - window;
-    const int j = t - len;
-    return (m[i] >> j & 1) && (window <= 0 || depth[i] - depth[j] < window);
-}
-
 // Work space of block_kth in shared memory.
 struct KthSpace {
     uint32_t hist[2048], found[2], sums[32];

@@ -50,89 +50,40 @@ __device__ __forceinline__ uint4 ldg_shared(const void *p) {
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
-// Joins the parts of R rows in shared memory (out [part][R][STRIDE], ml [part][R]: maximum in powers of two and sum) and, in a cluster, the CTAs, and
-// writes the rows, each CTA its share.  dst(r): the row's place in the output (< 0: padding), sink(r): its sink in powers of two or -infinity.  First the rows'
-// factors, then the values.  All threads call it, after a barrier; ml has room for R more.
-template <int HD, int STRIDE, int R, class Dst, class Sink>
-__device__ __forceinline__ void join_parts(float *out, float2 *ml, int parts, float *o, float *lse, Dst dst, Sink sink) {
-    __shared__ float weight[16][R], scale[R];
-    __shared__ long long place[R];
-    cg::cluster_group cl = cg::this_cluster();
-    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank(), threads = (int)blockDim.x;
-    if (C > 1 && parts > 1) {
-        // this CTA's parts into part 0
-        for (int r = threadIdx.x; r < R; r += threads) {
-            float m = -INFINITY, l = 0.0f;
-            for (int p = 0; p < parts; p++) m = fmaxf(m, ml[p * R + r].x);
-            const float safe = m == -INFINITY ? 0.0f : m;
-            for (int p = 0; p < parts; p++) {
-                const float2 part = ml[p * R + r];
-                const float w = exp2_approx(part.x - safe);
-                weight[p][r] = w;
-                l = __fmaf_rn(w, part.y, l);
-            }
-            ml[parts * R + r] = make_float2(m, l);
-        }
-        __syncthreads();
-        for (int u = threadIdx.x; u < R * (HD / 4); u += threads) {
-            const int r = u / (HD / 4), d = u % (HD / 4) * 4;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-            for (int p = 0; p < parts; p++) {
-                const float w = weight[p][r];
-                const float4 y = *reinterpret_cast<const float4 *>(out + (p * R + r) * STRIDE + d);
-                x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
-            }
-            *reinterpret_cast<float4 *>(out + r * STRIDE + d) = x;
-        }
-        ml += parts * R;
-        parts = 1;
-    }
-    if (C > 1) cl.sync();
-    // this CTA's rows: r0 .. r0 + rows - 1
-    const int n = C > 1 ? C : parts, each = (R + C - 1) / C, r0 = c * each, rows = max(0, min(each, R - r0));
-    for (int i = threadIdx.x; i < rows; i += threads) {
-        const int r = r0 + i;
-        place[i] = dst(r);
-        if (place[i] < 0) continue;
-        const float sk = sink(r);
-        float2 part[16];
+// Partial results of a row - maximum in powers of two, sum, values - join as
+//   M = max m_p,  sum = sum_p l_p 2^(m_p - M),  x = sum_p x_p 2^(m_p - M),
+// the row's sink as one more part without values.  In a cluster a row has an owner, the CTA rank r / owned_rows(R, C): the others write their parts into its
+// shared memory, [CTA][owned row][STRIDE] and [CTA][owned row] of (m, l), and the owner adds them up in the order of the CTAs.
+__host__ __device__ constexpr int owned_rows(int R, int C) { return (R + C - 1) / C; }
+// The owner's end: n parts of `rows` rows.  dst(i): the owned row's place in the output (< 0: padding), sink(i): its sink in powers of two or -infinity.
+template <int HD, int STRIDE, class Dst, class Sink>
+__device__ __forceinline__ void join_rows(const float *x, const float2 *ml, int n, int rows, float *o, float *lse, Dst dst, Sink sink) {
+    for (int u = threadIdx.x; u < rows * (HD / 4); u += blockDim.x) {
+        const int i = u / (HD / 4), d = u % (HD / 4) * 4;
+        const long long to = dst(i);
+        if (to < 0) continue;
+        const float sk = sink(i);
         float m = sk;
-#pragma unroll
-        for (int p = 0; p < 16; p++)
-            if (p < n) part[p] = C > 1 ? cl.map_shared_rank(ml, p)[r] : ml[p * R + r];
-#pragma unroll
-        for (int p = 0; p < 16; p++)
-            if (p < n) m = fmaxf(m, part[p].x);
+#pragma unroll 8
+        for (int p = 0; p < n; p++) m = fmaxf(m, ml[p * rows + i].x);
         const float safe = m == -INFINITY ? 0.0f : m;
         float l = exp2_approx(sk - safe);
-#pragma unroll
-        for (int p = 0; p < 16; p++)
-            if (p < n) {
-                const float w = exp2_approx(part[p].x - safe);
-                weight[p][i] = w;
-                l = __fmaf_rn(w, part[p].y, l);
-            }
-        scale[i] = __fdividef(1.0f, l == 0.0f ? 1.0f : l);
-        if (lse) lse[place[i]] = (m + log2f(l)) * LN2;
-    }
-    __syncthreads();
-    for (int u = threadIdx.x; u < rows * (HD / 4); u += threads) {
-        const int i = u / (HD / 4), d = u % (HD / 4) * 4, at = (r0 + i) * STRIDE + d;
-        const long long to = place[i];
-        if (to < 0) continue;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
         for (int p = 0; p < n; p++) {
-            const float w = weight[p][i];
-            const float4 y = *reinterpret_cast<const float4 *>(C > 1 ? cl.map_shared_rank(out, p) + at : out + p * R * STRIDE + at);
-            x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
+            const float2 part = ml[p * rows + i];
+            const float w = exp2_approx(part.x - safe);
+            const float4 z = *reinterpret_cast<const float4 *>(x + (p * rows + i) * STRIDE + d);
+            l = __fmaf_rn(w, part.y, l);
+            y.x = __fmaf_rn(w, z.x, y.x); y.y = __fmaf_rn(w, z.y, y.y); y.z = __fmaf_rn(w, z.z, y.z); y.w = __fmaf_rn(w, z.w, y.w);
         }
-        const float k = scale[i];
-        *reinterpret_cast<float4 *>(o + to * HD + d) = make_float4(x.x * k, x.y * k, x.z * k, x.w * k);
+        const float k = __fdividef(1.0f, l == 0.0f ? 1.0f : l);
+        *reinterpret_cast<float4 *>(o + to * HD + d) = make_float4(y.x * k, y.y * k, y.z * k, y.w * k);
+        if (lse && d == 0) lse[to] = (m + log2f(l)) * LN2;
     }
-    if (C > 1) cl.sync();          // nobody leaves while its memory is read
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // ---------------------------------------------------------------- trees
 // What the rows of an entry see: cached slots from lo on, drafted rows by mask (windows applied, rows behind the count cut off).
@@ -141,24 +92,29 @@ struct TreeRows {
     int lo[KV_TREE_MAX];
     int first, full;                        // smallest lo, largest lo: from there to len every row sees every slot
 };
-// All threads call it; complete for them after the next barrier.
-__device__ __forceinline__ void tree_rows(const TreeArgs &a, int b, const KvEntry &e, TreeRows &w) {
+// Thread i's mask of its entry, wanted before the entry's count is known (chains have none).
+__device__ __forceinline__ uint64_t tree_mask(const TreeArgs &a, int b) {
+    const int i = threadIdx.x;
+    return i >= a.rows ? 0 : a.mask ? a.mask[(long long)b * a.rows + i] : i == 63 ? ~0ull : (1ull << (i + 1)) - 1;
+}
+// All threads call it with their mask; complete for them after the next barrier.
+__device__ __forceinline__ void tree_rows(const TreeArgs &a, const KvEntry &e, uint64_t mine, TreeRows &w) {
     __shared__ int depth[KV_TREE_MAX];
     const int i = threadIdx.x;
+    mine &= e.count == 64 ? ~0ull : (1ull << e.count) - 1;
     if (a.window <= 0) {
-        tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
-        if (i < e.count) w.lo[i] = 0;
+        if (i < e.count) { w.mask[i] = mine; w.lo[i] = 0; }
         if (i == 0) w.first = w.full = 0;
         return;
     }
     if (i == 0) { w.first = e.len; w.full = 0; }
-    tree_masks(a.mask, b, a.rows, e.count, w.mask, depth);
+    if (i < e.count) depth[i] = __popcll(mine & ~(1ull << i));
     __syncthreads();
     if (i < e.count) {
         uint64_t in = 0;
         for (int j = 0; j < e.count; j++) in |= (uint64_t)(depth[i] - depth[j] < a.window) << j;
         const int lo = max(0, min(e.len, e.len + depth[i] + 1 - a.window));
-        w.mask[i] &= in;
+        w.mask[i] = mine & in;
         w.lo[i] = lo;
         atomicMin(&w.first, lo);
         atomicMax(&w.full, lo);

@@ -245,59 +245,99 @@ struct Running {
     }
 };
 
-// grid (C, kv heads x blocks of 16 WM rows, entries), clusters of C
-template <class T, int HD, int NK, int WM>
-__global__ void __launch_bounds__(AW * 32, WM == 1 && HD == 64 ? 2 : 1) tree_kernel(KvDev kv, TreeArgs a) {
-    constexpr int WK = AW / WM, R = 16 * WM, STEP = 8 * NK;
-    extern __shared__ __align__(16) float4 frag[];          // the queries, then the parts: out [WK][R][HD], ml [WK][R]
-    __shared__ TreeRows see;
-    const int per = a.nh / kv.nkv, blocks = (a.rows * per + R - 1) / R;
-    const int kvh = blockIdx.y / blocks, row0 = blockIdx.y % blocks * R, b = blockIdx.z;
-    const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
-    if (!e.ok || row0 >= e.count * per) {
-        if (!e.ok && threadIdx.x == 0) kv_error(kv);
+// The parts of a CTA's warps (out [parts][16][HD], ml [parts][16] in shared memory) to the rows' places or, in a cluster, by way of the owners; got, gml: room for
+// the owner's parts, 16 + 15 rows.  All threads call it, after a barrier; the cluster's CTAs have arrived once at its barrier before.
+template <int HD, class Dst, class Sink>
+__device__ __forceinline__ void join_warps(float *out, float2 *ml, int parts, float *got, float2 *gml, float *o, float *lse, Dst dst, Sink sink) {
+    constexpr int R = 16;
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
+    if (C == 1) {
+        join_rows<HD, HD>(out, ml, parts, R, o, lse, dst, sink);
         return;
     }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp % WM, wk = warp / WM, end = e.len + e.count;
+    const int each = owned_rows(R, C);
+    cluster_wait();                // every CTA has begun: its memory may be written
+    for (int u = threadIdx.x; u < R * (HD / 4); u += AW * 32) {
+        const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int p = 0; p < AW; p++) m = fmaxf(m, ml[p * R + r].x);
+        const float safe = m == -INFINITY ? 0.0f : m;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int p = 0; p < AW; p++) {
+            const float2 part = ml[p * R + r];
+            const float w = exp2_approx(part.x - safe);
+            const float4 y = *reinterpret_cast<const float4 *>(out + (p * R + r) * HD + d);
+            l = __fmaf_rn(w, part.y, l);
+            x.x = __fmaf_rn(w, y.x, x.x); x.y = __fmaf_rn(w, y.y, x.y); x.z = __fmaf_rn(w, y.z, x.z); x.w = __fmaf_rn(w, y.w, x.w);
+        }
+        const int owner = r / each, at = c * each + r % each;
+        *reinterpret_cast<float4 *>(cl.map_shared_rank(got, owner) + at * HD + d) = x;
+        if (d == 0) cl.map_shared_rank(gml, owner)[at] = make_float2(m, l);
+    }
+    cluster_arrive();
+    cluster_wait();
+    join_rows<HD, HD>(got, gml, C, each, o, lse, [&](int i) -> long long { return c * each + i < R ? dst(c * each + i) : -1; }, [&](int i) { return sink(c * each + i); });
+}
+
+// grid (C, kv heads, entries), clusters of C
+template <class T, int HD, int NK>
+__global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) tree_kernel(KvDev kv, TreeArgs a) {
+    constexpr int R = 16, STEP = 8 * NK;
+    extern __shared__ __align__(16) float4 frag[];          // the queries, then the parts: out [AW][R][HD], ml [AW][R]; behind them the owner's parts
+    __shared__ TreeRows see;
+    const int per = a.nh / kv.nkv, kvh = blockIdx.y, b = blockIdx.z;
+    const uint64_t mine = tree_mask(a, b);
+    if (gridDim.x > 1) cluster_arrive();
+    const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
+    if (!e.ok || e.count == 0) {
+        if (!e.ok && threadIdx.x == 0) kv_error(kv);
+        if (gridDim.x > 1) cluster_wait();
+        return;
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, end = e.len + e.count;
     const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh), *vc = (const typename T::Val *)kv.v + kv.head(e.seq, kvh);
     int s0 = 0;
     if (a.window > 0) {
-        tree_rows(a, b, e, see);
+        tree_rows(a, e, mine, see);
         __syncthreads();
         s0 = see.first / STEP;
     }
     // the CTA's steps, the warp's among them; the first is on its way while masks and queries are prepared
     const int steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
     const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps);
-    int s = from + wk;
+    int s = from + warp;
     KvStep<T, HD, NK> st;
     if (s < to) {
-        st.template load_k<WM == 1>(kc, s * STEP, end);
-        st.template load_v<WM == 1>(vc, s * STEP, end);
+        st.template load_k<true>(kc, s * STEP, end);
+        st.template load_v<true>(vc, s * STEP, end);
     }
-    if (a.window <= 0) tree_rows(a, b, e, see);
-    stage_queries<T, HD>(frag, WM, [&](int r) -> const float * {
-        const int i = (row0 + r) / per;
-        return i < e.count ? a.q + (((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per) * HD : nullptr;
-    });
+    if (a.window <= 0) tree_rows(a, e, mine, see);
+    auto place = [&](int r) -> long long {
+        const int i = r / per;
+        return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + r % per : -1;
+    };
+    stage_queries<T, HD>(frag, 1, [&](int r) -> const float * { return place(r) >= 0 ? a.q + place(r) * HD : nullptr; });
     __syncthreads();
     // this lane's two rows
     uint64_t mask[2];
     int lo[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const int i = (row0 + wm * 16 + (lane >> 2) + 8 * h) / per;
+        const int i = ((lane >> 2) + 8 * h) / per;
         mask[h] = i < e.count ? see.mask[i] : 0;
         lo[h] = i < e.count ? see.lo[i] : 0x7fffffff;
     }
     const float c = a.scale * LOG2E;
     Running<T, HD, NK> run;
     run.clear();
-    for (; s < to; s += WK) {
+    for (; s < to; s += AW) {
         const int base = s * STEP;
         float x[NK][4];
-        step_scores<T, HD, NK>(st, frag + wm * (HD / 8) * 64, x);
-        if (s + WK < to) st.template load_k<WM == 1>(kc, (s + WK) * STEP, end);
+        step_scores<T, HD, NK>(st, frag, x);
+        if (s + AW < to) st.template load_k<true>(kc, (s + AW) * STEP, end);
         const bool partial = base < see.full || base + STEP > e.len;
 #pragma unroll
         for (int j = 0; j < NK; j++)
@@ -311,44 +351,36 @@ __global__ void __launch_bounds__(AW * 32, WM == 1 && HD == 64 ? 2 : 1) tree_ker
                 }
             }
         run.add(st, x, partial);
-        if (s + WK < to) st.template load_v<WM == 1>(vc, (s + WK) * STEP, end);
+        if (s + AW < to) st.template load_v<true>(vc, (s + AW) * STEP, end);
     }
     __syncthreads();                 // the queries have been read
-    float *out = reinterpret_cast<float *>(frag);
-    float2 *ml = reinterpret_cast<float2 *>(out + WK * R * HD);
-    run.store(out + (wk * R + wm * 16) * HD, ml + wk * R + wm * 16);
+    float *out = reinterpret_cast<float *>(frag), *got = out + AW * R * HD;
+    float2 *gml = reinterpret_cast<float2 *>(got + 31 * HD), *ml = gml + 31;
+    run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
-    join_parts<HD, HD, R>(out, ml, WK, a.out, a.lse,
-                     [&](int r) -> long long {
-                         const int i = (row0 + r) / per;
-                         return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
-                     },
-                     [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
+    join_warps<HD>(out, ml, AW, got, gml, a.out, a.lse, place, [&](int r) { return a.sinks ? a.sinks[kvh * per + r % per] * LOG2E : -INFINITY; });
 }
 
-// bytes of a CTA's shared memory: the queries, later the parts
-__host__ __device__ constexpr size_t attn_smem(int hd, int wm) {
-    const size_t parts = (size_t)AW * 16 * (hd * 4 + 8) + 16 * wm * 8, queries = (size_t)wm * hd * 128;
-    return parts > queries ? parts : queries;
-}
+// bytes of a CTA's shared memory: the queries, later the parts, and the owner's parts
+__host__ __device__ constexpr size_t attn_smem(int hd) { return (size_t)(AW * 16 + 31) * (hd * 4 + 8); }
+static_assert(attn_smem(64) >= 64 * 128 && attn_smem(128) >= 128 * 128, "");
 
-template <class T, int HD, int NK, int WM>
+template <class T, int HD, int NK>
 static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
-    const int per = a.nh / kv.nkv, blocks = (a.rows * per + 16 * WM - 1) / (16 * WM);
-    constexpr size_t smem = attn_smem(HD, WM);
-    constexpr auto K = tree_kernel<T, HD, NK, WM>;
+    constexpr size_t smem = attn_smem(HD);
+    constexpr auto K = tree_kernel<T, HD, NK>;
     cudaError_t e = cudaSuccess;
-    const int c = cluster_size<K>((long long)a.n * kv.nkv * blocks, (slots + 8 * NK - 1) / (8 * NK), AW / WM, 4, AW * 32, smem, smem, &e);
+    const int c = cluster_size<K>((long long)a.n * kv.nkv, (slots + 8 * NK - 1) / (8 * NK), AW, 4, AW * 32, smem, smem, &e);
     if (e != cudaSuccess) return e;
-    return launch_cluster<K>(dim3(c, kv.nkv * blocks, a.n), AW * 32, c, smem, smem, st, kv, a);
+    return launch_cluster<K>(dim3(c, kv.nkv, a.n), AW * 32, c, smem, smem, st, kv, a);
 }
 
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
     int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
     if (a.window > 0) slots = min(slots, a.window + a.rows);
     if (a.rows * (a.nh / kv.nkv) > 16) return launch_tree_tc(kv, a, slots, st);
-    if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2, 1>(kv, a, slots, st) : launch_tree<KvBf16, 128, 2, 1>(kv, a, slots, st);
-    return kv.hd == 64 ? launch_tree<KvF32, 64, 1, 1>(kv, a, slots, st) : launch_tree<KvF32, 128, 1, 1>(kv, a, slots, st);
+    if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2>(kv, a, slots, st) : launch_tree<KvBf16, 128, 2>(kv, a, slots, st);
+    return kv.hd == 64 ? launch_tree<KvF32, 64, 1>(kv, a, slots, st) : launch_tree<KvF32, 128, 1>(kv, a, slots, st);
 }
 
 // ---------------------------------------------------------------- book of weights
@@ -361,12 +393,13 @@ __global__ void __launch_bounds__(AW * 32) weigh_kernel(KvDev kv, TreeArgs a, co
     __shared__ TreeRows see;
     __shared__ float lse[R];
     const int kvh = blockIdx.y, b = blockIdx.z, per = a.nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t mine = tree_mask(a, b);
     const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
     if (kv_named_before(a.seq, b) || !e.ok) {
         if (threadIdx.x == 0) kv_error(kv);
         return;
     }
-    tree_rows(a, b, e, see);
+    tree_rows(a, e, mine, see);
     __syncthreads();
     const uint64_t rows = picked ? picked[b] : ~0ull;
     const int end = e.len + e.count, steps = (end + STEP - 1) / STEP, s0 = see.first / STEP;
@@ -502,16 +535,18 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
                                                          const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *o, float *lse) {
     constexpr int R = 16, STEP = 8 * NK;
     extern __shared__ __align__(16) float4 frag[];
-    uint32_t *keys = reinterpret_cast<uint32_t *>(frag) + attn_smem(HD, 1) / 4;      // [cap / block + 1]
+    uint32_t *keys = reinterpret_cast<uint32_t *>(frag) + attn_smem(HD) / 4;      // [cap / block + 1]
     __shared__ int32_t chosen[256];
     __shared__ float qs[16 * HD];
     __shared__ KthSpace kth;
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks();
     const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (C > 1) cluster_arrive();
     const int s = seq ? seq[r] : r, n = len[r];
     if ((unsigned)s >= (unsigned)kv.n_seq || (unsigned)n > (unsigned)kv.cap) {
         if (threadIdx.x == 0) kv_error(kv);
+        if (C > 1) cluster_wait();
         return;
     }
     const long long row = (long long)r * nh + kvh * per;
@@ -524,7 +559,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
         // scores of the blocks that are not taken anyhow
         const float *mean = means + ((long long)s * kv.nkv + kvh) * (kv.cap / block) * HD;
         const int hi = nb - local, tiles = (hi - first + 7) / 8;
-        if (C > 1) cl.sync();          // every CTA is there: its memory may be written
+        if (C > 1) cluster_wait();     // every CTA is there: its memory may be written
         for (int i = blockIdx.x * AW + warp; i < tiles; i += C * AW) {
             uint32_t key[2];
             const int j0 = first + 8 * i, j = j0 + 2 * (lane & 3);
@@ -535,8 +570,13 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
                 if (j + 1 < hi) there[j + 1] = key[1];
             }
         }
-        if (C > 1) cl.sync();
-        else __syncthreads();
+        if (C > 1) {
+            cluster_arrive();
+            cluster_wait();
+            cluster_arrive();          // for the join
+        } else {
+            __syncthreads();
+        }
         uint32_t ties;
         const int want = nsel - first - local;
         const uint32_t last = want > 0 ? block_kth(hi - first, want, [&](int i) { return keys[first + i]; }, kth, &ties) : 0xFFFFFFFFu;
@@ -595,11 +635,11 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
         if (i + hop < steps) st.template load_v<true>(vc, slot(i + hop), n);
     }
     __syncthreads();
-    float *out = reinterpret_cast<float *>(frag);
-    float2 *ml = reinterpret_cast<float2 *>(out + AW * R * HD);
+    float *out = reinterpret_cast<float *>(frag), *got = out + AW * R * HD;
+    float2 *gml = reinterpret_cast<float2 *>(got + 31 * HD), *ml = gml + 31;
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
-    join_parts<HD, HD, R>(out, ml, AW, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
+    join_warps<HD>(out, ml, AW, got, gml, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
                    [&](int i) { return sinks ? sinks[kvh * per + i] * LOG2E : -INFINITY; });
 }
 
@@ -609,9 +649,9 @@ static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, 
     const int longest = len_hint > 0 ? min(len_hint, kv.cap) : kv.cap, nb = longest / block, each = block / (8 * NK);
     // a tile of eight blocks' scores costs about as much as a step
     const int steps = min(nsel, nb + 1) * each + (nb > nsel ? nb / 8 : 0);
-    const size_t smem = attn_smem(HD, 1) + (size_t)(kv.cap / block + 1) * 4, most = attn_smem(HD, 1) + 16385 * 4;
+    const size_t smem = attn_smem(HD) + (size_t)(kv.cap / block + 1) * 4, most = attn_smem(HD) + 16385 * 4;
     cudaError_t e = cudaSuccess;
-    const int c = cluster_size<blocks_kernel<T, HD, NK>>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, attn_smem(HD, 1), most, &e);
+    const int c = cluster_size<blocks_kernel<T, HD, NK>>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, attn_smem(HD), most, &e);
     if (e != cudaSuccess) return e;
     return launch_cluster<blocks_kernel<T, HD, NK>>(dim3(c, rows, kv.nkv), AW * 32, c, smem, most, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
                                                     sinks, sel, out, lse);

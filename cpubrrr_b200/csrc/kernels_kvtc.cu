@@ -40,7 +40,7 @@ struct Tc {
     // columns: twice scores, which become the pieces hi | mid by halves, and the pieces lo behind; the output tile; the queries
     static constexpr uint32_t BUF = N + N / 2, D = 2 * BUF, Q = D + HD;
     static constexpr int OUT = HD + 4;                                 // floats from row to row of the result in shared memory
-    static_assert(Q + QT * HD / 2 <= 512 && SMEM + 1024 <= 227 * 1024 - 4608 && TC_M * OUT * 4 + TC_M * 16 <= 2 * ST * STAGE, "");
+    static_assert(Q + QT * HD / 2 <= 512 && SMEM + 1024 <= 227 * 1024 - 4608 && (TC_M + 15) * (OUT * 4 + 8) <= 2 * ST * STAGE, "");
 };
 
 __device__ __forceinline__ void tc_mma_ss(uint32_t issue, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -161,33 +161,78 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
         for (int i = 0; i < HD / 8; i++) qx[i] = node < a.rows ? p[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (a.sinks) sink = a.sinks[head] * LOG2E;
     }
+    const uint64_t mine = tree_mask(a, b);
     const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
     if (!e.ok || row0 >= e.count * per) {
         if (!e.ok && threadIdx.x == 0) kv_error(kv);
         return;
     }
-    if (tid == 0) {
-        for (int i = 0; i < S::ST; i++) { mbar_init(&kfull[i], T::SPLIT ? TC_LOAD : 1); mbar_init(&vfull[i], TC_LOAD); mbar_init(&vraw[i], 1); mbar_init(&kempty[i], 1); mbar_init(&vempty[i], 1); }
-        for (int i = 0; i < S::UNITS; i++) { mbar_init(&rfull[i], 1); mbar_init(&rempty[i], TC_LOAD); }
-        mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1); mbar_init(&pready, TC_SOFT); mbar_init(&dfull, 1); mbar_init(&qfull, TC_SOFT);
-        mbar_fence_init();
-    }
     if (warp == TC_ISSUE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    tree_rows(a, b, e, see);
+    const uint32_t base0 = smem_u32(tsm);
+    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh), *vc = (const typename T::Val *)kv.v + kv.head(e.seq, kvh);
+    const int end = e.len + e.count;
+    int from = 0, tiles = 0;
+    auto share = [&](int first) {          // this CTA's tiles
+        const int s0 = first / N, all = (end + N - 1) / N - s0, chunk = (all + gridDim.x - 1) / gridDim.x;
+        from = s0 + blockIdx.x * chunk;
+        tiles = max(0, min(chunk, s0 + all - from));
+    };
+    TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
+    // copies, from half operand (f32) or tile (bf16) u0 to u1
+    auto bring = [&](int u0, int u1) {
+        if constexpr (T::SPLIT) {
+            // the ring, half a tile's rows to a copy (rows behind the end are not read)
+            for (int u = u0; u < u1; u++) {
+                const Half x = half_of(u, tiles);
+                const int slot = u % S::UNITS, t = (from + x.tile) * N + x.second * S::UROWS, rows = max(0, min(S::UROWS, end - t));
+                if (u >= S::UNITS) wait(&rempty[slot], ((u / S::UNITS) & 1) ^ 1);
+                if (rows) {
+                    mbar_expect_tx(&rfull[slot], rows * HD * 4);
+                    bulk_g2s(tsm + S::RAW + slot * S::UNIT, (x.val ? vc : kc) + (long long)t * HD, rows * HD * 4, &rfull[slot]);
+                } else {
+                    mbar_arrive(&rfull[slot]);
+                }
+            }
+        } else {
+            // a tile's keys and values (slots behind the end come along: nobody sees them)
+            for (int i = u0; i < u1; i++) {
+                const int st = i % S::ST, t = (from + i) * N;
+                if (i >= S::ST) wait(&kempty[st], (i / S::ST - 1) & 1);
+                mbar_expect_tx(&kfull[st], S::PLANE);
+                for (int x = 0; x < HD; x += 64) tensor_rows(base0 + S::K + st * S::STAGE + x * N * 2, &maps.k, x, t, kvh, e.seq, &kfull[st]);
+                if (i >= S::ST) wait(&vempty[st], (i / S::ST - 1) & 1);
+                mbar_expect_tx(&vraw[st], S::PLANE);
+                for (int x = 0; x < HD; x += 64) tensor_rows(base0 + S::V + st * S::STAGE + x * N * 2, &maps.v, x, t, kvh, e.seq, &vraw[st]);
+            }
+        }
+    };
+    const int room = T::SPLIT ? S::UNITS : S::ST;
+    int brought = 0;
+    if (tid == TC_BULK * 32) {
+        for (int i = 0; i < S::ST; i++) { mbar_init(&kfull[i], T::SPLIT ? TC_LOAD : 1); mbar_init(&vfull[i], TC_LOAD); mbar_init(&vraw[i], 1); mbar_init(&kempty[i], 1); mbar_init(&vempty[i], 1); }
+        for (int i = 0; i < S::UNITS; i++) { mbar_init(&rfull[i], 1); mbar_init(&rempty[i], TC_LOAD); }
+        mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1); mbar_init(&pready, TC_SOFT); mbar_init(&dfull, 1); mbar_init(&qfull, TC_SOFT);
+        mbar_fence_init();
+        if (a.window <= 0) {               // what there is room for, before the others are ready
+            share(0);
+            brought = min(room, T::SPLIT ? 4 * tiles : tiles);
+            bring(0, brought);
+        }
+    }
+    tree_rows(a, e, mine, see);
     tl_fence_before();
     __syncthreads();
     tl_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_sh, 0), base0 = smem_u32(tsm);
-    const int end = e.len + e.count, s0 = see.first / N, all = (end + N - 1) / N - s0, chunk = (all + gridDim.x - 1) / gridDim.x;
-    const int from = s0 + blockIdx.x * chunk, tiles = max(0, min(chunk, s0 + all - from));
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_sh, 0);
+    share(see.first);
     auto partial = [&](int i) { return (from + i) * N < see.full || (from + i + 1) * N > e.len; };
-    TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
-    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh), *vc = (const typename T::Val *)kv.v + kv.head(e.seq, kvh);
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)gridDim.x, rank = (int)blockIdx.x, each = owned_rows(TC_M, C);
     float *out = reinterpret_cast<float *>(tsm + S::K);
-    float2 *ml = reinterpret_cast<float2 *>(out + TC_M * S::OUT);
+    float2 *ml = reinterpret_cast<float2 *>(out + (TC_M + 15) * S::OUT);
 
     if (warp < TC_SOFT) {
         // ---------------- queries, softmax, output
@@ -316,11 +361,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
         asm volatile("bar.sync %0, 256;" ::"r"(9) : "memory");
         l += part_max[0][half ^ 1][r];
         const float m2 = m == -INFINITY ? m : m * c;
-        if (gridDim.x > 1) {
-            // keys and values are done with: their place takes the rows
-            if (half == 0) ml[r] = make_float2(m2, l);
+        if (C > 1) {
+            // nobody in the cluster uses keys and values any more: their place takes the parts of the rows that a CTA owns
+            cluster_arrive();
+            cluster_wait();
+            const int owner = r / each, at = rank * each + r % each;
+            if (half == 0) cl.map_shared_rank(ml, owner)[at] = make_float2(m2, l);
+            float *to = cl.map_shared_rank(out, owner) + at * S::OUT + half * (HD / 2);
 #pragma unroll
-            for (int d = 0; d < HD / 4; d += 2) *reinterpret_cast<ulonglong2 *>(out + r * S::OUT + half * (HD / 2) + 2 * d) = make_ulonglong2(o[d], o[d + 1]);
+            for (int d = 0; d < HD / 4; d += 2) *reinterpret_cast<ulonglong2 *>(to + 2 * d) = make_ulonglong2(o[d], o[d + 1]);
         } else if (node < e.count) {
             const float top = fmaxf(m2, sink), safe = top == -INFINITY ? 0.0f : top, w = exp2_approx(m2 - safe);
             l = __fmaf_rn(l, w, exp2_approx(sink - safe));
@@ -426,31 +475,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
             }
         }
     } else if (warp == TC_BULK) {
-        if (T::SPLIT && lane == 0) {
-            // ---------------- f32: the ring, half a tile's rows to a copy (rows behind the end are not read)
-            for (int u = 0; u < 4 * tiles; u++) {
-                const Half x = half_of(u, tiles);
-                const int slot = u % max(S::UNITS, 1), t = (from + x.tile) * N + x.second * S::UROWS, rows = max(0, min(S::UROWS, end - t));
-                if (u >= S::UNITS) wait(&rempty[slot], ((u / max(S::UNITS, 1)) & 1) ^ 1);
-                if (rows) {
-                    mbar_expect_tx(&rfull[slot], rows * HD * 4);
-                    bulk_g2s(tsm + S::RAW + slot * S::UNIT, (x.val ? vc : kc) + (long long)t * HD, rows * HD * 4, &rfull[slot]);
-                } else {
-                    mbar_arrive(&rfull[slot]);
-                }
-            }
-        } else if (!T::SPLIT && lane == 0) {
-            // ---------------- bf16: a tile's keys and values (slots behind the end come along: nobody sees them)
-            for (int i = 0; i < tiles; i++) {
-                const int st = i % S::ST, t = (from + i) * N;
-                if (i >= S::ST) wait(&kempty[st], (i / S::ST - 1) & 1);
-                mbar_expect_tx(&kfull[st], S::PLANE);
-                for (int x = 0; x < HD; x += 64) tensor_rows(base0 + S::K + st * S::STAGE + x * N * 2, &maps.k, x, t, kvh, e.seq, &kfull[st]);
-                if (i >= S::ST) wait(&vempty[st], (i / S::ST - 1) & 1);
-                mbar_expect_tx(&vraw[st], S::PLANE);
-                for (int x = 0; x < HD; x += 64) tensor_rows(base0 + S::V + st * S::STAGE + x * N * 2, &maps.v, x, t, kvh, e.seq, &vraw[st]);
-            }
-        }
+        // ---------------- copies
+        if (lane == 0) bring(brought, T::SPLIT ? 4 * tiles : tiles);
         __syncwarp();
     } else {
         // ---------------- products (the whole warp walks the loop, an elected lane issues)
@@ -505,16 +531,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
             }
         }
     }
+    if (C > 1 && warp >= TC_SOFT) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
     tl_fence_before();
     __syncthreads();
     if (warp == TC_ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    if (gridDim.x == 1) return;
-    join_parts<HD, S::OUT, TC_M>(out, ml, 1, a.out, a.lse,
-                           [&](int r) -> long long {
-                               const int i = (row0 + r) / per;
-                               return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
-                           },
-                           [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
+    if (C == 1) return;
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    join_rows<HD, S::OUT>(out, ml, C, each, a.out, a.lse,
+                          [&](int i) -> long long {
+                              const int r = rank * each + i, node = (row0 + r) / per;
+                              return r < TC_M && node < e.count ? ((long long)b * a.rows + node) * a.nh + kvh * per + (row0 + r) % per : -1;
+                          },
+                          [&](int i) { return a.sinks ? a.sinks[kvh * per + (row0 + rank * each + i) % per] * LOG2E : -INFINITY; });
 }
 
 template <class T, int HD>
