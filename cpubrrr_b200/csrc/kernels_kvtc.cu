@@ -23,17 +23,19 @@ namespace brrr {
 
 namespace {
 
-constexpr int TC_SOFT = 8, TC_LOAD = 4, TC_ISSUE = TC_SOFT + TC_LOAD, TC_BULK = TC_ISSUE + 1, TC_THREADS = (TC_BULK + 1) * 32, TC_M = 128;
+constexpr int TC_SOFT = 8, TC_M = 128;
 
 template <class T, int HD>
 struct Tc {
+    // warps: softmax, then these, then one that issues and one that copies
+    static constexpr int LOAD = T::SPLIT ? 8 : 4, ISSUE = TC_SOFT + LOAD, BULK = ISSUE + 1, THREADS = T::SPLIT ? 640 : 448;
     static constexpr int N = HD == 64 ? 128 : 64;                      // slots of a tile: 8192 values of keys and of values each
     static constexpr int PL = T::SPLIT ? 3 : 1;                       // pieces of a cached value
     static constexpr int ST = T::SPLIT ? 1 : 4;                        // stages of operands
     static constexpr int NC = HD / 8;                                  // 16-byte pieces of a row
     static constexpr int PLANE = N * HD * 2, STAGE = PL * PLANE;
     static constexpr int QT = HD == 64 ? 2 : 3;                        // pieces of the queries in tensor memory
-    static constexpr int UNITS = T::SPLIT ? 6 : 0, UROWS = N / 2, UNIT = UROWS * HD * 4;      // ring of raw f32 rows: half a tile each
+    static constexpr int UNITS = T::SPLIT ? 3 : 0, UNIT = N * HD * 4;      // ring of raw f32 rows: a tile's keys or values each
     static constexpr int Q2 = 0, K = QT == 2 ? TC_M * HD * 2 : 0, V = K + ST * STAGE, RAW = V + ST * STAGE, BYTES = RAW + UNITS * UNIT;
     // above half of an SM's shared memory: one CTA per SM, since each takes all of tensor memory
     static constexpr size_t SMEM = BYTES > 118784 ? BYTES : 118784;
@@ -98,27 +100,24 @@ struct Products {
     static __device__ __forceinline__ constexpr int b(int p) { return B >> (4 * p) & 15; }
 };
 
-// The order in which halves of operands are made: keys of tiles 0 and 1, then values of tile i and keys of tile i + 2 in turn (the scores of tile i + 2 follow the
+// The order in which f32 operands are made: keys of tiles 0 and 1, then values of tile i and keys of tile i + 2 in turn (the scores of tile i + 2 follow the
 // outputs of tile i, before the values of tile i + 1 have room).
-struct Half {
-    int tile, second;
+struct Operand {
+    int tile;
     bool val;
 };
-__device__ __forceinline__ Half half_of(int u, int tiles) {
-    const int op = u >> 1, keys = min(op, (op + 2) >> 1);       // K0 K1 V0 K2 V1 K3 ...: operands 0, 1, 3, 5 ... are keys while there are any
-    Half h;
-    h.second = u & 1;
-    if (op < 2) {
-        h.val = tiles == 1 && op == 1;
-        h.tile = h.val ? 0 : op;
-    } else if (op < 2 * tiles - 1) {
-        h.val = !(op & 1);
-        h.tile = h.val ? (op - 2) >> 1 : keys;
-    } else {
-        h.val = true;
-        h.tile = tiles - 1;
+__device__ __forceinline__ Operand operand_of(int u, int tiles) {          // K0 K1 V0 K2 V1 K3 ... V
+    if (u < 2) return {tiles == 1 ? 0 : u, tiles == 1 && u == 1};
+    if (u >= 2 * tiles - 1) return {tiles - 1, true};
+    return u & 1 ? Operand{(u + 1) >> 1, false} : Operand{(u - 2) >> 1, true};
+}
+// Registers of a thread from here on, for the four warps of a group (f32: 640 threads of 96 at launch, 480 among the five groups: 2 x 144 + 2 x 72 + 48).
+template <bool ON, bool MORE, int R>
+__device__ __forceinline__ void tc_regs() {
+    if constexpr (ON) {
+        if constexpr (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
     }
-    return h;
 }
 // K and V of a bf16 cache as tensors [sequence][kv head][slot][dim], boxes of 64 dims x a tile's slots in rows of 128 swizzled bytes
 struct alignas(64) KvMaps {
@@ -136,7 +135,7 @@ __device__ __forceinline__ uint64_t desc_rows128(uint32_t at, uint32_t lbo) {
 
 // grid (C, kv heads x blocks of 128 rows, entries), clusters of C
 template <class T, int HD>
-__global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeArgs a, const __grid_constant__ KvMaps maps) {
+__global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv, TreeArgs a, const __grid_constant__ KvMaps maps) {
     typedef Tc<T, HD> S;
     typedef Products<S::PL> Pr;
     constexpr int N = S::N;
@@ -167,7 +166,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
         if (!e.ok && threadIdx.x == 0) kv_error(kv);
         return;
     }
-    if (warp == TC_ISSUE) {
+    if (warp == S::ISSUE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -181,13 +180,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
         tiles = max(0, min(chunk, s0 + all - from));
     };
     TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
-    // copies, from half operand (f32) or tile (bf16) u0 to u1
+    // copies, from operand (f32) or tile (bf16) u0 to u1
     auto bring = [&](int u0, int u1) {
         if constexpr (T::SPLIT) {
-            // the ring, half a tile's rows to a copy (rows behind the end are not read)
+            // the ring (rows behind the end are not read)
             for (int u = u0; u < u1; u++) {
-                const Half x = half_of(u, tiles);
-                const int slot = u % S::UNITS, t = (from + x.tile) * N + x.second * S::UROWS, rows = max(0, min(S::UROWS, end - t));
+                const Operand x = operand_of(u, tiles);
+                const int slot = u % S::UNITS, t = (from + x.tile) * N, rows = max(0, min(N, end - t));
                 if (u >= S::UNITS) wait(&rempty[slot], ((u / S::UNITS) & 1) ^ 1);
                 if (rows) {
                     mbar_expect_tx(&rfull[slot], rows * HD * 4);
@@ -211,14 +210,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
     };
     const int room = T::SPLIT ? S::UNITS : S::ST;
     int brought = 0;
-    if (tid == TC_BULK * 32) {
-        for (int i = 0; i < S::ST; i++) { mbar_init(&kfull[i], T::SPLIT ? TC_LOAD : 1); mbar_init(&vfull[i], TC_LOAD); mbar_init(&vraw[i], 1); mbar_init(&kempty[i], 1); mbar_init(&vempty[i], 1); }
-        for (int i = 0; i < S::UNITS; i++) { mbar_init(&rfull[i], 1); mbar_init(&rempty[i], TC_LOAD); }
+    if (tid == S::BULK * 32) {
+        for (int i = 0; i < S::ST; i++) { mbar_init(&kfull[i], T::SPLIT ? S::LOAD : 1); mbar_init(&vfull[i], S::LOAD); mbar_init(&vraw[i], 1); mbar_init(&kempty[i], 1); mbar_init(&vempty[i], 1); }
+        for (int i = 0; i < S::UNITS; i++) { mbar_init(&rfull[i], 1); mbar_init(&rempty[i], S::LOAD); }
         mbar_init(&sfull[0], 1); mbar_init(&sfull[1], 1); mbar_init(&pready, TC_SOFT); mbar_init(&dfull, 1); mbar_init(&qfull, TC_SOFT);
         mbar_fence_init();
         if (a.window <= 0) {               // what there is room for, before the others are ready
             share(0);
-            brought = min(room, T::SPLIT ? 4 * tiles : tiles);
+            brought = min(room, T::SPLIT ? 2 * tiles : tiles);
             bring(0, brought);
         }
     }
@@ -236,6 +235,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
 
     if (warp < TC_SOFT) {
         // ---------------- queries, softmax, output
+        tc_regs<T::SPLIT, true, 144>();
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
 #pragma unroll
@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
             for (int d = 0; d < HD / 4; d += 2) to[d / 2] = make_ulonglong2(tl_mul2(o[d], kk), tl_mul2(o[d + 1], kk));
             if (a.lse && half == 0) a.lse[place] = (top + log2f(l)) * LN2;
         }
-    } else if (warp < TC_ISSUE) {
+    } else if (warp < S::ISSUE) {
+        tc_regs<T::SPLIT, false, 72>();
         const int lw = warp - TC_SOFT, lt = tid - TC_SOFT * 32;
         auto arrive = [&](uint64_t *bar) {
             fence_proxy_async();
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
         // a clean slate for the slots of a tile that turn out to be no numbers
         auto clean = [&](int st) {
             if (lt < N / 32) bad[st][lt] = 0;
-            asm volatile("bar.sync %0, 128;" ::"r"(10) : "memory");
+            asm volatile("bar.sync %0, %1;" ::"r"(10), "n"(S::LOAD * 32) : "memory");
         };
         if constexpr (!T::SPLIT) {
             // ---------------- bf16: values have come; where a row may not see all of them, those that are no numbers become zeros
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
                 wait(&vraw[st], (i / S::ST) & 1);
                 if (partial(i)) {
                     clean(st);
-                    for (int u = lt; u < N * S::NC; u += TC_LOAD * 32) {
+                    for (int u = lt; u < N * S::NC; u += S::LOAD * 32) {
                         const int row = u / S::NC, c = u % S::NC;
                         const uint32_t at = base0 + S::V + st * S::STAGE + (c >> 3) * (N * 128) + row * 128 + ((c & 7) ^ (row & 7)) * 16;
                         float x[8];
@@ -417,117 +418,109 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
                 arrive(&vfull[st]);
             }
         } else {
-            // ---------------- f32: rows out of the ring, cut into pieces.  A thread walks along a row of its own, its neighbours' rows one piece (and by fours
-            // half a piece) ahead: reads and writes meet no bank conflicts
-            const int row = lane & 7, first = row >> 2 & 1;
-            for (int u = 0; u < 4 * tiles; u++) {                       // halves of operands in the ring's order
-                const Half x = half_of(u, tiles);
+            // ---------------- f32: rows out of the ring, cut into pieces.  A thread walks along a row of its own, four values at a time, its neighbours four
+            // values ahead: reads and writes meet no bank conflicts
+            const int row = lane & 7;
+            for (int u = 0; u < 2 * tiles; u++) {
+                const Operand x = operand_of(u, tiles);
                 const bool val = x.val, part = partial(x.tile);
-                const int i = x.tile, h = x.second;
-                if (!h && i > 0) wait(val ? &vempty[0] : &kempty[0], (i - 1) & 1);
-                if (!h && val && part) clean(0);
-                {
-                    const int slot = u % S::UNITS;
-                    wait(&rfull[slot], (u / S::UNITS) & 1);
-                    const uint32_t raw = base0 + S::RAW + slot * S::UNIT, dst = base0 + (val ? S::V : S::K);
-                    constexpr int ITEMS = S::UROWS * S::NC / (TC_LOAD * 32);      // pieces of a thread
+                const int i = x.tile, slot = u % S::UNITS, t0 = (from + i) * N;
+                if (i > 0) wait(val ? &vempty[0] : &kempty[0], (i - 1) & 1);
+                if (val && part) clean(0);
+                wait(&rfull[slot], (u / S::UNITS) & 1);
+                const uint32_t raw = base0 + S::RAW + slot * S::UNIT, dst = base0 + (val ? S::V : S::K);
+                constexpr int ITEMS = N * HD / 4 / (S::LOAD * 32);         // of four values
+                auto item = [&](int k, bool look) {
+                    // a warp: four groups of eight rows, its share of their pieces
+                    const int groups = N / 32, rg = lw % groups * 4 + (lane >> 3), c = (lw / groups * ITEMS + k + row + (lane >> 3)) & (HD / 4 - 1), rr = rg * 8 + row;
+                    const uint4 y = lds128(raw + (rr * HD + c * 4) * 4);
+                    f32x2 v[2] = {tl_pack2(y.x, y.y), tl_pack2(y.z, y.w)};
+                    if (look) {
+                        bool any = false;
 #pragma unroll
-                    for (int k = 0; k < ITEMS; k++) {
-                        // a warp: four groups of eight rows at a time (128 dimensions: each warp one group of the unit's four, by its lanes a quarter of the pieces)
-                        int rg, c;
-                        if (S::UROWS == 64) {
-                            rg = (lw & 1) * 4 + (lane >> 3);
-                            c = ((lw >> 1) * (S::NC / 2) + k + row) & (S::NC - 1);
-                        } else {
-                            rg = lane >> 3;
-                            c = (lw * (S::NC / 4) + k + row) & (S::NC - 1);
+                        for (int d = 0; d < 2; d++) any |= not_finite(__uint_as_float((uint32_t)v[d])) || not_finite(__uint_as_float((uint32_t)(v[d] >> 32)));
+                        if (t0 + rr >= end) v[0] = v[1] = 0ull;
+                        else if (val && any) {
+                            v[0] = v[1] = 0ull;
+                            atomicOr(&bad[0][rr >> 5], 1u << (rr & 31));
                         }
-                        const int rr = rg * 8 + row, t = (from + i) * N + h * S::UROWS + rr;
-                        const uint32_t src = raw + (rr * HD + c * 8) * 4;
-                        const uint4 y = lds128(src + first * 16), z = lds128(src + (first ^ 1) * 16);
-                        const bool there = t < end;
-                        f32x2 x[4];
-                        x[0] = tl_pack2(first ? z.x : y.x, first ? z.y : y.y); x[1] = tl_pack2(first ? z.z : y.z, first ? z.w : y.w);
-                        x[2] = tl_pack2(first ? y.x : z.x, first ? y.y : z.y); x[3] = tl_pack2(first ? y.z : z.z, first ? y.w : z.w);
-                        if (!there) x[0] = x[1] = x[2] = x[3] = 0ull;
-                        if (val && part) {
-                            bool any = false;
-#pragma unroll
-                            for (int d = 0; d < 4; d++) any |= not_finite(__uint_as_float((uint32_t)x[d])) || not_finite(__uint_as_float((uint32_t)(x[d] >> 32)));
-                            if (any) {
-                                x[0] = x[1] = x[2] = x[3] = 0ull;
-                                const int tr = h * S::UROWS + rr;
-                                atomicOr(&bad[0][tr >> 5], 1u << (tr & 31));
-                            }
-                        }
-                        uint32_t p[3][4];
-#pragma unroll
-                        for (int d = 0; d < 4; d++) cut2(x[d], p[0][d], p[1][d], p[2][d]);
-                        const int g8 = h * (S::UROWS / 8) + rg;
-                        const uint32_t at = dst + (val ? g8 * S::NC + c : c * (N / 8) + g8) * 128 + row * 16;
-#pragma unroll
-                        for (int d = 0; d < 3; d++) st_shared16(at + d * S::PLANE, p[d]);
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&rempty[slot]);
-                    if (h) arrive(val ? &vfull[0] : &kfull[0]);
+                    uint32_t p[3][2];
+#pragma unroll
+                    for (int d = 0; d < 2; d++) cut2(v[d], p[0][d], p[1][d], p[2][d]);
+                    const int piece = c >> 1;
+                    const uint32_t at = dst + (val ? rg * S::NC + piece : piece * (N / 8) + rg) * 128 + row * 16 + (c & 1) * 8;
+#pragma unroll
+                    for (int d = 0; d < 3; d++) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + d * S::PLANE), "r"(p[d][0]), "r"(p[d][1]) : "memory");
+                };
+                if (part) {
+                    for (int k = 0; k < ITEMS; k++) item(k, true);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < ITEMS; k++) item(k, false);
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&rempty[slot]);
+                arrive(val ? &vfull[0] : &kfull[0]);
             }
         }
-    } else if (warp == TC_BULK) {
-        // ---------------- copies
-        if (lane == 0) bring(brought, T::SPLIT ? 4 * tiles : tiles);
-        __syncwarp();
     } else {
-        // ---------------- products (the whole warp walks the loop, an elected lane issues)
-        const uint32_t issue = elect_one() ? 1u : 0u;
-        constexpr uint32_t types = (1u << 4) | (1u << 7) | (1u << 10) | ((TC_M >> 4) << 24);       // f32 += bf16 x bf16
-        constexpr uint32_t id_s = types | ((uint32_t)(N >> 3) << 17), id_o = types | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-        const uint64_t dq = tl_smem_desc(tsm + S::Q2, TC_M * 16, 128), dk = T::SPLIT ? tl_smem_desc(tsm + S::K, N * 16, 128) : desc_rows128(base0 + S::K, 16),
-                       dv = T::SPLIT ? tl_smem_desc(tsm + S::V, S::NC * 128, 128) : desc_rows128(base0 + S::V, N * 128);
-        wait(&qfull, 0);
-        auto scores = [&](int i) {
-            const int st = i % S::ST;
-            wait(&kfull[st], (i / S::ST) & 1);
-            tl_fence_after();
-            const uint32_t d = tmem + (i & 1) * S::BUF;
-            const uint64_t k0 = dk + (uint64_t)(st * S::STAGE / 16);
-#pragma unroll
-            for (int p = 0; p < Pr::N; p++)
-#pragma unroll
-                for (int s = 0; s < HD / 16; s++) {
-                    const uint64_t db = k0 + (uint64_t)((T::SPLIT ? Pr::b(p) * S::PLANE + s * 2 * N * 16 : s / 4 * N * 128 + s % 4 * 32) / 16);
-                    if (Pr::a(p) < S::QT) tc_mma_ts(issue, d, tmem + S::Q + Pr::a(p) * (HD / 2) + s * 8, db, id_s, p > 0 || s > 0);
-                    else tc_mma_ss(issue, d, dq + (uint64_t)(s * 2 * TC_M * 16 / 16), db, id_s, p > 0 || s > 0);
-                }
-            tl_commit_if(issue, &sfull[i & 1]);
-            tl_commit_if(issue, &kempty[st]);
+        tc_regs<T::SPLIT, false, 48>();
+        if (warp == S::BULK) {
+            // ---------------- copies
+            if (lane == 0) bring(brought, T::SPLIT ? 2 * tiles : tiles);
             __syncwarp();
-        };
-        if (tiles > 0) scores(0);
-        if (tiles > 1) scores(1);
-        for (int i = 0; i < tiles; i++) {
-            const int st = i % S::ST;
-            wait(&vfull[st], (i / S::ST) & 1);
-            wait(&pready, i & 1);
-            tl_fence_after();
-            const uint32_t p0 = tmem + (i & 1) * S::BUF;
-            const uint64_t v0 = dv + (uint64_t)(st * S::STAGE / 16);
+        } else if (warp == S::ISSUE) {
+            // ---------------- products (the whole warp walks the loop, an elected lane issues)
+            const uint32_t issue = elect_one() ? 1u : 0u;
+            constexpr uint32_t types = (1u << 4) | (1u << 7) | (1u << 10) | ((TC_M >> 4) << 24);       // f32 += bf16 x bf16
+            constexpr uint32_t id_s = types | ((uint32_t)(N >> 3) << 17), id_o = types | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+            const uint64_t dq = tl_smem_desc(tsm + S::Q2, TC_M * 16, 128), dk = T::SPLIT ? tl_smem_desc(tsm + S::K, N * 16, 128) : desc_rows128(base0 + S::K, 16),
+                           dv = T::SPLIT ? tl_smem_desc(tsm + S::V, S::NC * 128, 128) : desc_rows128(base0 + S::V, N * 128);
+            wait(&qfull, 0);
+            auto scores = [&](int i) {
+                const int st = i % S::ST;
+                wait(&kfull[st], (i / S::ST) & 1);
+                tl_fence_after();
+                const uint32_t d = tmem + (i & 1) * S::BUF;
+                const uint64_t k0 = dk + (uint64_t)(st * S::STAGE / 16);
 #pragma unroll
-            for (int p = 0; p < Pr::N; p++)
+                for (int p = 0; p < Pr::N; p++)
 #pragma unroll
-                for (int s = 0; s < N / 16; s++) {
-                    constexpr int per_half = N / 32;
-                    const int h = s / per_half, k = s % per_half;
-                    const uint32_t at = p0 + (Pr::a(p) < 2 ? h * (N / 2) + Pr::a(p) * (N / 4) : N + h * (N / 4)) + k * 8;
-                    tc_mma_ts(issue, tmem + S::D, at, v0 + (uint64_t)((T::SPLIT ? Pr::b(p) * S::PLANE + s * 2 * S::NC * 128 : s * 2048) / 16), id_o, p > 0 || s > 0);
+                    for (int s = 0; s < HD / 16; s++) {
+                        const uint64_t db = k0 + (uint64_t)((T::SPLIT ? Pr::b(p) * S::PLANE + s * 2 * N * 16 : s / 4 * N * 128 + s % 4 * 32) / 16);
+                        if (Pr::a(p) < S::QT) tc_mma_ts(issue, d, tmem + S::Q + Pr::a(p) * (HD / 2) + s * 8, db, id_s, p > 0 || s > 0);
+                        else tc_mma_ss(issue, d, dq + (uint64_t)(s * 2 * TC_M * 16 / 16), db, id_s, p > 0 || s > 0);
+                    }
+                tl_commit_if(issue, &sfull[i & 1]);
+                tl_commit_if(issue, &kempty[st]);
+                __syncwarp();
+            };
+            if (tiles > 0) scores(0);
+            if (tiles > 1) scores(1);
+            for (int i = 0; i < tiles; i++) {
+                const int st = i % S::ST;
+                wait(&vfull[st], (i / S::ST) & 1);
+                wait(&pready, i & 1);
+                tl_fence_after();
+                const uint32_t p0 = tmem + (i & 1) * S::BUF;
+                const uint64_t v0 = dv + (uint64_t)(st * S::STAGE / 16);
+#pragma unroll
+                for (int p = 0; p < Pr::N; p++)
+#pragma unroll
+                    for (int s = 0; s < N / 16; s++) {
+                        constexpr int per_half = N / 32;
+                        const int h = s / per_half, k = s % per_half;
+                        const uint32_t at = p0 + (Pr::a(p) < 2 ? h * (N / 2) + Pr::a(p) * (N / 4) : N + h * (N / 4)) + k * 8;
+                        tc_mma_ts(issue, tmem + S::D, at, v0 + (uint64_t)((T::SPLIT ? Pr::b(p) * S::PLANE + s * 2 * S::NC * 128 : s * 2048) / 16), id_o, p > 0 || s > 0);
+                    }
+                tl_commit_if(issue, &dfull);
+                tl_commit_if(issue, &vempty[st]);
+                __syncwarp();
+                if (i + 2 < tiles) {
+                    wait(&dfull, i & 1);             // the weights of tile i stand where its scores go
+                    scores(i + 2);
                 }
-            tl_commit_if(issue, &dfull);
-            tl_commit_if(issue, &vempty[st]);
-            __syncwarp();
-            if (i + 2 < tiles) {
-                wait(&dfull, i & 1);             // the weights of tile i stand where its scores go
-                scores(i + 2);
             }
         }
     }
@@ -538,7 +531,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tree_tc_kernel(KvDev kv, TreeAr
     }
     tl_fence_before();
     __syncthreads();
-    if (warp == TC_ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == S::ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     if (C == 1) return;
     __syncwarp();
     cluster_arrive();
@@ -570,9 +563,9 @@ cudaError_t launch_tree_tc_as(const KvDev &kv, const TreeArgs &a, int slots, cud
     constexpr auto K = tree_tc_kernel<T, HD>;
     constexpr size_t smem = S::SMEM + 1024;
     cudaError_t e = cudaSuccess;
-    const int c = cluster_size<K>((long long)a.n * kv.nkv * blocks, (slots + S::N - 1) / S::N, 1, 4, TC_THREADS, smem, smem, &e);
+    const int c = cluster_size<K>((long long)a.n * kv.nkv * blocks, (slots + S::N - 1) / S::N, 1, 4, S::THREADS, smem, smem, &e);
     if (e != cudaSuccess) return e;
-    return launch_cluster<K>(dim3(c, kv.nkv * blocks, a.n), TC_THREADS, c, smem, smem, st, kv, a, maps);
+    return launch_cluster<K>(dim3(c, kv.nkv * blocks, a.n), S::THREADS, c, smem, smem, st, kv, a, maps);
 }
 
 }  // namespace
