@@ -104,6 +104,7 @@ cudaError_t launch_kv_evict(const KvDev &kv, const KvDev *dst, int n, const int3
 cudaError_t launch_kv_means(const KvDev &kv, int n, const int32_t *seq, const int32_t *since, const int32_t *len, int block, int len_hint, float *means, cudaStream_t st);
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st);
 cudaError_t launch_tree_tc(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st);      // kernels_kvtc.cu; slots: about as many per entry
+cudaError_t launch_weigh_tc(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int slots, cudaStream_t st);
 cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st);
 cudaError_t launch_attn_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,
                                int len_hint, const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *out, float *lse, cudaStream_t st);

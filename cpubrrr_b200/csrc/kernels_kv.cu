@@ -25,6 +25,8 @@ __device__ __forceinline__ void kv_store4(void *p, int type, long long at, float
 __global__ void kv_append_kernel(KvDev kv, int rows, const int32_t *seq, const int32_t *len, const int32_t *count, const int32_t *at,
                                  const float *__restrict__ qkv, long long ld, int nh, const float *__restrict__ rope, int n_rope, float *__restrict__ q) {
     const int i = blockIdx.x, b = blockIdx.y, half = kv.hd / 2, per = half / 4;
+    pdl_wait();
+    pdl_trigger();
     const KvEntry e = kv_entry(kv, b, rows, seq, len, count);
     if (kv_named_before(seq, b) || !e.ok) {
         if (threadIdx.x == 0) kv_error(kv);
@@ -70,8 +72,7 @@ __global__ void kv_append_kernel(KvDev kv, int rows, const int32_t *seq, const i
 
 cudaError_t launch_kv_append(const KvDev &kv, int n, int rows, const int32_t *seq, const int32_t *len, const int32_t *count, const int32_t *at, const float *qkv,
                              long long ld, int nh, const float *rope, int n_rope, float *q, cudaStream_t st) {
-    kv_append_kernel<<<dim3(rows, n), 512, 0, st>>>(kv, rows, seq, len, count, at, qkv, ld, nh, rope, n_rope, q);
-    return cudaGetLastError();
+    return launch_k(kv_append_kernel, dim3(rows, n), dim3(512), 0, st, true, kv, rows, seq, len, count, at, qkv, ld, nh, rope, n_rope, q);
 }
 
 // ---------------------------------------------------------------- commit
@@ -80,6 +81,8 @@ constexpr int CM_THREADS = 256;
 __global__ void __launch_bounds__(CM_THREADS) kv_commit_kernel(KvDev kv, int rows, const int32_t *seq, const int32_t *len, const int32_t *path, const int32_t *npath,
                                                                int32_t *new_len) {
     const int kvh = blockIdx.x, b = blockIdx.y;
+    pdl_wait();
+    pdl_trigger();
     const KvEntry e = kv_entry(kv, b, rows, seq, len, npath);
     bool bad = kv_named_before(seq, b) || !e.ok;
     if (!bad) {
@@ -123,8 +126,7 @@ __global__ void __launch_bounds__(CM_THREADS) kv_commit_kernel(KvDev kv, int row
 
 cudaError_t launch_kv_commit(const KvDev &kv, int n, int rows, const int32_t *seq, const int32_t *len, const int32_t *path, const int32_t *npath, int32_t *new_len,
                              cudaStream_t st) {
-    kv_commit_kernel<<<dim3(kv.nkv, n, 2), CM_THREADS, 0, st>>>(kv, rows, seq, len, path, npath, new_len);
-    return cudaGetLastError();
+    return launch_k(kv_commit_kernel, dim3(kv.nkv, n, 2), dim3(CM_THREADS), 0, st, true, kv, rows, seq, len, path, npath, new_len);
 }
 
 // ---------------------------------------------------------------- eviction
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
                                                               const int32_t *end, int32_t *map, int32_t *new_len) {
     extern __shared__ uint32_t sm[];
     __shared__ KthSpace kth;
-    pdl_trigger();
+    pdl_wait();
     const int kvh = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = EV_THREADS / 32;
     const KvEntry e = kv_entry(kv, b, 0, seq, len, nullptr);
     const bool bad = kv_named_before(seq, b) || !e.ok || e.seq >= dst.n_seq;
@@ -222,6 +224,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
         if (lane == 0) kept[i] |= mine;
     }
     __syncthreads();
+    pdl_trigger();
     // freed slots below m per word 0 .. mw, then kept ones behind per word mw .. words - 1 (one place further on)
     const uint32_t low = (1u << (m & 31)) - 1;
     for (int i = threadIdx.x; i <= words; i += EV_THREADS) {
@@ -253,6 +256,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
 constexpr int MV_BATCH = 4;
 __global__ void __launch_bounds__(256) kv_move_kernel(KvDev kv, KvDev dst, bool inplace, const int32_t *seq, int keep, const int32_t *map) {
     const int kvh = blockIdx.y, b = blockIdx.z, per = kv.hd * kv.size() / 16;       // a power of two
+    pdl_wait();
     const int s = seq ? seq[b] : b;
     if ((unsigned)s >= (unsigned)kv.n_seq || s >= dst.n_seq) return;
     const int32_t *from = map + ((long long)b * kv.nkv + kvh) * keep;
@@ -260,7 +264,6 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvDev kv, KvDev dst, bool 
     uint4 *k2 = reinterpret_cast<uint4 *>((char *)dst.k + dst.head(s, kvh) * dst.size()), *v2 = reinterpret_cast<uint4 *>((char *)dst.v + dst.head(s, kvh) * dst.size());
     const long long book = kv.book(s, kvh), book2 = dst.book(s, kvh);
     const int c = threadIdx.x % per, rows = 256 / per, d0 = blockIdx.x * rows * MV_BATCH + threadIdx.x / per;
-    pdl_wait();
     int t[MV_BATCH];
     uint4 x[MV_BATCH], y[MV_BATCH];
 #pragma unroll
@@ -291,8 +294,7 @@ cudaError_t launch_kv_evict(const KvDev &kv, const KvDev *dst, int n, const int3
     auto kern = keys ? kv_evict_kernel<true> : kv_evict_kernel<false>;
     cudaError_t e = smem > 36 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) : cudaSuccess;
     if (e != cudaSuccess) return e;
-    kern<<<dim3(kv.nkv, n), EV_THREADS, smem, st>>>(kv, to, seq, len, keep, first, recent, end, map, new_len);
-    e = cudaGetLastError();
+    e = launch_k(kern, dim3(kv.nkv, n), dim3(EV_THREADS), smem, st, true, kv, to, seq, len, keep, first, recent, end, map, new_len);
     if (e != cudaSuccess) return e;
     const int rows = 256 / (kv.hd * kv.size() / 16) * MV_BATCH;
     return launch_k(kv_move_kernel, dim3((keep + rows - 1) / rows, kv.nkv, n), dim3(256), 0, st, true, kv, to, dst == nullptr, seq, keep, (const int32_t *)map);
@@ -303,6 +305,8 @@ cudaError_t launch_kv_evict(const KvDev &kv, const KvDev *dst, int n, const int3
 __global__ void __launch_bounds__(256) kv_means_kernel(KvDev kv, const int32_t *seq, const int32_t *since, const int32_t *len, int block, float *__restrict__ means) {
     __shared__ double part[256 * 4];
     const int kvh = blockIdx.y, b = blockIdx.z;
+    pdl_wait();
+    pdl_trigger();
     const KvEntry e = kv_entry(kv, b, 0, seq, len, nullptr);
     const int s0 = since ? since[b] : 0;
     if (kv_named_before(seq, b) || !e.ok || s0 < 0) {
@@ -340,8 +344,7 @@ __global__ void __launch_bounds__(256) kv_means_kernel(KvDev kv, const int32_t *
 
 cudaError_t launch_kv_means(const KvDev &kv, int n, const int32_t *seq, const int32_t *since, const int32_t *len, int block, int len_hint, float *means, cudaStream_t st) {
     const int blocks = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) / block + 1;
-    kv_means_kernel<<<dim3(min(blocks, 4096), kv.nkv, n), 256, 0, st>>>(kv, seq, since, len, block, means);
-    return cudaGetLastError();
+    return launch_k(kv_means_kernel, dim3(min(blocks, 4096), kv.nkv, n), dim3(256), 0, st, true, kv, seq, since, len, block, means);
 }
 
 }  // namespace brrr

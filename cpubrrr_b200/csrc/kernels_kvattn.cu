@@ -289,8 +289,10 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) tree_kernel(KvDev k
     extern __shared__ __align__(16) float4 frag[];          // the queries, then the parts: out [AW][R][HD], ml [AW][R]; behind them the owner's parts
     __shared__ TreeRows see;
     const int per = a.nh / kv.nkv, kvh = blockIdx.y, b = blockIdx.z;
-    const uint64_t mine = tree_mask(a, b);
     if (gridDim.x > 1) cluster_arrive();
+    pdl_wait();
+    pdl_trigger();
+    const uint64_t mine = tree_mask(a, b);
     const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
     if (!e.ok || e.count == 0) {
         if (!e.ok && threadIdx.x == 0) kv_error(kv);
@@ -393,6 +395,8 @@ __global__ void __launch_bounds__(AW * 32) weigh_kernel(KvDev kv, TreeArgs a, co
     __shared__ TreeRows see;
     __shared__ float lse[R];
     const int kvh = blockIdx.y, b = blockIdx.z, per = a.nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    pdl_trigger();
     const uint64_t mine = tree_mask(a, b);
     const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
     if (kv_named_before(a.seq, b) || !e.ok) {
@@ -483,6 +487,9 @@ static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64
 }
 
 cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
+    int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
+    if (a.window > 0) slots = min(slots, a.window + a.rows);
+    if (a.rows * (a.nh / kv.nkv) > 16) return launch_weigh_tc(kv, a, picked, slots, st);
     if (kv.type) return kv.hd == 64 ? launch_weigh<KvBf16, 64, 2>(kv, a, picked, len_hint, st) : launch_weigh<KvBf16, 128, 2>(kv, a, picked, len_hint, st);
     return kv.hd == 64 ? launch_weigh<KvF32, 64, 2>(kv, a, picked, len_hint, st) : launch_weigh<KvF32, 128, 2>(kv, a, picked, len_hint, st);
 }
@@ -543,6 +550,8 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
     const int C = (int)cl.num_blocks();
     const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (C > 1) cluster_arrive();
+    pdl_wait();
+    pdl_trigger();
     const int s = seq ? seq[r] : r, n = len[r];
     if ((unsigned)s >= (unsigned)kv.n_seq || (unsigned)n > (unsigned)kv.cap) {
         if (threadIdx.x == 0) kv_error(kv);

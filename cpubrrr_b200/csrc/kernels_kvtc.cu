@@ -19,6 +19,8 @@
 #include "brrr_tc.cuh"
 #include "brrr_tmap.h"
 
+#include <algorithm>
+
 namespace brrr {
 
 namespace {
@@ -133,6 +135,96 @@ __device__ __forceinline__ uint64_t desc_rows128(uint32_t at, uint32_t lbo) {
     return (uint64_t)((at >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 | (uint64_t)64 << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+// A thread's half of its row of queries as operand A: the first QT pieces into tensor memory at `at` (this warp's lanes), a third that has no room there into
+// core matrices in shared memory at q2 (row r).  Complete for the tensor cores after the fences that the caller makes.
+template <int HD, int QT>
+__device__ __forceinline__ void stage_pieces(const float4 (&qx)[HD / 8], bool negative, uint32_t at, uint32_t q2, int half, int r) {
+    const uint32_t flip = negative ? 0x80008000u : 0;
+#pragma unroll
+    for (int i = 0; i < HD / 8; i += 8) {
+        uint32_t p[3][16];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            cut2(pack2(qx[i + j].x, qx[i + j].y), p[0][2 * j], p[1][2 * j], p[2][2 * j]);
+            cut2(pack2(qx[i + j].z, qx[i + j].w), p[0][2 * j + 1], p[1][2 * j + 1], p[2][2 * j + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) p[k][j] ^= flip;
+            if (k < QT) tc_st16(at + k * (HD / 2) + half * (HD / 4) + i * 2, p[k]);
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t v[4] = {p[k][4 * j], p[k][4 * j + 1], p[k][4 * j + 2], p[k][4 * j + 3]};
+                    st_shared16(q2 + ((half * (HD / 16) + i / 2 + j) * (TC_M / 8) + (r >> 3)) * 128 + (r & 7) * 16, v);
+                }
+        }
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    fence_proxy_async();
+    tl_fence_before();
+}
+
+// Which of the slots t0 .. t0 + 63 a row sees that sees cached slots from lo on and the drafted ones of its mask.
+__device__ __forceinline__ uint64_t slots_seen(uint64_t mask, int lo, int len, int t0) {
+    auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
+    const int d = len - t0;                                    // where the drafted ones begin
+    return (below(d) & ~below(lo - t0)) | (d >= 64 || d <= -64 ? 0ull : d >= 0 ? mask << d : mask >> -d);
+}
+
+// One warp's share (lw of eight) of a tile of f32 rows: out of the ring, cut into pieces, into the planes of an operand (values: MN-major).  A thread walks along a
+// row of its own, four values at a time, its neighbours four values ahead: reads and writes meet no bank conflicts.  look: rows from `rows` on are zeros, and values
+// that are no numbers become zeros and are noted in bad (keys: they stay).
+template <int HD, int N>
+__device__ __forceinline__ void cut_tile(uint32_t raw, uint32_t dst, int lw, bool val, bool look, int rows, uint32_t *bad) {
+    constexpr int ITEMS = N * HD / 4 / 256, GROUPS = N / 32, NC = HD / 8, PLANE = N * HD * 2;
+    const int lane = threadIdx.x & 31, row = lane & 7;
+    auto item = [&](int k) {
+        const int rg = lw % GROUPS * 4 + (lane >> 3), c = (lw / GROUPS * ITEMS + k + row + (lane >> 3)) & (HD / 4 - 1), rr = rg * 8 + row;
+        const uint4 y = lds128(raw + (rr * HD + c * 4) * 4);
+        f32x2 v[2] = {tl_pack2(y.x, y.y), tl_pack2(y.z, y.w)};
+        if (look) {
+            bool any = false;
+#pragma unroll
+            for (int d = 0; d < 2; d++) any |= not_finite(__uint_as_float((uint32_t)v[d])) || not_finite(__uint_as_float((uint32_t)(v[d] >> 32)));
+            if (rr >= rows) v[0] = v[1] = 0ull;
+            else if (val && any) {
+                v[0] = v[1] = 0ull;
+                atomicOr(&bad[rr >> 5], 1u << (rr & 31));
+            }
+        }
+        uint32_t p[3][2];
+#pragma unroll
+        for (int d = 0; d < 2; d++) cut2(v[d], p[0][d], p[1][d], p[2][d]);
+        const int piece = c >> 1;
+        const uint32_t at = dst + (val ? rg * NC + piece : piece * (N / 8) + rg) * 128 + row * 16 + (c & 1) * 8;
+#pragma unroll
+        for (int d = 0; d < 3; d++) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + d * PLANE), "r"(p[d][0]), "r"(p[d][1]) : "memory");
+    };
+    if (look) {
+        for (int k = 0; k < ITEMS; k++) item(k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++) item(k);
+    }
+}
+
+// The scores' products of a tile: queries (tensor memory qt, the piece behind in shared memory dq) against keys at k0, into column d.
+template <class T, int HD, int N, int QT>
+__device__ __forceinline__ void issue_scores(uint32_t issue, uint32_t d, uint32_t qt, uint64_t dq, uint64_t k0) {
+    typedef Products<T::SPLIT ? 3 : 1> Pr;
+    constexpr uint32_t id = (1u << 4) | (1u << 7) | (1u << 10) | ((TC_M >> 4) << 24) | ((uint32_t)(N >> 3) << 17);       // f32 += bf16 x bf16
+#pragma unroll
+    for (int p = 0; p < Pr::N; p++)
+#pragma unroll
+        for (int s = 0; s < HD / 16; s++) {
+            const uint64_t db = k0 + (uint64_t)((T::SPLIT ? Pr::b(p) * N * HD * 2 + s * 2 * N * 16 : s / 4 * N * 128 + s % 4 * 32) / 16);
+            if (Pr::a(p) < QT) tc_mma_ts(issue, d, qt + Pr::a(p) * (HD / 2) + s * 8, db, id, p > 0 || s > 0);
+            else tc_mma_ss(issue, d, dq + (uint64_t)(s * 2 * TC_M * 16 / 16), db, id, p > 0 || s > 0);
+        }
+}
+
 // grid (C, kv heads x blocks of 128 rows, entries), clusters of C
 template <class T, int HD>
 __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv, TreeArgs a, const __grid_constant__ KvMaps maps) {
@@ -152,6 +244,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
     // this thread's half of its row of queries and the row's sink, on their way before anything else is known
     const int quarter = warp & 3, half = warp >> 2 & 1, r = quarter * 32 + lane, node = (row0 + r) / per, head = kvh * per + (row0 + r) % per;
     const long long place = ((long long)b * a.rows + node) * a.nh + head;
+    pdl_wait();
     float4 qx[HD / 8];
     float sink = -INFINITY;
     if (warp < TC_SOFT) {
@@ -225,6 +318,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
     tl_fence_before();
     __syncthreads();
     tl_fence_after();
+    pdl_trigger();                 // not before this CTA holds its tensor memory: the next kernel's might wait for this one with it
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_sh, 0);
     share(see.first);
     auto partial = [&](int i) { return (from + i) * N < see.full || (from + i + 1) * N > e.len; };
@@ -237,42 +331,12 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
         // ---------------- queries, softmax, output
         tc_regs<T::SPLIT, true, 144>();
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0;
-#pragma unroll
-        for (int i = 0; i < HD / 8; i += 8) {
-            uint32_t p[3][16];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                cut2(pack2(qx[i + j].x, qx[i + j].y), p[0][2 * j], p[1][2 * j], p[2][2 * j]);
-                cut2(pack2(qx[i + j].z, qx[i + j].w), p[0][2 * j + 1], p[1][2 * j + 1], p[2][2 * j + 1]);
-            }
-#pragma unroll
-            for (int k = 0; k < 3; k++) {
-#pragma unroll
-                for (int j = 0; j < 16; j++) p[k][j] ^= flip;
-                if (k < S::QT) tc_st16(lanes + S::Q + k * (HD / 2) + half * (HD / 4) + i * 2, p[k]);
-                else
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t v[4] = {p[k][4 * j], p[k][4 * j + 1], p[k][4 * j + 2], p[k][4 * j + 3]};
-                        st_shared16(base0 + S::Q2 + ((half * (S::NC / 2) + i / 2 + j) * (TC_M / 8) + (r >> 3)) * 128 + (r & 7) * 16, v);
-                    }
-            }
-        }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        fence_proxy_async();
-        tl_fence_before();
+        stage_pieces<HD, S::QT>(qx, a.scale < 0.0f, lanes + S::Q, base0 + S::Q2, half, r);
         __syncwarp();
         if (lane == 0) mbar_arrive(&qfull);
         const uint64_t mask = node < e.count ? see.mask[node] : 0;
         const int lo = node < e.count ? see.lo[node] : 0x7fffffff;
         const bool idle = row0 + quarter * 32 >= e.count * per;         // a warp of padding
-        // which of the slots t0 .. t0 + 63 this row sees
-        auto sees = [&](int t0) {
-            auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
-            const int d = e.len - t0;                                    // where the drafted ones begin
-            return (below(d) & ~below(lo - t0)) | (d >= 64 || d <= -64 ? 0ull : d >= 0 ? mask << d : mask >> -d);
-        };
         const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);           // above zero: -infinity stays what it is
         const f32x2 cc = pack2(c, c);
         float m = -INFINITY, l = 0.0f, f = 1.0f;
@@ -304,7 +368,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
 #pragma unroll
                 for (int k = 0; k < N / 2; k += 32) tc_ld32(mine + k, s + k);
                 if (part) {
-                    const uint64_t seen = sees(t0);
+                    const uint64_t seen = slots_seen(mask, lo, e.len, t0);
 #pragma unroll
                     for (int k = 0; k < N / 2; k++)
                         if (!((uint32_t)(seen >> (k & 32)) >> (k & 31) & 1)) s[k] = -INFINITY;
@@ -348,7 +412,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
                 wait(&vfull[i % S::ST], (i / S::ST) & 1);
                 const uint32_t *g = &bad[i % S::ST][half * (N / 64)];
                 const uint64_t gone = N == 64 ? g[0] : g[0] | (uint64_t)g[N / 64 - 1] << 32;
-                if (gone & sees(t0)) l = NAN;
+                if (gone & slots_seen(mask, lo, e.len, t0)) l = NAN;
             }
             if (i > 0) join_output(i - 1);
             f = fn;
@@ -418,47 +482,17 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
                 arrive(&vfull[st]);
             }
         } else {
-            // ---------------- f32: rows out of the ring, cut into pieces.  A thread walks along a row of its own, four values at a time, its neighbours four
-            // values ahead: reads and writes meet no bank conflicts
-            const int row = lane & 7;
+            // ---------------- f32: rows out of the ring, cut into pieces
             for (int u = 0; u < 2 * tiles; u++) {
                 const Operand x = operand_of(u, tiles);
                 const bool val = x.val, part = partial(x.tile);
-                const int i = x.tile, slot = u % S::UNITS, t0 = (from + i) * N;
+                const int i = x.tile, slot = u % S::UNITS;
                 if (i > 0) wait(val ? &vempty[0] : &kempty[0], (i - 1) & 1);
                 if (val && part) clean(0);
                 wait(&rfull[slot], (u / S::UNITS) & 1);
                 const uint32_t raw = base0 + S::RAW + slot * S::UNIT, dst = base0 + (val ? S::V : S::K);
-                constexpr int ITEMS = N * HD / 4 / (S::LOAD * 32);         // of four values
-                auto item = [&](int k, bool look) {
-                    // a warp: four groups of eight rows, its share of their pieces
-                    const int groups = N / 32, rg = lw % groups * 4 + (lane >> 3), c = (lw / groups * ITEMS + k + row + (lane >> 3)) & (HD / 4 - 1), rr = rg * 8 + row;
-                    const uint4 y = lds128(raw + (rr * HD + c * 4) * 4);
-                    f32x2 v[2] = {tl_pack2(y.x, y.y), tl_pack2(y.z, y.w)};
-                    if (look) {
-                        bool any = false;
-#pragma unroll
-                        for (int d = 0; d < 2; d++) any |= not_finite(__uint_as_float((uint32_t)v[d])) || not_finite(__uint_as_float((uint32_t)(v[d] >> 32)));
-                        if (t0 + rr >= end) v[0] = v[1] = 0ull;
-                        else if (val && any) {
-                            v[0] = v[1] = 0ull;
-                            atomicOr(&bad[0][rr >> 5], 1u << (rr & 31));
-                        }
-                    }
-                    uint32_t p[3][2];
-#pragma unroll
-                    for (int d = 0; d < 2; d++) cut2(v[d], p[0][d], p[1][d], p[2][d]);
-                    const int piece = c >> 1;
-                    const uint32_t at = dst + (val ? rg * S::NC + piece : piece * (N / 8) + rg) * 128 + row * 16 + (c & 1) * 8;
-#pragma unroll
-                    for (int d = 0; d < 3; d++) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + d * S::PLANE), "r"(p[d][0]), "r"(p[d][1]) : "memory");
-                };
-                if (part) {
-                    for (int k = 0; k < ITEMS; k++) item(k, true);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < ITEMS; k++) item(k, false);
-                }
+                if (part) cut_tile<HD, N>(raw, dst, lw, val, true, end - (from + i) * N, bad[0]);
+                else cut_tile<HD, N>(raw, dst, lw, val, false, 0, nullptr);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&rempty[slot]);
                 arrive(val ? &vfull[0] : &kfull[0]);
@@ -474,7 +508,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
             // ---------------- products (the whole warp walks the loop, an elected lane issues)
             const uint32_t issue = elect_one() ? 1u : 0u;
             constexpr uint32_t types = (1u << 4) | (1u << 7) | (1u << 10) | ((TC_M >> 4) << 24);       // f32 += bf16 x bf16
-            constexpr uint32_t id_s = types | ((uint32_t)(N >> 3) << 17), id_o = types | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+            constexpr uint32_t id_o = types | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
             const uint64_t dq = tl_smem_desc(tsm + S::Q2, TC_M * 16, 128), dk = T::SPLIT ? tl_smem_desc(tsm + S::K, N * 16, 128) : desc_rows128(base0 + S::K, 16),
                            dv = T::SPLIT ? tl_smem_desc(tsm + S::V, S::NC * 128, 128) : desc_rows128(base0 + S::V, N * 128);
             wait(&qfull, 0);
@@ -482,16 +516,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
                 const int st = i % S::ST;
                 wait(&kfull[st], (i / S::ST) & 1);
                 tl_fence_after();
-                const uint32_t d = tmem + (i & 1) * S::BUF;
-                const uint64_t k0 = dk + (uint64_t)(st * S::STAGE / 16);
-#pragma unroll
-                for (int p = 0; p < Pr::N; p++)
-#pragma unroll
-                    for (int s = 0; s < HD / 16; s++) {
-                        const uint64_t db = k0 + (uint64_t)((T::SPLIT ? Pr::b(p) * S::PLANE + s * 2 * N * 16 : s / 4 * N * 128 + s % 4 * 32) / 16);
-                        if (Pr::a(p) < S::QT) tc_mma_ts(issue, d, tmem + S::Q + Pr::a(p) * (HD / 2) + s * 8, db, id_s, p > 0 || s > 0);
-                        else tc_mma_ss(issue, d, dq + (uint64_t)(s * 2 * TC_M * 16 / 16), db, id_s, p > 0 || s > 0);
-                    }
+                issue_scores<T, HD, N, S::QT>(issue, tmem + (i & 1) * S::BUF, tmem + S::Q, dq, dk + (uint64_t)(st * S::STAGE / 16));
                 tl_commit_if(issue, &sfull[i & 1]);
                 tl_commit_if(issue, &kempty[st]);
                 __syncwarp();
@@ -544,31 +569,218 @@ __global__ void __launch_bounds__(Tc<T, HD>::THREADS, 1) tree_tc_kernel(KvDev kv
                           [&](int i) { return a.sinks ? a.sinks[kvh * per + (row0 + rank * each + i) % per] * LOG2E : -INFINITY; });
 }
 
+// ---------------------------------------------------------------- book of weights
+// The same scores, 2^(score - lse) of each, and their sum over the rows of the lanes: halves change places in a butterfly, so that a sum of 64 columns over 32 lanes
+// takes 62 exchanges; four warps' sums meet in shared memory and go to the book by one thread per slot.  A CTA takes its tiles once for every 128
+// rows, in order.
+template <class T, int HD>
+struct Wc {
+    typedef Tc<T, HD> S;
+    static constexpr int N = S::N, CUT = T::SPLIT ? 8 : 0, ISSUE = TC_SOFT + CUT, BULK = ISSUE + 1, THREADS = (BULK + 1) * 32;
+    static constexpr int ST = T::SPLIT ? 1 : 4, UNITS = T::SPLIT ? 3 : 1;
+    static constexpr int K = S::K, RAW = K + ST * S::STAGE, BYTES = RAW + (T::SPLIT ? UNITS * S::UNIT : 0);
+    static constexpr size_t SMEM = BYTES > 118784 ? BYTES : 118784;
+    static constexpr uint32_t Q = 2 * N;                        // columns: scores twice, the queries
+};
+template <class T, int HD>
+__global__ void __launch_bounds__(Wc<T, HD>::THREADS, 1) weigh_tc_kernel(KvDev kv, TreeArgs a, const uint64_t *picked, const __grid_constant__ KvMaps maps) {
+    typedef Wc<T, HD> W;
+    typedef Tc<T, HD> S;
+    constexpr int N = W::N;
+    extern __shared__ unsigned char tsm_[];
+    unsigned char *tsm = tsm_ + ((1024u - (smem_u32(tsm_) & 1023u)) & 1023u);
+    __shared__ __align__(8) uint64_t kfull[W::ST], kempty[W::ST], sfull[2], sfree[2], qfull, rfull[W::UNITS], rempty[W::UNITS];
+    __shared__ TreeRows see;
+    __shared__ float part[2][4][N];
+    __shared__ uint32_t tmem_sh;
+    const int per = a.nh / kv.nkv, kvh = blockIdx.y, b = blockIdx.z;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    pdl_wait();
+    const uint64_t mine = tree_mask(a, b);
+    const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
+    if (kv_named_before(a.seq, b) || !e.ok) {
+        if (tid == 0) kv_error(kv);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < W::ST; i++) { mbar_init(&kfull[i], T::SPLIT ? W::CUT : 1); mbar_init(&kempty[i], 1); }
+        for (int i = 0; i < W::UNITS; i++) { mbar_init(&rfull[i], 1); mbar_init(&rempty[i], T::SPLIT ? W::CUT : 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(&sfull[i], 1); mbar_init(&sfree[i], TC_SOFT); }
+        mbar_init(&qfull, TC_SOFT);
+        mbar_fence_init();
+    }
+    if (warp == W::ISSUE) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tree_rows(a, e, mine, see);
+    tl_fence_before();
+    __syncthreads();
+    tl_fence_after();
+    pdl_trigger();                 // see tree_tc_kernel
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_sh, 0), base0 = smem_u32(tsm);
+    const int end = e.len + e.count, s0 = see.first / N, all = (end + N - 1) / N - s0, chunk = (all + gridDim.x - 1) / gridDim.x;
+    const int from = s0 + blockIdx.x * chunk, tiles = max(0, min(chunk, s0 + all - from)), blocks = (e.count * per + TC_M - 1) / TC_M, total = tiles * blocks;
+    TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
+    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh);
+
+    if (warp < TC_SOFT) {
+        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint64_t rows = picked ? picked[b] : ~0ull;
+        const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);
+        float *weight = kv.weight + kv.book(e.seq, kvh);
+        int j = 0;
+        for (int blk = 0; blk < blocks && tiles > 0; blk++) {
+            const int node = (blk * TC_M + r) / per;
+            const long long place = ((long long)b * a.rows + node) * a.nh + kvh * per + (blk * TC_M + r) % per;
+            {
+                // the products with the block's queries before are done: their last scores have been seen
+                float4 qx[HD / 8];
+                const float4 *p = reinterpret_cast<const float4 *>(a.q + place * HD + half * (HD / 2));
+#pragma unroll
+                for (int i = 0; i < HD / 8; i++) qx[i] = node < e.count ? p[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                stage_pieces<HD, S::QT>(qx, a.scale < 0.0f, lanes + W::Q, base0 + S::Q2, half, r);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&qfull);
+            }
+            const bool counts = node < e.count && (rows >> node & 1);
+            const uint64_t mask = counts ? see.mask[node] : 0;
+            const int lo = counts ? see.lo[node] : 0x7fffffff;
+            const float z = counts ? a.lse[place] * LOG2E : 0.0f;
+            const bool every = __all_sync(0xffffffffu, counts);
+            for (int i = 0; i < tiles; i++, j++) {
+                const int t0 = (from + i) * N;
+                const bool look = !every || t0 < see.full || t0 + N > e.len;
+                wait(&sfull[j & 1], (j >> 1) & 1);
+                tl_fence_after();
+                float s[N / 2];
+#pragma unroll
+                for (int k = 0; k < N / 2; k += 32) tc_ld32(lanes + (j & 1) * N + half * (N / 2) + k, s + k);
+                tl_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfree[j & 1]);
+                if (look) {
+                    const uint64_t seen = counts ? slots_seen(mask, lo, e.len, t0 + half * (N / 2)) : 0;
+#pragma unroll
+                    for (int k = 0; k < N / 2; k++)
+                        if (!((uint32_t)(seen >> (k & 32)) >> (k & 31) & 1)) s[k] = -INFINITY;
+                }
+#pragma unroll
+                for (int k = 0; k < N / 2; k++) s[k] = exp2_approx(__fmaf_rn(s[k], c, -z));
+#pragma unroll
+                for (int n = N / 4, o = 16; n > 0; n >>= 1, o >>= 1) {
+                    if (o == 0) break;
+                    const bool up = lane & o;
+#pragma unroll
+                    for (int k = 0; k < n; k++) {
+                        const float keep = up ? s[k + n] : s[k], give = up ? s[k] : s[k + n];
+                        s[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                    }
+                }
+                // 32 columns: one is left in a lane, 64: two
+                float *to = &part[j & 1][quarter][half * (N / 2)];
+                if (N == 64) to[lane] = s[0];
+                else *reinterpret_cast<float2 *>(to + 2 * lane) = make_float2(s[0], s[1]);
+                asm volatile("bar.sync %0, 256;" ::"r"(9) : "memory");
+                if (tid < N && t0 + tid < end) weight[t0 + tid] += (part[j & 1][0][tid] + part[j & 1][1][tid]) + (part[j & 1][2][tid] + part[j & 1][3][tid]);
+            }
+        }
+    } else if (T::SPLIT && warp < W::ISSUE) {
+        for (int j = 0; j < total; j++) {
+            const int t = (from + j % tiles) * N, slot = j % W::UNITS;
+            if (j > 0) wait(&kempty[0], (j - 1) & 1);
+            wait(&rfull[slot], (j / W::UNITS) & 1);
+            cut_tile<HD, N>(base0 + W::RAW + slot * S::UNIT, base0 + W::K, warp - TC_SOFT, false, t + N > end, end - t, nullptr);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&rempty[slot]);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kfull[0]);
+        }
+    } else if (warp == W::BULK) {
+        if (lane == 0)
+            for (int j = 0; j < total; j++) {
+                const int t = (from + j % tiles) * N;
+                if constexpr (T::SPLIT) {
+                    const int slot = j % W::UNITS, rows = min(N, end - t);
+                    if (j >= W::UNITS) wait(&rempty[slot], (j / W::UNITS - 1) & 1);
+                    mbar_expect_tx(&rfull[slot], rows * HD * 4);
+                    bulk_g2s(tsm + W::RAW + slot * S::UNIT, kc + (long long)t * HD, rows * HD * 4, &rfull[slot]);
+                } else {
+                    const int st = j % W::ST;
+                    if (j >= W::ST) wait(&kempty[st], (j / W::ST - 1) & 1);
+                    mbar_expect_tx(&kfull[st], S::PLANE);
+                    for (int x = 0; x < HD; x += 64) tensor_rows(base0 + W::K + st * S::STAGE + x * N * 2, &maps.k, x, t, kvh, e.seq, &kfull[st]);
+                }
+            }
+        __syncwarp();
+    } else if (warp == W::ISSUE) {
+        const uint32_t issue = elect_one() ? 1u : 0u;
+        const uint64_t dq = tl_smem_desc(tsm + S::Q2, TC_M * 16, 128), dk = T::SPLIT ? tl_smem_desc(tsm + W::K, N * 16, 128) : desc_rows128(base0 + W::K, 16);
+        for (int j = 0; j < total; j++) {
+            const int st = j % W::ST;
+            if (j % tiles == 0) wait(&qfull, (j / tiles) & 1);
+            if (j >= 2) wait(&sfree[j & 1], ((j >> 1) - 1) & 1);
+            wait(&kfull[st], (j / W::ST) & 1);
+            tl_fence_after();
+            issue_scores<T, HD, N, S::QT>(issue, tmem + (j & 1) * N, tmem + W::Q, dq, dk + (uint64_t)(st * S::STAGE / 16));
+            tl_commit_if(issue, &sfull[j & 1]);
+            tl_commit_if(issue, &kempty[st]);
+            __syncwarp();
+        }
+    }
+    tl_fence_before();
+    __syncthreads();
+    if (warp == W::ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// K and V of a bf16 cache for the tensor copies
+cudaError_t kv_maps(const KvDev &kv, int slots, KvMaps *m) {
+    const tmap_encode_t encode = tmap_encode();
+    if (!encode) return cudaErrorNotSupported;
+    const cuuint64_t dims[4] = {(cuuint64_t)kv.hd, (cuuint64_t)kv.cap, (cuuint64_t)kv.nkv, (cuuint64_t)kv.n_seq};
+    const cuuint64_t strides[3] = {(cuuint64_t)kv.hd * 2, (cuuint64_t)kv.hs * 2, (cuuint64_t)kv.ss * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)slots, 1, 1}, ones[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 2; i++)
+        if (encode(i ? &m->v : &m->k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? kv.v : kv.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    return cudaSuccess;
+}
+
 template <class T, int HD>
 cudaError_t launch_tree_tc_as(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
     typedef Tc<T, HD> S;
     const int blocks = (a.rows * (a.nh / kv.nkv) + TC_M - 1) / TC_M;
     KvMaps maps{};
-    if (!T::SPLIT) {
-        const tmap_encode_t encode = tmap_encode();
-        if (!encode) return cudaErrorNotSupported;
-        const cuuint64_t dims[4] = {(cuuint64_t)HD, (cuuint64_t)kv.cap, (cuuint64_t)kv.nkv, (cuuint64_t)kv.n_seq};
-        const cuuint64_t strides[3] = {HD * 2, (cuuint64_t)kv.hs * 2, (cuuint64_t)kv.ss * 2};
-        const cuuint32_t box[4] = {64, S::N, 1, 1}, ones[4] = {1, 1, 1, 1};
-        for (int i = 0; i < 2; i++)
-            if (encode(i ? &maps.v : &maps.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? kv.v : kv.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-                return cudaErrorInvalidValue;
-    }
+    cudaError_t e = T::SPLIT ? cudaSuccess : kv_maps(kv, S::N, &maps);
+    if (e != cudaSuccess) return e;
     constexpr auto K = tree_tc_kernel<T, HD>;
     constexpr size_t smem = S::SMEM + 1024;
-    cudaError_t e = cudaSuccess;
     const int c = cluster_size<K>((long long)a.n * kv.nkv * blocks, (slots + S::N - 1) / S::N, 1, 4, S::THREADS, smem, smem, &e);
     if (e != cudaSuccess) return e;
     return launch_cluster<K>(dim3(c, kv.nkv * blocks, a.n), S::THREADS, c, smem, smem, st, kv, a, maps);
 }
 
+template <class T, int HD>
+cudaError_t launch_weigh_tc_as(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int slots, cudaStream_t st) {
+    typedef Wc<T, HD> W;
+    KvMaps maps{};
+    const cudaError_t e = T::SPLIT ? cudaSuccess : kv_maps(kv, W::N, &maps);
+    if (e != cudaSuccess) return e;
+    // one wave of CTAs, while each has a tile
+    const int jobs = a.n * kv.nkv, tiles = (slots + W::N - 1) / W::N;
+    constexpr size_t smem = W::SMEM + 1024;
+    return launch_cluster<weigh_tc_kernel<T, HD>>(dim3(std::max(1, std::min(tiles, 148 / jobs)), kv.nkv, a.n), W::THREADS, 1, smem, smem, st, kv, a, picked, maps);
+}
+
 }  // namespace
+
+cudaError_t launch_weigh_tc(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int slots, cudaStream_t st) {
+    if (kv.type) return kv.hd == 64 ? launch_weigh_tc_as<KvBf16, 64>(kv, a, picked, slots, st) : launch_weigh_tc_as<KvBf16, 128>(kv, a, picked, slots, st);
+    return kv.hd == 64 ? launch_weigh_tc_as<KvF32, 64>(kv, a, picked, slots, st) : launch_weigh_tc_as<KvF32, 128>(kv, a, picked, slots, st);
+}
 
 cudaError_t launch_tree_tc(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
     if (kv.type) return kv.hd == 64 ? launch_tree_tc_as<KvBf16, 64>(kv, a, slots, st) : launch_tree_tc_as<KvBf16, 128>(kv, a, slots, st);
