@@ -158,7 +158,7 @@ static cudaError_t launch_cluster(dim3 grid, int threads, int cluster, size_t sm
 
 // CTAs (1..16) that share the steps of one of `jobs` pieces of work, `lanes` steps of a CTA going on at a time: the least time of all waves, where a
 // CTA's start and end cost about as much as `fixed` steps.  How many clusters of a size the GPU holds at once is asked for once per kernel, size and device.
-template <auto K>
+template <auto K, bool CLUSTER = true>
 static int cluster_size(long long jobs, int steps, int lanes, int fixed, int threads, size_t smem, size_t most, cudaError_t *err) {
     static std::atomic<int> room[64][17];
     int dev = 0;
@@ -167,26 +167,27 @@ static int cluster_size(long long jobs, int steps, int lanes, int fixed, int thr
     if (*err != cudaSuccess) return 1;
     int best = 1;
     double least = 0.0;
-    for (int c = 1; c <= 16; c++) {
-        int held = dev < 64 ? room[dev][c].load() : 0;
+    for (int c = 1; c <= 16; c++) {           // without clusters c CTAs take c of the places for one
+        const int c_room = CLUSTER ? c : 1;
+        int held = dev < 64 ? room[dev][c_room].load() : 0;
         if (!held) {
             cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(c);
+            cfg.gridDim = dim3(c_room);
             cfg.blockDim = dim3(threads);
             cfg.dynamicSmemBytes = smem;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = c;
+            attr[0].val.clusterDim.x = c_room;
             attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
             if (cudaOccupancyMaxActiveClusters(&held, K, &cfg) != cudaSuccess) { (void)cudaGetLastError(); held = 0; }
             held = held > 0 ? held : -1;
-            if (dev < 64) room[dev][c].store(held);
+            if (dev < 64) room[dev][c_room].store(held);
         }
         if (held < 0) continue;
         const int turns = (steps + c * lanes - 1) / (c * lanes);
-        const double t = (double)((jobs + held - 1) / held) * (turns + fixed);
+        const double t = (double)(CLUSTER ? (jobs + held - 1) / held : (jobs * c + held - 1) / held) * (turns + fixed);
         if (c == 1 || t < least) { best = c; least = t; }
         if (turns <= 1) break;
     }

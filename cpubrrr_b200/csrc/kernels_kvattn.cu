@@ -7,19 +7,21 @@
 // head_dim / 8 additions, a step's share of the output starts at zero and joins the running output by one fused multiply-add that also
 // rescales it to the new running maximum.
 //
-// Operand B comes from global memory straight into registers.  Its k index may be any order of the dimensions (keys) that operand A
-// has too, so a lane's k = t, t + 4 of consecutive products are the consecutive values of one 16-byte load; the accumulator of the scores, with keys 2t and
-// 2t + 1 in a lane, is operand A of the second product as it stands.  Queries are split once and wait in shared memory in fragment order.
+// Every warp has a ring of steps of its own in shared memory, filled by bulk copies of consecutive rows several steps ahead, and waits for nobody else.  The k
+// index of operand B may be any order of the dimensions (keys) that operand A has too, so a lane's k = t, t + 4 of consecutive products are the
+// consecutive values of one 16-byte read; the accumulator of the scores, with keys 2t and 2t + 1 in a lane, is operand A of the second product as it
+// stands.  Queries are split once and wait in shared memory in fragment order.
 //
 // The slots of an entry are split over the warps of a CTA and the CTAs of a cluster, each with its own maximum and sum; partial results meet
 // in shared memory, those of the cluster through distributed shared memory, in a fixed order: one launch, no workspace, no atomics.
 #include "brrr_kernels.h"
 #include "brrr_block.cuh"
 #include "brrr_kvattn.cuh"
+#include "brrr_tc.cuh"
 
 namespace brrr {
 
-constexpr int AW = 8;                       // warps of an attention CTA
+constexpr int AW = 4;                       // warps of an attention CTA; three CTAs on an SM
 
 __device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u); }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const float4 &a, float b0, float b1) {
@@ -29,38 +31,47 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const float4 &a, float b
 }
 
 
-// What a lane keeps of a step of 8 NK slots.  Keys: of slot 8 j + lane / 4 the values 4V c + V (lane % 4) ...  Values: of slots 8 j + 2 (lane % 4) and the next
-// the values 8V c + V (lane / 4) ...
-template <class T, int HD, int NK>
-struct KvStep {
-    static constexpr int NC = HD / (4 * T::V), NVC = HD / (8 * T::V);
-    uint4 k[NK][NC], v[NK][2][NVC];
-    // slots base .. base + 8 NK - 1, those from end on left out (zeros)
-    template <bool STREAM>
-    __device__ __forceinline__ void load_k(const typename T::Val *kc, int base, int end) {
-        const int lane = threadIdx.x & 31;
-#pragma unroll
-        for (int j = 0; j < NK; j++) {
-            const int t = base + 8 * j + (lane >> 2);
-            const typename T::Val *p = kc + (long long)t * HD + T::V * (lane & 3);
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-                k[j][c] = t < end ? (STREAM ? ldg_stream(p + 4 * T::V * c) : ldg_shared(p + 4 * T::V * c)) : make_uint4(0, 0, 0, 0);
+// A warp's ring: D steps of 8 NK slots, 16 KB in all, keys and (both) values of a step side by side.  Lane 0 copies.
+template <class T, int HD, int NK, bool BOTH>
+struct Ring {
+    static constexpr int STEP = 8 * NK, ROW = HD * (int)sizeof(typename T::Val), HALF = STEP * ROW, SLOT = HALF * (BOTH ? 2 : 1), D = 16384 / SLOT;
+    static constexpr int NC = HD / (4 * T::V), NVC = HD / (8 * T::V);       // 16-byte reads of a lane per slot: keys, values
+    static_assert(D >= 2 && D * SLOT == 16384, "");
+    uint32_t at;             // of the ring, in shared memory
+    uint64_t *full;          // [D]
+    __device__ __forceinline__ Ring(unsigned char *mem, uint64_t *bars) {
+        const int warp = threadIdx.x >> 5;
+        at = smem_u32(mem) + warp * 16384;
+        full = bars + warp * 8;
+        if ((threadIdx.x & 31) == 0) {
+            for (int i = 0; i < D; i++) mbar_init(&full[i], 1);
+            mbar_fence_init();
+        }
+        __syncwarp();
+    }
+    // step n of this warp: slots base .. base + 8 NK - 1, those from end on not read (their place keeps what it had)
+    __device__ __forceinline__ void bring(int n, const typename T::Val *kc, const typename T::Val *vc, int base, int end) {
+        if ((threadIdx.x & 31) == 0) {
+            const int i = n % D, bytes = min(STEP, end - base) * ROW;
+            uint64_t *bar = &full[i];
+            mbar_expect_tx(bar, BOTH ? 2 * bytes : bytes);
+            const uint32_t dst = at + i * SLOT;
+            copy(dst, kc + (long long)base * HD, bytes, bar);
+            if (BOTH) copy(dst + HALF, vc + (long long)base * HD, bytes, bar);
         }
     }
-    template <bool STREAM>
-    __device__ __forceinline__ void load_v(const typename T::Val *vc, int base, int end) {
+    __device__ __forceinline__ static void copy(uint32_t dst, const void *src, int bytes, uint64_t *bar) {
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+    }
+    __device__ __forceinline__ uint32_t step(int n) const { return at + n % D * SLOT; }
+    // this lane's 16 bytes c of the key of slot 8 j + lane / 4, and of the value of slot 8 j + 2 (lane % 4) + h
+    __device__ __forceinline__ static uint4 key(uint32_t st, int j, int c) {
         const int lane = threadIdx.x & 31;
-#pragma unroll
-        for (int j = 0; j < NK; j++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int t = base + 8 * j + 2 * (lane & 3) + h;
-                const typename T::Val *p = vc + (long long)t * HD + T::V * (lane >> 2);
-#pragma unroll
-                for (int c = 0; c < NVC; c++)
-                    v[j][h][c] = t < end ? (STREAM ? ldg_stream(p + 8 * T::V * c) : ldg_shared(p + 8 * T::V * c)) : make_uint4(0, 0, 0, 0);
-            }
+        return lds128(st + (8 * j + (lane >> 2)) * ROW + (lane & 3) * 16 + c * 64);
+    }
+    __device__ __forceinline__ static uint4 value(uint32_t st, int j, int h, int c) {
+        const int lane = threadIdx.x & 31;
+        return lds128(st + HALF + (8 * j + 2 * (lane & 3) + h) * ROW + (lane >> 2) * 16 + c * 128);
     }
 };
 
@@ -87,8 +98,8 @@ __device__ __forceinline__ void stage_queries(float4 *frag, int tiles, Row row) 
 }
 
 // Scores of a tile of rows against a step's slots: s[j] as the accumulator of slots 8 j .. 8 j + 7.
-template <class T, int HD, int NK>
-__device__ __forceinline__ void step_scores(const KvStep<T, HD, NK> &st, const float4 *frag, float (&s)[NK][4]) {
+template <class T, int HD, int NK, class R>
+__device__ __forceinline__ void step_scores(uint32_t st, const float4 *frag, float (&s)[NK][4]) {
     constexpr int P = T::V / 2;                 // products per load
     const int lane = threadIdx.x & 31;
     float lo1[NK][4], lo2[NK][4];
@@ -97,10 +108,10 @@ __device__ __forceinline__ void step_scores(const KvStep<T, HD, NK> &st, const f
 #pragma unroll
         for (int e = 0; e < 4; e++) s[j][e] = lo1[j][e] = lo2[j][e] = 0.0f;
 #pragma unroll
-    for (int c = 0; c < st.NC; c++) {
+    for (int c = 0; c < R::NC; c++) {
         float x[NK][T::V];
 #pragma unroll
-        for (int j = 0; j < NK; j++) T::get(st.k[j][c], x[j]);
+        for (int j = 0; j < NK; j++) T::get(R::key(st, j, c), x[j]);
 #pragma unroll
         for (int p = 0; p < P; p++) {
             const float4 ah = frag[(c * P + p) * 64 + lane], al = frag[(c * P + p) * 64 + 32 + lane];
@@ -127,7 +138,7 @@ __device__ __forceinline__ void step_scores(const KvStep<T, HD, NK> &st, const f
 
 // A warp's running attention of 16 rows: maxima and sums in powers of two of rows lane / 4 and lane / 4 + 8 (the sum: this lane's slots only), and
 // the outputs, o[8 c' + V..]: see finish.
-template <class T, int HD, int NK>
+template <class T, int HD, int NK, class Rg>
 struct Running {
     static constexpr int NN = HD / 8;           // 8 values wide products of the output
     float m[2], l[2], o[NN][4];
@@ -141,7 +152,7 @@ struct Running {
     }
     // s: scaled scores in powers of two, -infinity where a row does not see the slot.  partial: some row may not see some slot, whose values may be anything: a
     // value that is no number goes into the sum of the rows that see it, and no further.
-    __device__ __forceinline__ void add(KvStep<T, HD, NK> &st, float (&s)[NK][4], bool partial) {
+    __device__ __forceinline__ void add(uint32_t st, float (&s)[NK][4], bool partial) {
         float top[2] = {m[0], m[1]};
 #pragma unroll
         for (int j = 0; j < NK; j++) {
@@ -170,14 +181,11 @@ struct Running {
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int c = 0; c < st.NVC; c++) {
+                    for (int c = 0; c < Rg::NVC; c++) {
                         float x[T::V];
-                        T::get(st.v[j][h][c], x);
-                        bool any = false;
+                        T::get(Rg::value(st, j, h, c), x);
 #pragma unroll
-                        for (int i = 0; i < T::V; i++) any |= not_finite(x[i]);
-                        bad[h] |= any;
-                        if (any) st.v[j][h][c] = make_uint4(0, 0, 0, 0);
+                        for (int i = 0; i < T::V; i++) bad[h] |= not_finite(x[i]);
                     }
                 const uint32_t mine = 0x11111111u << (threadIdx.x & 3);
 #pragma unroll
@@ -194,7 +202,7 @@ struct Running {
             pl[j] = make_float4(p[0] - ph[j].x, p[2] - ph[j].y, p[1] - ph[j].z, p[3] - ph[j].w);
         }
 #pragma unroll
-        for (int c = 0; c < st.NVC; c++) {
+        for (int c = 0; c < Rg::NVC; c++) {
             float d[T::V][4];
 #pragma unroll
             for (int i = 0; i < T::V; i++)
@@ -203,8 +211,15 @@ struct Running {
 #pragma unroll
             for (int j = 0; j < NK; j++) {
                 float x0[T::V], x1[T::V];
-                T::get(st.v[j][0][c], x0);
-                T::get(st.v[j][1][c], x1);
+                T::get(Rg::value(st, j, 0, c), x0);
+                T::get(Rg::value(st, j, 1, c), x1);
+                if (partial) {
+#pragma unroll
+                    for (int i = 0; i < T::V; i++) {
+                        if (not_finite(x0[i])) x0[i] = 0.0f;
+                        if (not_finite(x1[i])) x1[i] = 0.0f;
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < T::V; i++) {
                     if (T::SPLIT) {
@@ -284,12 +299,16 @@ __device__ __forceinline__ void join_warps(float *out, float2 *ml, int parts, fl
 
 // grid (C, kv heads, entries), clusters of C
 template <class T, int HD, int NK>
-__global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) tree_kernel(KvDev kv, TreeArgs a) {
+__global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev kv, TreeArgs a) {
+    typedef Ring<T, HD, NK, true> Rg;
     constexpr int R = 16, STEP = 8 * NK;
-    extern __shared__ __align__(16) float4 frag[];          // the queries, then the parts: out [AW][R][HD], ml [AW][R]; behind them the owner's parts
+    extern __shared__ __align__(128) unsigned char asm_[];  // the warps' rings, later the parts: out [AW][R][HD], ml [AW][R]; the queries; the owner's parts
+    __shared__ __align__(8) uint64_t bars[AW * 8];
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * 16384);
     __shared__ TreeRows see;
     const int per = a.nh / kv.nkv, kvh = blockIdx.y, b = blockIdx.z;
     if (gridDim.x > 1) cluster_arrive();
+    Rg ring(asm_, bars);
     pdl_wait();
     pdl_trigger();
     const uint64_t mine = tree_mask(a, b);
@@ -307,15 +326,11 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) tree_kernel(KvDev k
         __syncthreads();
         s0 = see.first / STEP;
     }
-    // the CTA's steps, the warp's among them; the first is on its way while masks and queries are prepared
+    // the CTA's steps, the warp's among them; the first are on their way while masks and queries are prepared
     const int steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
-    const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps);
-    int s = from + warp;
-    KvStep<T, HD, NK> st;
-    if (s < to) {
-        st.template load_k<true>(kc, s * STEP, end);
-        st.template load_v<true>(vc, s * STEP, end);
-    }
+    const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps), count = max(0, (to - from - warp + AW - 1) / AW);
+    auto base_of = [&](int n) { return (from + warp + n * AW) * STEP; };
+    for (int n = 0; n < min(count, Rg::D); n++) ring.bring(n, kc, vc, base_of(n), end);
     if (a.window <= 0) tree_rows(a, e, mine, see);
     auto place = [&](int r) -> long long {
         const int i = r / per;
@@ -333,13 +348,15 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) tree_kernel(KvDev k
         lo[h] = i < e.count ? see.lo[i] : 0x7fffffff;
     }
     const float c = a.scale * LOG2E;
-    Running<T, HD, NK> run;
+    Running<T, HD, NK, Rg> run;
     run.clear();
-    for (; s < to; s += AW) {
-        const int base = s * STEP;
+    TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
+    for (int n = 0; n < count; n++) {
+        const int base = base_of(n);
+        const uint32_t st = ring.step(n);
+        wait(&ring.full[n % Rg::D], (n / Rg::D) & 1);
         float x[NK][4];
-        step_scores<T, HD, NK>(st, frag, x);
-        if (s + AW < to) st.template load_k<true>(kc, (s + AW) * STEP, end);
+        step_scores<T, HD, NK, Rg>(st, frag, x);
         const bool partial = base < see.full || base + STEP > e.len;
 #pragma unroll
         for (int j = 0; j < NK; j++)
@@ -353,19 +370,20 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) tree_kernel(KvDev k
                 }
             }
         run.add(st, x, partial);
-        if (s + AW < to) st.template load_v<true>(vc, (s + AW) * STEP, end);
+        __syncwarp();
+        if (n + Rg::D < count) ring.bring(n + Rg::D, kc, vc, base_of(n + Rg::D), end);
     }
-    __syncthreads();                 // the queries have been read
-    float *out = reinterpret_cast<float *>(frag), *got = out + AW * R * HD;
+    __syncthreads();                 // nobody reads the rings any more
+    float *out = reinterpret_cast<float *>(asm_), *got = reinterpret_cast<float *>(frag) + 32 * HD;
     float2 *gml = reinterpret_cast<float2 *>(got + 31 * HD), *ml = gml + 31;
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
     join_warps<HD>(out, ml, AW, got, gml, a.out, a.lse, place, [&](int r) { return a.sinks ? a.sinks[kvh * per + r % per] * LOG2E : -INFINITY; });
 }
 
-// bytes of a CTA's shared memory: the queries, later the parts, and the owner's parts
-__host__ __device__ constexpr size_t attn_smem(int hd) { return (size_t)(AW * 16 + 31) * (hd * 4 + 8); }
-static_assert(attn_smem(64) >= 64 * 128 && attn_smem(128) >= 128 * 128, "");
+// bytes of a CTA's shared memory: the rings (later the parts of the warps), the queries, the owner's parts
+__host__ __device__ constexpr size_t attn_smem(int hd) { return (size_t)AW * 16384 + hd * 128 + 31 * (hd * 4 + 8) + AW * 16 * 8; }
+static_assert(16 * 128 * 4 <= 16384, "a warp's part fits its ring");
 
 template <class T, int HD, int NK>
 static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
@@ -382,19 +400,21 @@ cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, c
     if (a.window > 0) slots = min(slots, a.window + a.rows);
     if (a.rows * (a.nh / kv.nkv) > 16) return launch_tree_tc(kv, a, slots, st);
     if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2>(kv, a, slots, st) : launch_tree<KvBf16, 128, 2>(kv, a, slots, st);
-    return kv.hd == 64 ? launch_tree<KvF32, 64, 1>(kv, a, slots, st) : launch_tree<KvF32, 128, 1>(kv, a, slots, st);
+    return kv.hd == 64 ? launch_tree<KvF32, 64, 2>(kv, a, slots, st) : launch_tree<KvF32, 128, 1>(kv, a, slots, st);
 }
 
 // ---------------------------------------------------------------- book of weights
-// A CTA per run of slots, kv head and entry; a warp owns a step of slots and takes the rows 16 WT at a time, whose queries wait in shared memory: every
-// slot's weight is formed and added by one warp in the order of the rows.
-template <class T, int HD, int NK, int WT>
-__global__ void __launch_bounds__(AW * 32) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked) {
-    constexpr int R = 16 * WT, STEP = 8 * NK;
-    extern __shared__ __align__(16) float4 frag[];
+// Up to 16 rows per kv head (more: kernels_kvtc.cu).  A warp owns a step of slots: the scores of its keys, their powers, the sum over the rows.
+template <class T, int HD, int NK>
+__global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked) {
+    typedef Ring<T, HD, NK, false> Rg;
+    constexpr int STEP = 8 * NK;
+    extern __shared__ __align__(128) unsigned char asm_[];       // the warps' rings, the queries
+    __shared__ __align__(8) uint64_t bars[AW * 8];
     __shared__ TreeRows see;
-    __shared__ float lse[R];
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * 16384);
     const int kvh = blockIdx.y, b = blockIdx.z, per = a.nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Rg ring(asm_, bars);
     pdl_wait();
     pdl_trigger();
     const uint64_t mine = tree_mask(a, b);
@@ -403,95 +423,108 @@ __global__ void __launch_bounds__(AW * 32) weigh_kernel(KvDev kv, TreeArgs a, co
         if (threadIdx.x == 0) kv_error(kv);
         return;
     }
-    tree_rows(a, e, mine, see);
-    __syncthreads();
-    const uint64_t rows = picked ? picked[b] : ~0ull;
-    const int end = e.len + e.count, steps = (end + STEP - 1) / STEP, s0 = see.first / STEP;
+    const int end = e.len + e.count;
     const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh);
     float *weight = kv.weight + kv.book(e.seq, kvh);
-    const float c = a.scale * LOG2E;
-    for (int row0 = 0; row0 < e.count * per; row0 += R) {
-        const int tiles = min(WT, (e.count * per - row0 + 15) / 16);
+    int s0 = 0;
+    if (a.window > 0) {
+        tree_rows(a, e, mine, see);
         __syncthreads();
-        stage_queries<T, HD>(frag, tiles, [&](int r) -> const float * {
-            const int i = (row0 + r) / per;
-            return i < e.count ? a.q + (((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per) * HD : nullptr;
-        });
-        for (int r = threadIdx.x; r < R; r += AW * 32) {
-            const int i = (row0 + r) / per;
-            // a row that does not count has an infinite sum: weights of zero
-            lse[r] = i < e.count && (rows >> i & 1) ? a.lse[((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per] * LOG2E : INFINITY;
-        }
-        __syncthreads();
-        const int hop = gridDim.x * AW;
-        int s = s0 + blockIdx.x * AW + warp;
-        KvStep<T, HD, NK> st;
-        if (s < steps) st.template load_k<WT == 1>(kc, s * STEP, end);
-        for (; s < steps; s += hop) {
-            const int base = s * STEP;
-            const bool partial = base < see.full || base + STEP > e.len;
-            float sum[NK][2];
+        s0 = see.first / STEP;
+    }
+    const int steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
+    const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps), count = max(0, (to - from - warp + AW - 1) / AW);
+    auto base_of = [&](int n) { return (from + warp + n * AW) * STEP; };
+    for (int n = 0; n < min(count, Rg::D); n++) ring.bring(n, kc, nullptr, base_of(n), end);
+    if (a.window <= 0) tree_rows(a, e, mine, see);
+    const uint64_t rows = picked ? picked[b] : ~0ull;
+    auto place = [&](int r) -> long long {
+        const int i = r / per;
+        return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + r % per : -1;
+    };
+    stage_queries<T, HD>(frag, 1, [&](int r) -> const float * { return place(r) >= 0 ? a.q + place(r) * HD : nullptr; });
+    // this lane's two rows; one that does not count sees nothing
+    bool counts[2];
+    float z[2];
 #pragma unroll
-            for (int j = 0; j < NK; j++) sum[j][0] = sum[j][1] = 0.0f;
-            for (int w = 0; w < tiles; w++) {
-                float x[NK][4];
-                step_scores<T, HD, NK>(st, frag + w * (HD / 8) * 64, x);
-                if (w == tiles - 1 && s + hop < steps) st.template load_k<WT == 1>(kc, (s + hop) * STEP, end);
+    for (int h = 0; h < 2; h++) {
+        const int r = (lane >> 2) + 8 * h, i = r / per;
+        counts[h] = i < e.count && (rows >> i & 1);
+        z[h] = counts[h] ? a.lse[place(r)] * LOG2E : 0.0f;
+    }
+    __syncthreads();
+    uint64_t mask[2];
+    int lo[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int i = ((lane >> 2) + 8 * h) / per;
+        mask[h] = counts[h] ? see.mask[i] : 0;
+        lo[h] = counts[h] ? see.lo[i] : 0x7fffffff;
+    }
+    const float c = a.scale * LOG2E;
+    TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
+    for (int n = 0; n < count; n++) {
+        const int base = base_of(n);
+        // the two slots of lane t < 4 per eight: what the book has
+        float2 had[NK];
+#pragma unroll
+        for (int j = 0; j < NK; j++) {
+            const int t = base + 8 * j + 2 * lane;
+            had[j] = make_float2(lane < 4 && t < end ? weight[t] : 0.0f, lane < 4 && t + 1 < end ? weight[t + 1] : 0.0f);
+        }
+        wait(&ring.full[n % Rg::D], (n / Rg::D) & 1);
+        float x[NK][4], sum[NK][2];
+        step_scores<T, HD, NK, Rg>(ring.step(n), frag, x);
+        __syncwarp();
+        if (n + Rg::D < count) ring.bring(n + Rg::D, kc, nullptr, base_of(n + Rg::D), end);
+        const bool partial = base < see.full || base + STEP > e.len;
+#pragma unroll
+        for (int j = 0; j < NK; j++) {
+#pragma unroll
+            for (int f = 0; f < 2; f++) {
+                float p[2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int r = w * 16 + (lane >> 2) + 8 * h, i = (row0 + r) / per;
-                    const float z = lse[r];
-                    const uint64_t mask = partial && i < e.count ? see.mask[i] : 0;
-                    const int lo = i < e.count ? see.lo[i] : 0x7fffffff;
-#pragma unroll
-                    for (int j = 0; j < NK; j++)
-#pragma unroll
-                        for (int f = 0; f < 2; f++) {
-                            float p = exp2_approx(__fmaf_rn(x[j][2 * h + f], c, -z));
-                            if (partial) {
-                                const int t = base + 8 * j + 2 * (lane & 3) + f;
-                                if (!(t < e.len ? t >= lo : t < end && (mask >> (t - e.len) & 1))) p = 0.0f;
-                            }
-                            sum[j][f] += z == INFINITY ? 0.0f : p;
-                        }
+                    p[h] = exp2_approx(__fmaf_rn(x[j][2 * h + f], c, -z[h]));
+                    bool sees = counts[h];
+                    if (partial) {
+                        const int t = base + 8 * j + 2 * (lane & 3) + f;
+                        sees = t < e.len ? t >= lo[h] : t < end && (mask[h] >> (t - e.len) & 1);
+                    }
+                    if (!sees) p[h] = 0.0f;
                 }
+                sum[j][f] = p[0] + p[1];
             }
 #pragma unroll
-            for (int j = 0; j < NK; j++) {
+            for (int f = 0; f < 2; f++)
 #pragma unroll
-                for (int f = 0; f < 2; f++)
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) sum[j][f] += __shfl_xor_sync(0xffffffffu, sum[j][f], o);
-                const int t = base + 8 * j + 2 * lane;
-                if (lane < 4) {
-                    if (t < end) weight[t] += sum[j][0];
-                    if (t + 1 < end) weight[t + 1] += sum[j][1];
-                }
+                for (int o = 4; o < 32; o <<= 1) sum[j][f] += __shfl_xor_sync(0xffffffffu, sum[j][f], o);
+            const int t = base + 8 * j + 2 * lane;
+            if (lane < 4) {
+                if (t < end) weight[t] = had[j].x + sum[j][0];
+                if (t + 1 < end) weight[t + 1] = had[j].y + sum[j][1];
             }
         }
     }
 }
 
 template <class T, int HD, int NK>
-static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
-    const int per = a.nh / kv.nkv, tiles = (a.rows * per + 15) / 16;
-    int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
-    if (a.window > 0) slots = min(slots, a.window + a.rows);
-    const int steps = (slots + 8 * NK - 1) / (8 * NK), jobs = kv.nkv * a.n;
-    // two CTAs on an SM, a few times over so that the last ones are short; no more than there are steps
-    const dim3 grid(max(1, min((steps + AW - 1) / AW, (3 * 296 + jobs - 1) / jobs)), kv.nkv, a.n);
-    constexpr size_t q = (size_t)HD * 128;
-    if (tiles == 1) return launch_cluster<weigh_kernel<T, HD, NK, 1>>(grid, AW * 32, 1, q, q, st, kv, a, picked);
-    if (tiles <= 4) return launch_cluster<weigh_kernel<T, HD, NK, 4>>(grid, AW * 32, 1, 4 * q, 4 * q, st, kv, a, picked);
-    return launch_cluster<weigh_kernel<T, HD, NK, 8>>(grid, AW * 32, 1, 8 * q, 8 * q, st, kv, a, picked);
+static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int slots, cudaStream_t st) {
+    constexpr size_t smem = (size_t)AW * 16384 + HD * 128;
+    constexpr auto K = weigh_kernel<T, HD, NK>;
+    // CTAs of an entry and head: as with clusters, the least time of all waves
+    cudaError_t e = cudaSuccess;
+    const int c = cluster_size<K, false>((long long)kv.nkv * a.n, (slots + 8 * NK - 1) / (8 * NK), AW, 4, AW * 32, smem, smem, &e);
+    if (e != cudaSuccess) return e;
+    return launch_cluster<K>(dim3(c, kv.nkv, a.n), AW * 32, 1, smem, smem, st, kv, a, picked);
 }
 
 cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
     int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
     if (a.window > 0) slots = min(slots, a.window + a.rows);
     if (a.rows * (a.nh / kv.nkv) > 16) return launch_weigh_tc(kv, a, picked, slots, st);
-    if (kv.type) return kv.hd == 64 ? launch_weigh<KvBf16, 64, 2>(kv, a, picked, len_hint, st) : launch_weigh<KvBf16, 128, 2>(kv, a, picked, len_hint, st);
-    return kv.hd == 64 ? launch_weigh<KvF32, 64, 2>(kv, a, picked, len_hint, st) : launch_weigh<KvF32, 128, 2>(kv, a, picked, len_hint, st);
+    if (kv.type) return kv.hd == 64 ? launch_weigh<KvBf16, 64, 2>(kv, a, picked, slots, st) : launch_weigh<KvBf16, 128, 2>(kv, a, picked, slots, st);
+    return kv.hd == 64 ? launch_weigh<KvF32, 64, 2>(kv, a, picked, slots, st) : launch_weigh<KvF32, 128, 2>(kv, a, picked, slots, st);
 }
 
 // ---------------------------------------------------------------- chosen blocks
@@ -538,11 +571,14 @@ __device__ __forceinline__ void block_keys(const float *__restrict__ q, int per,
 }
 
 template <class T, int HD, int NK>
-__global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel, int first, int local,
+__global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel, int first, int local,
                                                          const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *o, float *lse) {
+    typedef Ring<T, HD, NK, true> Rg;
     constexpr int R = 16, STEP = 8 * NK;
-    extern __shared__ __align__(16) float4 frag[];
-    uint32_t *keys = reinterpret_cast<uint32_t *>(frag) + attn_smem(HD) / 4;      // [cap / block + 1]
+    extern __shared__ __align__(128) unsigned char asm_[];
+    __shared__ __align__(8) uint64_t bars[AW * 8];
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * 16384);
+    uint32_t *keys = reinterpret_cast<uint32_t *>(asm_) + attn_smem(HD) / 4;      // [cap / block + 1]
     __shared__ int32_t chosen[256];
     __shared__ float qs[16 * HD];
     __shared__ KthSpace kth;
@@ -550,6 +586,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
     const int C = (int)cl.num_blocks();
     const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (C > 1) cluster_arrive();
+    Rg ring(asm_, bars);
     pdl_wait();
     pdl_trigger();
     const int s = seq ? seq[r] : r, n = len[r];
@@ -621,30 +658,35 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 2 : 1) blocks_kernel(KvDev
     const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(s, kvh), *vc = (const typename T::Val *)kv.v + kv.head(s, kvh);
     const float c = scale * LOG2E;
     const int each = block / STEP, steps = taken * each;
-    Running<T, HD, NK> run;
+    Running<T, HD, NK, Rg> run;
     run.clear();
-    KvStep<T, HD, NK> st;
-    const int hop = C * AW;
-    int i = blockIdx.x * AW + warp;
-    auto slot = [&](int i) { return chosen[i / each] * block + i % each * STEP; };
-    if (i < steps) {
-        st.template load_k<true>(kc, slot(i), n);
-        st.template load_v<true>(vc, slot(i), n);
-    }
-    for (; i < steps; i += hop) {
-        const int base = slot(i);
+    TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
+    const int hop = C * AW, i0 = blockIdx.x * AW + warp, count = max(0, (steps - i0 + hop - 1) / hop);
+    auto base_of = [&](int m) {
+        const int i = i0 + m * hop;
+        return chosen[i / each] * block + i % each * STEP;
+    };
+    auto bring = [&](int m) {
+        if (base_of(m) < n) ring.bring(m, kc, vc, base_of(m), n);       // the last block may end before
+    };
+    for (int m = 0; m < min(count, Rg::D); m++) bring(m);
+    for (int m = 0; m < count; m++) {
+        const int base = base_of(m);
+        if (base >= n) break;                                           // nothing but such steps follows
+        const uint32_t st = ring.step(m);
+        wait(&ring.full[m % Rg::D], (m / Rg::D) & 1);
         float x[NK][4];
-        step_scores<T, HD, NK>(st, frag, x);
-        if (i + hop < steps) st.template load_k<true>(kc, slot(i + hop), n);
+        step_scores<T, HD, NK, Rg>(st, frag, x);
 #pragma unroll
         for (int j = 0; j < NK; j++)
 #pragma unroll
             for (int f = 0; f < 4; f++) x[j][f] = base + 8 * j + 2 * (lane & 3) + (f & 1) < n ? x[j][f] * c : -INFINITY;
-        run.add(st, x, false);
-        if (i + hop < steps) st.template load_v<true>(vc, slot(i + hop), n);
+        run.add(st, x, base + STEP > n);
+        __syncwarp();
+        if (m + Rg::D < count) bring(m + Rg::D);
     }
     __syncthreads();
-    float *out = reinterpret_cast<float *>(frag), *got = out + AW * R * HD;
+    float *out = reinterpret_cast<float *>(asm_), *got = reinterpret_cast<float *>(frag) + 32 * HD;
     float2 *gml = reinterpret_cast<float2 *>(got + 31 * HD), *ml = gml + 31;
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
@@ -660,7 +702,7 @@ static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, 
     const int steps = min(nsel, nb + 1) * each + (nb > nsel ? nb / 8 : 0);
     const size_t smem = attn_smem(HD) + (size_t)(kv.cap / block + 1) * 4, most = attn_smem(HD) + 16385 * 4;
     cudaError_t e = cudaSuccess;
-    const int c = cluster_size<blocks_kernel<T, HD, NK>>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, attn_smem(HD), most, &e);
+    const int c = cluster_size<blocks_kernel<T, HD, NK>>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, attn_smem(HD) + 4096, most, &e);
     if (e != cudaSuccess) return e;
     return launch_cluster<blocks_kernel<T, HD, NK>>(dim3(c, rows, kv.nkv), AW * 32, c, smem, most, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
                                                     sinks, sel, out, lse);
@@ -668,7 +710,7 @@ static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, 
 
 cudaError_t launch_attn_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,
                                int len_hint, const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *out, float *lse, cudaStream_t st) {
-    auto go = kv.type ? (kv.hd == 64 ? launch_blocks<KvBf16, 64, 2> : launch_blocks<KvBf16, 128, 2>) : (kv.hd == 64 ? launch_blocks<KvF32, 64, 1> : launch_blocks<KvF32, 128, 1>);
+    auto go = kv.type ? (kv.hd == 64 ? launch_blocks<KvBf16, 64, 2> : launch_blocks<KvBf16, 128, 2>) : (kv.hd == 64 ? launch_blocks<KvF32, 64, 2> : launch_blocks<KvF32, 128, 1>);
     return go(kv, rows, seq, len, block, means, nsel, first, local, len_hint, q, nh, scale, sinks, sel, out, lse, st);
 }
 
