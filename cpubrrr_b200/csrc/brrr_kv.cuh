@@ -54,20 +54,23 @@ struct TreeArgs {
     const float *sinks;
     float *out, *lse;
 };
-// Work space of block_kth in shared memory.
+// Work space of block_kth in shared memory.  BITS at a time: eleven for a block of 1024 (the first hold sign, exponent and two more: fewer counts meet in
+// one word), eight for smaller ones (a thread has few words to clear and to add up).
+template <int BITS>
 struct KthSpace {
-    uint32_t hist[2048], found[2], sums[32];
+    uint32_t hist[1 << BITS], found[2], sums[32];
 };
-// The key of the k-th largest (1 <= k <= n) of key(0) .. key(n - 1), and how many of the keys that equal it are among the k largest: eleven bits at a time
-// (the first hold sign, exponent and two more: fewer counts meet in one word than with eight).  All threads call it; it ends with a barrier.
-template <class Key>
-__device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpace &w, uint32_t *ties) {
+// The key of the k-th largest (1 <= k <= n) of key(0) .. key(n - 1), and how many of the keys that equal it are among the k largest.  All threads call it (at most
+// 1 << BITS of them); it ends with a barrier.
+template <int BITS, class Key>
+__device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpace<BITS> &w, uint32_t *ties) {
     uint32_t prefix = 0, known = 0;
-    const int each = 2048 / blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t digit = pass == 2 ? 1023u : 2047u;
-        for (int i = threadIdx.x; i < 2048; i += blockDim.x) w.hist[i] = 0;
+    const int each = (1 << BITS) / blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int left = 32; left > 0;) {
+        const int shift = max(0, left - BITS);
+        const uint32_t digit = (1u << (left - shift)) - 1;
+        left = shift;
+        for (int i = threadIdx.x; i < 1 << BITS; i += blockDim.x) w.hist[i] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < n; i += blockDim.x) {
             const uint32_t x = key(i);
@@ -75,7 +78,7 @@ __device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpa
         }
         __syncthreads();
         // thread i: `each` digits, the largest first
-        const int top = 2047 - threadIdx.x * each;
+        const int top = (1 << BITS) - 1 - threadIdx.x * each;
         uint32_t sum = 0;
         for (int j = 0; j < each; j++) sum += w.hist[top - j];
         uint32_t upto = sum;

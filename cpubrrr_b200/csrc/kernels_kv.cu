@@ -174,7 +174,7 @@ template <bool KEEP_KEYS>
 __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev dst, const int32_t *seq, const int32_t *len, int keep, int first, int recent,
                                                               const int32_t *end, int32_t *map, int32_t *new_len) {
     extern __shared__ uint32_t sm[];
-    __shared__ KthSpace kth;
+    __shared__ KthSpace<11> kth;
     pdl_wait();
     const int kvh = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = EV_THREADS / 32;
     const KvEntry e = kv_entry(kv, b, 0, seq, len, nullptr);

@@ -534,30 +534,36 @@ __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
     asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
 }
 
-// Keys of blocks j0 .. j0 + 7 by one warp: lane 4 g + t has those of blocks 2t and 2t + 1 (the same for every g).
+// The means of blocks j0 .. j0 + 7 (not beyond last): lane 4 g + t has values 16 c + 4 t .. of block j0 + g.
 template <int HD>
-__device__ __forceinline__ void block_keys(const float *__restrict__ q, int per, const float *__restrict__ mean, int j0, int nb, uint32_t (&key)[2]) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const float *m = mean + (long long)min(j0 + g, nb - 1) * HD + 4 * t;
-    float4 x[HD / 16];
+__device__ __forceinline__ void load_means(const float *__restrict__ mean, int j0, int last, float4 (&x)[HD / 16]) {
+    const int lane = threadIdx.x & 31;
+    const float *m = mean + (long long)min(j0 + (lane >> 2), last) * HD + 4 * (lane & 3);
 #pragma unroll
     for (int c = 0; c < HD / 16; c++) x[c] = *reinterpret_cast<const float4 *>(m + 16 * c);
+}
+// Their keys: lane 4 g + t has those of blocks j0 + 2t and j0 + 2t + 1 (the same for every g).
+template <int HD>
+__device__ __forceinline__ void block_keys(const float *__restrict__ q, int per, const float4 (&x)[HD / 16], uint32_t (&key)[2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     key[0] = key[1] = 0;
     for (int h0 = 0; h0 < per; h0 += 8) {
-        double even[2] = {0.0, 0.0}, odd[2] = {0.0, 0.0};
+        double sum[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[i][0] = sum[i][1] = 0.0;
         const float *p = q + (h0 + g) * HD + 4 * t;
 #pragma unroll
         for (int c = 0; c < HD / 16; c++) {
             const float4 a = h0 + g < per ? *reinterpret_cast<const float4 *>(p + 16 * c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            mma_f64(even, a.x, x[c].x);
-            mma_f64(odd, a.y, x[c].y);
-            mma_f64(even, a.z, x[c].z);
-            mma_f64(odd, a.w, x[c].w);
+            mma_f64(sum[0], a.x, x[c].x);
+            mma_f64(sum[1], a.y, x[c].y);
+            mma_f64(sum[2], a.z, x[c].z);
+            mma_f64(sum[3], a.w, x[c].w);
         }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             // the rounding keeps the order, so the largest may be taken afterwards; what is no number wins here and loses in the end
-            const float f = (float)(even[i] + odd[i]);
+            const float f = (float)((sum[0][i] + sum[1][i]) + (sum[2][i] + sum[3][i]));
             uint32_t k = f != f ? 0xFFFFFFFFu : float_orderable(f == 0.0f ? 0.0f : f);
             if (h0 + g >= per) k = 0;
 #pragma unroll
@@ -581,7 +587,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
     uint32_t *keys = reinterpret_cast<uint32_t *>(asm_) + attn_smem(HD) / 4;      // [cap / block + 1]
     __shared__ int32_t chosen[256];
     __shared__ float qs[16 * HD];
-    __shared__ KthSpace kth;
+    __shared__ KthSpace<8> kth;
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks();
     const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -606,10 +612,21 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
         const float *mean = means + ((long long)s * kv.nkv + kvh) * (kv.cap / block) * HD;
         const int hi = nb - local, tiles = (hi - first + 7) / 8;
         if (C > 1) cluster_wait();     // every CTA is there: its memory may be written
-        for (int i = blockIdx.x * AW + warp; i < tiles; i += C * AW) {
+        float4 x[2][HD / 16];
+        const int step = C * AW;
+        int i = blockIdx.x * AW + warp;
+        load_means<HD>(mean, first + 8 * i, hi - 1, x[0]);
+        for (int turn = 0; i < tiles; i += step, turn++) {
+            // the next tile's means come while this one's are used
+            const int j = first + 8 * i + 2 * (lane & 3);
             uint32_t key[2];
-            const int j0 = first + 8 * i, j = j0 + 2 * (lane & 3);
-            block_keys<HD>(qs, per, mean, j0, hi, key);
+            if (turn & 1) {
+                load_means<HD>(mean, first + 8 * (i + step), hi - 1, x[0]);
+                block_keys<HD>(qs, per, x[1], key);
+            } else {
+                load_means<HD>(mean, first + 8 * (i + step), hi - 1, x[1]);
+                block_keys<HD>(qs, per, x[0], key);
+            }
             for (int p = lane >> 2; p < C; p += 8) {
                 uint32_t *there = C > 1 ? cl.map_shared_rank(keys, p) : keys;
                 if (j < hi) there[j] = key[0];
@@ -627,28 +644,32 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
         const int want = nsel - first - local;
         const uint32_t last = want > 0 ? block_kth(hi - first, want, [&](int i) { return keys[first + i]; }, kth, &ties) : 0xFFFFFFFFu;
         if (want <= 0) ties = 0;
-        // the places of the chosen ones, in ascending order of blocks
-        uint32_t before = 0, same_before = 0;
-        for (int at = 0; at < nb; at += AW * 32) {
-            const int j = at + threadIdx.x;
-            const bool must = j < nb && (j < first || j >= hi), free = j >= first && j < hi;
+        // the places of the chosen ones, in ascending order of blocks: a warp has a run of 32 w blocks and counts them first; both counts in one word
+        const int run = (nb + 32 * AW - 1) / (32 * AW), j0 = warp * run * 32 + lane;
+        auto kind = [&](int j, bool &over, bool &same) {
+            const bool free = j >= first && j < hi;
             const uint32_t k = free ? keys[j] : 0;
-            const bool over = must || (free && k > last), same = free && k == last && want > 0;
-            // counts of both kinds in one word: block <= 256 of each
+            over = (j < nb && !free) || (free && want > 0 && k > last);
+            same = free && want > 0 && k == last;
+        };
+        uint32_t count = 0;
+        for (int w = 0; w < run; w++) {
+            bool over, same;
+            kind(j0 + 32 * w, over, same);
+            count += __popc(__ballot_sync(0xffffffffu, over)) | __popc(__ballot_sync(0xffffffffu, same)) << 16;
+        }
+        if (lane == 0) kth.sums[warp] = count;
+        __syncthreads();
+        uint32_t before = 0;
+        for (int w = 0; w < warp; w++) before += kth.sums[w];
+        for (int w = 0; w < run; w++) {
+            bool over, same;
+            kind(j0 + 32 * w, over, same);
             const uint32_t b_over = __ballot_sync(0xffffffffu, over), b_same = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1;
-            if (lane == 0) kth.sums[warp] = __popc(b_over) | __popc(b_same) << 16;
-            __syncthreads();
-            uint32_t mine = __popc(b_over & below) | __popc(b_same & below) << 16, all = 0;
-            for (int w = 0; w < AW; w++) {
-                if (w < warp) mine += kth.sums[w];
-                all += kth.sums[w];
-            }
-            __syncthreads();
-            const uint32_t o_rank = before + (mine & 0xFFFF), s_rank = same_before + (mine >> 16);
-            if (over) chosen[o_rank + min(s_rank, ties)] = j;
-            else if (same && s_rank < ties) chosen[o_rank + s_rank] = j;
-            before += all & 0xFFFF;
-            same_before += all >> 16;
+            const uint32_t o_rank = (before & 0xFFFF) + __popc(b_over & below), s_rank = (before >> 16) + __popc(b_same & below);
+            if (over) chosen[o_rank + min(s_rank, ties)] = j0 + 32 * w;
+            else if (same && s_rank < ties) chosen[o_rank + s_rank] = j0 + 32 * w;
+            before += __popc(b_over) | __popc(b_same) << 16;
         }
     }
     stage_queries<T, HD>(frag, 1, [&](int i) -> const float * { return i < per ? qs + i * HD : nullptr; });
@@ -657,14 +678,14 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
         for (int i = threadIdx.x; i < nsel; i += AW * 32) sel[((long long)r * kv.nkv + kvh) * nsel + i] = i < taken ? chosen[i] : -1;
     const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(s, kvh), *vc = (const typename T::Val *)kv.v + kv.head(s, kvh);
     const float c = scale * LOG2E;
-    const int each = block / STEP, steps = taken * each;
+    const int shift = 31 - __clz(block / STEP), steps = taken << shift;       // steps of a block: a power of two
     Running<T, HD, NK, Rg> run;
     run.clear();
     TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
     const int hop = C * AW, i0 = blockIdx.x * AW + warp, count = max(0, (steps - i0 + hop - 1) / hop);
     auto base_of = [&](int m) {
         const int i = i0 + m * hop;
-        return chosen[i / each] * block + i % each * STEP;
+        return chosen[i >> shift] * block + (i & ((1 << shift) - 1)) * STEP;
     };
     auto bring = [&](int m) {
         if (base_of(m) < n) ring.bring(m, kc, vc, base_of(m), n);       // the last block may end before
