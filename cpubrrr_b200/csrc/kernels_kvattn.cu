@@ -31,17 +31,20 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const float4 &a, float b
 }
 
 
-// A warp's ring: D steps of 8 NK slots, 16 KB in all, keys and (both) values of a step side by side.  Lane 0 copies.
-template <class T, int HD, int NK, bool BOTH>
+// A warp's ring: D places for the keys or the values of a step of 8 NK slots each, 12 KB in all.  Lane 0 copies; operand u is u-th in the order in which the warp
+// uses them (keys, values, keys, ...).
+constexpr int RING = 12288;
+template <class T, int HD, int NK>
 struct Ring {
-    static constexpr int STEP = 8 * NK, ROW = HD * (int)sizeof(typename T::Val), HALF = STEP * ROW, SLOT = HALF * (BOTH ? 2 : 1), D = 16384 / SLOT;
+    static constexpr int STEP = 8 * NK, ROW = HD * (int)sizeof(typename T::Val), PLACE = STEP * ROW, D = RING / PLACE;
     static constexpr int NC = HD / (4 * T::V), NVC = HD / (8 * T::V);       // 16-byte reads of a lane per slot: keys, values
-    static_assert(D >= 2 && D * SLOT == 16384, "");
+    static_assert(D >= 2 && D <= 8, "");
     uint32_t at;             // of the ring, in shared memory
     uint64_t *full;          // [D]
+    int in = 0, out = 0, in_turn = 0;      // places that the next copy and the next use take, and the parity of the next use
     __device__ __forceinline__ Ring(unsigned char *mem, uint64_t *bars) {
         const int warp = threadIdx.x >> 5;
-        at = smem_u32(mem) + warp * 16384;
+        at = smem_u32(mem) + warp * RING;
         full = bars + warp * 8;
         if ((threadIdx.x & 31) == 0) {
             for (int i = 0; i < D; i++) mbar_init(&full[i], 1);
@@ -49,21 +52,24 @@ struct Ring {
         }
         __syncwarp();
     }
-    // step n of this warp: slots base .. base + 8 NK - 1, those from end on not read (their place keeps what it had)
-    __device__ __forceinline__ void bring(int n, const typename T::Val *kc, const typename T::Val *vc, int base, int end) {
+    // slots base .. base + 8 NK - 1 of p, those from end on not read (their place keeps what it had), to the next place, which must have been used
+    __device__ __forceinline__ void bring(const typename T::Val *p, int base, int end) {
         if ((threadIdx.x & 31) == 0) {
-            const int i = n % D, bytes = min(STEP, end - base) * ROW;
-            uint64_t *bar = &full[i];
-            mbar_expect_tx(bar, BOTH ? 2 * bytes : bytes);
-            const uint32_t dst = at + i * SLOT;
-            copy(dst, kc + (long long)base * HD, bytes, bar);
-            if (BOTH) copy(dst + HALF, vc + (long long)base * HD, bytes, bar);
+            const int bytes = min(STEP, end - base) * ROW;
+            mbar_expect_tx(&full[in], bytes);
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at + in * PLACE), "l"(p + (long long)base * HD), "r"(bytes),
+                         "r"(smem_u32(&full[in]))
+                         : "memory");
         }
+        in = in + 1 == D ? 0 : in + 1;
     }
-    __device__ __forceinline__ static void copy(uint32_t dst, const void *src, int bytes, uint64_t *bar) {
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+    // the next operand's place, once it has come
+    __device__ __forceinline__ uint32_t next(TlWaiter &wait) {
+        wait(&full[out], in_turn);
+        const uint32_t p = at + out * PLACE;
+        if (++out == D) { out = 0; in_turn ^= 1; }
+        return p;
     }
-    __device__ __forceinline__ uint32_t step(int n) const { return at + n % D * SLOT; }
     // this lane's 16 bytes c of the key of slot 8 j + lane / 4, and of the value of slot 8 j + 2 (lane % 4) + h
     __device__ __forceinline__ static uint4 key(uint32_t st, int j, int c) {
         const int lane = threadIdx.x & 31;
@@ -71,7 +77,7 @@ struct Ring {
     }
     __device__ __forceinline__ static uint4 value(uint32_t st, int j, int h, int c) {
         const int lane = threadIdx.x & 31;
-        return lds128(st + HALF + (8 * j + 2 * (lane & 3) + h) * ROW + (lane >> 2) * 16 + c * 128);
+        return lds128(st + (8 * j + 2 * (lane & 3) + h) * ROW + (lane >> 2) * 16 + c * 128);
     }
 };
 
@@ -300,11 +306,11 @@ __device__ __forceinline__ void join_warps(float *out, float2 *ml, int parts, fl
 // grid (C, kv heads, entries), clusters of C
 template <class T, int HD, int NK>
 __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev kv, TreeArgs a) {
-    typedef Ring<T, HD, NK, true> Rg;
+    typedef Ring<T, HD, NK> Rg;
     constexpr int R = 16, STEP = 8 * NK;
     extern __shared__ __align__(128) unsigned char asm_[];  // the warps' rings, later the parts: out [AW][R][HD], ml [AW][R]; the queries; the owner's parts
     __shared__ __align__(8) uint64_t bars[AW * 8];
-    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * 16384);
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * RING);
     __shared__ TreeRows see;
     const int per = a.nh / kv.nkv, kvh = blockIdx.y, b = blockIdx.z;
     if (gridDim.x > 1) cluster_arrive();
@@ -330,7 +336,11 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
     const int steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
     const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps), count = max(0, (to - from - warp + AW - 1) / AW);
     auto base_of = [&](int n) { return (from + warp + n * AW) * STEP; };
-    for (int n = 0; n < min(count, Rg::D); n++) ring.bring(n, kc, vc, base_of(n), end);
+    // operand u: keys (u even) or values of step u / 2
+    auto bring = [&](int u) {
+        if (u < 2 * count) ring.bring(u & 1 ? vc : kc, base_of(u >> 1), end);
+    };
+    for (int u = 0; u < Rg::D; u++) bring(u);
     if (a.window <= 0) tree_rows(a, e, mine, see);
     auto place = [&](int r) -> long long {
         const int i = r / per;
@@ -353,10 +363,10 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
     TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
     for (int n = 0; n < count; n++) {
         const int base = base_of(n);
-        const uint32_t st = ring.step(n);
-        wait(&ring.full[n % Rg::D], (n / Rg::D) & 1);
         float x[NK][4];
-        step_scores<T, HD, NK, Rg>(st, frag, x);
+        step_scores<T, HD, NK, Rg>(ring.next(wait), frag, x);
+        __syncwarp();
+        bring(2 * n + Rg::D);
         const bool partial = base < see.full || base + STEP > e.len;
 #pragma unroll
         for (int j = 0; j < NK; j++)
@@ -369,9 +379,9 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
                     if (!sees) x[j][f] = -INFINITY;
                 }
             }
-        run.add(st, x, partial);
+        run.add(ring.next(wait), x, partial);
         __syncwarp();
-        if (n + Rg::D < count) ring.bring(n + Rg::D, kc, vc, base_of(n + Rg::D), end);
+        bring(2 * n + 1 + Rg::D);
     }
     __syncthreads();                 // nobody reads the rings any more
     float *out = reinterpret_cast<float *>(asm_), *got = reinterpret_cast<float *>(frag) + 32 * HD;
@@ -382,8 +392,8 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
 }
 
 // bytes of a CTA's shared memory: the rings (later the parts of the warps), the queries, the owner's parts
-__host__ __device__ constexpr size_t attn_smem(int hd) { return (size_t)AW * 16384 + hd * 128 + 31 * (hd * 4 + 8) + AW * 16 * 8; }
-static_assert(16 * 128 * 4 <= 16384, "a warp's part fits its ring");
+__host__ __device__ constexpr size_t attn_smem(int hd) { return (size_t)AW * RING + hd * 128 + 31 * (hd * 4 + 8) + AW * 16 * 8; }
+static_assert(16 * 128 * 4 <= RING, "a warp's part fits its ring");
 
 template <class T, int HD, int NK>
 static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
@@ -407,12 +417,12 @@ cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, c
 // Up to 16 rows per kv head (more: kernels_kvtc.cu).  A warp owns a step of slots: the scores of its keys, their powers, the sum over the rows.
 template <class T, int HD, int NK>
 __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked) {
-    typedef Ring<T, HD, NK, false> Rg;
+    typedef Ring<T, HD, NK> Rg;
     constexpr int STEP = 8 * NK;
     extern __shared__ __align__(128) unsigned char asm_[];       // the warps' rings, the queries
     __shared__ __align__(8) uint64_t bars[AW * 8];
     __shared__ TreeRows see;
-    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * 16384);
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * RING);
     const int kvh = blockIdx.y, b = blockIdx.z, per = a.nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Rg ring(asm_, bars);
     pdl_wait();
@@ -435,7 +445,7 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
     const int steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
     const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps), count = max(0, (to - from - warp + AW - 1) / AW);
     auto base_of = [&](int n) { return (from + warp + n * AW) * STEP; };
-    for (int n = 0; n < min(count, Rg::D); n++) ring.bring(n, kc, nullptr, base_of(n), end);
+    for (int n = 0; n < min(count, Rg::D); n++) ring.bring(kc, base_of(n), end);
     if (a.window <= 0) tree_rows(a, e, mine, see);
     const uint64_t rows = picked ? picked[b] : ~0ull;
     auto place = [&](int r) -> long long {
@@ -472,11 +482,10 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
             const int t = base + 8 * j + 2 * lane;
             had[j] = make_float2(lane < 4 && t < end ? weight[t] : 0.0f, lane < 4 && t + 1 < end ? weight[t + 1] : 0.0f);
         }
-        wait(&ring.full[n % Rg::D], (n / Rg::D) & 1);
         float x[NK][4], sum[NK][2];
-        step_scores<T, HD, NK, Rg>(ring.step(n), frag, x);
+        step_scores<T, HD, NK, Rg>(ring.next(wait), frag, x);
         __syncwarp();
-        if (n + Rg::D < count) ring.bring(n + Rg::D, kc, nullptr, base_of(n + Rg::D), end);
+        if (n + Rg::D < count) ring.bring(kc, base_of(n + Rg::D), end);
         const bool partial = base < see.full || base + STEP > e.len;
 #pragma unroll
         for (int j = 0; j < NK; j++) {
@@ -510,7 +519,7 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
 
 template <class T, int HD, int NK>
 static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int slots, cudaStream_t st) {
-    constexpr size_t smem = (size_t)AW * 16384 + HD * 128;
+    constexpr size_t smem = (size_t)AW * RING + HD * 128;
     constexpr auto K = weigh_kernel<T, HD, NK>;
     // CTAs of an entry and head: as with clusters, the least time of all waves
     cudaError_t e = cudaSuccess;
@@ -524,7 +533,7 @@ cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *
     if (a.window > 0) slots = min(slots, a.window + a.rows);
     if (a.rows * (a.nh / kv.nkv) > 16) return launch_weigh_tc(kv, a, picked, slots, st);
     if (kv.type) return kv.hd == 64 ? launch_weigh<KvBf16, 64, 2>(kv, a, picked, slots, st) : launch_weigh<KvBf16, 128, 2>(kv, a, picked, slots, st);
-    return kv.hd == 64 ? launch_weigh<KvF32, 64, 2>(kv, a, picked, slots, st) : launch_weigh<KvF32, 128, 2>(kv, a, picked, slots, st);
+    return kv.hd == 64 ? launch_weigh<KvF32, 64, 2>(kv, a, picked, slots, st) : launch_weigh<KvF32, 128, 1>(kv, a, picked, slots, st);
 }
 
 // ---------------------------------------------------------------- chosen blocks
@@ -579,11 +588,11 @@ __device__ __forceinline__ void block_keys(const float *__restrict__ q, int per,
 template <class T, int HD, int NK>
 __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel, int first, int local,
                                                          const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *o, float *lse) {
-    typedef Ring<T, HD, NK, true> Rg;
+    typedef Ring<T, HD, NK> Rg;
     constexpr int R = 16, STEP = 8 * NK;
     extern __shared__ __align__(128) unsigned char asm_[];
     __shared__ __align__(8) uint64_t bars[AW * 8];
-    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * 16384);
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * RING);
     uint32_t *keys = reinterpret_cast<uint32_t *>(asm_) + attn_smem(HD) / 4;      // [cap / block + 1]
     __shared__ int32_t chosen[256];
     __shared__ float qs[16 * HD];
@@ -687,24 +696,25 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
         const int i = i0 + m * hop;
         return chosen[i >> shift] * block + (i & ((1 << shift) - 1)) * STEP;
     };
-    auto bring = [&](int m) {
-        if (base_of(m) < n) ring.bring(m, kc, vc, base_of(m), n);       // the last block may end before
+    // the last block may end before its last steps: nothing but such steps follows
+    auto bring = [&](int u) {
+        if (u < 2 * count && base_of(u >> 1) < n) ring.bring(u & 1 ? vc : kc, base_of(u >> 1), n);
     };
-    for (int m = 0; m < min(count, Rg::D); m++) bring(m);
+    for (int u = 0; u < Rg::D; u++) bring(u);
     for (int m = 0; m < count; m++) {
         const int base = base_of(m);
-        if (base >= n) break;                                           // nothing but such steps follows
-        const uint32_t st = ring.step(m);
-        wait(&ring.full[m % Rg::D], (m / Rg::D) & 1);
+        if (base >= n) break;
         float x[NK][4];
-        step_scores<T, HD, NK, Rg>(st, frag, x);
+        step_scores<T, HD, NK, Rg>(ring.next(wait), frag, x);
+        __syncwarp();
+        bring(2 * m + Rg::D);
 #pragma unroll
         for (int j = 0; j < NK; j++)
 #pragma unroll
             for (int f = 0; f < 4; f++) x[j][f] = base + 8 * j + 2 * (lane & 3) + (f & 1) < n ? x[j][f] * c : -INFINITY;
-        run.add(st, x, base + STEP > n);
+        run.add(ring.next(wait), x, base + STEP > n);
         __syncwarp();
-        if (m + Rg::D < count) bring(m + Rg::D);
+        bring(2 * m + 1 + Rg::D);
     }
     __syncthreads();
     float *out = reinterpret_cast<float *>(asm_), *got = reinterpret_cast<float *>(frag) + 32 * HD;
