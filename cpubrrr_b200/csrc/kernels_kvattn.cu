@@ -303,7 +303,7 @@ __device__ __forceinline__ void join_warps(float *out, float2 *ml, int parts, fl
     join_rows<HD, HD>(got, gml, C, each, o, lse, [&](int i) -> long long { return c * each + i < R ? dst(c * each + i) : -1; }, [&](int i) { return sink(c * each + i); });
 }
 
-// grid (C, kv heads, entries), clusters of C
+// grid (C, kv heads x tiles of 16 rows, entries), clusters of C
 template <class T, int HD, int NK>
 __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev kv, TreeArgs a) {
     typedef Ring<T, HD, NK> Rg;
@@ -312,14 +312,14 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
     __shared__ __align__(8) uint64_t bars[AW * 8];
     float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * RING);
     __shared__ TreeRows see;
-    const int per = a.nh / kv.nkv, kvh = blockIdx.y, b = blockIdx.z;
+    const int per = a.nh / kv.nkv, tiles = (a.rows * per + R - 1) / R, kvh = blockIdx.y / tiles, row0 = blockIdx.y % tiles * R, b = blockIdx.z;
     if (gridDim.x > 1) cluster_arrive();
     Rg ring(asm_, bars);
     pdl_wait();
     pdl_trigger();
     const uint64_t mine = tree_mask(a, b);
     const KvEntry e = kv_entry(kv, b, a.rows, a.seq, a.len, a.count);
-    if (!e.ok || e.count == 0) {
+    if (!e.ok || row0 >= e.count * per) {
         if (!e.ok && threadIdx.x == 0) kv_error(kv);
         if (gridDim.x > 1) cluster_wait();
         return;
@@ -343,8 +343,8 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
     for (int u = 0; u < Rg::D; u++) bring(u);
     if (a.window <= 0) tree_rows(a, e, mine, see);
     auto place = [&](int r) -> long long {
-        const int i = r / per;
-        return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + r % per : -1;
+        const int i = (row0 + r) / per;
+        return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
     };
     stage_queries<T, HD>(frag, 1, [&](int r) -> const float * { return place(r) >= 0 ? a.q + place(r) * HD : nullptr; });
     __syncthreads();
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
     int lo[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const int i = ((lane >> 2) + 8 * h) / per;
+        const int i = (row0 + (lane >> 2) + 8 * h) / per;
         mask[h] = i < e.count ? see.mask[i] : 0;
         lo[h] = i < e.count ? see.lo[i] : 0x7fffffff;
     }
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
     float2 *gml = reinterpret_cast<float2 *>(got + 31 * HD), *ml = gml + 31;
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
-    join_warps<HD>(out, ml, AW, got, gml, a.out, a.lse, place, [&](int r) { return a.sinks ? a.sinks[kvh * per + r % per] * LOG2E : -INFINITY; });
+    join_warps<HD>(out, ml, AW, got, gml, a.out, a.lse, place, [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
 }
 
 // bytes of a CTA's shared memory: the rings (later the parts of the warps), the queries, the owner's parts
@@ -400,15 +400,27 @@ static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int slots, cu
     constexpr size_t smem = attn_smem(HD);
     constexpr auto K = tree_kernel<T, HD, NK>;
     cudaError_t e = cudaSuccess;
-    const int c = cluster_size<K>((long long)a.n * kv.nkv, (slots + 8 * NK - 1) / (8 * NK), AW, 4, AW * 32, smem, smem, &e);
+    const int tiles = (a.rows * (a.nh / kv.nkv) + 15) / 16;
+    const int c = cluster_size<K>((long long)a.n * kv.nkv * tiles, (slots + 8 * NK - 1) / (8 * NK), AW, 4, AW * 32, smem, smem, &e);
     if (e != cudaSuccess) return e;
-    return launch_cluster<K>(dim3(c, kv.nkv, a.n), AW * 32, c, smem, smem, st, kv, a);
+    return launch_cluster<K>(dim3(c, kv.nkv * tiles, a.n), AW * 32, c, smem, smem, st, kv, a);
+}
+
+// Whether the kernel of 128-row tiles (kernels_kvtc.cu) takes less time than CTAs of 16 rows.  Both were measured with 8 to 256 rows, 1 and 8 sequences, 40 to 2500 slots
+// (20 calls in a graph, in L2): beyond a start that costs the other `start` ns more, 128 slots cost `few` ns per 16 rows here and `many` ns per 128 rows there.  64
+// dimensions f32, 8 heads: 64 rows over 200 slots 6.3 and 13.0 us, over 2500 15.2 and 17.1; 8 sequences: 32 rows over 700 15.4 and 18.8, 128 rows over 2500
+// 146 and 40.
+static bool wide_rows_pay(const KvDev &kv, const TreeArgs &a, int slots) {
+    static const struct { double few, many, start; } cost[2][2] = {{{14.0, 22.0, 7000.0}, {29.0, 45.0, 7000.0}}, {{11.0, 12.4, 4000.0}, {17.0, 24.0, 4500.0}}};
+    const auto &c = cost[kv.type][kv.hd == 128];
+    const int rows = a.rows * (a.nh / kv.nkv);
+    return (double)a.n * kv.nkv * (slots / 128.0) * (c.few * ((rows + 15) / 16) - c.many * ((rows + 127) / 128)) > c.start;
 }
 
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
     int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
     if (a.window > 0) slots = min(slots, a.window + a.rows);
-    if (a.rows * (a.nh / kv.nkv) > 16) return launch_tree_tc(kv, a, slots, st);
+    if (wide_rows_pay(kv, a, slots)) return launch_tree_tc(kv, a, slots, st);
     if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2>(kv, a, slots, st) : launch_tree<KvBf16, 128, 2>(kv, a, slots, st);
     return kv.hd == 64 ? launch_tree<KvF32, 64, 2>(kv, a, slots, st) : launch_tree<KvF32, 128, 1>(kv, a, slots, st);
 }
