@@ -54,6 +54,35 @@ struct TreeArgs {
     const float *sinks;
     float *out, *lse;
 };
+__device__ __forceinline__ uint32_t warp_scan(uint32_t x) {          // sums of this lane and those before it
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if ((int)(threadIdx.x & 31) >= o) x += y;
+    }
+    return x;
+}
+// Sum over the threads before this one, and over all; sums: a word per warp.  All threads call it; one barrier inside, and one before sums is used again.
+__device__ __forceinline__ uint32_t block_before(uint32_t x, uint32_t *sums, uint32_t &all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t upto = warp_scan(x);
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    const uint32_t of_warps = warp_scan(lane < (int)(blockDim.x >> 5) ? sums[lane] : 0);
+    all = __shfl_sync(0xffffffffu, of_warps, 31);
+    return upto - x + (warp ? __shfl_sync(0xffffffffu, of_warps, warp - 1) : 0);
+}
+// Place of the n-th set bit (from 0) of a word that has more.
+__device__ __forceinline__ int nth_bit(uint32_t w, int n) {
+    int at = 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const int c = __popc(w & ((1u << o) - 1));
+        if (n >= c) { n -= c; at += o; w >>= o; }
+    }
+    return at;
+}
+
 // Work space of block_kth in shared memory.  BITS at a time: eleven for a block of 1024 (the first hold sign, exponent and two more: fewer counts meet in
 // one word), eight for smaller ones (a thread has few words to clear and to add up).
 template <int BITS>
@@ -65,7 +94,7 @@ struct KthSpace {
 template <int BITS, class Key>
 __device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpace<BITS> &w, uint32_t *ties) {
     uint32_t prefix = 0, known = 0;
-    const int each = (1 << BITS) / blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int each = (1 << BITS) / blockDim.x;
     for (int left = 32; left > 0;) {
         const int shift = max(0, left - BITS);
         const uint32_t digit = (1u << (left - shift)) - 1;
@@ -81,16 +110,9 @@ __device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpa
         const int top = (1 << BITS) - 1 - threadIdx.x * each;
         uint32_t sum = 0;
         for (int j = 0; j < each; j++) sum += w.hist[top - j];
-        uint32_t upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-        }
-        if (lane == 31) w.sums[warp] = upto;
-        __syncthreads();
-        for (int i = 0; i < warp; i++) upto += w.sums[i];
-        uint32_t above = upto - sum;
+        uint32_t all;
+        uint32_t above = block_before(sum, w.sums, all);
+        const uint32_t upto = above + sum;
         if (above < k && k <= upto)
             for (int j = 0; j < each; j++) {
                 const uint32_t c = w.hist[top - j];

@@ -144,30 +144,26 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int first, long 
 
 // Exclusive running sums of v[0 .. n), in place; returns the total.  All threads call it; v is complete afterwards.
 __device__ __forceinline__ uint32_t block_scan(uint32_t *v, int n, uint32_t *warp_sums) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = blockDim.x >> 5;
     uint32_t carry = 0;
     for (int at = 0; at < n; at += blockDim.x) {
         const int i = at + threadIdx.x;
-        const uint32_t x = i < n ? v[i] : 0;
-        uint32_t s = x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += y;
-        }
-        if (lane == 31) warp_sums[warp] = s;
-        __syncthreads();
-        uint32_t before = 0, all = 0;
-        for (int w = 0; w < nwarp; w++) {
-            const uint32_t y = warp_sums[w];
-            if (w < warp) before += y;
-            all += y;
-        }
-        if (i < n) v[i] = carry + before + s - x;
+        uint32_t all;
+        const uint32_t before = block_before(i < n ? v[i] : 0, warp_sums, all);
+        if (i < n) v[i] = carry + before;
         carry += all;
         __syncthreads();
     }
     return carry;
+}
+// The last i of v[0 .. n) with v[i] <= x; v[0] is 0 and v does not fall.
+__device__ __forceinline__ int last_upto(const uint32_t *v, int n, uint32_t x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (v[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
 }
 
 template <bool KEEP_KEYS>
@@ -234,21 +230,14 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     }
     __syncthreads();
     block_scan(run, mw + 1, kth.sums);
-    block_scan(run + mw + 1, words - mw, kth.sums);
-    for (int i = warp; i < words; i += nwarp) {
-        const int t = i * 32 + lane;
-        if (!(kept[i] >> lane & 1)) continue;
-        if (t < m) { out[t] = t; continue; }
-        const uint32_t j = run[i + 1] + __popc((i == mw ? kept[i] & ~low : kept[i]) & ((1u << lane) - 1));       // the j-th kept entry behind takes the j-th freed slot
-        int lo = 0, hi = mw;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (run[mid] <= j) lo = mid;
-            else hi = mid - 1;
-        }
-        uint32_t holes = ~kept[lo] & (lo == mw ? low : 0xffffffffu);
-        for (uint32_t s = j - run[lo]; s > 0; s--) holes &= holes - 1;
-        out[lo * 32 + __ffs(holes) - 1] = t;
+    const int moved = (int)block_scan(run + mw + 1, words - mw, kth.sums);
+    for (int t = threadIdx.x; t < m; t += EV_THREADS)
+        if (kept[t >> 5] >> (t & 31) & 1) out[t] = t;
+    // the j-th kept entry behind takes the j-th freed slot
+    for (int j = threadIdx.x; j < moved; j += EV_THREADS) {
+        const int h = last_upto(run, mw + 1, j), f = mw + last_upto(run + mw + 1, words - mw, j);
+        const uint32_t holes = ~kept[h] & (h == mw ? low : 0xffffffffu), behind = f == mw ? kept[f] & ~low : kept[f];
+        out[h * 32 + nth_bit(holes, j - run[h])] = f * 32 + nth_bit(behind, j - run[f + 1]);
     }
 }
 
