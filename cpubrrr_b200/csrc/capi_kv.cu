@@ -8,13 +8,16 @@ using namespace brrr;
 namespace {
 
 static_assert(KV_TREE_MAX == BRRR_TREE_MAX, "");
+constexpr int KV_HEADS_MAX = 512;         // heads x tiles of rows are a grid's second dimension
 
 bool off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
+template <class... P>
+bool off4(const P *...p) { return ((... | (uintptr_t)p) & 3) != 0; }
 
 // The view for the kernels; false where it describes no cache.
 bool view(const brrr_kv *c, KvDev *out) {
     if (!c || !c->k || !c->v || (c->type != BRRR_KV_F32 && c->type != BRRR_KV_BF16)) return false;
-    if (c->n_seq <= 0 || c->n_head_kv <= 0 || c->n_head_kv > 65535 || (c->head_dim != 64 && c->head_dim != 128) || c->cap <= 0 || c->cap > BRRR_KV_CAP_MAX) return false;
+    if (c->n_seq <= 0 || c->n_head_kv <= 0 || c->n_head_kv > KV_HEADS_MAX || (c->head_dim != 64 && c->head_dim != 128) || c->cap <= 0 || c->cap > BRRR_KV_CAP_MAX) return false;
     if (off16(c->k) || off16(c->v) || ((uintptr_t)c->weight & 3) || ((uintptr_t)c->pos & 3) || ((uintptr_t)c->err & 3)) return false;
     const int64_t head = (int64_t)c->cap * c->head_dim;
     if (c->head_stride < 0 || c->seq_stride < 0 || c->head_stride % 8 || c->seq_stride % 8) return false;
@@ -40,6 +43,7 @@ bool apart(const void *a, int64_t na, const void *b, int64_t nb) {
     return x + (uintptr_t)na <= y || y + (uintptr_t)nb <= x;
 }
 
+bool finite(float x) { return x - x == 0.0f; }
 bool heads_ok(const KvDev &d, int n_head) { return n_head > 0 && n_head % d.nkv == 0 && n_head / d.nkv <= 16; }
 
 // The memory belongs to the device whose stream the kernels go to: a pointer of another one (or of the host) would fault there.
@@ -63,7 +67,7 @@ extern "C" int brrr_kv_append(const brrr_kv *kv, int n, int rows, const int32_t 
     KvDev d;
     if (!view(kv, &d) || !d_len || !d_qkv || off16(d_qkv) || off16(d_q) || ((uintptr_t)d_rope & 15)) return BRRR_ERR_ARG;
     if (n <= 0 || n > 65535 || rows <= 0 || rows > d.cap || n_head < 0 || (n_head > 0 && !heads_ok(d, n_head)) || (d_q && n_head == 0)) return BRRR_ERR_ARG;
-    if ((d_rope && n_rope <= 0) || (!d_seq && n > d.n_seq)) return BRRR_ERR_ARG;
+    if ((d_rope && n_rope <= 0) || (!d_seq && n > d.n_seq) || off4(d_seq, d_len, d_count, d_at)) return BRRR_ERR_ARG;
     const int64_t width = (int64_t)(n_head + 2 * d.nkv) * d.hd;
     if (ld == 0) ld = width;
     if (ld < width || ld % 4) return BRRR_ERR_ARG;
@@ -76,6 +80,7 @@ extern "C" int brrr_attn_tree(const brrr_kv *kv, int n, int rows, const int32_t 
     KvDev d;
     if (!view(kv, &d) || !d_len || !d_q || !d_out || off16(d_q) || off16(d_out) || ((uintptr_t)d_mask & 7)) return BRRR_ERR_ARG;
     if (n <= 0 || n > 65535 || rows <= 0 || rows > BRRR_TREE_MAX || !heads_ok(d, n_head) || window < 0 || (!d_seq && n > d.n_seq)) return BRRR_ERR_ARG;
+    if (!finite(scale) || off4(d_seq, d_len, d_count, d_sinks, d_lse)) return BRRR_ERR_ARG;
     if (int rc = on_this_device(d)) return rc;
     const TreeArgs a{n, rows, d_seq, d_len, d_count, d_mask, d_q, n_head, scale, window, d_sinks, d_out, d_lse};
     return done(launch_attn_tree(d, a, len_hint, (cudaStream_t)stream));
@@ -85,7 +90,7 @@ extern "C" int brrr_kv_commit(const brrr_kv *kv, int n, int rows, const int32_t 
                               int32_t *d_new_len, void *stream) {
     KvDev d;
     if (!view(kv, &d) || !d_len || !d_path || !d_npath || d_new_len == d_len) return BRRR_ERR_ARG;
-    if (n <= 0 || n > 65535 || rows <= 0 || rows > BRRR_TREE_MAX || (!d_seq && n > d.n_seq)) return BRRR_ERR_ARG;
+    if (n <= 0 || n > 65535 || rows <= 0 || rows > BRRR_TREE_MAX || (!d_seq && n > d.n_seq) || off4(d_seq, d_len, d_path, d_npath, d_new_len)) return BRRR_ERR_ARG;
     if (int rc = on_this_device(d)) return rc;
     return done(launch_kv_commit(d, n, rows, d_seq, d_len, d_path, d_npath, d_new_len, (cudaStream_t)stream));
 }
@@ -95,6 +100,7 @@ extern "C" int brrr_kv_weigh(const brrr_kv *kv, int n, int rows, const int32_t *
     KvDev d;
     if (!view(kv, &d) || !d.weight || !d_len || !d_q || !d_lse || off16(d_q) || ((uintptr_t)d_mask & 7) || ((uintptr_t)d_rows & 7)) return BRRR_ERR_ARG;
     if (n <= 0 || n > 65535 || rows <= 0 || rows > BRRR_TREE_MAX || !heads_ok(d, n_head) || window < 0 || (!d_seq && n > d.n_seq)) return BRRR_ERR_ARG;
+    if (!finite(scale) || off4(d_seq, d_len, d_count, d_lse)) return BRRR_ERR_ARG;
     if (int rc = on_this_device(d)) return rc;
     const TreeArgs a{n, rows, d_seq, d_len, d_count, d_mask, d_q, n_head, scale, window, nullptr, nullptr, const_cast<float *>(d_lse)};
     return done(launch_kv_weigh(d, a, d_rows, len_hint, (cudaStream_t)stream));
@@ -105,7 +111,7 @@ extern "C" int brrr_kv_evict(const brrr_kv *kv, const brrr_kv *dst, int n, const
     KvDev d, to;
     if (!view(kv, &d) || !d.weight || !d.pos || !d_len || !d_map || d_new_len == d_len) return BRRR_ERR_ARG;
     if (n <= 0 || n > 65535 || keep <= 0 || keep > d.cap || first < 0 || recent < 0 || first > keep || recent > keep - first) return BRRR_ERR_ARG;
-    if ((recent > 0 && !d_end) || (!d_seq && n > d.n_seq)) return BRRR_ERR_ARG;
+    if ((recent > 0 && !d_end) || (!d_seq && n > d.n_seq) || off4(d_seq, d_len, d_end, d_map, d_new_len)) return BRRR_ERR_ARG;
     if (dst) {
         if (!view(dst, &to) || !to.weight || !to.pos || to.type != d.type || to.nkv != d.nkv || to.hd != d.hd || to.cap < keep || (!d_seq && n > to.n_seq)) return BRRR_ERR_ARG;
         const int64_t x = extent(d), y = extent(to), bx = (int64_t)d.n_seq * d.nkv * d.cap * 4, by = (int64_t)to.n_seq * to.nkv * to.cap * 4;
@@ -123,7 +129,7 @@ extern "C" int brrr_kv_means(const brrr_kv *kv, int n, const int32_t *d_seq, con
     KvDev d;
     if (!view(kv, &d) || !d_len || off16(d_means) || (block != 16 && block != 32 && block != 64 && block != 128)) return BRRR_ERR_ARG;
     if (!d_means && d.cap >= block) return BRRR_ERR_ARG;         // a cache shorter than a block has no means
-    if (n <= 0 || n > 65535 || (!d_seq && n > d.n_seq)) return BRRR_ERR_ARG;
+    if (n <= 0 || n > 65535 || (!d_seq && n > d.n_seq) || off4(d_seq, d_since, d_len)) return BRRR_ERR_ARG;
     if (int rc = on_this_device(d)) return rc;
     return done(launch_kv_means(d, n, d_seq, d_since, d_len, block, len_hint, d_means, (cudaStream_t)stream));
 }
@@ -135,7 +141,7 @@ extern "C" int brrr_attn_blocks(const brrr_kv *kv, int rows, const int32_t *d_se
     if (!view(kv, &d) || !d_len || !d_q || !d_sel || !d_out || off16(d_means) || off16(d_q) || off16(d_out)) return BRRR_ERR_ARG;
     if ((block != 16 && block != 32 && block != 64 && block != 128) || (!d_means && d.cap >= block)) return BRRR_ERR_ARG;
     if (rows <= 0 || rows > 65535 || !heads_ok(d, n_head) || nsel <= 0 || nsel > 256 || first < 0 || local < 1 || first > nsel || local > nsel - first) return BRRR_ERR_ARG;
-    if (!d_seq && rows > d.n_seq) return BRRR_ERR_ARG;
+    if ((!d_seq && rows > d.n_seq) || !finite(scale) || off4(d_seq, d_len, d_sinks, d_sel, d_lse)) return BRRR_ERR_ARG;
     if (d.cap / block > 16384) return BRRR_ERR_RANGE;
     if (int rc = on_this_device(d)) return rc;
     return done(launch_attn_blocks(d, rows, d_seq, d_len, block, d_means, nsel, first, local, len_hint, d_q, n_head, scale, d_sinks, d_sel, d_out, d_lse,

@@ -6,11 +6,7 @@ with data_ptr() (a contiguous torch tensor); `stream` is a cudaStream_t as an in
 """
 import ctypes as C
 
-from ._lib import Kv, check, lib
-
-
-def _p(x):
-    return x if x is None or isinstance(x, int) else x.data_ptr()
+from ._lib import BrrrError, Kv, check, lib
 
 
 class KvCache:
@@ -19,37 +15,65 @@ class KvCache:
 
     def __init__(self, k, v, n_seq, n_head_kv, head_dim, cap, bf16=False, head_stride=0, seq_stride=0, weight=None, pos=None, err=None):
         self._held = (k, v, weight, pos, err)      # the memory stays as long as the view
-        self.view = Kv(_p(k), _p(v), int(bool(bf16)), n_seq, n_head_kv, head_dim, cap, head_stride, seq_stride, _p(weight), _p(pos), _p(err))
+        self._dev = None if isinstance(k, int) or k is None else k.get_device()
+        # k and v may have any strides: head_stride and seq_stride describe them
+        size, book = 2 if bf16 else 4, n_seq * n_head_kv * cap
+        self.view = Kv(self._at(k, 0, size, False), self._at(v, 0, size, False), int(bool(bf16)), n_seq, n_head_kv, head_dim, cap, head_stride, seq_stride,
+                       self._at(weight, book), self._at(pos, book), self._at(err, 1))
         self._ref = C.byref(self.view)
+        self._lib = lib()
+
+    def _at(self, x, need=0, size=4, dense=True):
+        """The address of a device array; a tensor has to be dense, of `size` bytes a value, of `need` values at least and on the cache's device."""
+        if x is None or isinstance(x, int):
+            return x
+        if (x.element_size() != size or x.numel() < need or (dense and not x.is_contiguous()) or
+                (x.get_device() != self._dev if self._dev is not None else x.get_device() < 0)):
+            raise BrrrError(f"KvCache: a contiguous array of {need} or more {size}-byte values on the cache's device is wanted, not {tuple(x.shape)} {x.dtype} on {x.device}")
+        return x.data_ptr()
 
     def append(self, n, rows, length, qkv, n_head=0, q=None, at=None, rope=None, n_rope=0, count=None, seq=None, ld=0, stream=None):
         """Rows of q | k | v into the cache at slots length[b] + i, rotated by their positions; rotated q to `q`."""
-        check(lib().brrr_kv_append(self._ref, n, rows, _p(seq), _p(length), _p(count), _p(at), _p(qkv), ld, n_head, _p(rope), n_rope, _p(q), stream), "brrr_kv_append")
+        p, v = self._at, self.view
+        width = (n_head + 2 * v.n_head_kv) * v.head_dim
+        check(self._lib.brrr_kv_append(self._ref, n, rows, p(seq, n), p(length, n), p(count, n), p(at, n * rows), p(qkv, (n * rows - 1) * (ld or width) + width), ld, n_head,
+                                       p(rope, n_rope * v.head_dim), n_rope, p(q, n * rows * n_head * v.head_dim), stream), "brrr_kv_append")
 
     def attn_tree(self, n, rows, length, q, n_head, out, scale, seq=None, count=None, mask=None, len_hint=0, window=0, sinks=None, lse=None, stream=None):
         """Attention of drafted tokens (ancestor masks; None: a chain) over the cache and their own entries."""
-        check(lib().brrr_attn_tree(self._ref, n, rows, _p(seq), _p(length), _p(count), _p(mask), len_hint, _p(q), n_head, scale, window, _p(sinks), _p(out), _p(lse),
-                                   stream), "brrr_attn_tree")
+        p, heads = self._at, n * rows * n_head
+        values = heads * self.view.head_dim
+        check(self._lib.brrr_attn_tree(self._ref, n, rows, p(seq, n), p(length, n), p(count, n), p(mask, n * rows, 8), len_hint, p(q, values), n_head, scale, window,
+                                       p(sinks, n_head), p(out, values), p(lse, heads), stream), "brrr_attn_tree")
 
     def commit(self, n, rows, length, path, npath, seq=None, new_len=None, stream=None):
         """The accepted rows of each tree to the slots behind the cached entries."""
-        check(lib().brrr_kv_commit(self._ref, n, rows, _p(seq), _p(length), _p(path), _p(npath), _p(new_len), stream), "brrr_kv_commit")
+        p = self._at
+        check(self._lib.brrr_kv_commit(self._ref, n, rows, p(seq, n), p(length, n), p(path, n * rows), p(npath, n), p(new_len, n), stream), "brrr_kv_commit")
 
     def weigh(self, n, rows, length, q, n_head, lse, scale, seq=None, count=None, mask=None, picked=None, len_hint=0, window=0, stream=None):
         """The attention weights of the rows (of those whose bit in `picked` is set) added to the cache's book."""
-        check(lib().brrr_kv_weigh(self._ref, n, rows, _p(seq), _p(length), _p(count), _p(mask), _p(picked), len_hint, _p(q), n_head, scale, window, _p(lse), stream),
-              "brrr_kv_weigh")
+        p, heads = self._at, n * rows * n_head
+        check(self._lib.brrr_kv_weigh(self._ref, n, rows, p(seq, n), p(length, n), p(count, n), p(mask, n * rows, 8), p(picked, n, 8), len_hint,
+                                      p(q, heads * self.view.head_dim), n_head, scale, window, p(lse, heads), stream), "brrr_kv_weigh")
 
     def evict(self, n, length, keep, first, recent, end, map, seq=None, dst=None, new_len=None, len_hint=0, stream=None):
         """The `keep` entries of each head with the largest weights (and the first and latest ones) in place, or into another KvCache."""
-        check(lib().brrr_kv_evict(self._ref, None if dst is None else dst._ref, n, _p(seq), _p(length), keep, first, recent, _p(end), _p(map), _p(new_len), len_hint,
-                                  stream), "brrr_kv_evict")
+        p = self._at
+        check(self._lib.brrr_kv_evict(self._ref, None if dst is None else dst._ref, n, p(seq, n), p(length, n), keep, first, recent, p(end, n),
+                                      p(map, n * self.view.n_head_kv * keep), p(new_len, n), len_hint, stream), "brrr_kv_evict")
 
     def means(self, n, length, block, means, seq=None, since=None, len_hint=0, stream=None):
         """Means of the keys of the whole blocks between since[b] and length[b]."""
-        check(lib().brrr_kv_means(self._ref, n, _p(seq), _p(since), _p(length), block, len_hint, _p(means), stream), "brrr_kv_means")
+        p = self._at
+        check(self._lib.brrr_kv_means(self._ref, n, p(seq, n), p(since, n), p(length, n), block, len_hint, p(means, self._means(block)), stream), "brrr_kv_means")
 
     def attn_blocks(self, rows, seq, length, block, means, nsel, first, local, q, n_head, out, scale, sel, len_hint=0, sinks=None, lse=None, stream=None):
         """Attention of each row over the nsel blocks of its sequence that it scores highest; the choice goes to `sel`."""
-        check(lib().brrr_attn_blocks(self._ref, rows, _p(seq), _p(length), block, _p(means), nsel, first, local, len_hint, _p(q), n_head, scale, _p(sinks), _p(sel),
-                                     _p(out), _p(lse), stream), "brrr_attn_blocks")
+        p, values = self._at, rows * n_head * self.view.head_dim
+        check(self._lib.brrr_attn_blocks(self._ref, rows, p(seq, rows), p(length, rows), block, p(means, self._means(block)), nsel, first, local, len_hint, p(q, values), n_head,
+                                         scale, p(sinks, n_head), p(sel, rows * self.view.n_head_kv * nsel), p(out, values), p(lse, rows * n_head), stream), "brrr_attn_blocks")
+
+    def _means(self, block):
+        v = self.view
+        return v.n_seq * v.n_head_kv * (v.cap // block) * v.head_dim if block > 0 else 0

@@ -304,14 +304,15 @@ int brrr_qwen_cli_main(int argc, char **argv);
  * commit, weigh, evict, means) has named already, is left out, its outputs stay as they were, and *err (if given) becomes 1.
  * d_seq [n] names the sequences of a call; NULL: entry b is sequence b.  len_hint: about the largest length among the entries (0: unknown);
  * it steers how work is split, never what is computed.
- * A slot that a row does not see may hold anything, infinities and NaN included; a row that sees such a value has no defined result. */
+ * A slot that a row does not see may hold anything, infinities and NaN included; a row that sees such a value has no defined result.  A sink may be
+ * -infinity (no sink for that head), not +infinity; `scale` is any finite number. */
 enum { BRRR_KV_F32 = 0, BRRR_KV_BF16 = 1 };
 #define BRRR_TREE_MAX 64     /* rows per sequence of brrr_attn_tree, brrr_kv_commit and brrr_kv_weigh */
 #define BRRR_KV_CAP_MAX (1 << 19)     /* largest capacity */
 typedef struct brrr_kv {
     void *k, *v;                      /* [n_seq][n_head_kv][cap][head_dim] values of `type`, keys rotated; 16-byte aligned */
     int32_t type;                     /* BRRR_KV_F32 (the engines' caches) or BRRR_KV_BF16 */
-    int32_t n_seq, n_head_kv;
+    int32_t n_seq, n_head_kv;         /* n_head_kv <= 512 */
     int32_t head_dim;                 /* 64 or 128 */
     int32_t cap;                      /* slots per head */
     int64_t head_stride, seq_stride;  /* values from one head to the next and from one sequence to the next, multiples of 8; 0: dense */

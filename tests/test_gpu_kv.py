@@ -275,6 +275,146 @@ def test_offsets_beyond_32_bits(brrr, dev):
     assert int(err) == 0
 
 
+# ---------------------------------------------------------------- many rows: the kernels of 128-row tiles
+WIDE = [
+    dict(n=1, rows=64, lens=[700], heads=64, kv=4, hd=64, masks="tree"),
+    dict(n=3, rows=33, lens=[1301, 0, 640], heads=64, kv=4, hd=64, masks="any", counts=[33, 17, 33], sinks=True),
+    dict(n=2, rows=64, lens=[1025, 1152], heads=32, kv=2, hd=64, masks="tree", window=200),
+    dict(n=4, rows=64, lens=[130, 127, 129, 64], heads=48, kv=6, hd=64, masks="chain", seq=[4, 1, 0, 2], pad=16),
+    dict(n=2, rows=40, lens=[900, 77], heads=48, kv=3, hd=128, masks="tree"),
+    dict(n=2, rows=64, lens=[511, 1090], heads=32, kv=2, hd=128, masks="any", window=64, sinks=True),
+    dict(n=3, rows=50, lens=[641, 640, 639], heads=48, kv=4, hd=128, masks="chain", counts=[50, 1, 49], heads_outside=True),
+    dict(n=1, rows=61, lens=[1999], heads=32, kv=2, hd=64, masks="tree", bf16=True),
+    dict(n=2, rows=64, lens=[500, 1301], heads=64, kv=4, hd=64, masks="any", bf16=True, counts=[0, 64], sinks=True, window=333),
+    dict(n=24, rows=64, lens=[30 + 2 * i for i in range(24)], heads=16, kv=2, hd=64, masks="tree", bf16=True),
+    dict(n=2, rows=47, lens=[1280, 831], heads=32, kv=2, hd=128, masks="tree", bf16=True, seq=[2, 2], pad=8),
+    dict(n=1, rows=64, lens=[2500], heads=16, kv=1, hd=128, masks="chain", bf16=True, window=1000),
+]
+
+
+def reference(s, c, q, scale):
+    """The definition in 64 bits on the GPU, entry by entry: out, lse, and the weights of every row [n][rows][heads][slots]."""
+    import torch
+    k, v = s.k.double().nan_to_num(0.0, 0.0, 0.0), s.v.double().nan_to_num(0.0, 0.0, 0.0)       # what is no number here nobody sees
+    n, rows, heads, hd = q.shape
+    out, lse, weights = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape[:3], dtype=torch.float64, device=q.device), []
+    for b in range(n):
+        m, ln = s.counts[b], s.lens[b]
+        if not m:
+            weights.append(None)
+            continue
+        live = [x & ((1 << m) - 1) for x in s.masks[b][:m]]
+        seen = torch.zeros((m, ln + m), dtype=torch.bool, device=q.device)
+        for i in range(m):
+            di = R.depth(live[i], i)
+            seen[i, max(0, ln + di + 1 - s.window) if s.window else 0: ln] = True
+            seen[i, ln:] = torch.tensor([bool(live[i] >> j & 1) and (not s.window or di - R.depth(live[j], j) < s.window) for j in range(m)], device=q.device)
+        per = heads // c["kv"]
+        x = torch.einsum("ihd,htd->iht", q[b, :m].double(), k[s.seq[b], :, : ln + m].repeat_interleave(per, 0)) * scale
+        x = x.masked_fill(~seen[:, None], -math.inf)
+        full = x if s.sinks is None else torch.cat([x, s.up(s.sinks).double().view(1, -1, 1).expand(m, -1, 1)], -1)
+        lse[b, :m] = torch.logsumexp(full, -1)
+        w = torch.exp(x - lse[b, :m, :, None]).nan_to_num(0.0)
+        out[b, :m] = torch.einsum("iht,htd->ihd", w, v[s.seq[b], :, : ln + m].repeat_interleave(per, 0))
+        weights.append(w)
+    return out, lse, weights
+
+
+@pytest.mark.parametrize("scale", [1.0, -1.3])
+@pytest.mark.parametrize("c", WIDE, ids=lambda c: "-".join(str(c[k]) for k in ("n", "rows", "heads", "kv", "hd", "masks")) + ("-bf16" if c.get("bf16") else ""))
+def test_wide_trees_and_their_weights(brrr, dev, c, scale):
+    import torch
+    s = prepared_tree(dev, c, seed=31)
+    s.scale *= scale
+    n, rows, per = c["n"], c["rows"], c["heads"] // c["kv"]
+    want, want_lse, weights = reference(s, c, s.up(s.q), s.scale)
+    for hint in (0, 1):              # a small hint sends the same call to the kernel of 16-row tiles
+        out, lse = run_tree(brrr, s, c, hint=hint)
+        assert s.ok()
+        again, _ = run_tree(brrr, s, c, hint=hint)
+        assert torch.equal(out, again)
+        for b in range(n):
+            m = s.counts[b]
+            if m:
+                close(out[b, :m].cpu().numpy().reshape(m, c["heads"], c["hd"]), want[b, :m].cpu().numpy())
+                close_lse(lse[b, :m].cpu().numpy(), want_lse[b, :m].cpu().numpy())
+            assert (out[b, m:] == 7.0).all() and (lse[b, m:] == 7.0).all()
+    if "seq" in c and len(set(s.seq)) < n:
+        return                       # a sequence may be weighed once in a call
+    picked = [int(x) for x in s.rng.integers(0, 1 << 63, n)]
+    for pick in (None, picked):
+        s.weight.fill_(1.0)
+        s.view(brrr).weigh(n, rows, s.up(s.lens, np.int32), s.up(s.q), c["heads"], lse, s.scale, seq=s.up(s.seq, np.int32) if "seq" in c else None,
+                           count=s.up(s.counts, np.int32) if "counts" in c else None, mask=None if c["masks"] == "chain" else s.up(np.array(s.masks, np.uint64)),
+                           picked=None if pick is None else s.up(np.array(pick, np.uint64)), window=s.window)
+        torch.cuda.synchronize()
+        assert s.ok()
+        book = torch.ones(s.weight.shape, dtype=torch.float64, device=dev)
+        for b in range(n):
+            m = s.counts[b]
+            if m:
+                rows_in = torch.tensor([pick is None or bool(pick[b] >> i & 1) for i in range(m)], device=dev)
+                book[s.seq[b], :, : s.lens[b] + m] += (weights[b] * rows_in[:, None, None]).sum(0).view(c["kv"], per, -1).sum(1)
+        close(s.weight.cpu().numpy(), book.cpu().numpy())
+        untouched = book == 1.0
+        assert (s.weight[untouched] == 1.0).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_wide_rows_do_not_touch_what_other_rows_see(brrr, dev, bf16, hd):
+    """As for few rows: drafted rows and cached slots that are no numbers concern the rows that see them, in outputs and in the book."""
+    import torch
+    c = dict(n=1, rows=64, lens=[900], heads=32, kv=2, hd=hd, masks="tree", bf16=bf16)
+    s = prepared_tree(dev, c, seed=9)
+    s.masks, s.window = [[1 << i | (s.masks[0][i] & 1) for i in range(64)]], 300       # rows see row 0 or nobody but themselves
+    s.masks[0][0] = 1
+    s.k.nan_to_num_(0.1), s.v.nan_to_num_(0.2, 0.3, 0.4)
+    want, _, weights = reference(s, c, s.up(s.q), s.scale)
+    s.v[0, :, 917] = float("inf"); s.k[0, :, 917] = float("nan")      # row 17
+    s.v[0, 1, 930, 3] = float("nan")                                  # row 30, one dimension of one head
+    shallow = [i for i in range(64) if R.depth(s.masks[0][i], i) == 0]
+    s.v[0, :, 601] = float("nan"); s.k[0, :, 601] = float("inf")      # seen by depth 0 alone (601 = 900 + 0 + 1 - 300)
+    out, lse = run_tree(brrr, s, c)
+    out = out.cpu().numpy().reshape(64, 32, hd)
+    fine = [i for i in range(64) if i not in shallow and i not in (17, 30)]
+    close(out[fine], want[0, fine].cpu().numpy())
+    close(out[30, :16], want[0, 30, :16].cpu().numpy()) if 30 not in shallow else None
+    picked = sum(1 << i for i in fine)
+    s.view(brrr).weigh(1, 64, s.up(s.lens, np.int32), s.up(s.q), 32, lse, s.scale, mask=s.up(np.array(s.masks, np.uint64)), picked=s.up(np.array([picked], np.uint64)), window=300)
+    torch.cuda.synchronize()
+    book = (weights[0][fine].sum(0)).view(2, 16, -1).sum(1)
+    close(s.weight[0, :, :964].cpu().numpy(), book.cpu().numpy())
+
+
+def test_wide_rows_far_beyond_32_bits(brrr, dev):
+    import torch
+    stride, cap, hd, kv, rows, heads, ln = (1 << 32) + 64, 1000, 64, 2, 64, 32, 900
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 20 GB of device memory")
+    buf = [torch.empty(stride + kv * cap * hd, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    rng = np.random.default_rng(5)
+    x = [torch.from_numpy(rng.standard_normal((1, kv, cap, hd)).astype(np.float32)).to(dev).bfloat16() for _ in range(2)]
+    for b, y in zip(buf, x):
+        b[stride:] = y.flatten()
+    weight, err = torch.zeros((2, kv, cap), device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    view = brrr.KvCache(buf[0], buf[1], 2, kv, hd, cap, bf16=True, seq_stride=stride, weight=weight, err=err)
+    q = torch.from_numpy(rng.standard_normal((1, rows, heads, hd)).astype(np.float32)).to(dev)
+    out, lse, seq, lens = torch.zeros((1, rows, heads * hd), device=dev), torch.zeros((1, rows, heads), device=dev), torch.ones(1, dtype=torch.int32, device=dev), \
+        torch.full((1,), ln, dtype=torch.int32, device=dev)
+    view.attn_tree(1, rows, lens, q, heads, out, 0.125, seq=seq, lse=lse)
+    view.weigh(1, rows, lens, q, heads, lse, 0.125, seq=seq)
+    torch.cuda.synchronize()
+
+    class Near:
+        k, v, counts, lens, masks, window, sinks, seq = x[0], x[1], [rows], [ln], [R.chain(rows)], 0, None, [0]
+    want, want_lse, weights = reference(Near, dict(kv=kv), q, 0.125)
+    close(out.cpu().numpy().reshape(want.shape), want.cpu().numpy())
+    close_lse(lse.cpu().numpy(), want_lse.cpu().numpy())
+    close(weight[1, :, : ln + rows].cpu().numpy(), weights[0].sum(0).view(kv, 16, -1).sum(1).cpu().numpy())
+    assert int(err) == 0 and not weight[0].any()
+
+
 # ---------------------------------------------------------------- append
 @pytest.mark.parametrize("hd,bf16,turn,nh,out_q", [(64, False, True, 9, True), (128, True, True, 6, True), (64, True, False, 0, False), (128, False, False, 3, True), (64, False, True, 6, False)])
 def test_append(brrr, dev, hd, bf16, turn, nh, out_q):
@@ -652,6 +792,8 @@ def test_graphs_and_streams(brrr, dev):
     import torch
     c = dict(n=2, rows=11, lens=[600, 410], heads=16, kv=2, hd=64, masks="tree")
     s = prepared_tree(dev, c)
+    wide = prepared_tree(dev, dict(n=1, rows=64, lens=[700], heads=64, kv=4, hd=64, masks="tree", bf16=True))
+    wq, wmask, wlen, wview = wide.up(wide.q), wide.up(np.array(wide.masks, np.uint64)), wide.up([700], np.int32), wide.view(brrr)
     view = s.view(brrr)
     s.k.nan_to_num_(0.0), s.v.nan_to_num_(0.0, 0.0, 0.0)
     n, rows = 2, 11
@@ -661,11 +803,13 @@ def test_graphs_and_streams(brrr, dev):
     q1 = q[:, 0].contiguous()
 
     def bufs():
-        return (torch.zeros((n, rows, 16 * 64), device=dev), torch.zeros((n, rows, 16), device=dev), torch.zeros((2, 2, 5), dtype=torch.int32, device=dev), torch.zeros((2, 16 * 64), device=dev))
+        return (torch.zeros((n, rows, 16 * 64), device=dev), torch.zeros((n, rows, 16), device=dev), torch.zeros((2, 2, 5), dtype=torch.int32, device=dev), torch.zeros((2, 16 * 64), device=dev),
+                torch.zeros((1, 64, 64 * 64), device=dev))
 
     def read(o, st):
         view.attn_tree(n, rows, lens, q, 16, o[0], 0.125, mask=mask, lse=o[1], stream=st)
         view.attn_blocks(2, None, lens, 16, means, 5, 1, 1, q1, 16, o[3], 0.125, o[2], stream=st)
+        wview.attn_tree(1, 64, wlen, wq, 64, o[4], 0.125, mask=wmask, stream=st)
     eager = bufs()
     read(eager, None)
     torch.cuda.synchronize()

@@ -13,7 +13,7 @@ def view(B, **kw):
     return B._lib.Kv(*[d[n] for n, _ in B._lib.Kv._fields_])
 
 
-BAD_VIEWS = [dict(k=None), dict(v=None), dict(k=P + 8), dict(v=2 * P + 4), dict(type=2), dict(type=-1), dict(n_seq=0), dict(n_head_kv=0), dict(n_head_kv=65536),
+BAD_VIEWS = [dict(k=None), dict(v=None), dict(k=P + 8), dict(v=2 * P + 4), dict(type=2), dict(type=-1), dict(n_seq=0), dict(n_head_kv=0), dict(n_head_kv=513),
              dict(head_dim=96), dict(head_dim=0), dict(cap=0), dict(cap=(1 << 19) + 1), dict(head_stride=-64), dict(head_stride=6404), dict(head_stride=6392),
              dict(seq_stride=6400 * 4 - 8), dict(seq_stride=6408), dict(n_head_kv=1, head_stride=8, seq_stride=6392), dict(head_stride=6400, seq_stride=1 << 51),
              dict(weight=3 * P + 2), dict(pos=4 * P + 1), dict(err=5 * P + 3)]
@@ -58,14 +58,15 @@ def test_append(brrr):
 def test_tree_and_weigh(brrr):
     L, v, bare = brrr.lib(), view(brrr), view(brrr, weight=None)
 
-    def tree(n=1, rows=1, len=P, mask=None, q=P, nh=8, window=0, out=P):
-        return L.brrr_attn_tree(C.byref(v), n, rows, None, len, None, mask, 0, q, nh, 1.0, window, None, out, None, None)
+    def tree(n=1, rows=1, seq=None, len=P, count=None, mask=None, q=P, nh=8, scale=1.0, window=0, sinks=None, out=P, lse=None):
+        return L.brrr_attn_tree(C.byref(v), n, rows, seq, len, count, mask, 0, q, nh, scale, window, sinks, out, lse, None)
 
-    def weigh(n=1, rows=1, len=P, mask=None, picked=None, q=P, nh=8, window=0, lse=P, v=v):
-        return L.brrr_kv_weigh(C.byref(v), n, rows, None, len, None, mask, picked, 0, q, nh, 1.0, window, lse, None)
-    both = dict(n=[0, -1, 4, 65536], rows=[0, 65, -2], len=[None], mask=[P + 4], q=[None, P + 4], nh=[0, -4, 6, 68], window=[-1])
-    refuse(tree, {}, {**both, "out": [None, P + 8]})
-    refuse(weigh, {}, {**both, "picked": [P + 4], "lse": [None], "v": [bare]})
+    def weigh(n=1, rows=1, seq=None, len=P, count=None, mask=None, picked=None, q=P, nh=8, scale=1.0, window=0, lse=P, v=v):
+        return L.brrr_kv_weigh(C.byref(v), n, rows, seq, len, count, mask, picked, 0, q, nh, scale, window, lse, None)
+    both = dict(n=[0, -1, 4, 65536], rows=[0, 65, -2], seq=[P + 2], len=[None, P + 1], count=[P + 2], mask=[P + 4], q=[None, P + 4], nh=[0, -4, 6, 68], window=[-1],
+                scale=[float("nan"), float("inf"), -float("inf")])
+    refuse(tree, {}, {**both, "out": [None, P + 8], "sinks": [P + 1], "lse": [P + 2]})
+    refuse(weigh, {}, {**both, "picked": [P + 4], "lse": [None, P + 2], "v": [bare]})
 
 
 def test_commit(brrr):
@@ -118,3 +119,14 @@ def test_the_binding_passes_what_the_header_says(brrr):
     with pytest.raises(brrr.BrrrError, match="brrr_kv_weigh.*argument"):
         kv.weigh(1, 1, P, P, 8, P, 1.0)
     assert kv.TREE_MAX == int(re.search(r"#define BRRR_TREE_MAX (\d+)", src).group(1))
+
+
+def test_the_class_takes_tensors_of_the_right_kind_only(brrr):
+    """Arrays of another value size, with strides, or in host memory beside a device cache never become addresses."""
+    import torch
+    kv = brrr.KvCache(P, 2 * P, 3, 4, 64, 100, weight=3 * P, pos=4 * P)
+    i32, i64 = torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int64)
+    for call in (lambda: kv.attn_tree(1, 1, i32, P, 8, P, 1.0), lambda: kv.commit(1, 1, P, i64, P), lambda: kv.evict(1, i64, 5, 0, 0, None, P),
+                 lambda: kv.weigh(1, 1, P, P, 8, P, 1.0, picked=i32)):
+        with pytest.raises(brrr.BrrrError, match="cache's device"):
+            call()
