@@ -1,16 +1,17 @@
 // Attention over KV caches that the caller owns: trees of drafted tokens, chosen blocks, and the book of attention weights.
 //
-// Rows are (drafted token, query head of one kv head) pairs, 16 to a tile of mma.sync (m16n8k8, tf32 operands, f32 sums); a warp holds one tile of
-// rows and walks slots in steps of 16.  Results are single precision: an f32 operand x is split into hi = x rounded to tf32's 11 bits and the
-// rest lo = x - hi, exact, of which tf32 takes 11 bits again; hi hi + hi lo + lo hi leaves out 2^-22 of a product at most.  bf16 values are tf32
-// values: for such a cache two products are enough.  The tensor cores' adders truncate, so no long sum is left to them: a step's scores take
-// head_dim / 8 additions, a step's share of the output starts at zero and joins the running output by one fused multiply-add that also
-// rescales it to the new running maximum.
+// Rows are (drafted token, query head of one kv head) pairs, 8 or 16 to a CTA; a warp walks slots in steps of 16.  Scores and outputs are formed
+// transposed, S^T = K Q^T and O^T = V^T P^T, with mma.sync (m16n8k8, tf32 operands, f32 sums): slots and dimensions are the 16 rows of operand A, and the
+// 8 columns of operand B are the rows above, of which a token has 8 (64 query heads over 8): nothing is padded.  Results are single precision: an f32 operand
+// x is split into hi = x rounded to tf32's 11 bits and the rest lo = x - hi, exact, of which tf32 takes 11 bits again; hi hi + hi lo + lo hi leaves out
+// 2^-22 of a product at most.  bf16 values are tf32 values: for such a cache two products are enough.  The tensor cores' adders truncate, so no long sum is
+// left to them: a step's scores take head_dim / 16 additions, a step's share of the output starts at zero and joins the running output by one fused
+// multiply-add that also rescales it to the new running maximum.
 //
-// Every warp has a ring of steps of its own in shared memory, filled by bulk copies of consecutive rows several steps ahead, and waits for nobody else.  The k
-// index of operand B may be any order of the dimensions (keys) that operand A has too, so a lane's k = t, t + 4 of consecutive products are the
-// consecutive values of one 16-byte read; the accumulator of the scores, with keys 2t and 2t + 1 in a lane, is operand A of the second product as it
-// stands.  Queries are split once and wait in shared memory in fragment order.
+// Every warp has a ring of operands of its own in shared memory, filled by bulk copies of consecutive rows several operands ahead, and waits for nobody
+// else.  The k index of a product may be any order of the dimensions (slots) that both operands have, so a lane's k = t, t + 4 of consecutive products are the
+// consecutive values of one 16-byte read, and the rows of V^T may be any order of the dimensions.  Weights change from the accumulator's place (slot
+// g, rows 2t, 2t + 1 in lane 4 g + t) to operand B's (slots 2t, 2t + 1, row g) by shuffles.  Queries are split once and wait in shared memory in fragment order.
 //
 // The slots of an entry are split over the warps of a CTA and the CTAs of a cluster, each with its own maximum and sum; partial results meet
 // in shared memory, those of the cluster through distributed shared memory, in a fixed order: one launch, no workspace, no atomics.
@@ -31,12 +32,12 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const float4 &a, float b
 }
 
 
-// A warp's ring: D places for the keys or the values of a step of 8 NK slots each, 12 KB in all.  Lane 0 copies; operand u is u-th in the order in which the warp
-// uses them (keys, values, keys, ...).
-constexpr int RING = 12288;
-template <class T, int HD, int NK>
+// A warp's ring: D places for the keys or the values of a step of 16 slots each.  Lane 0 copies; operands are used in the order in which they are copied (keys,
+// values, keys, ...).
+constexpr int STEP = 16;
+template <class T, int HD>
 struct Ring {
-    static constexpr int STEP = 8 * NK, ROW = HD * (int)sizeof(typename T::Val), PLACE = STEP * ROW, D = RING / PLACE;
+    static constexpr int ROW = HD * (int)sizeof(typename T::Val), PLACE = STEP * ROW, BYTES = PLACE == 8192 ? 16384 : 12288, D = BYTES / PLACE;
     static constexpr int NC = HD / (4 * T::V), NVC = HD / (8 * T::V);       // 16-byte reads of a lane per slot: keys, values
     static_assert(D >= 2 && D <= 8, "");
     uint32_t at;             // of the ring, in shared memory
@@ -44,7 +45,7 @@ struct Ring {
     int in = 0, out = 0, in_turn = 0;      // places that the next copy and the next use take, and the parity of the next use
     __device__ __forceinline__ Ring(unsigned char *mem, uint64_t *bars) {
         const int warp = threadIdx.x >> 5;
-        at = smem_u32(mem) + warp * RING;
+        at = smem_u32(mem) + warp * BYTES;
         full = bars + warp * 8;
         if ((threadIdx.x & 31) == 0) {
             for (int i = 0; i < D; i++) mbar_init(&full[i], 1);
@@ -52,7 +53,7 @@ struct Ring {
         }
         __syncwarp();
     }
-    // slots base .. base + 8 NK - 1 of p, those from end on not read (their place keeps what it had), to the next place, which must have been used
+    // slots base .. base + 15 of p, those from end on not read (their place keeps what it had), to the next place, which must have been used
     __device__ __forceinline__ void bring(const typename T::Val *p, int base, int end) {
         if ((threadIdx.x & 31) == 0) {
             const int bytes = min(STEP, end - base) * ROW;
@@ -81,144 +82,164 @@ struct Ring {
     }
 };
 
-// Queries of `tiles` tiles of 16 rows in fragment order, hi and lo parts: per product (8 dimensions) and lane 16 bytes each.  row(r): the row's
+// Queries of NT tiles of 8 rows as operand B: per product (8 dimensions), tile and lane 16 bytes, the hi and the lo parts of its two values.  row(r): the row's
 // values, or null for a row of padding (zeros).
-template <class T, int HD, class Row>
-__device__ __forceinline__ void stage_queries(float4 *frag, int tiles, Row row) {
-    constexpr int W = 4 * T::V;                 // dimensions that one load of the four lanes of a slot covers
+template <class T, int HD, int NT, class Row>
+__device__ __forceinline__ void stage_queries(float4 *frag, Row row) {
+    constexpr int W = 4 * T::V;                 // dimensions that one read of the four lanes of a slot covers
     float *f = reinterpret_cast<float *>(frag);
-    for (int u = threadIdx.x; u < tiles * 16 * (HD / 4); u += AW * 32) {
+    for (int u = threadIdx.x; u < NT * 8 * (HD / 4); u += AW * 32) {
         const int r = u / (HD / 4), d0 = u % (HD / 4) * 4;
         const float *p = row(r);
         const float4 x4 = p ? *reinterpret_cast<const float4 *>(p + d0) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         const float x[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int d = d0 + i, t = d % W / T::V, step = d / W * (T::V / 2) + d % T::V / 2, odd = d & 1;
-            const int at = ((((r / 16) * (HD / 8) + step) * 2) * 32 + (r % 8) * 4 + t) * 4 + (r % 16) / 8 + 2 * odd;
+            const int d = d0 + i, t = d % W / T::V, product = d / W * (T::V / 2) + d % T::V / 2, odd = d & 1;
+            const int at = ((product * NT + r / 8) * 32 + (r & 7) * 4 + t) * 4 + odd;
             const float hi = tf32_hi(x[i]);
             f[at] = hi;
-            f[at + 32 * 4] = x[i] - hi;
+            f[at + 2] = x[i] - hi;
         }
     }
 }
 
-// Scores of a tile of rows against a step's slots: s[j] as the accumulator of slots 8 j .. 8 j + 7.
-template <class T, int HD, int NK, class R>
-__device__ __forceinline__ void step_scores(uint32_t st, const float4 *frag, float (&s)[NK][4]) {
-    constexpr int P = T::V / 2;                 // products per load
+// Scores of 16 slots: s[n] is the accumulator of rows 8 n ..: slot g (+ 8), rows 2t, 2t + 1.
+template <class T, int HD, int NT>
+__device__ __forceinline__ void step_scores(uint32_t st, const float4 *frag, float (&s)[NT][4]) {
+    typedef Ring<T, HD> R;
+    constexpr int P = T::V / 2;                 // products per read
     const int lane = threadIdx.x & 31;
-    float lo1[NK][4], lo2[NK][4];
+    float sum[NT][T::SPLIT ? 6 : 4][4];         // big and small products of even and odd steps
 #pragma unroll
-    for (int j = 0; j < NK; j++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[j][e] = lo1[j][e] = lo2[j][e] = 0.0f;
+        for (int i = 0; i < (T::SPLIT ? 6 : 4); i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[n][i][e] = 0.0f;
 #pragma unroll
     for (int c = 0; c < R::NC; c++) {
-        float x[NK][T::V];
-#pragma unroll
-        for (int j = 0; j < NK; j++) T::get(R::key(st, j, c), x[j]);
+        float x[2][T::V];
+        T::get(R::key(st, 0, c), x[0]);
+        T::get(R::key(st, 1, c), x[1]);
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            const float4 ah = frag[(c * P + p) * 64 + lane], al = frag[(c * P + p) * 64 + 32 + lane];
+            float4 ah, al;
+            if (T::SPLIT) {
+                ah = make_float4(tf32_hi(x[0][2 * p]), tf32_hi(x[1][2 * p]), tf32_hi(x[0][2 * p + 1]), tf32_hi(x[1][2 * p + 1]));
+                al = make_float4(x[0][2 * p] - ah.x, x[1][2 * p] - ah.y, x[0][2 * p + 1] - ah.z, x[1][2 * p + 1] - ah.w);
+            } else {
+                ah = make_float4(x[0][2 * p], x[1][2 * p], x[0][2 * p + 1], x[1][2 * p + 1]);
+            }
 #pragma unroll
-            for (int j = 0; j < NK; j++) {
-                const float b0 = x[j][2 * p], b1 = x[j][2 * p + 1];
-                if (T::SPLIT) {
-                    const float h0 = tf32_hi(b0), h1 = tf32_hi(b1);
-                    mma_tf32(s[j], ah, h0, h1);
-                    mma_tf32(lo1[j], ah, b0 - h0, b1 - h1);
-                    mma_tf32(lo2[j], al, h0, h1);
-                } else {
-                    mma_tf32(s[j], ah, b0, b1);
-                    mma_tf32(lo1[j], al, b0, b1);
-                }
+            for (int n = 0; n < NT; n++) {
+                const float4 b = frag[((c * P + p) * NT + n) * 32 + lane];
+                constexpr int S = T::SPLIT ? 3 : 2;
+                float(&to)[T::SPLIT ? 6 : 4][4] = sum[n];
+                const int o = p & 1 ? S : 0;
+                mma_tf32(to[o], ah, b.x, b.y);
+                mma_tf32(to[o + 1], ah, b.z, b.w);
+                if (T::SPLIT) mma_tf32(to[o + S - 1], al, b.x, b.y);
             }
         }
     }
 #pragma unroll
-    for (int j = 0; j < NK; j++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[j][e] += T::SPLIT ? lo1[j][e] + lo2[j][e] : lo1[j][e];
+        for (int e = 0; e < 4; e++) {
+            if (T::SPLIT) s[n][e] = (sum[n][0][e] + sum[n][3][e]) + ((sum[n][1][e] + sum[n][2][e]) + (sum[n][4][e] + sum[n][T::SPLIT ? 5 : 0][e]));
+            else s[n][e] = (sum[n][0][e] + sum[n][2][e]) + (sum[n][1][e] + sum[n][3][e]);
+        }
 }
 
-// A warp's running attention of 16 rows: maxima and sums in powers of two of rows lane / 4 and lane / 4 + 8 (the sum: this lane's slots only), and
-// the outputs, o[8 c' + V..]: see finish.
-template <class T, int HD, int NK, class Rg>
+// A warp's running attention of 8 NT rows: maxima and sums in powers of two of rows 8 n + 2t, 2t + 1 (the sum: this lane's slots only), and the outputs.
+template <class T, int HD, int NT>
 struct Running {
-    static constexpr int NN = HD / 8;           // 8 values wide products of the output
-    float m[2], l[2], o[NN][4];
+    typedef Ring<T, HD> R;
+    static constexpr int MT = HD / 16, PER = T::V / 2;      // 16 dimensions each; how many of them a 16-byte read of values serves
+    float m[NT][2], l[NT][2], o[MT][NT][4];
     __device__ __forceinline__ void clear() {
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NN; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[n][e] = 0.0f;
+            for (int f = 0; f < 2; f++) { m[n][f] = -INFINITY; l[n][f] = 0.0f; }
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[i][n][e] = 0.0f;
     }
     // s: scaled scores in powers of two, -infinity where a row does not see the slot.  partial: some row may not see some slot, whose values may be anything: a
     // value that is no number goes into the sum of the rows that see it, and no further.
-    __device__ __forceinline__ void add(uint32_t st, float (&s)[NK][4], bool partial) {
-        float top[2] = {m[0], m[1]};
+    __device__ __forceinline__ void add(uint32_t st, float (&s)[NT][4], bool partial) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        float corr[NT][2];
 #pragma unroll
-        for (int j = 0; j < NK; j++) {
-            top[0] = fmaxf(top[0], fmaxf(s[j][0], s[j][1]));
-            top[1] = fmaxf(top[1], fmaxf(s[j][2], s[j][3]));
-        }
-        float corr[2];
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-            const float safe = top[h] == -INFINITY ? 0.0f : top[h];
-            corr[h] = exp2_approx(m[h] - safe);
-            m[h] = top[h];
-            top[h] = safe;
-            l[h] *= corr[h];
-        }
-        float4 ph[NK], pl[NK];
+            for (int f = 0; f < 2; f++) {
+                float top = fmaxf(m[n][f], fmaxf(s[n][f], s[n][f + 2]));
 #pragma unroll
-        for (int j = 0; j < NK; j++) {
-            float p[4];
+                for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float safe = top == -INFINITY ? 0.0f : top;
+                corr[n][f] = exp2_approx(m[n][f] - safe);
+                m[n][f] = top;
+                s[n][f] = exp2_approx(s[n][f] - safe);
+                s[n][f + 2] = exp2_approx(s[n][f + 2] - safe);
+            }
+        if (partial) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) p[e] = exp2_approx(s[j][e] - top[e >> 1]);
-            if (partial) {
+            for (int k = 0; k < 2; k++) {
                 bool bad[2] = {false, false};
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int c = 0; c < Rg::NVC; c++) {
+                    for (int c = 0; c < R::NVC; c++) {
                         float x[T::V];
-                        T::get(Rg::value(st, j, h, c), x);
+                        T::get(R::value(st, k, h, c), x);
 #pragma unroll
                         for (int i = 0; i < T::V; i++) bad[h] |= not_finite(x[i]);
                     }
-                const uint32_t mine = 0x11111111u << (threadIdx.x & 3);
+                const uint32_t even = __ballot_sync(0xffffffffu, bad[0]), odd = __ballot_sync(0xffffffffu, bad[1]);
+                if ((g & 1 ? odd : even) & (0x11111111u << (g >> 1)))         // this lane's slot; a weight of zero: not seen (or of no weight)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (__ballot_sync(0xffffffffu, bad[h]) & mine) {
-                        if (s[j][h] != -INFINITY) p[h] = NAN;
-                        if (s[j][2 + h] != -INFINITY) p[2 + h] = NAN;
-                    }
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int f = 0; f < 2; f++)
+                            if (s[n][2 * k + f] != 0.0f) s[n][2 * k + f] = NAN;
             }
-            l[0] += p[0] + p[1];
-            l[1] += p[2] + p[3];
-            // operand A: k = t is slot 2t, k = t + 4 slot 2t + 1
-            ph[j] = make_float4(tf32_hi(p[0]), tf32_hi(p[2]), tf32_hi(p[1]), tf32_hi(p[3]));
-            pl[j] = make_float4(p[0] - ph[j].x, p[2] - ph[j].y, p[1] - ph[j].z, p[3] - ph[j].w);
+        }
+        // operand B: slots 2t and 2t + 1 of eight, row g
+        float bh[NT][2][2], bl[NT][2][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            l[n][0] = __fmaf_rn(l[n][0], corr[n][0], s[n][0] + s[n][2]);
+            l[n][1] = __fmaf_rn(l[n][1], corr[n][1], s[n][1] + s[n][3]);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int from = 8 * t + 4 * h + (g >> 1);
+                    const float x = __shfl_sync(0xffffffffu, s[n][2 * k], from), y = __shfl_sync(0xffffffffu, s[n][2 * k + 1], from), p = g & 1 ? y : x;
+                    bh[n][k][h] = tf32_hi(p);
+                    bl[n][k][h] = p - bh[n][k][h];
+                }
         }
 #pragma unroll
-        for (int c = 0; c < Rg::NVC; c++) {
-            float d[T::V][4];
+        for (int c = 0; c < R::NVC; c++) {
+            float d[PER][NT][4];
 #pragma unroll
-            for (int i = 0; i < T::V; i++)
+            for (int i = 0; i < PER; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) d[i][e] = 0.0f;
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int j = 0; j < NK; j++) {
+                    for (int e = 0; e < 4; e++) d[i][n][e] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
                 float x0[T::V], x1[T::V];
-                T::get(Rg::value(st, j, 0, c), x0);
-                T::get(Rg::value(st, j, 1, c), x1);
+                T::get(R::value(st, k, 0, c), x0);
+                T::get(R::value(st, k, 1, c), x1);
                 if (partial) {
 #pragma unroll
                     for (int i = 0; i < T::V; i++) {
@@ -227,54 +248,62 @@ struct Running {
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < T::V; i++) {
+                for (int i = 0; i < PER; i++) {
+                    const float4 a = make_float4(x0[2 * i], x0[2 * i + 1], x1[2 * i], x1[2 * i + 1]);
                     if (T::SPLIT) {
-                        const float h0 = tf32_hi(x0[i]), h1 = tf32_hi(x1[i]);
-                        mma_tf32(d[i], ph[j], x0[i] - h0, x1[i] - h1);
-                        mma_tf32(d[i], pl[j], h0, h1);
-                        mma_tf32(d[i], ph[j], h0, h1);
+                        const float4 ah = make_float4(tf32_hi(a.x), tf32_hi(a.y), tf32_hi(a.z), tf32_hi(a.w)), al = make_float4(a.x - ah.x, a.y - ah.y, a.z - ah.z, a.w - ah.w);
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            mma_tf32(d[i][n], al, bh[n][k][0], bh[n][k][1]);
+                            mma_tf32(d[i][n], ah, bl[n][k][0], bl[n][k][1]);
+                            mma_tf32(d[i][n], ah, bh[n][k][0], bh[n][k][1]);
+                        }
                     } else {
-                        mma_tf32(d[i], pl[j], x0[i], x1[i]);
-                        mma_tf32(d[i], ph[j], x0[i], x1[i]);
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            mma_tf32(d[i][n], a, bl[n][k][0], bl[n][k][1]);
+                            mma_tf32(d[i][n], a, bh[n][k][0], bh[n][k][1]);
+                        }
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < T::V; i++)
+            for (int i = 0; i < PER; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[c * T::V + i][e] = __fmaf_rn(o[c * T::V + i][e], corr[e >> 1], d[i][e]);
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[c * PER + i][n][e] = __fmaf_rn(o[c * PER + i][n][e], corr[n][e & 1], d[i][n][e]);
         }
     }
-    // Into shared memory: out [16][HD] (rows of this tile), ml [16][2].
+    // Into shared memory: out [8 NT][HD], ml [8 NT].
     __device__ __forceinline__ void store(float *out, float2 *ml) {
-        const int lane = threadIdx.x & 31, t = lane & 3;
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            const int r = (lane >> 2) + 8 * h;
-            if (t == 0) ml[r] = make_float2(m[h], l[h]);
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int c = 0; c < HD / (8 * T::V); c++)
+            for (int f = 0; f < 2; f++) {
 #pragma unroll
-                for (int n = 0; n < 2; n++)      // column 2t + n of products c V .. c V + V - 1: values 8V c + V (2t + n) ...
+                for (int d = 4; d < 32; d <<= 1) l[n][f] += __shfl_xor_sync(0xffffffffu, l[n][f], d);
+                const int r = 8 * n + 2 * t + f;
+                if (g == 0) ml[r] = make_float2(m[n][f], l[n][f]);
 #pragma unroll
-                    for (int i = 0; i < T::V; i += 4)
-                        *reinterpret_cast<float4 *>(out + r * HD + 8 * T::V * c + T::V * (2 * t + n) + i) =
-                            make_float4(o[c * T::V + i][2 * h + n], o[c * T::V + i + 1][2 * h + n], o[c * T::V + i + 2][2 * h + n], o[c * T::V + i + 3][2 * h + n]);
-        }
+                for (int c = 0; c < R::NVC; c++)
+#pragma unroll
+                    for (int i = 0; i < PER; i += 2)         // products i, i + 1: values 8V c + V g + 2i ...
+                        *reinterpret_cast<float4 *>(out + r * HD + 8 * T::V * c + T::V * g + 2 * i) =
+                            make_float4(o[c * PER + i][n][f], o[c * PER + i][n][f + 2], o[c * PER + i + 1][n][f], o[c * PER + i + 1][n][f + 2]);
+            }
     }
 };
 
-// The parts of a CTA's warps (out [parts][16][HD], ml [parts][16] in shared memory) to the rows' places or, in a cluster, by way of the owners; got, gml: room for
-// the owner's parts, 16 + 15 rows.  All threads call it, after a barrier; the cluster's CTAs have arrived once at its barrier before.
-template <int HD, class Dst, class Sink>
-__device__ __forceinline__ void join_warps(float *out, float2 *ml, int parts, float *got, float2 *gml, float *o, float *lse, Dst dst, Sink sink) {
-    constexpr int R = 16;
+// The parts of a CTA's warps (out [AW][R][HD], ml [AW][R] in shared memory) to the rows' places or, in a cluster, by way of the owners; got, gml: room for
+// the owner's parts, R + 15 rows.  All threads call it, after a barrier; the cluster's CTAs have arrived once at its barrier before.
+template <int HD, int R, class Dst, class Sink>
+__device__ __forceinline__ void join_warps(float *out, float2 *ml, float *got, float2 *gml, float *o, float *lse, Dst dst, Sink sink) {
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), c = (int)cl.block_rank();
     if (C == 1) {
-        join_rows<HD, HD>(out, ml, parts, R, o, lse, dst, sink);
+        join_rows<HD, HD>(out, ml, AW, R, o, lse, dst, sink);
         return;
     }
     const int each = owned_rows(R, C);
@@ -303,14 +332,22 @@ __device__ __forceinline__ void join_warps(float *out, float2 *ml, int parts, fl
     join_rows<HD, HD>(got, gml, C, each, o, lse, [&](int i) -> long long { return c * each + i < R ? dst(c * each + i) : -1; }, [&](int i) { return sink(c * each + i); });
 }
 
-// grid (C, kv heads x tiles of 16 rows, entries), clusters of C
-template <class T, int HD, int NK>
+// A CTA's shared memory: the warps' rings, later their parts; the queries; the owner's parts; the warps' maxima and sums.
+template <class T, int HD, int NT>
+struct Room {
+    static constexpr int R = 8 * NT, RINGS = AW * Ring<T, HD>::BYTES, GOT = RINGS + R * HD * 8, GML = GOT + (R + 15) * HD * 4, ML = GML + (R + 15) * 8, BYTES = ML + AW * R * 8;
+    static_assert(R * HD * 4 <= Ring<T, HD>::BYTES, "a warp's part fits its ring");
+};
+
+// grid (C, kv heads x tiles of 8 NT rows, entries), clusters of C
+template <class T, int HD, int NT>
 __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev kv, TreeArgs a) {
-    typedef Ring<T, HD, NK> Rg;
-    constexpr int R = 16, STEP = 8 * NK;
-    extern __shared__ __align__(128) unsigned char asm_[];  // the warps' rings, later the parts: out [AW][R][HD], ml [AW][R]; the queries; the owner's parts
+    typedef Ring<T, HD> Rg;
+    typedef Room<T, HD, NT> Rm;
+    constexpr int R = 8 * NT;
+    extern __shared__ __align__(128) unsigned char asm_[];
     __shared__ __align__(8) uint64_t bars[AW * 8];
-    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * RING);
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + Rm::RINGS);
     __shared__ TreeRows see;
     const int per = a.nh / kv.nkv, tiles = (a.rows * per + R - 1) / R, kvh = blockIdx.y / tiles, row0 = blockIdx.y % tiles * R, b = blockIdx.z;
     if (gridDim.x > 1) cluster_arrive();
@@ -346,37 +383,39 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
         const int i = (row0 + r) / per;
         return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + (row0 + r) % per : -1;
     };
-    stage_queries<T, HD>(frag, 1, [&](int r) -> const float * { return place(r) >= 0 ? a.q + place(r) * HD : nullptr; });
+    stage_queries<T, HD, NT>(frag, [&](int r) -> const float * { return place(r) >= 0 ? a.q + place(r) * HD : nullptr; });
     __syncthreads();
-    // this lane's two rows
-    uint64_t mask[2];
-    int lo[2];
+    // this lane's rows 8 n + 2t, 2t + 1
+    uint64_t mask[NT][2];
+    int lo[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int i = (row0 + (lane >> 2) + 8 * h) / per;
-        mask[h] = i < e.count ? see.mask[i] : 0;
-        lo[h] = i < e.count ? see.lo[i] : 0x7fffffff;
-    }
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            const int i = (row0 + 8 * n + 2 * (lane & 3) + f) / per;
+            mask[n][f] = i < e.count ? see.mask[i] : 0;
+            lo[n][f] = i < e.count ? see.lo[i] : 0x7fffffff;
+        }
     const float c = a.scale * LOG2E;
-    Running<T, HD, NK, Rg> run;
+    Running<T, HD, NT> run;
     run.clear();
     TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
     for (int n = 0; n < count; n++) {
         const int base = base_of(n);
-        float x[NK][4];
-        step_scores<T, HD, NK, Rg>(ring.next(wait), frag, x);
+        float x[NT][4];
+        step_scores<T, HD, NT>(ring.next(wait), frag, x);
         __syncwarp();
         bring(2 * n + Rg::D);
         const bool partial = base < see.full || base + STEP > e.len;
 #pragma unroll
-        for (int j = 0; j < NK; j++)
+        for (int i = 0; i < NT; i++)
 #pragma unroll
             for (int f = 0; f < 4; f++) {
-                x[j][f] *= c;
+                x[i][f] *= c;
                 if (partial) {
-                    const int t = base + 8 * j + 2 * (lane & 3) + (f & 1), h = f >> 1;
-                    const bool sees = t < e.len ? t >= lo[h] : t < end && (mask[h] >> (t - e.len) & 1);
-                    if (!sees) x[j][f] = -INFINITY;
+                    const int t = base + (lane >> 2) + 8 * (f >> 1);
+                    const bool sees = t < e.len ? t >= lo[i][f & 1] : t < end && (mask[i][f & 1] >> (t - e.len) & 1);
+                    if (!sees) x[i][f] = -INFINITY;
                 }
             }
         run.add(ring.next(wait), x, partial);
@@ -384,24 +423,20 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
         bring(2 * n + 1 + Rg::D);
     }
     __syncthreads();                 // nobody reads the rings any more
-    float *out = reinterpret_cast<float *>(asm_), *got = reinterpret_cast<float *>(frag) + 32 * HD;
-    float2 *gml = reinterpret_cast<float2 *>(got + 31 * HD), *ml = gml + 31;
+    float *out = reinterpret_cast<float *>(asm_), *got = reinterpret_cast<float *>(asm_ + Rm::GOT);
+    float2 *gml = reinterpret_cast<float2 *>(asm_ + Rm::GML), *ml = reinterpret_cast<float2 *>(asm_ + Rm::ML);
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
-    join_warps<HD>(out, ml, AW, got, gml, a.out, a.lse, place, [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
+    join_warps<HD, R>(out, ml, got, gml, a.out, a.lse, place, [&](int r) { return a.sinks ? a.sinks[kvh * per + (row0 + r) % per] * LOG2E : -INFINITY; });
 }
 
-// bytes of a CTA's shared memory: the rings (later the parts of the warps), the queries, the owner's parts
-__host__ __device__ constexpr size_t attn_smem(int hd) { return (size_t)AW * RING + hd * 128 + 31 * (hd * 4 + 8) + AW * 16 * 8; }
-static_assert(16 * 128 * 4 <= RING, "a warp's part fits its ring");
-
-template <class T, int HD, int NK>
+template <class T, int HD, int NT>
 static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
-    constexpr size_t smem = attn_smem(HD);
-    constexpr auto K = tree_kernel<T, HD, NK>;
+    constexpr size_t smem = Room<T, HD, NT>::BYTES;
+    constexpr auto K = tree_kernel<T, HD, NT>;
     cudaError_t e = cudaSuccess;
-    const int tiles = (a.rows * (a.nh / kv.nkv) + 15) / 16;
-    const int c = cluster_size<K>((long long)a.n * kv.nkv * tiles, (slots + 8 * NK - 1) / (8 * NK), AW, 4, AW * 32, smem, smem, &e);
+    const int tiles = (a.rows * (a.nh / kv.nkv) + 8 * NT - 1) / (8 * NT);
+    const int c = cluster_size<K>((long long)a.n * kv.nkv * tiles, (slots + STEP - 1) / STEP, AW, 4, AW * 32, smem, smem, &e);
     if (e != cudaSuccess) return e;
     return launch_cluster<K>(dim3(c, kv.nkv * tiles, a.n), AW * 32, c, smem, smem, st, kv, a);
 }
@@ -421,20 +456,21 @@ cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, c
     int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
     if (a.window > 0) slots = min(slots, a.window + a.rows);
     if (wide_rows_pay(kv, a, slots)) return launch_tree_tc(kv, a, slots, st);
-    if (kv.type) return kv.hd == 64 ? launch_tree<KvBf16, 64, 2>(kv, a, slots, st) : launch_tree<KvBf16, 128, 2>(kv, a, slots, st);
-    return kv.hd == 64 ? launch_tree<KvF32, 64, 2>(kv, a, slots, st) : launch_tree<KvF32, 128, 1>(kv, a, slots, st);
+    const bool one = a.rows * (a.nh / kv.nkv) <= 8;
+    auto go = kv.type ? (kv.hd == 64 ? (one ? launch_tree<KvBf16, 64, 1> : launch_tree<KvBf16, 64, 2>) : (one ? launch_tree<KvBf16, 128, 1> : launch_tree<KvBf16, 128, 2>))
+                      : (kv.hd == 64 ? (one ? launch_tree<KvF32, 64, 1> : launch_tree<KvF32, 64, 2>) : (one ? launch_tree<KvF32, 128, 1> : launch_tree<KvF32, 128, 2>));
+    return go(kv, a, slots, st);
 }
 
 // ---------------------------------------------------------------- book of weights
 // Up to 16 rows per kv head (more: kernels_kvtc.cu).  A warp owns a step of slots: the scores of its keys, their powers, the sum over the rows.
-template <class T, int HD, int NK>
+template <class T, int HD, int NT>
 __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked) {
-    typedef Ring<T, HD, NK> Rg;
-    constexpr int STEP = 8 * NK;
+    typedef Ring<T, HD> Rg;
     extern __shared__ __align__(128) unsigned char asm_[];       // the warps' rings, the queries
     __shared__ __align__(8) uint64_t bars[AW * 8];
     __shared__ TreeRows see;
-    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * RING);
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * Rg::BYTES);
     const int kvh = blockIdx.y, b = blockIdx.z, per = a.nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Rg ring(asm_, bars);
     pdl_wait();
@@ -464,78 +500,70 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
         const int i = r / per;
         return i < e.count ? ((long long)b * a.rows + i) * a.nh + kvh * per + r % per : -1;
     };
-    stage_queries<T, HD>(frag, 1, [&](int r) -> const float * { return place(r) >= 0 ? a.q + place(r) * HD : nullptr; });
-    // this lane's two rows; one that does not count sees nothing
-    bool counts[2];
-    float z[2];
+    stage_queries<T, HD, NT>(frag, [&](int r) -> const float * { return place(r) >= 0 ? a.q + place(r) * HD : nullptr; });
+    // this lane's rows 8 n + 2t, 2t + 1; one that does not count sees nothing
+    bool counts[NT][2];
+    float z[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int r = (lane >> 2) + 8 * h, i = r / per;
-        counts[h] = i < e.count && (rows >> i & 1);
-        z[h] = counts[h] ? a.lse[place(r)] * LOG2E : 0.0f;
-    }
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            const int r = 8 * n + 2 * (lane & 3) + f, i = r / per;
+            counts[n][f] = i < e.count && (rows >> i & 1);
+            z[n][f] = counts[n][f] ? a.lse[place(r)] * LOG2E : 0.0f;
+        }
     __syncthreads();
-    uint64_t mask[2];
-    int lo[2];
+    uint64_t mask[NT][2];
+    int lo[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int i = ((lane >> 2) + 8 * h) / per;
-        mask[h] = counts[h] ? see.mask[i] : 0;
-        lo[h] = counts[h] ? see.lo[i] : 0x7fffffff;
-    }
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            const int i = (8 * n + 2 * (lane & 3) + f) / per;
+            mask[n][f] = counts[n][f] ? see.mask[i] : 0;
+            lo[n][f] = counts[n][f] ? see.lo[i] : 0x7fffffff;
+        }
     const float c = a.scale * LOG2E;
     TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
     for (int n = 0; n < count; n++) {
         const int base = base_of(n);
-        // the two slots of lane t < 4 per eight: what the book has
-        float2 had[NK];
-#pragma unroll
-        for (int j = 0; j < NK; j++) {
-            const int t = base + 8 * j + 2 * lane;
-            had[j] = make_float2(lane < 4 && t < end ? weight[t] : 0.0f, lane < 4 && t + 1 < end ? weight[t + 1] : 0.0f);
-        }
-        float x[NK][4], sum[NK][2];
-        step_scores<T, HD, NK, Rg>(ring.next(wait), frag, x);
+        // lane t < 2 writes slot g + 8t: what the book has
+        const int mine_at = base + (lane >> 2) + 8 * (lane & 3);
+        const bool writes = (lane & 3) < 2 && mine_at < end;
+        const float had = writes ? weight[mine_at] : 0.0f;
+        float x[NT][4], sum[2] = {0.0f, 0.0f};
+        step_scores<T, HD, NT>(ring.next(wait), frag, x);
         __syncwarp();
         if (n + Rg::D < count) ring.bring(kc, base_of(n + Rg::D), end);
         const bool partial = base < see.full || base + STEP > e.len;
 #pragma unroll
-        for (int j = 0; j < NK; j++) {
+        for (int i = 0; i < NT; i++)
 #pragma unroll
-            for (int f = 0; f < 2; f++) {
-                float p[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    p[h] = exp2_approx(__fmaf_rn(x[j][2 * h + f], c, -z[h]));
-                    bool sees = counts[h];
-                    if (partial) {
-                        const int t = base + 8 * j + 2 * (lane & 3) + f;
-                        sees = t < e.len ? t >= lo[h] : t < end && (mask[h] >> (t - e.len) & 1);
-                    }
-                    if (!sees) p[h] = 0.0f;
+            for (int f = 0; f < 4; f++) {
+                float p = exp2_approx(__fmaf_rn(x[i][f], c, -z[i][f & 1]));
+                bool sees = counts[i][f & 1];
+                if (partial) {
+                    const int t = base + (lane >> 2) + 8 * (f >> 1);
+                    sees = t < e.len ? t >= lo[i][f & 1] : t < end && (mask[i][f & 1] >> (t - e.len) & 1);
                 }
-                sum[j][f] = p[0] + p[1];
+                sum[f >> 1] += sees ? p : 0.0f;
             }
 #pragma unroll
-            for (int f = 0; f < 2; f++)
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) sum[j][f] += __shfl_xor_sync(0xffffffffu, sum[j][f], o);
-            const int t = base + 8 * j + 2 * lane;
-            if (lane < 4) {
-                if (t < end) weight[t] = had[j].x + sum[j][0];
-                if (t + 1 < end) weight[t + 1] = had[j].y + sum[j][1];
-            }
+        for (int f = 0; f < 2; f++) {
+            sum[f] += __shfl_xor_sync(0xffffffffu, sum[f], 1);
+            sum[f] += __shfl_xor_sync(0xffffffffu, sum[f], 2);
         }
+        if (writes) weight[mine_at] = had + sum[lane & 1];
     }
 }
 
-template <class T, int HD, int NK>
+template <class T, int HD, int NT>
 static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int slots, cudaStream_t st) {
-    constexpr size_t smem = (size_t)AW * RING + HD * 128;
-    constexpr auto K = weigh_kernel<T, HD, NK>;
+    constexpr size_t smem = (size_t)AW * Ring<T, HD>::BYTES + HD * 64 * NT;
+    constexpr auto K = weigh_kernel<T, HD, NT>;
     // CTAs of an entry and head: as with clusters, the least time of all waves
     cudaError_t e = cudaSuccess;
-    const int c = cluster_size<K, false>((long long)kv.nkv * a.n, (slots + 8 * NK - 1) / (8 * NK), AW, 4, AW * 32, smem, smem, &e);
+    const int c = cluster_size<K, false>((long long)kv.nkv * a.n, (slots + STEP - 1) / STEP, AW, 4, AW * 32, smem, smem, &e);
     if (e != cudaSuccess) return e;
     return launch_cluster<K>(dim3(c, kv.nkv, a.n), AW * 32, 1, smem, smem, st, kv, a, picked);
 }
@@ -544,8 +572,10 @@ cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *
     int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
     if (a.window > 0) slots = min(slots, a.window + a.rows);
     if (a.rows * (a.nh / kv.nkv) > 16) return launch_weigh_tc(kv, a, picked, slots, st);
-    if (kv.type) return kv.hd == 64 ? launch_weigh<KvBf16, 64, 2>(kv, a, picked, slots, st) : launch_weigh<KvBf16, 128, 2>(kv, a, picked, slots, st);
-    return kv.hd == 64 ? launch_weigh<KvF32, 64, 2>(kv, a, picked, slots, st) : launch_weigh<KvF32, 128, 1>(kv, a, picked, slots, st);
+    const bool one = a.rows * (a.nh / kv.nkv) <= 8;
+    auto go = kv.type ? (kv.hd == 64 ? (one ? launch_weigh<KvBf16, 64, 1> : launch_weigh<KvBf16, 64, 2>) : (one ? launch_weigh<KvBf16, 128, 1> : launch_weigh<KvBf16, 128, 2>))
+                      : (kv.hd == 64 ? (one ? launch_weigh<KvF32, 64, 1> : launch_weigh<KvF32, 64, 2>) : (one ? launch_weigh<KvF32, 128, 1> : launch_weigh<KvF32, 128, 2>));
+    return go(kv, a, picked, slots, st);
 }
 
 // ---------------------------------------------------------------- chosen blocks
@@ -597,15 +627,16 @@ __device__ __forceinline__ void block_keys(const float *__restrict__ q, int per,
         if (key[i] == 0xFFFFFFFFu) key[i] = 0;
 }
 
-template <class T, int HD, int NK>
+template <class T, int HD, int NT>
 __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel, int first, int local,
                                                          const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *o, float *lse) {
-    typedef Ring<T, HD, NK> Rg;
-    constexpr int R = 16, STEP = 8 * NK;
+    typedef Ring<T, HD> Rg;
+    typedef Room<T, HD, NT> Rm;
+    constexpr int R = 8 * NT;
     extern __shared__ __align__(128) unsigned char asm_[];
     __shared__ __align__(8) uint64_t bars[AW * 8];
-    float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * RING);
-    uint32_t *keys = reinterpret_cast<uint32_t *>(asm_) + attn_smem(HD) / 4;      // [cap / block + 1]
+    float4 *frag = reinterpret_cast<float4 *>(asm_ + Rm::RINGS);
+    uint32_t *keys = reinterpret_cast<uint32_t *>(asm_ + Rm::BYTES);      // [cap / block + 1]
     __shared__ int32_t chosen[256];
     __shared__ float qs[16 * HD];
     __shared__ KthSpace<8> kth;
@@ -693,14 +724,14 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
             before += __popc(b_over) | __popc(b_same) << 16;
         }
     }
-    stage_queries<T, HD>(frag, 1, [&](int i) -> const float * { return i < per ? qs + i * HD : nullptr; });
+    stage_queries<T, HD, NT>(frag, [&](int i) -> const float * { return i < per ? qs + i * HD : nullptr; });
     __syncthreads();
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < nsel; i += AW * 32) sel[((long long)r * kv.nkv + kvh) * nsel + i] = i < taken ? chosen[i] : -1;
     const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(s, kvh), *vc = (const typename T::Val *)kv.v + kv.head(s, kvh);
     const float c = scale * LOG2E;
     const int shift = 31 - __clz(block / STEP), steps = taken << shift;       // steps of a block: a power of two
-    Running<T, HD, NK, Rg> run;
+    Running<T, HD, NT> run;
     run.clear();
     TlWaiter wait{kv.err ? reinterpret_cast<uint32_t *>(kv.err) : nullptr, false};
     const int hop = C * AW, i0 = blockIdx.x * AW + warp, count = max(0, (steps - i0 + hop - 1) / hop);
@@ -716,44 +747,47 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
     for (int m = 0; m < count; m++) {
         const int base = base_of(m);
         if (base >= n) break;
-        float x[NK][4];
-        step_scores<T, HD, NK, Rg>(ring.next(wait), frag, x);
+        float x[NT][4];
+        step_scores<T, HD, NT>(ring.next(wait), frag, x);
         __syncwarp();
         bring(2 * m + Rg::D);
 #pragma unroll
-        for (int j = 0; j < NK; j++)
+        for (int j = 0; j < NT; j++)
 #pragma unroll
-            for (int f = 0; f < 4; f++) x[j][f] = base + 8 * j + 2 * (lane & 3) + (f & 1) < n ? x[j][f] * c : -INFINITY;
+            for (int f = 0; f < 4; f++) x[j][f] = base + (lane >> 2) + 8 * (f >> 1) < n ? x[j][f] * c : -INFINITY;
         run.add(ring.next(wait), x, base + STEP > n);
         __syncwarp();
         bring(2 * m + 1 + Rg::D);
     }
     __syncthreads();
-    float *out = reinterpret_cast<float *>(asm_), *got = reinterpret_cast<float *>(frag) + 32 * HD;
-    float2 *gml = reinterpret_cast<float2 *>(got + 31 * HD), *ml = gml + 31;
+    float *out = reinterpret_cast<float *>(asm_), *got = reinterpret_cast<float *>(asm_ + Rm::GOT);
+    float2 *gml = reinterpret_cast<float2 *>(asm_ + Rm::GML), *ml = reinterpret_cast<float2 *>(asm_ + Rm::ML);
     run.store(out + warp * R * HD, ml + warp * R);
     __syncthreads();
-    join_warps<HD>(out, ml, AW, got, gml, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
+    join_warps<HD, R>(out, ml, got, gml, o, lse, [&](int i) -> long long { return i < per ? row + i : -1; },
                    [&](int i) { return sinks ? sinks[kvh * per + i] * LOG2E : -INFINITY; });
 }
 
-template <class T, int HD, int NK>
+template <class T, int HD, int NT>
 static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,
                                  int len_hint, const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *out, float *lse, cudaStream_t st) {
-    const int longest = len_hint > 0 ? min(len_hint, kv.cap) : kv.cap, nb = longest / block, each = block / (8 * NK);
+    const int longest = len_hint > 0 ? min(len_hint, kv.cap) : kv.cap, nb = longest / block;
     // a tile of eight blocks' scores costs about as much as a step
-    const int steps = min(nsel, nb + 1) * each + (nb > nsel ? nb / 8 : 0);
-    const size_t smem = attn_smem(HD) + (size_t)(kv.cap / block + 1) * 4, most = attn_smem(HD) + 16385 * 4;
+    const int steps = min(nsel, nb + 1) * (block / STEP) + (nb > nsel ? nb / 8 : 0);
+    constexpr size_t room = Room<T, HD, NT>::BYTES, most = room + 16385 * 4;
+    constexpr auto K = blocks_kernel<T, HD, NT>;
     cudaError_t e = cudaSuccess;
-    const int c = cluster_size<blocks_kernel<T, HD, NK>>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, attn_smem(HD) + 4096, most, &e);
+    const int c = cluster_size<K>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, room + 4096, most, &e);
     if (e != cudaSuccess) return e;
-    return launch_cluster<blocks_kernel<T, HD, NK>>(dim3(c, rows, kv.nkv), AW * 32, c, smem, most, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
-                                                    sinks, sel, out, lse);
+    return launch_cluster<K>(dim3(c, rows, kv.nkv), AW * 32, c, room + (size_t)(kv.cap / block + 1) * 4, most, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
+                             sinks, sel, out, lse);
 }
 
 cudaError_t launch_attn_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,
                                int len_hint, const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *out, float *lse, cudaStream_t st) {
-    auto go = kv.type ? (kv.hd == 64 ? launch_blocks<KvBf16, 64, 2> : launch_blocks<KvBf16, 128, 2>) : (kv.hd == 64 ? launch_blocks<KvF32, 64, 2> : launch_blocks<KvF32, 128, 1>);
+    const bool one = nh / kv.nkv <= 8;
+    auto go = kv.type ? (kv.hd == 64 ? (one ? launch_blocks<KvBf16, 64, 1> : launch_blocks<KvBf16, 64, 2>) : (one ? launch_blocks<KvBf16, 128, 1> : launch_blocks<KvBf16, 128, 2>))
+                      : (kv.hd == 64 ? (one ? launch_blocks<KvF32, 64, 1> : launch_blocks<KvF32, 64, 2>) : (one ? launch_blocks<KvF32, 128, 1> : launch_blocks<KvF32, 128, 2>));
     return go(kv, rows, seq, len, block, means, nsel, first, local, len_hint, q, nh, scale, sinks, sel, out, lse, st);
 }
 
