@@ -3,6 +3,7 @@
 #include "brrr_block.cuh"
 #include "brrr_kv.cuh"
 #include "brrr_tma.cuh"
+#include "brrr_tmap.h"
 
 #include <atomic>
 #include <cooperative_groups.h>
@@ -37,17 +38,6 @@ struct KvBf16 {
         for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
     }
 };
-
-__device__ __forceinline__ uint4 ldg_stream(const void *p) {
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-    return r;
-}
-__device__ __forceinline__ uint4 ldg_shared(const void *p) {
-    uint4 r;
-    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-    return r;
-}
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
@@ -120,6 +110,30 @@ __device__ __forceinline__ void tree_rows(const TreeArgs &a, const KvEntry &e, u
         atomicMin(&w.first, lo);
         atomicMax(&w.full, lo);
     }
+}
+
+// K and V as tensors [sequence][kv head][slot][dim], boxes of 128 bytes of a row x `slots` rows, rows of a box 128 swizzled bytes in shared memory (16-byte piece
+// c of row r at c ^ (r & 7)).  A box may reach behind an entry's end: what stands there nobody sees.
+struct alignas(64) KvMaps {
+    CUtensorMap k, v;
+};
+static inline cudaError_t kv_maps(const KvDev &kv, int slots, KvMaps *m) {
+    const tmap_encode_t encode = tmap_encode();
+    if (!encode) return cudaErrorNotSupported;
+    const cuuint64_t size = kv.size(), dims[4] = {(cuuint64_t)kv.hd, (cuuint64_t)kv.cap, (cuuint64_t)kv.nkv, (cuuint64_t)kv.n_seq};
+    const cuuint64_t strides[3] = {kv.hd * size, kv.hs * size, kv.ss * size};
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / size), (cuuint32_t)slots, 1, 1}, ones[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 2; i++)
+        if (encode(i ? &m->v : &m->k, kv.type ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, i ? kv.v : kv.k, dims, strides, box, ones,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    return cudaSuccess;
+}
+__device__ __forceinline__ void tensor_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+__device__ __forceinline__ void tensor_rows(uint32_t dst, const CUtensorMap *map, int x, int slot, int kvh, int seq, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(slot),
+                 "r"(kvh), "r"(seq), "r"(smem_u32(bar))
+                 : "memory");
 }
 
 // Once per kernel and device: the shared memory it may ask for, clusters of up to 16.

@@ -8,10 +8,12 @@
 // left to them: a step's scores take head_dim / 16 additions, a step's share of the output starts at zero and joins the running output by one fused
 // multiply-add that also rescales it to the new running maximum.
 //
-// Every warp has a ring of operands of its own in shared memory, filled by bulk copies of consecutive rows several operands ahead, and waits for nobody
-// else.  The k index of a product may be any order of the dimensions (slots) that both operands have, so a lane's k = t, t + 4 of consecutive products are the
-// consecutive values of one 16-byte read, and the rows of V^T may be any order of the dimensions.  Weights change from the accumulator's place (slot
-// g, rows 2t, 2t + 1 in lane 4 g + t) to operand B's (slots 2t, 2t + 1, row g) by shuffles.  Queries are split once and wait in shared memory in fragment order.
+// Every warp has a ring of operands of its own in shared memory, filled by tensor copies of 16 rows several operands ahead, and waits for nobody else.  The
+// copies swizzle the rows: with rows as they are, 16-byte reads of keys met two and of values four to a bank (201 tokens x 8 heads over 24 blocks of 32 f32
+// slots took 159 us, now 144).  The k index of a product may be any order of the dimensions (slots) that both operands have, so a lane's k = t, t + 4 of
+// consecutive products are the consecutive values of one 16-byte read, and the rows of V^T may be any order of the dimensions.  Weights change from the
+// accumulator's place (slot g, rows 2t, 2t + 1 in lane 4 g + t) to operand B's (slots 2t, 2t + 1, row g) by shuffles.  Queries are split once and wait in
+// shared memory in fragment order.
 //
 // The slots of an entry are split over the warps of a CTA and the CTAs of a cluster, each with its own maximum and sum; partial results meet
 // in shared memory, those of the cluster through distributed shared memory, in a fixed order: one launch, no workspace, no atomics.
@@ -31,7 +33,6 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const float4 &a, float b
                  : "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(a.z)), "r"(__float_as_uint(a.w)), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
 
-
 // A warp's ring: D places for the keys or the values of a step of 16 slots each.  Lane 0 copies; operands are used in the order in which they are copied (keys,
 // values, keys, ...).
 constexpr int STEP = 16;
@@ -43,24 +44,24 @@ struct Ring {
     uint32_t at;             // of the ring, in shared memory
     uint64_t *full;          // [D]
     int in = 0, out = 0, in_turn = 0;      // places that the next copy and the next use take, and the parity of the next use
-    __device__ __forceinline__ Ring(unsigned char *mem, uint64_t *bars) {
+    __device__ __forceinline__ Ring(unsigned char *mem, uint64_t *bars, const KvMaps &maps) {
         const int warp = threadIdx.x >> 5;
         at = smem_u32(mem) + warp * BYTES;
         full = bars + warp * 8;
         if ((threadIdx.x & 31) == 0) {
+            tensor_prefetch(&maps.k);
+            tensor_prefetch(&maps.v);
             for (int i = 0; i < D; i++) mbar_init(&full[i], 1);
             mbar_fence_init();
         }
         __syncwarp();
     }
-    // slots base .. base + 15 of p, those from end on not read (their place keeps what it had), to the next place, which must have been used
-    __device__ __forceinline__ void bring(const typename T::Val *p, int base, int end) {
+    // slots base .. base + 15 of a head to the next place, which must have been used
+    __device__ __forceinline__ void bring(const CUtensorMap *map, int base, int kvh, int seq) {
         if ((threadIdx.x & 31) == 0) {
-            const int bytes = min(STEP, end - base) * ROW;
-            mbar_expect_tx(&full[in], bytes);
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at + in * PLACE), "l"(p + (long long)base * HD), "r"(bytes),
-                         "r"(smem_u32(&full[in]))
-                         : "memory");
+            mbar_expect_tx(&full[in], PLACE);
+#pragma unroll
+            for (int i = 0; i < ROW / 128; i++) tensor_rows(at + in * PLACE + i * 2048, map, i * 8 * T::V, base, kvh, seq, &full[in]);
         }
         in = in + 1 == D ? 0 : in + 1;
     }
@@ -71,14 +72,15 @@ struct Ring {
         if (++out == D) { out = 0; in_turn ^= 1; }
         return p;
     }
-    // this lane's 16 bytes c of the key of slot 8 j + lane / 4, and of the value of slot 8 j + 2 (lane % 4) + h
+    // this lane's 16 bytes c of the key of slot 8 j + lane / 4: piece 2 (lane % 4) + c % 2 of its 128 bytes c / 2; and of the value of slot 8 k + 2 (lane % 4) + h:
+    // piece lane / 4 of its 128 bytes c
     __device__ __forceinline__ static uint4 key(uint32_t st, int j, int c) {
-        const int lane = threadIdx.x & 31;
-        return lds128(st + (8 * j + (lane >> 2)) * ROW + (lane & 3) * 16 + c * 64);
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        return lds128(st + (c >> 1) * 2048 + j * 1024 + g * 128 + (((2 * t) ^ g ^ (c & 1)) << 4));
     }
-    __device__ __forceinline__ static uint4 value(uint32_t st, int j, int h, int c) {
-        const int lane = threadIdx.x & 31;
-        return lds128(st + (8 * j + 2 * (lane & 3) + h) * ROW + (lane >> 2) * 16 + c * 128);
+    __device__ __forceinline__ static uint4 value(uint32_t st, int k, int h, int c) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        return lds128(st + c * 2048 + k * 1024 + (2 * t + h) * 128 + ((g ^ (2 * t + h)) << 4));
     }
 };
 
@@ -86,7 +88,7 @@ struct Ring {
 // values, or null for a row of padding (zeros).
 template <class T, int HD, int NT, class Row>
 __device__ __forceinline__ void stage_queries(float4 *frag, Row row) {
-    constexpr int W = 4 * T::V;                 // dimensions that one read of the four lanes of a slot covers
+    constexpr int W = 8 * T::V;                 // dimensions of 128 bytes
     float *f = reinterpret_cast<float *>(frag);
     for (int u = threadIdx.x; u < NT * 8 * (HD / 4); u += AW * 32) {
         const int r = u / (HD / 4), d0 = u % (HD / 4) * 4;
@@ -95,7 +97,7 @@ __device__ __forceinline__ void stage_queries(float4 *frag, Row row) {
         const float x[4] = {x4.x, x4.y, x4.z, x4.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int d = d0 + i, t = d % W / T::V, product = d / W * (T::V / 2) + d % T::V / 2, odd = d & 1;
+            const int d = d0 + i, piece = d % W / T::V, t = piece >> 1, product = (d / W * 2 + (piece & 1)) * (T::V / 2) + d % T::V / 2, odd = d & 1;
             const int at = ((product * NT + r / 8) * 32 + (r & 7) * 4 + t) * 4 + odd;
             const float hi = tf32_hi(x[i]);
             f[at] = hi;
@@ -341,17 +343,18 @@ struct Room {
 
 // grid (C, kv heads x tiles of 8 NT rows, entries), clusters of C
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev kv, TreeArgs a) {
+__global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev kv, TreeArgs a, const __grid_constant__ KvMaps maps) {
     typedef Ring<T, HD> Rg;
     typedef Room<T, HD, NT> Rm;
     constexpr int R = 8 * NT;
-    extern __shared__ __align__(128) unsigned char asm_[];
+    extern __shared__ unsigned char raw_[];
+    unsigned char *asm_ = raw_ + ((1024u - (smem_u32(raw_) & 1023u)) & 1023u);          // swizzled rows want 1024-byte alignment
     __shared__ __align__(8) uint64_t bars[AW * 8];
     float4 *frag = reinterpret_cast<float4 *>(asm_ + Rm::RINGS);
     __shared__ TreeRows see;
     const int per = a.nh / kv.nkv, tiles = (a.rows * per + R - 1) / R, kvh = blockIdx.y / tiles, row0 = blockIdx.y % tiles * R, b = blockIdx.z;
     if (gridDim.x > 1) cluster_arrive();
-    Rg ring(asm_, bars);
+    Rg ring(asm_, bars, maps);
     pdl_wait();
     pdl_trigger();
     const uint64_t mine = tree_mask(a, b);
@@ -362,7 +365,6 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
         return;
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, end = e.len + e.count;
-    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh), *vc = (const typename T::Val *)kv.v + kv.head(e.seq, kvh);
     int s0 = 0;
     if (a.window > 0) {
         tree_rows(a, e, mine, see);
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
     auto base_of = [&](int n) { return (from + warp + n * AW) * STEP; };
     // operand u: keys (u even) or values of step u / 2
     auto bring = [&](int u) {
-        if (u < 2 * count) ring.bring(u & 1 ? vc : kc, base_of(u >> 1), end);
+        if (u < 2 * count) ring.bring(u & 1 ? &maps.v : &maps.k, base_of(u >> 1), kvh, e.seq);
     };
     for (int u = 0; u < Rg::D; u++) bring(u);
     if (a.window <= 0) tree_rows(a, e, mine, see);
@@ -432,24 +434,26 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev k
 
 template <class T, int HD, int NT>
 static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st) {
-    constexpr size_t smem = Room<T, HD, NT>::BYTES;
+    constexpr size_t smem = Room<T, HD, NT>::BYTES + 1024;
     constexpr auto K = tree_kernel<T, HD, NT>;
-    cudaError_t e = cudaSuccess;
+    KvMaps maps;
+    cudaError_t e = kv_maps(kv, STEP, &maps);
+    if (e != cudaSuccess) return e;
     const int tiles = (a.rows * (a.nh / kv.nkv) + 8 * NT - 1) / (8 * NT);
     const int c = cluster_size<K>((long long)a.n * kv.nkv * tiles, (slots + STEP - 1) / STEP, AW, 4, AW * 32, smem, smem, &e);
     if (e != cudaSuccess) return e;
-    return launch_cluster<K>(dim3(c, kv.nkv * tiles, a.n), AW * 32, c, smem, smem, st, kv, a);
+    return launch_cluster<K>(dim3(c, kv.nkv * tiles, a.n), AW * 32, c, smem, smem, st, kv, a, maps);
 }
 
-// Whether the kernel of 128-row tiles (kernels_kvtc.cu) takes less time than CTAs of 16 rows.  Both were measured with 8 to 256 rows, 1 and 8 sequences, 40 to 2500 slots
-// (20 calls in a graph, in L2): beyond a start that costs the other `start` ns more, 128 slots cost `few` ns per 16 rows here and `many` ns per 128 rows there.  64
-// dimensions f32, 8 heads: 64 rows over 200 slots 6.3 and 13.0 us, over 2500 15.2 and 17.1; 8 sequences: 32 rows over 700 15.4 and 18.8, 128 rows over 2500
-// 146 and 40.
+// Whether the kernel of 128-row tiles (kernels_kvtc.cu) takes less time than CTAs of 16 rows.  Both were measured with 8 to 256 rows, 1 and 8 sequences, 40 to 2500
+// slots (20 calls in a graph, in L2): a tile of 128 rows takes the time of one and a half of 16, and a start of `start` tiles of 16 rows x 128 slots (spread over
+// the GPU) more.  The rule takes at most 14 % more than the better one of the two (38 % for 256 rows of 128 f32 dimensions over 700 slots: 17.0 and 23.4 us).  64
+// dimensions f32, 8 heads: 64 rows over 200 slots 6.4 and 13.0 us, over 2500 15.8 and 17.0; 8 sequences: 32 rows over 700 16.0 and 18.7, 128 rows over 2500
+// 151 and 40.
 static bool wide_rows_pay(const KvDev &kv, const TreeArgs &a, int slots) {
-    static const struct { double few, many, start; } cost[2][2] = {{{14.0, 22.0, 7000.0}, {29.0, 45.0, 7000.0}}, {{11.0, 12.4, 4000.0}, {17.0, 24.0, 4500.0}}};
-    const auto &c = cost[kv.type][kv.hd == 128];
+    static const double start[2][2] = {{400, 200}, {175, 150}};         // f32, bf16 of 64 and of 128 dimensions
     const int rows = a.rows * (a.nh / kv.nkv);
-    return (double)a.n * kv.nkv * (slots / 128.0) * (c.few * ((rows + 15) / 16) - c.many * ((rows + 127) / 128)) > c.start;
+    return (double)a.n * kv.nkv * (slots / 128.0) * ((rows + 15) / 16 - 1.5 * ((rows + 127) / 128)) > start[kv.type][kv.hd == 128];
 }
 
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
@@ -465,14 +469,15 @@ cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, c
 // ---------------------------------------------------------------- book of weights
 // Up to 16 rows per kv head (more: kernels_kvtc.cu).  A warp owns a step of slots: the scores of its keys, their powers, the sum over the rows.
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked) {
+__global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked, const __grid_constant__ KvMaps maps) {
     typedef Ring<T, HD> Rg;
-    extern __shared__ __align__(128) unsigned char asm_[];       // the warps' rings, the queries
+    extern __shared__ unsigned char raw_[];
+    unsigned char *asm_ = raw_ + ((1024u - (smem_u32(raw_) & 1023u)) & 1023u);          // the warps' rings, the queries
     __shared__ __align__(8) uint64_t bars[AW * 8];
     __shared__ TreeRows see;
     float4 *frag = reinterpret_cast<float4 *>(asm_ + AW * Rg::BYTES);
     const int kvh = blockIdx.y, b = blockIdx.z, per = a.nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Rg ring(asm_, bars);
+    Rg ring(asm_, bars, maps);
     pdl_wait();
     pdl_trigger();
     const uint64_t mine = tree_mask(a, b);
@@ -482,7 +487,6 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
         return;
     }
     const int end = e.len + e.count;
-    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(e.seq, kvh);
     float *weight = kv.weight + kv.book(e.seq, kvh);
     int s0 = 0;
     if (a.window > 0) {
@@ -493,7 +497,7 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
     const int steps = (end + STEP - 1) / STEP - s0, chunk = (steps + gridDim.x - 1) / gridDim.x;
     const int from = s0 + blockIdx.x * chunk, to = min(from + chunk, s0 + steps), count = max(0, (to - from - warp + AW - 1) / AW);
     auto base_of = [&](int n) { return (from + warp + n * AW) * STEP; };
-    for (int n = 0; n < min(count, Rg::D); n++) ring.bring(kc, base_of(n), end);
+    for (int n = 0; n < min(count, Rg::D); n++) ring.bring(&maps.k, base_of(n), kvh, e.seq);
     if (a.window <= 0) tree_rows(a, e, mine, see);
     const uint64_t rows = picked ? picked[b] : ~0ull;
     auto place = [&](int r) -> long long {
@@ -534,7 +538,7 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
         float x[NT][4], sum[2] = {0.0f, 0.0f};
         step_scores<T, HD, NT>(ring.next(wait), frag, x);
         __syncwarp();
-        if (n + Rg::D < count) ring.bring(kc, base_of(n + Rg::D), end);
+        if (n + Rg::D < count) ring.bring(&maps.k, base_of(n + Rg::D), kvh, e.seq);
         const bool partial = base < see.full || base + STEP > e.len;
 #pragma unroll
         for (int i = 0; i < NT; i++)
@@ -559,13 +563,15 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
 
 template <class T, int HD, int NT>
 static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int slots, cudaStream_t st) {
-    constexpr size_t smem = (size_t)AW * Ring<T, HD>::BYTES + HD * 64 * NT;
+    constexpr size_t smem = (size_t)AW * Ring<T, HD>::BYTES + HD * 64 * NT + 1024;
     constexpr auto K = weigh_kernel<T, HD, NT>;
+    KvMaps maps;
+    cudaError_t e = kv_maps(kv, STEP, &maps);
+    if (e != cudaSuccess) return e;
     // CTAs of an entry and head: as with clusters, the least time of all waves
-    cudaError_t e = cudaSuccess;
     const int c = cluster_size<K, false>((long long)kv.nkv * a.n, (slots + STEP - 1) / STEP, AW, 4, AW * 32, smem, smem, &e);
     if (e != cudaSuccess) return e;
-    return launch_cluster<K>(dim3(c, kv.nkv, a.n), AW * 32, 1, smem, smem, st, kv, a, picked);
+    return launch_cluster<K>(dim3(c, kv.nkv, a.n), AW * 32, 1, smem, smem, st, kv, a, picked, maps);
 }
 
 cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
@@ -629,11 +635,13 @@ __device__ __forceinline__ void block_keys(const float *__restrict__ q, int per,
 
 template <class T, int HD, int NT>
 __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel, int first, int local,
-                                                         const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *o, float *lse) {
+                                                         const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *o, float *lse,
+                                                         const __grid_constant__ KvMaps maps) {
     typedef Ring<T, HD> Rg;
     typedef Room<T, HD, NT> Rm;
     constexpr int R = 8 * NT;
-    extern __shared__ __align__(128) unsigned char asm_[];
+    extern __shared__ unsigned char raw_[];
+    unsigned char *asm_ = raw_ + ((1024u - (smem_u32(raw_) & 1023u)) & 1023u);          // swizzled rows want 1024-byte alignment
     __shared__ __align__(8) uint64_t bars[AW * 8];
     float4 *frag = reinterpret_cast<float4 *>(asm_ + Rm::RINGS);
     uint32_t *keys = reinterpret_cast<uint32_t *>(asm_ + Rm::BYTES);      // [cap / block + 1]
@@ -644,7 +652,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
     const int C = (int)cl.num_blocks();
     const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (C > 1) cluster_arrive();
-    Rg ring(asm_, bars);
+    Rg ring(asm_, bars, maps);
     pdl_wait();
     pdl_trigger();
     const int s = seq ? seq[r] : r, n = len[r];
@@ -728,7 +736,6 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
     __syncthreads();
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < nsel; i += AW * 32) sel[((long long)r * kv.nkv + kvh) * nsel + i] = i < taken ? chosen[i] : -1;
-    const typename T::Val *kc = (const typename T::Val *)kv.k + kv.head(s, kvh), *vc = (const typename T::Val *)kv.v + kv.head(s, kvh);
     const float c = scale * LOG2E;
     const int shift = 31 - __clz(block / STEP), steps = taken << shift;       // steps of a block: a power of two
     Running<T, HD, NT> run;
@@ -741,7 +748,7 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev
     };
     // the last block may end before its last steps: nothing but such steps follows
     auto bring = [&](int u) {
-        if (u < 2 * count && base_of(u >> 1) < n) ring.bring(u & 1 ? vc : kc, base_of(u >> 1), n);
+        if (u < 2 * count && base_of(u >> 1) < n) ring.bring(u & 1 ? &maps.v : &maps.k, base_of(u >> 1), kvh, s);
     };
     for (int u = 0; u < Rg::D; u++) bring(u);
     for (int m = 0; m < count; m++) {
@@ -774,13 +781,15 @@ static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, 
     const int longest = len_hint > 0 ? min(len_hint, kv.cap) : kv.cap, nb = longest / block;
     // a tile of eight blocks' scores costs about as much as a step
     const int steps = min(nsel, nb + 1) * (block / STEP) + (nb > nsel ? nb / 8 : 0);
-    constexpr size_t room = Room<T, HD, NT>::BYTES, most = room + 16385 * 4;
+    constexpr size_t room = Room<T, HD, NT>::BYTES + 1024, most = room + 16385 * 4;
     constexpr auto K = blocks_kernel<T, HD, NT>;
-    cudaError_t e = cudaSuccess;
+    KvMaps maps;
+    cudaError_t e = kv_maps(kv, STEP, &maps);
+    if (e != cudaSuccess) return e;
     const int c = cluster_size<K>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, room + 4096, most, &e);
     if (e != cudaSuccess) return e;
     return launch_cluster<K>(dim3(c, rows, kv.nkv), AW * 32, c, room + (size_t)(kv.cap / block + 1) * 4, most, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
-                             sinks, sel, out, lse);
+                             sinks, sel, out, lse, maps);
 }
 
 cudaError_t launch_attn_blocks(const KvDev &kv, int rows, const int32_t *seq, const int32_t *len, int block, const float *means, int nsel, int first, int local,

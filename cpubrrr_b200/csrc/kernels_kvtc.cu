@@ -17,7 +17,6 @@
 #include "brrr_kernels.h"
 #include "brrr_kvattn.cuh"
 #include "brrr_tc.cuh"
-#include "brrr_tmap.h"
 
 #include <algorithm>
 
@@ -120,15 +119,6 @@ __device__ __forceinline__ void tc_regs() {
         if constexpr (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
     }
-}
-// K and V of a bf16 cache as tensors [sequence][kv head][slot][dim], boxes of 64 dims x a tile's slots in rows of 128 swizzled bytes
-struct alignas(64) KvMaps {
-    CUtensorMap k, v;
-};
-__device__ __forceinline__ void tensor_rows(uint32_t dst, const CUtensorMap *map, int x, int slot, int kvh, int seq, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(slot),
-                 "r"(kvh), "r"(seq), "r"(smem_u32(bar))
-                 : "memory");
 }
 // descriptor of rows of 128 swizzled bytes: groups of eight rows 1024 bytes apart, blocks of 64 values `lbo` bytes apart (MN-major)
 __device__ __forceinline__ uint64_t desc_rows128(uint32_t at, uint32_t lbo) {
@@ -733,20 +723,6 @@ __global__ void __launch_bounds__(Wc<T, HD>::THREADS, 1) weigh_tc_kernel(KvDev k
     tl_fence_before();
     __syncthreads();
     if (warp == W::ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-}
-
-// K and V of a bf16 cache for the tensor copies
-cudaError_t kv_maps(const KvDev &kv, int slots, KvMaps *m) {
-    const tmap_encode_t encode = tmap_encode();
-    if (!encode) return cudaErrorNotSupported;
-    const cuuint64_t dims[4] = {(cuuint64_t)kv.hd, (cuuint64_t)kv.cap, (cuuint64_t)kv.nkv, (cuuint64_t)kv.n_seq};
-    const cuuint64_t strides[3] = {(cuuint64_t)kv.hd * 2, (cuuint64_t)kv.hs * 2, (cuuint64_t)kv.ss * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)slots, 1, 1}, ones[4] = {1, 1, 1, 1};
-    for (int i = 0; i < 2; i++)
-        if (encode(i ? &m->v : &m->k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? kv.v : kv.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return cudaErrorInvalidValue;
-    return cudaSuccess;
 }
 
 template <class T, int HD>
