@@ -121,6 +121,8 @@ extern "C" int brrr_kv_evict(const brrr_kv *kv, const brrr_kv *dst, int n, const
                 if (!apart(f.p, f.n, t.p, t.n)) return BRRR_ERR_ARG;
     }
     if (int rc = on_this_device(d)) return rc;
+    if (dst)
+        if (int rc = on_this_device(to)) return rc;
     return done(launch_kv_evict(d, dst ? &to : nullptr, n, d_seq, d_len, keep, first, recent, d_end, d_map, d_new_len, len_hint, (cudaStream_t)stream));
 }
 

@@ -513,8 +513,8 @@ __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a,
 #pragma unroll
         for (int f = 0; f < 2; f++) {
             const int r = 8 * n + 2 * (lane & 3) + f, i = r / per;
-            counts[n][f] = i < e.count && (rows >> i & 1);
-            z[n][f] = counts[n][f] ? a.lse[place(r)] * LOG2E : 0.0f;
+            z[n][f] = i < e.count ? a.lse[place(r)] * LOG2E : -INFINITY;          // -infinity: the row has no weights
+            counts[n][f] = i < e.count && (rows >> i & 1) && z[n][f] != -INFINITY;
         }
     __syncthreads();
     uint64_t mask[NT][2];

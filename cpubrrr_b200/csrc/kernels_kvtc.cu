@@ -6,9 +6,9 @@
 // three: the six products down to 2^-16 are formed, what is left out is 2^-22 of the product.  The small ones come first in the accumulator, so that few
 // of its (truncating) additions carry weight; an output tile starts at zero and joins the running output in registers, scaled to the new maximum.
 //
-// Warp roles: 0-7 softmax and output (thread = row and half of a tile's slots, then half of the dimensions); 13 brings keys and values (bf16: tensor copies
-// in operand order, swizzled; f32: bulk copies of raw rows into a ring, which warps 8-11 cut into pieces in operand order); 8-11 look at the values of
-// tiles that not every row sees whole; 12 issues.  Queries are operand A in tensor memory (64 dimensions: the two upper pieces, there is no room for the third,
+// Warp roles: 0-7 softmax and output (thread = row and half of a tile's slots, then half of the dimensions).  bf16: 13 brings keys and values, tensor copies in
+// operand order, swizzled; 8-11 look at the values of tiles that not every row sees whole; 12 issues.  f32: 17 brings raw rows into a ring, 8-15 cut them
+// into pieces in operand order, 16 issues.  Queries are operand A in tensor memory (64 dimensions: the two upper pieces, there is no room for the third,
 // which stays in shared memory).  Scores of two tiles alternate in tensor memory; the pieces of a tile's weights take the place of its scores as operand A.
 // While the softmax warps work on tile i + 1 the tensor cores do the values of tile i and the scores of tile i + 2.
 //
@@ -634,10 +634,11 @@ __global__ void __launch_bounds__(Wc<T, HD>::THREADS, 1) weigh_tc_kernel(KvDev k
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&qfull);
             }
-            const bool counts = node < e.count && (rows >> node & 1);
+            const float of_row = node < e.count ? a.lse[place] : -INFINITY;          // -infinity: the row has no weights
+            const bool counts = node < e.count && (rows >> node & 1) && of_row != -INFINITY;
             const uint64_t mask = counts ? see.mask[node] : 0;
             const int lo = counts ? see.lo[node] : 0x7fffffff;
-            const float z = counts ? a.lse[place] * LOG2E : 0.0f;
+            const float z = counts ? of_row * LOG2E : 0.0f;
             const bool every = __all_sync(0xffffffffu, counts);
             for (int i = 0; i < tiles; i++, j++) {
                 const int t0 = (from + i) * N;

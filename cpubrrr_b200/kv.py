@@ -17,17 +17,28 @@ class KvCache:
         self._held = (k, v, weight, pos, err)      # the memory stays as long as the view
         self._dev = None if isinstance(k, int) or k is None else k.get_device()
         # k and v may have any strides: head_stride and seq_stride describe them
-        size, book = 2 if bf16 else 4, n_seq * n_head_kv * cap
-        self.view = Kv(self._at(k, 0, size, False), self._at(v, 0, size, False), int(bool(bf16)), n_seq, n_head_kv, head_dim, cap, head_stride, seq_stride,
+        book, head = n_seq * n_head_kv * cap, cap * head_dim
+        hs = head_stride if head_stride and n_head_kv > 1 else head
+        values = (n_seq - 1) * (seq_stride if seq_stride and n_seq > 1 else hs * n_head_kv) + (n_head_kv - 1) * hs + head
+        self.view = Kv(self._rows(k, values, bf16), self._rows(v, values, bf16), int(bool(bf16)), n_seq, n_head_kv, head_dim, cap, head_stride, seq_stride,
                        self._at(weight, book), self._at(pos, book), self._at(err, 1))
         self._ref = C.byref(self.view)
         self._lib = lib()
 
-    def _at(self, x, need=0, size=4, dense=True):
+    def _rows(self, x, need, bf16):
+        """The address of keys or values; behind a tensor's first value its memory has to hold all of them."""
+        if x is None or isinstance(x, int):
+            return x
+        dtype, left = "torch.bfloat16" if bf16 else "torch.float32", x.untyped_storage().nbytes() // x.element_size() - x.storage_offset()
+        if str(x.dtype) != dtype or left < need or x.get_device() != self._dev:
+            raise BrrrError(f"KvCache: {need} values of {dtype} on one device are wanted, not {left} of {x.dtype} on {x.device}")
+        return x.data_ptr()
+
+    def _at(self, x, need=0, size=4):
         """The address of a device array; a tensor has to be dense, of `size` bytes a value, of `need` values at least and on the cache's device."""
         if x is None or isinstance(x, int):
             return x
-        if (x.element_size() != size or x.numel() < need or (dense and not x.is_contiguous()) or
+        if (x.element_size() != size or x.numel() < need or not x.is_contiguous() or
                 (x.get_device() != self._dev if self._dev is not None else x.get_device() < 0)):
             raise BrrrError(f"KvCache: a contiguous array of {need} or more {size}-byte values on the cache's device is wanted, not {tuple(x.shape)} {x.dtype} on {x.device}")
         return x.data_ptr()
@@ -60,6 +71,8 @@ class KvCache:
     def evict(self, n, length, keep, first, recent, end, map, seq=None, dst=None, new_len=None, len_hint=0, stream=None):
         """The `keep` entries of each head with the largest weights (and the first and latest ones) in place, or into another KvCache."""
         p = self._at
+        if dst is not None and None not in (dst._dev, self._dev) and dst._dev != self._dev:
+            raise BrrrError("KvCache: dst is on another device")
         check(self._lib.brrr_kv_evict(self._ref, None if dst is None else dst._ref, n, p(seq, n), p(length, n), keep, first, recent, p(end, n),
                                       p(map, n * self.view.n_head_kv * keep), p(new_len, n), len_hint, stream), "brrr_kv_evict")
 

@@ -305,7 +305,8 @@ int brrr_qwen_cli_main(int argc, char **argv);
  * d_seq [n] names the sequences of a call; NULL: entry b is sequence b.  len_hint: about the largest length among the entries (0: unknown);
  * it steers how work is split, never what is computed.
  * A slot that a row does not see may hold anything, infinities and NaN included; a row that sees such a value has no defined result.  A sink may be
- * -infinity (no sink for that head), not +infinity; `scale` is any finite number. */
+ * -infinity (no sink for that head), not +infinity; `scale` is any finite number (scaled scores beyond single precision give no defined result).
+ * An output overlaps no input, except that d_out may be d_q. */
 enum { BRRR_KV_F32 = 0, BRRR_KV_BF16 = 1 };
 #define BRRR_TREE_MAX 64     /* rows per sequence of brrr_attn_tree, brrr_kv_commit and brrr_kv_weigh */
 #define BRRR_KV_CAP_MAX (1 << 19)     /* largest capacity */
@@ -349,7 +350,8 @@ int brrr_kv_commit(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, con
 
 /* Attention weights into the book: weight[seq][kv head][t] += sum over the rows i and the query heads h of that kv head of
  * exp(scale q.k_t - lse[b][i][h]) for every slot t that row i sees (as in brrr_attn_tree, with its d_lse).  d_rows [n] (nullable: all): bit i
- * says whether row i counts, so that only the accepted rows of a tree do.  The view needs a weight book. */
+ * says whether row i counts, so that only the accepted rows of a tree do; a d_lse of -infinity (the row sees nothing) adds nothing.  The view needs a
+ * weight book. */
 int brrr_kv_weigh(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, const int32_t *d_len, const int32_t *d_count, const uint64_t *d_mask,
                   const uint64_t *d_rows, int len_hint, const float *d_q, int n_head, float scale, int window, const float *d_lse, void *stream);
 
@@ -359,7 +361,7 @@ int brrr_kv_weigh(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, cons
  * ascending order, with their weights and positions: attention does not ask for an order, so no more than that moves.  d_map [n][n_head_kv][keep]: the
  * slot that each entry came from, -1 from m on.  dst NULL: in place (what lies behind m is then nobody's); else all kept entries are written to the same sequence of
  * dst, another view of the same type, heads and dimension with cap >= keep whose memory does not overlap.  d_new_len (nullable, not d_len) [n] = m.
- * first + recent <= keep.  Views need both books. */
+ * first + recent <= keep.  Views need both books.  For an entry that is left out: d_map -1, d_new_len len[b]. */
 int brrr_kv_evict(const brrr_kv *kv, const brrr_kv *dst, int n, const int32_t *d_seq, const int32_t *d_len, int keep, int first, int recent,
                   const int32_t *d_end, int32_t *d_map, int32_t *d_new_len, int len_hint, void *stream);
 

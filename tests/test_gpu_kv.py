@@ -169,6 +169,12 @@ def test_tree(brrr, dev, c):
         assert (out[b, m:] == 7.0).all() and (lse[b, m:] == 7.0).all()      # rows behind the count
     again, _ = run_tree(brrr, s, c, lse=False, hint=0)
     assert np.array_equal(again.cpu().numpy().reshape(out.shape), out)
+    inplace = s.up(s.q).view(c["n"], c["rows"], -1)
+    args = dict(seq=s.up(s.seq, np.int32) if "seq" in c else None, count=s.up(s.counts, np.int32) if "counts" in c else None,
+                mask=None if c["masks"] == "chain" else s.up(np.array(s.masks, np.uint64)), window=s.window, sinks=None if s.sinks is None else s.up(s.sinks))
+    s.view(brrr).attn_tree(c["n"], c["rows"], s.up(s.lens, np.int32), inplace, c["heads"], inplace, s.scale, **args)
+    for b in range(c["n"]):
+        assert np.array_equal(inplace.cpu().numpy().reshape(out.shape)[b, : s.counts[b]], out[b, : s.counts[b]])
     for hint in (1, s.cap, 1 << 20):                                          # a hint is no more than that
         other, _ = run_tree(brrr, s, c, lse=False, hint=hint)
         for b in range(c["n"]):
@@ -333,6 +339,12 @@ def test_wide_trees_and_their_weights(brrr, dev, c, scale):
         assert s.ok()
         again, _ = run_tree(brrr, s, c, hint=hint)
         assert torch.equal(out, again)
+        same = s.up(s.q).view(out.shape)
+        s.view(brrr).attn_tree(n, rows, s.up(s.lens, np.int32), same, c["heads"], same, s.scale, seq=s.up(s.seq, np.int32) if "seq" in c else None,
+                               count=s.up(s.counts, np.int32) if "counts" in c else None, mask=None if c["masks"] == "chain" else s.up(np.array(s.masks, np.uint64)),
+                               len_hint=hint, window=s.window, sinks=None if s.sinks is None else s.up(s.sinks))
+        for b in range(n):
+            assert torch.equal(same[b, : s.counts[b]], out[b, : s.counts[b]])
         for b in range(n):
             m = s.counts[b]
             if m:
@@ -385,6 +397,33 @@ def test_wide_rows_do_not_touch_what_other_rows_see(brrr, dev, bf16, hd):
     torch.cuda.synchronize()
     book = (weights[0][fine].sum(0)).view(2, 16, -1).sum(1)
     close(s.weight[0, :, :964].cpu().numpy(), book.cpu().numpy())
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_wide_rows_that_see_nothing(brrr, dev, bf16, hd, sinks):
+    """Rows without a slot stand between rows that have some: zeros, the sink or -infinity, and nothing in the book."""
+    import torch
+    c = dict(n=2, rows=64, lens=[0, 150], heads=32, kv=2, hd=hd, masks="tree", bf16=bf16, sinks=sinks)
+    s = prepared_tree(dev, c, seed=12)
+    s.k.nan_to_num_(0.1), s.v.nan_to_num_(0.2, 0.3, 0.4)
+    s.masks = [[m if i % 3 else 0 for i, m in enumerate(masks)] for masks in s.masks]
+    want, want_lse, weights = reference(s, c, s.up(s.q), s.scale)
+    assert (want_lse[0, ::3] == -math.inf).all() != sinks
+    for hint in (0, 1):
+        out, lse = run_tree(brrr, s, c, hint=hint)
+        close(out.cpu().numpy().reshape(want.shape), want.cpu().numpy())
+        close_lse(lse.cpu().numpy(), want_lse.cpu().numpy())
+        assert not out[0, ::3].any()
+    s.weight.fill_(1.0)
+    s.view(brrr).weigh(2, 64, s.up(s.lens, np.int32), s.up(s.q), 32, lse, s.scale, mask=s.up(np.array(s.masks, np.uint64)))
+    torch.cuda.synchronize()
+    book = torch.ones(s.weight.shape, dtype=torch.float64, device=dev)
+    for b in range(2):
+        book[b, :, : s.lens[b] + 64] += weights[b].sum(0).view(2, 16, -1).sum(1)
+    assert s.ok()
+    close(s.weight.cpu().numpy(), book.cpu().numpy())
 
 
 def test_wide_rows_far_beyond_32_bits(brrr, dev):
@@ -704,6 +743,10 @@ def test_blocks(brrr, dev, c):
                          sinks=None if sinks is None else s.up(sinks))
         torch.cuda.synchronize()
         close(other.cpu().numpy().reshape(want.shape), want)
+    inplace = s.up(q).view(rows, -1)
+    view.attn_blocks(rows, s.up(seq, np.int32), s.up(c["lens"], np.int32), block, means, nsel, c["first"], c["local"], inplace, c["heads"], inplace, scale, sel,
+                     sinks=None if sinks is None else s.up(sinks))
+    assert torch.equal(inplace, out)
 
 
 def test_blocks_leave_out(brrr, dev):

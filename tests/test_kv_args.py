@@ -126,6 +126,19 @@ def test_the_class_takes_tensors_of_the_right_kind_only(brrr):
     import torch
     kv = brrr.KvCache(P, 2 * P, 3, 4, 64, 100, weight=3 * P, pos=4 * P)
     i32, i64 = torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int64)
+    k = torch.zeros((1, 2, 16, 64))
+    for bad in (k.half(), k.bfloat16(), k.int(), k[:, :1], k.view(-1)[1:]):          # another type, memory that ends early
+        with pytest.raises(brrr.BrrrError, match="values of torch.float32"):
+            brrr.KvCache(k, bad if bad.dtype != k.dtype else bad.clone(), 1, 2, 64, 16)
+    with pytest.raises(brrr.BrrrError, match="values of torch.bfloat16"):
+        brrr.KvCache(k.half(), k.half(), 1, 2, 64, 16, bf16=True)
+    with pytest.raises(brrr.BrrrError, match="values of torch.float32"):
+        brrr.KvCache(k, k, 1, 2, 64, 16, head_stride=16 * 64 + 8)
+    assert brrr.KvCache(k[:, 1:], k[:, 1:], 1, 1, 64, 16, head_stride=8).view.cap == 16          # one head: its stride says nothing
+    here, there = brrr.KvCache(k, k, 1, 2, 64, 16), brrr.KvCache(k, k, 1, 2, 64, 16)
+    there._dev = 1
+    with pytest.raises(brrr.BrrrError, match="another device"):
+        here.evict(1, P, 5, 0, 0, None, P, dst=there)
     for call in (lambda: kv.attn_tree(1, 1, i32, P, 8, P, 1.0), lambda: kv.commit(1, 1, P, i64, P), lambda: kv.evict(1, i64, 5, 0, 0, None, P),
                  lambda: kv.weigh(1, 1, P, P, 8, P, 1.0, picked=i32)):
         with pytest.raises(brrr.BrrrError, match="cache's device"):
