@@ -38,7 +38,7 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const float4 &a, float b
 constexpr int STEP = 16;
 template <class T, int HD>
 struct Ring {
-    static constexpr int ROW = HD * (int)sizeof(typename T::Val), PLACE = STEP * ROW, BYTES = PLACE == 8192 ? 16384 : 12288, D = BYTES / PLACE;
+    static constexpr int ROW = HD * (int)sizeof(typename T::Val), PLACE = STEP * ROW, BYTES = PLACE == 8192 ? 16384 : HD == 64 ? 8192 : 12288, D = BYTES / PLACE;
     static constexpr int NC = HD / (4 * T::V), NVC = HD / (8 * T::V);       // 16-byte reads of a lane per slot: keys, values
     static_assert(D >= 2 && D <= 8, "");
     uint32_t at;             // of the ring, in shared memory
@@ -343,7 +343,7 @@ struct Room {
 
 // grid (C, kv heads x tiles of 8 NT rows, entries), clusters of C
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) tree_kernel(KvDev kv, TreeArgs a, const __grid_constant__ KvMaps maps) {
+__global__ void __launch_bounds__(AW * 32, HD == 64 ? (NT == 1 ? 4 : 3) : 2) tree_kernel(KvDev kv, TreeArgs a, const __grid_constant__ KvMaps maps) {
     typedef Ring<T, HD> Rg;
     typedef Room<T, HD, NT> Rm;
     constexpr int R = 8 * NT;
@@ -634,7 +634,7 @@ __device__ __forceinline__ void block_keys(const float *__restrict__ q, int per,
 }
 
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(AW * 32, HD == 64 ? 3 : 2) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel, int first, int local,
+__global__ void __launch_bounds__(AW * 32, HD == 64 ? (NT == 1 ? 4 : 3) : 2) blocks_kernel(KvDev kv, const int32_t *seq, const int32_t *len, int block, const float *__restrict__ means, int nsel, int first, int local,
                                                          const float *q, int nh, float scale, const float *sinks, int32_t *sel, float *o, float *lse,
                                                          const __grid_constant__ KvMaps maps) {
     typedef Ring<T, HD> Rg;
