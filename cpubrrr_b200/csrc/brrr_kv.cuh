@@ -83,47 +83,54 @@ __device__ __forceinline__ int nth_bit(uint32_t w, int n) {
     return at;
 }
 
-// Work space of block_kth in shared memory.  BITS at a time: eleven for a block of 1024 (the first hold sign, exponent and two more: fewer counts meet in
-// one word), eight for smaller ones (a thread has few words to clear and to add up).
+// Work space of block_kth in shared memory, for blocks of 1 << (BITS - 1) threads: a warp has 64 digits.
 template <int BITS>
 struct KthSpace {
-    uint32_t hist[1 << BITS], found[2], sums[32];
+    alignas(8) uint32_t hist[3][1 << BITS];
+    uint32_t sums[32], of_warps[32];                // of_warps: the caller's
+    __device__ __forceinline__ void clear() {       // before a barrier before block_kth
+        for (int i = threadIdx.x; i < 3 << BITS; i += blockDim.x) hist[0][i] = 0;
+    }
 };
-// The key of the k-th largest (1 <= k <= n) of key(0) .. key(n - 1), and how many of the keys that equal it are among the k largest.  All threads call it (at most
-// 1 << BITS of them); it ends with a barrier.
+// The key of the k-th largest (1 <= k <= n) of key(0) .. key(n - 1); how many of the keys that equal it are among the k largest, and how many there are.  All
+// threads call it.  BITS bits at a time, the highest first: counts of the digits among the keys that agree with what is known, sums per warp of 64 digits, then
+// every warp finds the digit for itself.  Two barriers a digit: counts stand in three places in turn, of which the one after the next is cleared.
 template <int BITS, class Key>
-__device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpace<BITS> &w, uint32_t *ties) {
+__device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpace<BITS> &w, uint32_t *ties, uint32_t *equal) {
+    constexpr int B = 1 << BITS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t prefix = 0, known = 0;
-    const int each = (1 << BITS) / blockDim.x;
+    uint32_t *hist = w.hist[0], *next = w.hist[1], *after = w.hist[2];
     for (int left = 32; left > 0;) {
         const int shift = max(0, left - BITS);
-        const uint32_t digit = (1u << (left - shift)) - 1;
-        left = shift;
-        for (int i = threadIdx.x; i < 1 << BITS; i += blockDim.x) w.hist[i] = 0;
-        __syncthreads();
+        const uint32_t mask = (1u << (left - shift)) - 1;
         for (int i = threadIdx.x; i < n; i += blockDim.x) {
             const uint32_t x = key(i);
-            if ((x & known) == prefix) atomicAdd(&w.hist[x >> shift & digit], 1u);
+            if ((x & known) == prefix) atomicAdd(&hist[x >> shift & mask], 1u);
         }
         __syncthreads();
-        // thread i: `each` digits, the largest first
-        const int top = (1 << BITS) - 1 - threadIdx.x * each;
-        uint32_t sum = 0;
-        for (int j = 0; j < each; j++) sum += w.hist[top - j];
-        uint32_t all;
-        uint32_t above = block_before(sum, w.sums, all);
-        const uint32_t upto = above + sum;
-        if (above < k && k <= upto)
-            for (int j = 0; j < each; j++) {
-                const uint32_t c = w.hist[top - j];
-                if (above < k && k <= above + c) { w.found[0] = top - j; w.found[1] = k - above; }
-                above += c;
-            }
+        if (left < 32)
+            for (int i = threadIdx.x; i < B; i += blockDim.x) after[i] = 0;
+        // digits B - 1 - 64 warp - 2 lane (the larger one: y) and the one below
+        uint2 c = *reinterpret_cast<const uint2 *>(&hist[B - 2 - 64 * warp - 2 * lane]);
+        const uint32_t all = __reduce_add_sync(0xffffffffu, c.x + c.y);
+        if (lane == 0) w.sums[warp] = all;
         __syncthreads();
-        prefix |= w.found[0] << shift;
-        known |= digit << shift;
-        k = w.found[1];
-        __syncthreads();
+        const uint32_t of_warp = lane < (int)(blockDim.x >> 5) ? w.sums[lane] : 0, upto = warp_scan(of_warp);
+        const int at = __ffs(__ballot_sync(0xffffffffu, upto >= k)) - 1;
+        k -= __shfl_sync(0xffffffffu, upto - of_warp, at);
+        c = *reinterpret_cast<const uint2 *>(&hist[B - 2 - 64 * at - 2 * lane]);
+        const uint32_t to = warp_scan(c.x + c.y), before = to - c.x - c.y;
+        const int hit = __ffs(__ballot_sync(0xffffffffu, to >= k)) - 1;
+        const bool lower = before + c.y < k;
+        const uint32_t digit = __shfl_sync(0xffffffffu, (uint32_t)(B - 1 - 64 * at - 2 * lane) - (lower ? 1u : 0u), hit);
+        k -= __shfl_sync(0xffffffffu, before + (lower ? c.y : 0u), hit);
+        *equal = __shfl_sync(0xffffffffu, lower ? c.x : c.y, hit);
+        prefix |= digit << shift;
+        known |= mask << shift;
+        left = shift;
+        uint32_t *old = hist;
+        hist = next; next = after; after = old;
     }
     *ties = k;
     return prefix;

@@ -155,7 +155,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t *v, int n, uint32_t *war
     }
     return carry;
 }
-// The last i of v[0 .. n) with v[i] <= x; v[0] is 0 and v does not fall.
+// The last i of v[0 .. n) with v[i] <= x; v[0] is, and v does not fall.
 __device__ __forceinline__ int last_upto(const uint32_t *v, int n, uint32_t x) {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
                                                               const int32_t *end, int32_t *map, int32_t *new_len) {
     extern __shared__ uint32_t sm[];
     __shared__ KthSpace<11> kth;
+    kth.clear();
     pdl_wait();
     const int kvh = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = EV_THREADS / 32;
     const KvEntry e = kv_entry(kv, b, 0, seq, len, nullptr);
@@ -194,50 +195,51 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     const int32_t *pos = kv.pos + kv.book(e.seq, kvh);
     const long long from = recent > 0 ? (long long)end[b] - recent : 1ll << 31;
     const int words = (e.len + 31) / 32, mw = m / 32;
-    uint32_t *kept = sm, *run = sm + words, *keys = run + words + 1;
+    uint32_t *kept = sm, *run = sm + words, *same_of = run + words + 1, *keys = same_of + words;
+    // a thread has slots t, t + 1024, ... throughout: nobody else reads its keys
     if (KEEP_KEYS) {
 #pragma unroll 4
         for (int t = threadIdx.x; t < e.len; t += EV_THREADS) keys[t] = evict_key(w[t], pos[t], first, from);
-        __syncthreads();
     }
+    __syncthreads();
     auto key = [&](int t) { return KEEP_KEYS ? keys[t] : evict_key(w[t], pos[t], first, from); };
-    uint32_t ties;
-    const uint32_t last = block_kth(e.len, m, key, kth, &ties);
-    // kept: bits of 32 slots each; run: running counts [words + 1]
+    uint32_t ties, equal;
+    const uint32_t last = block_kth(e.len, m, key, kth, &ties, &equal), below = (1u << lane) - 1;
+    if (ties < equal) {              // of those with the last one's key the lower slots: how many are before each word
+        for (int i = warp; i < words; i += nwarp) {
+            const int t = i * 32 + lane;
+            const uint32_t same = __ballot_sync(0xffffffffu, t < e.len && key(t) == last);
+            if (lane == 0) same_of[i] = __popc(same);
+        }
+        __syncthreads();
+        block_scan(same_of, words, kth.of_warps);
+    }
+    // kept: bits of 32 slots each; run: freed slots below m of words 0 .. mw, then kept ones behind of words mw .. words - 1 (one place further on)
+    const uint32_t low = (1u << (m & 31)) - 1;
     for (int i = warp; i < words; i += nwarp) {
         const int t = i * 32 + lane;
         const uint32_t x = t < e.len ? key(t) : 0;
-        const uint32_t over = __ballot_sync(0xffffffffu, t < e.len && x > last), same = __ballot_sync(0xffffffffu, t < e.len && x == last);
-        if (lane == 0) { kept[i] = over; run[i] = __popc(same); }
-    }
-    __syncthreads();
-    block_scan(run, words, kth.sums);
-    for (int i = warp; i < words; i += nwarp) {
-        const int t = i * 32 + lane;
-        const bool same = t < e.len && key(t) == last;
-        const uint32_t all = __ballot_sync(0xffffffffu, same);
-        const uint32_t mine = __ballot_sync(0xffffffffu, same && run[i] + __popc(all & ((1u << lane) - 1)) < ties);
-        if (lane == 0) kept[i] |= mine;
+        const uint32_t over = __ballot_sync(0xffffffffu, t < e.len && x > last);
+        uint32_t same = __ballot_sync(0xffffffffu, t < e.len && x == last);
+        if (ties < equal) same = __ballot_sync(0xffffffffu, (same >> lane & 1) && same_of[i] + __popc(same & below) < ties);
+        if (lane == 0) {
+            const uint32_t in = over | same;
+            kept[i] = in;
+            if (i <= mw) run[i] = __popc(~in & (i == mw ? low : 0xffffffffu));
+            if (i >= mw) run[i + 1] = __popc(in & (i == mw ? ~low : 0xffffffffu));
+        }
     }
     __syncthreads();
     pdl_trigger();
-    // freed slots below m per word 0 .. mw, then kept ones behind per word mw .. words - 1 (one place further on)
-    const uint32_t low = (1u << (m & 31)) - 1;
-    for (int i = threadIdx.x; i <= words; i += EV_THREADS) {
-        if (i < mw) run[i] = __popc(~kept[i]);
-        else if (i == mw) run[i] = __popc(~kept[i] & low);
-        else run[i] = __popc(i - 1 == mw ? kept[i - 1] & ~low : kept[i - 1]);
-    }
-    __syncthreads();
-    block_scan(run, mw + 1, kth.sums);
-    const int moved = (int)block_scan(run + mw + 1, words - mw, kth.sums);
+    block_scan(run, words + 1, kth.of_warps);
+    const int moved = (int)run[mw + 1];           // as many are freed as are kept behind
     for (int t = threadIdx.x; t < m; t += EV_THREADS)
         if (kept[t >> 5] >> (t & 31) & 1) out[t] = t;
     // the j-th kept entry behind takes the j-th freed slot
     for (int j = threadIdx.x; j < moved; j += EV_THREADS) {
-        const int h = last_upto(run, mw + 1, j), f = mw + last_upto(run + mw + 1, words - mw, j);
+        const int h = last_upto(run, mw + 1, j), f = mw + last_upto(run + mw + 1, words - mw, moved + j);
         const uint32_t holes = ~kept[h] & (h == mw ? low : 0xffffffffu), behind = f == mw ? kept[f] & ~low : kept[f];
-        out[h * 32 + nth_bit(holes, j - run[h])] = f * 32 + nth_bit(behind, j - run[f + 1]);
+        out[h * 32 + nth_bit(holes, j - run[h])] = f * 32 + nth_bit(behind, moved + j - run[f + 1]);
     }
 }
 
@@ -277,11 +279,11 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvDev kv, KvDev dst, bool 
 cudaError_t launch_kv_evict(const KvDev &kv, const KvDev *dst, int n, const int32_t *seq, const int32_t *len, int keep, int first, int recent, const int32_t *end,
                             int32_t *map, int32_t *new_len, int len_hint, cudaStream_t st) {
     const KvDev &to = dst ? *dst : kv;
-    const size_t bits = ((size_t)(kv.cap + 31) / 32 * 2 + 1) * 4, all = bits + (size_t)kv.cap * 4, most = 200 * 1024;
+    const size_t bits = ((size_t)(kv.cap + 31) / 32 * 3 + 1) * 4, all = bits + (size_t)kv.cap * 4, most = 200 * 1024;
     const bool keys = all <= most;
     const size_t smem = keys ? all : bits;
     auto kern = keys ? kv_evict_kernel<true> : kv_evict_kernel<false>;
-    cudaError_t e = smem > 36 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) : cudaSuccess;
+    cudaError_t e = smem > 20 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) : cudaSuccess;
     if (e != cudaSuccess) return e;
     e = launch_k(kern, dim3(kv.nkv, n), dim3(EV_THREADS), smem, st, true, kv, to, seq, len, keep, first, recent, end, map, new_len);
     if (e != cudaSuccess) return e;

@@ -648,11 +648,13 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? (NT == 1 ? 4 : 3) : 2) blo
     __shared__ int32_t chosen[256];
     __shared__ float qs[16 * HD];
     __shared__ KthSpace<8> kth;
+    static_assert(AW * 32 == 1 << 7, "as block_kth wants it");
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks();
     const int r = blockIdx.y, kvh = blockIdx.z, per = nh / kv.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (C > 1) cluster_arrive();
     Rg ring(asm_, bars, maps);
+    kth.clear();
     pdl_wait();
     pdl_trigger();
     const int s = seq ? seq[r] : r, n = len[r];
@@ -700,9 +702,9 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? (NT == 1 ? 4 : 3) : 2) blo
         } else {
             __syncthreads();
         }
-        uint32_t ties;
+        uint32_t ties, equal;
         const int want = nsel - first - local;
-        const uint32_t last = want > 0 ? block_kth(hi - first, want, [&](int i) { return keys[first + i]; }, kth, &ties) : 0xFFFFFFFFu;
+        const uint32_t last = want > 0 ? block_kth(hi - first, want, [&](int i) { return keys[first + i]; }, kth, &ties, &equal) : 0xFFFFFFFFu;
         if (want <= 0) ties = 0;
         // the places of the chosen ones, in ascending order of blocks: a warp has a run of 32 w blocks and counts them first; both counts in one word
         const int run = (nb + 32 * AW - 1) / (32 * AW), j0 = warp * run * 32 + lane;
@@ -718,10 +720,10 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? (NT == 1 ? 4 : 3) : 2) blo
             kind(j0 + 32 * w, over, same);
             count += __popc(__ballot_sync(0xffffffffu, over)) | __popc(__ballot_sync(0xffffffffu, same)) << 16;
         }
-        if (lane == 0) kth.sums[warp] = count;
+        if (lane == 0) kth.of_warps[warp] = count;
         __syncthreads();
         uint32_t before = 0;
-        for (int w = 0; w < warp; w++) before += kth.sums[w];
+        for (int w = 0; w < warp; w++) before += kth.of_warps[w];
         for (int w = 0; w < run; w++) {
             bool over, same;
             kind(j0 + 32 * w, over, same);

@@ -603,7 +603,8 @@ EVICT = [dict(n=1, lens=[1], keep=1, first=0, recent=0), dict(n=1, lens=[2], kee
          dict(n=2, lens=[1025, 1024], keep=1024, first=4, recent=64, hd=128), dict(n=2, lens=[4000, 3999], keep=31, first=0, recent=31, bf16=True),
          dict(n=2, lens=[3000, 64], keep=64, first=64, recent=0, hd=128, bf16=True), dict(n=2, lens=[2500, 999], keep=1300, first=4, recent=100, seq=[2, 0]),
          dict(n=1, lens=[700], keep=350, first=0, recent=0, book="ties"), dict(n=1, lens=[700], keep=97, first=3, recent=9, book="odd"),
-         dict(n=1, lens=[96], keep=64, first=0, recent=0, book="ties"), dict(n=1, lens=[33000], keep=20011, first=100, recent=1000, kv=1)]
+         dict(n=1, lens=[96], keep=64, first=0, recent=0, book="ties"), dict(n=1, lens=[33000], keep=20011, first=100, recent=1000, kv=1),
+         dict(n=1, lens=[50001], keep=30011, first=7, recent=100, kv=1, book="ties"), dict(n=1, lens=[7001], keep=3500, first=0, recent=0, kv=2, book="odd")]
 
 
 def evict_setup(dev, c, seed):
