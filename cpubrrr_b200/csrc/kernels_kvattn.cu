@@ -341,7 +341,8 @@ struct Room {
     static_assert(R * HD * 4 <= Ring<T, HD>::BYTES, "a warp's part fits its ring");
 };
 
-// grid (C, kv heads x tiles of 8 NT rows, entries), clusters of C
+// grid (C, kv heads x tiles of 8 NT rows, entries), clusters of C.  One token, 73 slots: 7.5 us alone, of which about 3 are launch and lists; 12 sequences of 1023 slots
+// 17 us, 50 MB of keys and values at 3 TB/s: a warp's share is 16 steps, and the first copies and the join are not hidden behind so few.
 template <class T, int HD, int NT>
 __global__ void __launch_bounds__(AW * 32, HD == 64 ? (NT == 1 ? 4 : 3) : 2) tree_kernel(KvDev kv, TreeArgs a, const __grid_constant__ KvMaps maps) {
     typedef Ring<T, HD> Rg;
@@ -447,7 +448,7 @@ static cudaError_t launch_tree(const KvDev &kv, const TreeArgs &a, int slots, cu
 
 // Whether the kernel of 128-row tiles (kernels_kvtc.cu) takes less time than CTAs of 16 rows.  Both were measured with 8 to 256 rows, 1 and 8 sequences, 40 to 2500
 // slots (20 calls in a graph, in L2): a tile of 128 rows takes the time of one and a half of 16, and a start of `start` tiles of 16 rows x 128 slots (spread over
-// the GPU) more.  The rule takes at most 14 % more than the better one of the two (38 % for 256 rows of 128 f32 dimensions over 700 slots: 17.0 and 23.4 us).  64
+// the GPU) more.  The rule takes at most 10 % more than the better one of the two (38 % for 256 rows of 128 f32 dimensions over 700 slots: 17.0 and 23.4 us).  64
 // dimensions f32, 8 heads: 64 rows over 200 slots 6.4 and 13.0 us, over 2500 15.8 and 17.0; 8 sequences: 32 rows over 700 16.0 and 18.7, 128 rows over 2500
 // 151 and 40.
 static bool wide_rows_pay(const KvDev &kv, const TreeArgs &a, int slots) {
@@ -467,7 +468,8 @@ cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, c
 }
 
 // ---------------------------------------------------------------- book of weights
-// Up to 16 rows per kv head (more: kernels_kvtc.cu).  A warp owns a step of slots: the scores of its keys, their powers, the sum over the rows.
+// Up to 16 rows per kv head.  A warp owns a step of slots: the scores of its keys, their powers, the sum over the rows.  24 sequences of 3801 f32 slots: 29.8 us, keys at
+// 5 TB/s.  More rows go to kernels_kvtc.cu; 16 take 3.8 us here and 6.1 there over 200 slots of 64 f32 dimensions, 13.2 and 23.4 from 8 sequences of 2500.
 template <class T, int HD, int NT>
 __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked, const __grid_constant__ KvMaps maps) {
     typedef Ring<T, HD> Rg;
@@ -586,7 +588,9 @@ cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *
 
 // ---------------------------------------------------------------- chosen blocks
 // A cluster per (kv head, row).  Its CTAs share the blocks' scores: products of f64 (mma m8n8k4, 8 heads by 8 blocks), whose largest over the heads every CTA
-// gets as a 32-bit key in the order of the values.  Then each CTA finds the nsel largest keys and takes its share of the chosen blocks' steps.
+// gets as a 32-bit key in the order of the values.  Then each CTA finds the nsel largest keys and takes its share of the chosen blocks' steps.  201 rows x 8 heads over 282
+// blocks, 24 of 32 f32 slots chosen: 117 us, 632 MB of keys and values out of L2 at 5.4 TB/s, issue slots half full (rings of 12 KB and three CTAs on an SM:
+// 144 us).  One row over 954 bf16 blocks of 64: 18.8 us, a sequence of latencies (means, scores, cluster barrier, four digits, 16 steps, join).
 __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
     asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
 }
