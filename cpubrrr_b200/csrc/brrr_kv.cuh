@@ -92,16 +92,19 @@ struct KthSpace {
         for (int i = threadIdx.x; i < 3 << BITS; i += blockDim.x) hist[0][i] = 0;
     }
 };
-// The key of the k-th largest (1 <= k <= n) of key(0) .. key(n - 1); how many of the keys that equal it are among the k largest, and how many there are.  All
-// threads call it.  BITS bits at a time, the highest first: counts of the digits among the keys that agree with what is known, sums per warp of 64 digits, then
-// every warp finds the digit for itself.  Two barriers a digit: counts stand in three places in turn, of which the one after the next is cleared.
+// Of the k-th largest (1 <= k <= n) of key(0) .. key(n - 1) the leading bits, `known` of them, that tell it from the others; how many of the keys with these
+// bits are among the k largest, and how many there are: as many, or all bits are known.  All threads call it.  BITS bits at a time, the highest first: counts of the
+// digits among the keys that agree with what is known, sums per warp of 64 digits, then every warp finds the digit for itself.  Two barriers a digit: counts
+// stand in three places in turn, of which the one after the next is cleared.
 template <int BITS, class Key>
-__device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpace<BITS> &w, uint32_t *ties, uint32_t *equal) {
+__device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpace<BITS> &w, uint32_t &known, uint32_t &ties, uint32_t &equal) {
     constexpr int B = 1 << BITS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t prefix = 0, known = 0;
+    uint32_t prefix = 0;
+    known = 0;
+    equal = ~0u;
     uint32_t *hist = w.hist[0], *next = w.hist[1], *after = w.hist[2];
-    for (int left = 32; left > 0;) {
+    for (int left = 32; left > 0 && k != equal;) {
         const int shift = max(0, left - BITS);
         const uint32_t mask = (1u << (left - shift)) - 1;
         for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -125,14 +128,14 @@ __device__ __forceinline__ uint32_t block_kth(int n, uint32_t k, Key key, KthSpa
         const bool lower = before + c.y < k;
         const uint32_t digit = __shfl_sync(0xffffffffu, (uint32_t)(B - 1 - 64 * at - 2 * lane) - (lower ? 1u : 0u), hit);
         k -= __shfl_sync(0xffffffffu, before + (lower ? c.y : 0u), hit);
-        *equal = __shfl_sync(0xffffffffu, lower ? c.x : c.y, hit);
+        equal = __shfl_sync(0xffffffffu, lower ? c.x : c.y, hit);
         prefix |= digit << shift;
         known |= mask << shift;
         left = shift;
         uint32_t *old = hist;
         hist = next; next = after; after = old;
     }
-    *ties = k;
+    ties = k;
     return prefix;
 }
 

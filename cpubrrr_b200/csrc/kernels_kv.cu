@@ -199,19 +199,19 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     const long long from = recent > 0 ? (long long)end[b] - recent : 1ll << 31;
     const int words = (e.len + 31) / 32, mw = m / 32;
     uint32_t *kept = sm, *run = sm + words, *same_of = run + words + 1, *keys = same_of + words;
-    // a thread has slots t, t + 1024, ... throughout: nobody else reads its keys
+    // a thread has slots t, t + EV_THREADS, ... throughout: nobody else reads its keys
     if (KEEP_KEYS) {
 #pragma unroll 4
         for (int t = threadIdx.x; t < e.len; t += EV_THREADS) keys[t] = evict_key(w[t], pos[t], first, from);
     }
     __syncthreads();
     auto key = [&](int t) { return KEEP_KEYS ? keys[t] : evict_key(w[t], pos[t], first, from); };
-    uint32_t ties, equal;
-    const uint32_t last = block_kth(e.len, m, key, kth, &ties, &equal), below = (1u << lane) - 1;
+    uint32_t known, ties, equal;
+    const uint32_t last = block_kth(e.len, m, key, kth, known, ties, equal), below = (1u << lane) - 1;
     if (ties < equal) {              // of those with the last one's key the lower slots: how many are before each word
         for (int i = warp; i < words; i += nwarp) {
             const int t = i * 32 + lane;
-            const uint32_t same = __ballot_sync(0xffffffffu, t < e.len && key(t) == last);
+            const uint32_t same = __ballot_sync(0xffffffffu, t < e.len && key(t) == last);          // all bits are known
             if (lane == 0) same_of[i] = __popc(same);
         }
         __syncthreads();
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     const uint32_t low = (1u << (m & 31)) - 1;
     for (int i = warp; i < words; i += nwarp) {
         const int t = i * 32 + lane;
-        const uint32_t x = t < e.len ? key(t) : 0;
+        const uint32_t x = t < e.len ? key(t) & known : 0;
         const uint32_t over = __ballot_sync(0xffffffffu, t < e.len && x > last);
         uint32_t same = __ballot_sync(0xffffffffu, t < e.len && x == last);
         if (ties < equal) same = __ballot_sync(0xffffffffu, (same >> lane & 1) && same_of[i] + __popc(same & below) < ties);
@@ -236,9 +236,23 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     pdl_trigger();
     block_scan(run, words + 1, kth.of_warps);
     const int moved = (int)run[mw + 1];           // as many are freed as are kept behind
-    for (int t = threadIdx.x; t < m; t += EV_THREADS)
-        if (kept[t >> 5] >> (t & 31) & 1) out[t] = t;
     // the j-th kept entry behind takes the j-th freed slot
+    if (KEEP_KEYS) {
+        uint32_t *behind = keys;                  // which nobody needs any more
+        for (int t = mw * 32 + threadIdx.x; t < e.len; t += EV_THREADS) {
+            const int i = t >> 5;
+            const uint32_t in = i == mw ? kept[i] & ~low : kept[i];
+            if (in >> (t & 31) & 1) behind[run[i + 1] - moved + __popc(in & below)] = t;
+        }
+        __syncthreads();
+        for (int t = threadIdx.x; t < m; t += EV_THREADS) {
+            const uint32_t in = kept[t >> 5];
+            out[t] = in >> lane & 1 ? t : behind[run[t >> 5] + __popc(~in & below)];
+        }
+        return;
+    }
+    for (int t = threadIdx.x; t < m; t += EV_THREADS)
+        if (kept[t >> 5] >> lane & 1) out[t] = t;
     for (int j = threadIdx.x; j < moved; j += EV_THREADS) {
         const int h = last_upto(run, mw + 1, j), f = mw + last_upto(run + mw + 1, words - mw, moved + j);
         const uint32_t holes = ~kept[h] & (h == mw ? low : 0xffffffffu), behind = f == mw ? kept[f] & ~low : kept[f];

@@ -706,15 +706,14 @@ __global__ void __launch_bounds__(AW * 32, HD == 64 ? (NT == 1 ? 4 : 3) : 2) blo
         } else {
             __syncthreads();
         }
-        uint32_t ties, equal;
+        uint32_t known = ~0u, ties = 0, equal;
         const int want = nsel - first - local;
-        const uint32_t last = want > 0 ? block_kth(hi - first, want, [&](int i) { return keys[first + i]; }, kth, &ties, &equal) : 0xFFFFFFFFu;
-        if (want <= 0) ties = 0;
+        const uint32_t last = want > 0 ? block_kth(hi - first, want, [&](int i) { return keys[first + i]; }, kth, known, ties, equal) : 0xFFFFFFFFu;
         // the places of the chosen ones, in ascending order of blocks: a warp has a run of 32 w blocks and counts them first; both counts in one word
         const int run = (nb + 32 * AW - 1) / (32 * AW), j0 = warp * run * 32 + lane;
         auto kind = [&](int j, bool &over, bool &same) {
             const bool free = j >= first && j < hi;
-            const uint32_t k = free ? keys[j] : 0;
+            const uint32_t k = free ? keys[j] & known : 0;
             over = (j < nb && !free) || (free && want > 0 && k > last);
             same = free && want > 0 && k == last;
         };
