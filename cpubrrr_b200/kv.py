@@ -34,12 +34,15 @@ class KvCache:
             raise BrrrError(f"KvCache: {need} values of {dtype} on one device are wanted, not {left} of {x.dtype} on {x.device}")
         return x.data_ptr()
 
-    def _at(self, x, need=0, size=4):
+    def _at(self, x, need, size=4):
         """The address of a device array; a tensor has to be dense, of `size` bytes a value, of `need` values at least and on the cache's device."""
-        if x is None or isinstance(x, int):
-            return x
-        if (x.element_size() != size or x.numel() < need or not x.is_contiguous() or
-                (x.get_device() != self._dev if self._dev is not None else x.get_device() < 0)):
+        if x is None:
+            return None
+        try:
+            here = x.get_device()
+        except AttributeError:
+            return x                               # an address
+        if x.element_size() != size or x.numel() < need or not x.is_contiguous() or here < 0 or (here != self._dev and self._dev is not None):
             raise BrrrError(f"KvCache: a contiguous array of {need} or more {size}-byte values on the cache's device is wanted, not {tuple(x.shape)} {x.dtype} on {x.device}")
         return x.data_ptr()
 
