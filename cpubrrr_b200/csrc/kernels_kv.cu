@@ -132,10 +132,10 @@ cudaError_t launch_kv_commit(const KvDev &kv, int n, int rows, const int32_t *se
 
 // ---------------------------------------------------------------- eviction
 // Which entries stay: a CTA per (kv head, entry) finds the key of the last one kept digit by digit, then turns the keys into one bit per slot, and pairs the
-// freed slots below m with the kept entries behind.  Bits and running counts per 32 slots stand in shared memory, and the keys where there is
+// freed slots below m with the kept entries behind: by a list of these where the keys stood, by searches in the running counts where there is no such room.  Bits and running counts per 32 slots stand in shared memory, and the keys where there is
 // room for a cache's (46,000 slots; above, they are formed from the books again at every pass).  Bound by barriers and dependent reads, not by bytes: 8 heads x
-// 4096 entries 12.9 us alone, 128 heads of 32 caches x 3900 15.1.  Sums by walking instead of two levels of warp scans, and five barriers a digit: 19.4 and 15.2 us
-// for a whole eviction from one cache, now 12.8.
+// 4096 entries 11.9 us alone, 128 heads of 32 caches x 3900 13.8.  A whole eviction from one cache took 19.4 us with sums by walking, 15.2 with five barriers a digit,
+// 12.8 with pairs by two searches, and takes 12.4.  512 threads: 13.8 and 18.9 us in place of 12.9 and 15.1.
 constexpr int EV_THREADS = 1024;
 
 // protected entries above all weights, NaN below all, -0 as +0

@@ -589,8 +589,8 @@ cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *
 // ---------------------------------------------------------------- chosen blocks
 // A cluster per (kv head, row).  Its CTAs share the blocks' scores: products of f64 (mma m8n8k4, 8 heads by 8 blocks), whose largest over the heads every CTA
 // gets as a 32-bit key in the order of the values.  Then each CTA finds the nsel largest keys and takes its share of the chosen blocks' steps.  201 rows x 8 heads over 282
-// blocks, 24 of 32 f32 slots chosen: 117 us, 632 MB of keys and values out of L2 at 5.4 TB/s, issue slots half full (rings of 12 KB and three CTAs on an SM:
-// 144 us).  One row over 954 bf16 blocks of 64: 18.8 us, a sequence of latencies (means, scores, cluster barrier, four digits, 16 steps, join).
+// blocks, 24 of 32 f32 slots chosen: 115 us, 632 MB of keys and values out of L2 at 5.5 TB/s, issue slots half full (rings of 12 KB and three CTAs on an SM
+// took 24 us more).  One row over 954 bf16 blocks of 64: 18.2 us, a sequence of latencies (means, scores, cluster barrier, digits, steps, join).
 __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
     asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
 }
