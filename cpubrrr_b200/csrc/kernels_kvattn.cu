@@ -10,7 +10,7 @@
 //
 // Every warp has a ring of operands of its own in shared memory, filled by tensor copies of 16 rows several operands ahead, and waits for nobody else.  The
 // copies swizzle the rows: with rows as they are, 16-byte reads of keys met two and of values four to a bank (201 tokens x 8 heads over 24 blocks of 32 f32
-// slots took 159 us, now 144).  The k index of a product may be any order of the dimensions (slots) that both operands have, so a lane's k = t, t + 4 of
+// slots took 159 us in place of 144).  The k index of a product may be any order of the dimensions (slots) that both operands have, so a lane's k = t, t + 4 of
 // consecutive products are the consecutive values of one 16-byte read, and the rows of V^T may be any order of the dimensions.  Weights change from the
 // accumulator's place (slot g, rows 2t, 2t + 1 in lane 4 g + t) to operand B's (slots 2t, 2t + 1, row g) by shuffles.  Queries are split once and wait in
 // shared memory in fragment order.
