@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     block_scan(run, words + 1, kth.of_warps);
     const int moved = (int)run[mw + 1];           // as many are freed as are kept behind
     // the j-th kept entry behind takes the j-th freed slot
-    if (KEEP_KEYS) {
+    if constexpr (KEEP_KEYS) {
         uint32_t *behind = keys;                  // which nobody needs any more
         for (int t = mw * 32 + threadIdx.x; t < e.len; t += EV_THREADS) {
             const int i = t >> 5;
@@ -249,20 +249,21 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
             const uint32_t in = kept[t >> 5];
             out[t] = in >> lane & 1 ? t : behind[run[t >> 5] + __popc(~in & below)];
         }
-        return;
-    }
-    for (int t = threadIdx.x; t < m; t += EV_THREADS)
-        if (kept[t >> 5] >> lane & 1) out[t] = t;
-    for (int j = threadIdx.x; j < moved; j += EV_THREADS) {
-        const int h = last_upto(run, mw + 1, j), f = mw + last_upto(run + mw + 1, words - mw, moved + j);
-        const uint32_t holes = ~kept[h] & (h == mw ? low : 0xffffffffu), behind = f == mw ? kept[f] & ~low : kept[f];
-        out[h * 32 + nth_bit(holes, j - run[h])] = f * 32 + nth_bit(behind, moved + j - run[f + 1]);
+    } else {
+        for (int t = threadIdx.x; t < m; t += EV_THREADS)
+            if (kept[t >> 5] >> lane & 1) out[t] = t;
+        for (int j = threadIdx.x; j < moved; j += EV_THREADS) {
+            const int h = last_upto(run, mw + 1, j), f = mw + last_upto(run + mw + 1, words - mw, moved + j);
+            const uint32_t holes = ~kept[h] & (h == mw ? low : 0xffffffffu), behind = f == mw ? kept[f] & ~low : kept[f];
+            out[h * 32 + nth_bit(holes, j - run[h])] = f * 32 + nth_bit(behind, moved + j - run[f + 1]);
+        }
     }
 }
 
 // A thread moves 16 bytes of up to MV_BATCH entries' keys and values, all read before the first is written; the books go with an entry's first bytes.
-// 32 caches x 4 heads, 2001 entries of 256 bytes: 48.8 us, 4.9 TB/s read and written (four entries in flight per thread).
-constexpr int MV_BATCH = 4;
+// Bound by memory: evictions from 32 caches x 4 heads, 2001 entries of 256 bytes, take 54 us with two entries a thread (4.9 TB/s read and written, the
+// selection's 10 us among them), 59 with one, 57 with three, 61 with four, 79 with eight.
+constexpr int MV_BATCH = 2;
 __global__ void __launch_bounds__(256) kv_move_kernel(KvDev kv, KvDev dst, bool inplace, const int32_t *seq, int keep, const int32_t *map) {
     const int kvh = blockIdx.y, b = blockIdx.z, per = kv.hd * kv.size() / 16;       // a power of two
     pdl_wait();
