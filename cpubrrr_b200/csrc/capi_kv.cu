@@ -43,7 +43,8 @@ bool apart(const void *a, int64_t na, const void *b, int64_t nb) {
     return x + (uintptr_t)na <= y || y + (uintptr_t)nb <= x;
 }
 
-bool finite(float x) { return x - x == 0.0f; }
+// log2(e) times twice the scale stays in single precision: beyond, a score of zero would be no number
+bool scale_ok(float x) { return x >= -BRRR_KV_SCALE_MAX && x <= BRRR_KV_SCALE_MAX; }
 bool heads_ok(const KvDev &d, int n_head) { return n_head > 0 && n_head % d.nkv == 0 && n_head / d.nkv <= 16; }
 
 // The memory belongs to the device whose stream the kernels go to: a pointer of another one (or of the host) would fault there.
@@ -80,7 +81,7 @@ extern "C" int brrr_attn_tree(const brrr_kv *kv, int n, int rows, const int32_t 
     KvDev d;
     if (!view(kv, &d) || !d_len || !d_q || !d_out || off16(d_q) || off16(d_out) || ((uintptr_t)d_mask & 7)) return BRRR_ERR_ARG;
     if (n <= 0 || n > 65535 || rows <= 0 || rows > BRRR_TREE_MAX || !heads_ok(d, n_head) || window < 0 || (!d_seq && n > d.n_seq)) return BRRR_ERR_ARG;
-    if (!finite(scale) || off4(d_seq, d_len, d_count, d_sinks, d_lse)) return BRRR_ERR_ARG;
+    if (!scale_ok(scale) || off4(d_seq, d_len, d_count, d_sinks, d_lse)) return BRRR_ERR_ARG;
     if (int rc = on_this_device(d)) return rc;
     const TreeArgs a{n, rows, d_seq, d_len, d_count, d_mask, d_q, n_head, scale, window, d_sinks, d_out, d_lse};
     return done(launch_attn_tree(d, a, len_hint, (cudaStream_t)stream));
@@ -100,7 +101,7 @@ extern "C" int brrr_kv_weigh(const brrr_kv *kv, int n, int rows, const int32_t *
     KvDev d;
     if (!view(kv, &d) || !d.weight || !d_len || !d_q || !d_lse || off16(d_q) || ((uintptr_t)d_mask & 7) || ((uintptr_t)d_rows & 7)) return BRRR_ERR_ARG;
     if (n <= 0 || n > 65535 || rows <= 0 || rows > BRRR_TREE_MAX || !heads_ok(d, n_head) || window < 0 || (!d_seq && n > d.n_seq)) return BRRR_ERR_ARG;
-    if (!finite(scale) || off4(d_seq, d_len, d_count, d_lse)) return BRRR_ERR_ARG;
+    if (!scale_ok(scale) || off4(d_seq, d_len, d_count, d_lse)) return BRRR_ERR_ARG;
     if (int rc = on_this_device(d)) return rc;
     const TreeArgs a{n, rows, d_seq, d_len, d_count, d_mask, d_q, n_head, scale, window, nullptr, nullptr, const_cast<float *>(d_lse)};
     return done(launch_kv_weigh(d, a, d_rows, len_hint, (cudaStream_t)stream));
@@ -143,7 +144,7 @@ extern "C" int brrr_attn_blocks(const brrr_kv *kv, int rows, const int32_t *d_se
     if (!view(kv, &d) || !d_len || !d_q || !d_sel || !d_out || off16(d_means) || off16(d_q) || off16(d_out)) return BRRR_ERR_ARG;
     if ((block != 16 && block != 32 && block != 64 && block != 128) || (!d_means && d.cap >= block)) return BRRR_ERR_ARG;
     if (rows <= 0 || rows > 65535 || !heads_ok(d, n_head) || nsel <= 0 || nsel > 256 || first < 0 || local < 1 || first > nsel || local > nsel - first) return BRRR_ERR_ARG;
-    if ((!d_seq && rows > d.n_seq) || !finite(scale) || off4(d_seq, d_len, d_sinks, d_sel, d_lse)) return BRRR_ERR_ARG;
+    if ((!d_seq && rows > d.n_seq) || !scale_ok(scale) || off4(d_seq, d_len, d_sinks, d_sel, d_lse)) return BRRR_ERR_ARG;
     if (d.cap / block > 16384) return BRRR_ERR_RANGE;
     if (int rc = on_this_device(d)) return rc;
     return done(launch_attn_blocks(d, rows, d_seq, d_len, block, d_means, nsel, first, local, len_hint, d_q, n_head, scale, d_sinks, d_sel, d_out, d_lse,

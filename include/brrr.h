@@ -305,11 +305,12 @@ int brrr_qwen_cli_main(int argc, char **argv);
  * d_seq [n] names the sequences of a call; NULL: entry b is sequence b.  len_hint: about the largest length among the entries (0: unknown);
  * it steers how work is split, never what is computed.
  * A slot that a row does not see may hold anything, infinities and NaN included; a row that sees such a value has no defined result.  A sink may be
- * -infinity (no sink for that head), not +infinity; `scale` is any finite number (scaled scores beyond single precision give no defined result).
+ * -infinity (no sink for that head), not +infinity; `scale` is any number up to BRRR_KV_SCALE_MAX in magnitude (scaled scores beyond single precision give no defined result).
  * An output overlaps no input, except that d_out may be d_q. */
 enum { BRRR_KV_F32 = 0, BRRR_KV_BF16 = 1 };
 #define BRRR_TREE_MAX 64     /* rows per sequence of brrr_attn_tree, brrr_kv_commit and brrr_kv_weigh */
 #define BRRR_KV_CAP_MAX (1 << 19)     /* largest capacity */
+#define BRRR_KV_SCALE_MAX 1e38f
 typedef struct brrr_kv {
     void *k, *v;                      /* [n_seq][n_head_kv][cap][head_dim] values of `type`, keys rotated; 16-byte aligned */
     int32_t type;                     /* BRRR_KV_F32 (the engines' caches) or BRRR_KV_BF16 */
