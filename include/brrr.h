@@ -304,7 +304,8 @@ int brrr_qwen_cli_main(int argc, char **argv);
  * commit, weigh, evict, means) has named already, is left out, its outputs stay as they were, and *err (if given) becomes 1.
  * d_seq [n] names the sequences of a call; NULL: entry b is sequence b.  len_hint: about the largest length among the entries (0: unknown);
  * it steers how work is split, never what is computed.
- * A slot that a row does not see may hold anything, infinities and NaN included; a row that sees such a value has no defined result.  A sink may be
+ * A slot that a row does not see may hold anything, infinities, NaN and the largest finite values included; a row that sees an infinity or NaN, or whose weighted
+ * values add up beyond single precision, has no defined result.  A sink may be
  * -infinity (no sink for that head), not +infinity; `scale` is any number up to BRRR_KV_SCALE_MAX in magnitude (scaled scores beyond single precision give no defined result).
  * An output overlaps no input, except that d_out may be d_q. */
 enum { BRRR_KV_F32 = 0, BRRR_KV_BF16 = 1 };

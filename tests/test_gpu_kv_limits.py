@@ -1,0 +1,102 @@
+"""KV-cache operators at the limits of what their header allows, on the GPU: the largest finite numbers, more protected entries than are kept, the widest window,
+destinations between the source's heads, long lists of blocks, every piece of an operand.  The restatement, the set-up and, where none is derived here, the tolerances
+are those of test_gpu_kv.py."""
+import math
+
+import numpy as np
+import pytest
+
+import kv_ref as R
+from test_gpu_kv import Setup, close, close_lse, prepared_tree, reference, run_tree
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- the largest finite numbers
+def fill_idle(s, bf16):
+    """What no row sees holds the type's largest and lowest value in turn."""
+    import torch
+    big = torch.finfo(torch.bfloat16 if bf16 else torch.float32).max
+    sign = torch.where(torch.arange(s.hd, device=s.dev) % 2 == 0, 1.0, -1.0).to(s.k.dtype)
+    for x in (s.k, s.v):
+        idle = ~torch.isfinite(x[..., 0])
+        x[idle] = sign * big
+    return big, sign
+
+
+LARGEST = [dict(n=2, rows=1, lens=[72, 9], heads=16, kv=2, masks="chain", sinks=True), dict(n=2, rows=7, lens=[301, 33], heads=8, kv=4, masks="tree", counts=[7, 3], window=37),
+           dict(n=1, rows=64, lens=[700], heads=32, kv=2, masks="tree"), dict(n=2, rows=64, lens=[511, 1090], heads=32, kv=2, masks="any", window=64, sinks=True)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("c", LARGEST, ids=lambda c: "-".join(str(c[k]) for k in ("n", "rows", "lens", "heads", "kv", "masks")))
+def test_tree_largest_numbers_in_slots_that_nobody_sees(brrr, dev, c, hd, bf16):
+    import torch
+    c = dict(c, hd=hd, bf16=bf16)
+    s = prepared_tree(dev, c)
+    fill_idle(s, bf16)
+    want, want_lse, weights = reference(s, c, s.up(s.q), s.scale)
+    for hint in (0, 1):              # a small hint: the kernel of 16-row tiles
+        out, lse = run_tree(brrr, s, c, hint=hint)
+        assert s.ok()
+        for b in range(c["n"]):
+            m = s.counts[b]
+            close(out[b, :m].cpu().numpy().reshape(m, c["heads"], hd), want[b, :m].cpu().numpy())
+            close_lse(lse[b, :m].cpu().numpy(), want_lse[b, :m].cpu().numpy())
+    s.view(brrr).weigh(c["n"], c["rows"], s.up(s.lens, np.int32), s.up(s.q), c["heads"], lse, s.scale, count=s.up(s.counts, np.int32),
+                       mask=None if c["masks"] == "chain" else s.up(np.array(s.masks, np.uint64)), window=s.window)
+    torch.cuda.synchronize()
+    book = torch.zeros(s.weight.shape, dtype=torch.float64, device=dev)
+    for b in range(c["n"]):
+        book[b, :, : s.lens[b] + s.counts[b]] += weights[b].sum(0).view(c["kv"], c["heads"] // c["kv"], -1).sum(1)
+    close(s.weight.cpu().numpy(), book.cpu().numpy())
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("at", [7, 41, 62])
+def test_tree_rows_that_see_the_largest_value(brrr, dev, at, hd, bf16):
+    """One slot's value is the largest finite one - seen by all rows (7, in a step that everybody sees whole), by the shallow ones (41), by one drafted row and those
+    behind it (62): weighted it stays in single precision, and the others do not notice it."""
+    import torch
+    c = dict(n=1, rows=9, lens=[60], heads=8, kv=2, hd=hd, masks="tree", bf16=bf16)
+    s = prepared_tree(dev, c)
+    s.masks, s.window = [[1, 3, 5, 9, 16 | 1, 32 | 2 | 1, 64, 128 | 64, 256]], 20 if at == 41 else 0
+    s.k.nan_to_num_(0.1), s.v.nan_to_num_(0.2, 0.3, 0.4)
+    big = torch.finfo(s.v.dtype).max
+    s.v[0, :, at, ::2], s.v[0, :, at, 1::2] = big, -big
+    k, v = s.values()
+    want, want_lse, _ = R.tree(s.q.astype(np.float64), k, v, [0], [60], [9], s.masks, s.scale, s.window)
+    out, lse = run_tree(brrr, s, c)
+    for i in range(9):
+        close(out[0, i].cpu().numpy().reshape(8, hd), want[0, i])
+    close_lse(lse.cpu().numpy(), want_lse)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("heads", [8, 32])
+def test_blocks_largest_numbers_behind_the_end(brrr, dev, heads, hd, bf16):
+    import torch
+    kv, lens, block, nsel = 2, [500, 33, 5], 32, 4
+    s = Setup(dev, 13, 3, kv, hd, 520, bf16)
+    means, view = torch.zeros((3, kv, 520 // block, hd), device=dev), s.view(brrr)
+    view.means(3, s.up(lens, np.int32), block, means)
+    for b in range(3):
+        s.k[b, :, lens[b]:] = float("nan"); s.v[b, :, lens[b]:] = float("nan")
+    fill_idle(s, bf16)
+    q = s.f32(3, heads, hd)
+    out, lse, sel = torch.zeros((3, heads * hd), device=dev), torch.zeros((3, heads), device=dev), torch.zeros((3, kv, nsel), dtype=torch.int32, device=dev)
+    view.attn_blocks(3, None, s.up(lens, np.int32), block, means, nsel, 1, 1, s.up(q), heads, out, 0.125, sel, lse=lse)
+    torch.cuda.synchronize()
+    assert s.ok()
+    k, v = s.values()
+    per, m = heads // kv, means.cpu().numpy()
+    for r in range(3):
+        for h in range(heads):
+            chosen = R.choose(q[r, h // per * per: (h // per + 1) * per], m[r, h // per], lens[r], block, nsel, 1, 1)
+            slots = [t for j in chosen for t in range(j * block, min((j + 1) * block, lens[r]))]
+            want, z, _ = R.attend(q[r, h].astype(np.float64), k[r, h // per], v[r, h // per], slots, 0.125)
+            close(out[r].cpu().numpy().reshape(heads, hd)[h], want)
+            close_lse(lse[r, h].cpu().numpy()[None], np.array([z]))
