@@ -138,11 +138,14 @@ cudaError_t launch_kv_commit(const KvDev &kv, int n, int rows, const int32_t *se
 // 12.8 with pairs by two searches, and takes 12.4.  512 threads: 13.8 and 18.9 us in place of 12.9 and 15.1.
 constexpr int EV_THREADS = 1024;
 
-// protected entries above all weights, NaN below all, -0 as +0
-__device__ __forceinline__ uint32_t evict_key(float w, int pos, int first, long long from) {
-    if (pos < first || pos >= from) return 0xFFFFFFFFu;
-    if (w != w) return 0u;
-    return float_orderable(w == 0.0f ? 0.0f : w);
+// Protected entries above all weights, NaN below all, -0 as +0.  crowded: more entries are protected than are kept, so these alone are in question, by their
+// weights (NaN: 1), and the others are below.
+constexpr uint32_t EV_SAFE = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t evict_key(float w, int pos, int first, long long from, bool crowded) {
+    const bool safe = pos < first || pos >= from;
+    const uint32_t of_weight = w != w ? 0u : float_orderable(w == 0.0f ? 0.0f : w);
+    if (crowded) return safe ? max(of_weight, 1u) : 0u;
+    return safe ? EV_SAFE : of_weight;
 }
 
 // Exclusive running sums of v[0 .. n), in place; returns the total.  All threads call it; v is complete afterwards.
@@ -200,12 +203,21 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
     const int words = (e.len + 31) / 32, mw = m / 32;
     uint32_t *kept = sm, *run = sm + words, *same_of = run + words + 1, *keys = same_of + words;
     // a thread has slots t, t + EV_THREADS, ... throughout: nobody else reads its keys
-    if (KEEP_KEYS) {
+    uint32_t safe = 0;
 #pragma unroll 4
-        for (int t = threadIdx.x; t < e.len; t += EV_THREADS) keys[t] = evict_key(w[t], pos[t], first, from);
+    for (int t = threadIdx.x; t < e.len; t += EV_THREADS) {
+        const uint32_t x = evict_key(KEEP_KEYS ? w[t] : 0.0f, pos[t], first, from, false);
+        if (KEEP_KEYS) keys[t] = x;
+        safe += x == EV_SAFE;
     }
+    safe = __reduce_add_sync(0xffffffffu, safe);
+    if (lane == 0) kth.of_warps[warp] = safe;
     __syncthreads();
-    auto key = [&](int t) { return KEEP_KEYS ? keys[t] : evict_key(w[t], pos[t], first, from); };
+    const bool crowded = __reduce_add_sync(0xffffffffu, kth.of_warps[lane]) > (uint32_t)m;
+    static_assert(EV_THREADS == 32 * 32, "a word per warp, a lane per word");
+    if (KEEP_KEYS && crowded)
+        for (int t = threadIdx.x; t < e.len; t += EV_THREADS) keys[t] = evict_key(w[t], pos[t], first, from, true);
+    auto key = [&](int t) { return KEEP_KEYS ? keys[t] : evict_key(w[t], pos[t], first, from, crowded); };
     uint32_t known, ties, equal;
     const uint32_t last = block_kth(e.len, m, key, kth, known, ties, equal), below = (1u << lane) - 1;
     if (ties < equal) {              // of those with the last one's key the lower slots: how many are before each word

@@ -358,7 +358,7 @@ int brrr_kv_weigh(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, cons
                   const uint64_t *d_rows, int len_hint, const float *d_q, int n_head, float scale, int window, const float *d_lse, void *stream);
 
 /* Of the len[b] entries of each kv head keep m = min(len[b], keep): those with a position < first or >= end[b] - recent (end[b]: positions the
- * sequence has had; d_end may be NULL where recent is 0) before the others, then the larger weight (NaN below all), then the lower slot.
+ * sequence has had; d_end may be NULL where recent is 0) before the others, then - among these as among those - the larger weight (NaN below all), then the lower slot.
  * Kept entries in slots below m stay there; the slots below m that are freed take, in ascending order, the kept entries from the slots behind, in
  * ascending order, with their weights and positions: attention does not ask for an order, so no more than that moves.  d_map [n][n_head_kv][keep]: the
  * slot that each entry came from, -1 from m on.  dst NULL: in place (what lies behind m is then nobody's); else all kept entries are written to the same sequence of

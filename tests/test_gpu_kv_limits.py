@@ -100,3 +100,45 @@ def test_blocks_largest_numbers_behind_the_end(brrr, dev, heads, hd, bf16):
             want, z, _ = R.attend(q[r, h].astype(np.float64), k[r, h // per], v[r, h // per], slots, 0.125)
             close(out[r].cpu().numpy().reshape(heads, hd)[h], want)
             close_lse(lse[r, h].cpu().numpy()[None], np.array([z]))
+
+
+# ---------------------------------------------------------------- more protected entries than are kept
+CROWDED = [dict(lens=[5], keep=3, first=0, recent=1, spread=1, cap=8, kv=1), dict(lens=[700, 31], keep=50, first=20, recent=30, spread=40, cap=705),
+           dict(lens=[700, 333], keep=50, first=50, recent=0, spread=60, cap=705, book="odd"), dict(lens=[3000, 64], keep=64, first=0, recent=64, spread=3000, cap=3001, book="ties"),
+           dict(lens=[4096], keep=1000, first=500, recent=0, spread=2048, cap=4096), dict(lens=[4096], keep=1025, first=1025, recent=0, spread=1, cap=4096, book="odd"),
+           dict(lens=[50001], keep=1000, first=700, recent=300, spread=2000, cap=50010, kv=1, book="odd"), dict(lens=[47000], keep=8001, first=1, recent=0, spread=3, cap=47001, kv=1)]
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("c", CROWDED, ids=lambda c: f"{c['lens']}-{c['keep']}-{c['spread']}-{c.get('book', '')}")
+def test_evict_with_more_protected_entries_than_are_kept(brrr, dev, c, inplace):
+    """Positions that many entries share: among the protected ones the larger weight comes first, NaN last of them and still before every other entry."""
+    import torch
+    n, nkv, keep, first, recent = len(c["lens"]), c.get("kv", 2), c["keep"], c["first"], c["recent"]
+    s = Setup(dev, 17, n, nkv, 64, c["cap"])
+    w = np.exp(2 * s.f32(n, nkv, s.cap))
+    if c.get("book") == "ties":
+        w = s.rng.integers(0, 3, w.shape)
+    if c.get("book") == "odd":
+        w = s.rng.choice(np.float32([0.0, -0.0, np.nan, -np.nan, np.inf, -np.inf, -1.0, 1e-42, 2.0, 3.0e38]), w.shape)
+    if c["lens"] == [5]:
+        w[0, 0, :5] = [1, 2, 3, 4, 5]
+    s.weight.copy_(torch.from_numpy(w.astype(np.float32)))
+    s.pos.copy_(torch.from_numpy(s.rng.integers(0, c["spread"], w.shape).astype(np.int32)))
+    end = c["spread"]
+    weight, pos = s.weight.cpu().numpy(), s.pos.cpu().numpy()
+    old = [t.clone() for t in (s.k, s.v, s.weight, s.pos)]
+    d = s if inplace else Setup(dev, 18, n, nkv, 64, keep)
+    kept, new_len = torch.zeros((n, nkv, keep), dtype=torch.int32, device=dev), torch.zeros(n, dtype=torch.int32, device=dev)
+    s.view(brrr).evict(n, s.up(c["lens"], np.int32), keep, first, recent, s.up([end] * n, np.int32), kept, dst=None if inplace else d.view(brrr), new_len=new_len)
+    torch.cuda.synchronize()
+    assert s.ok() and new_len.tolist() == [min(x, keep) for x in c["lens"]]
+    for b in range(n):
+        for h in range(nkv):
+            src = R.evict(weight[b, h, : c["lens"][b]], pos[b, h, : c["lens"][b]], keep, first, recent, end)
+            assert kept[b, h].tolist() == src + [-1] * (keep - len(src))
+            if c["lens"] == [5]:
+                assert sorted(src) == [2, 3, 4]
+            at = torch.tensor(src, dtype=torch.long, device=dev)
+            for now, was in zip((d.k, d.v, d.weight, d.pos), old):
+                assert torch.equal(now[b, h, : len(src)].nan_to_num(99.0), was[b, h][at].nan_to_num(99.0))
