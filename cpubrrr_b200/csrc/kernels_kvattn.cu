@@ -472,9 +472,14 @@ static bool wide_rows_pay(const KvDev &kv, const TreeArgs &a, int slots) {
     return (double)a.n * kv.nkv * (slots / 128.0) * ((rows + 15) / 16 - 1.5 * ((rows + 127) / 128)) > start[kv.type][kv.hd == 128];
 }
 
+// About the slots of an entry that its rows see.  A window is up to INT_MAX wide: the cached slots are taken from it before the rows are added.
+static int tree_slots(const KvDev &kv, const TreeArgs &a, int len_hint) {
+    const int cached = len_hint > 0 ? min(len_hint, kv.cap) : kv.cap;
+    return (a.window > 0 ? min(cached, a.window) : cached) + a.rows;
+}
+
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st) {
-    int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
-    if (a.window > 0) slots = min(slots, a.window + a.rows);
+    const int slots = tree_slots(kv, a, len_hint);
     if (wide_rows_pay(kv, a, slots)) return launch_tree_tc(kv, a, slots, st);
     const bool one = a.rows * (a.nh / kv.nkv) <= 8;
     auto go = kv.type ? (kv.hd == 64 ? (one ? launch_tree<KvBf16, 64, 1> : launch_tree<KvBf16, 64, 2>) : (one ? launch_tree<KvBf16, 128, 1> : launch_tree<KvBf16, 128, 2>))
@@ -592,8 +597,7 @@ static cudaError_t launch_weigh(const KvDev &kv, const TreeArgs &a, const uint64
 }
 
 cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *picked, int len_hint, cudaStream_t st) {
-    int slots = (len_hint > 0 ? min(len_hint, kv.cap) : kv.cap) + a.rows;
-    if (a.window > 0) slots = min(slots, a.window + a.rows);
+    const int slots = tree_slots(kv, a, len_hint);
     if (a.rows * (a.nh / kv.nkv) > 16) return launch_weigh_tc(kv, a, picked, slots, st);
     const bool one = a.rows * (a.nh / kv.nkv) <= 8;
     auto go = kv.type ? (kv.hd == 64 ? (one ? launch_weigh<KvBf16, 64, 1> : launch_weigh<KvBf16, 64, 2>) : (one ? launch_weigh<KvBf16, 128, 1> : launch_weigh<KvBf16, 128, 2>))

@@ -142,3 +142,24 @@ def test_evict_with_more_protected_entries_than_are_kept(brrr, dev, c, inplace):
             at = torch.tensor(src, dtype=torch.long, device=dev)
             for now, was in zip((d.k, d.v, d.weight, d.pos), old):
                 assert torch.equal(now[b, h, : len(src)].nan_to_num(99.0), was[b, h][at].nan_to_num(99.0))
+
+
+# ---------------------------------------------------------------- the widest window
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,heads,kv,hd", [(1, 8, 8, 64), (5, 16, 4, 128), (64, 32, 2, 64), (64, 32, 2, 128)])
+def test_a_window_that_hides_nothing_changes_no_bit(brrr, dev, rows, heads, kv, hd, bf16):
+    """A window is a limit on what is seen and on the work, never more work than without one: one that hides nothing splits the slots as none does, up to the largest."""
+    import torch
+    c = dict(n=1, rows=rows, lens=[2000], heads=heads, kv=kv, hd=hd, masks="tree", bf16=bf16)
+    s = prepared_tree(dev, c)
+    want, want_lse = run_tree(brrr, s, c)
+    for window in (1 << 20, (1 << 31) - 64, (1 << 31) - 1):
+        s.window = window
+        out, lse = run_tree(brrr, s, c)
+        assert s.ok() and torch.equal(out, want) and torch.equal(lse, want_lse)
+        books = []
+        for x in (0, window):
+            s.weight.zero_()
+            s.view(brrr).weigh(1, rows, s.up(s.lens, np.int32), s.up(s.q), heads, lse, s.scale, mask=s.up(np.array(s.masks, np.uint64)), window=x)
+            books.append(s.weight.clone())
+        assert torch.equal(*books) and bool(books[0].any())
