@@ -19,3 +19,54 @@ def test_scales_whose_powers_of_two_leave_single_precision(brrr, scale, want):
         assert calls == [ARG] * 3
     elif not __import__("torch").cuda.is_available():
         assert calls == [CUDA] * 3
+
+
+class OnDevice:
+    """A tensor as one of device 0 would look to the class."""
+
+    def __init__(self, x):
+        self.x, self.dtype, self.shape, self.device = x, x.dtype, x.shape, "cuda:0"
+
+    def __getattr__(self, name):
+        return getattr(self.x, name)
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return P
+
+
+def test_the_class_reads_no_array_as_another_type(brrr):
+    """Lengths that are floats, or queries that are integers, have the right size and would be read as what they are not."""
+    import torch
+
+    def a(dtype, n=64 * 12 * 3):
+        return OnDevice(torch.zeros(n, dtype=dtype))
+    f, i, w, h = a(torch.float32), a(torch.int32), a(torch.int64), a(torch.float16)
+    kv = brrr.KvCache(P, 2 * P, 3, 4, 64, 16, weight=f, pos=i, err=i)
+    for bad in (dict(weight=i), dict(pos=f), dict(err=f), dict(pos=w), dict(weight=a(torch.float64))):
+        with pytest.raises(brrr.BrrrError, match="is wanted"):
+            brrr.KvCache(P, 2 * P, 3, 4, 64, 16, **{**dict(weight=f, pos=i, err=i), **bad})
+    i = a(torch.int32)
+    calls = {
+        "append": (lambda **k: kv.append(1, 1, k.pop("length"), k.pop("qkv"), n_head=4, n_rope=1, **k), dict(length=i, qkv=f, seq=i, count=i, at=i, rope=f, q=f)),
+        "attn_tree": (lambda **k: kv.attn_tree(1, 1, k.pop("length"), k.pop("q"), 4, k.pop("out"), 1.0, **k), dict(length=i, q=f, out=f, seq=i, count=i, mask=w, sinks=f, lse=f)),
+        "commit": (lambda **k: kv.commit(1, 1, k.pop("length"), k.pop("path"), k.pop("npath"), **k), dict(length=i, path=i, npath=i, seq=i, new_len=i)),
+        "weigh": (lambda **k: kv.weigh(1, 1, k.pop("length"), k.pop("q"), 4, k.pop("lse"), 1.0, **k), dict(length=i, q=f, lse=f, seq=i, count=i, mask=w, picked=w)),
+        "evict": (lambda **k: kv.evict(1, k.pop("length"), 4, 1, 1, k.pop("end"), k.pop("map"), **k), dict(length=i, end=i, map=i, seq=i, new_len=i)),
+        "means": (lambda **k: kv.means(1, k.pop("length"), 16, k.pop("means"), **k), dict(length=i, means=f, seq=i, since=i)),
+        "attn_blocks": (lambda **k: kv.attn_blocks(1, k.pop("seq"), k.pop("length"), 16, k.pop("means"), 4, 1, 1, k.pop("q"), 4, k.pop("out"), 1.0, k.pop("sel"), **k),
+                        dict(seq=i, length=i, means=f, q=f, out=f, sel=i, sinks=f, lse=f)),
+    }
+    for name, (call, good) in calls.items():
+        with pytest.raises(brrr.BrrrError, match=f"brrr_(kv|attn)_{name.split('_')[-1]}"):          # the arrays are taken; the memory is nobody's
+            call(**good)
+        for arg, x in good.items():
+            for bad in (f, i, w, h):
+                if bad.dtype != x.dtype:
+                    with pytest.raises(brrr.BrrrError, match="is wanted"):
+                        call(**{**good, arg: bad})
+    unsigned = dict(length=a(torch.uint32), q=f, out=f, mask=a(torch.uint64))
+    with pytest.raises(brrr.BrrrError, match="brrr_attn_tree"):
+        calls["attn_tree"][0](**unsigned)
