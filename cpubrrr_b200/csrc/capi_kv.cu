@@ -35,12 +35,36 @@ bool view(const brrr_kv *c, KvDev *out) {
     return true;
 }
 
-// bytes from the first value of k (or v) to the end of the last head
-int64_t extent(const KvDev &d) { return ((d.n_seq - 1) * d.ss + (d.nkv - 1) * d.hs + (int64_t)d.cap * d.hd) * d.size(); }
-
-bool apart(const void *a, int64_t na, const void *b, int64_t nb) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x + (uintptr_t)na <= y || y + (uintptr_t)nb <= x;
+// Pieces of memory of one length, in ascending order: `outer` times `inner` of them, a step apart each (view has seen that they do not overlap).
+struct Pieces {
+    uintptr_t at;
+    int64_t len, inner, inner_step, outer, outer_step;
+    int64_t count() const { return inner * outer; }
+    uintptr_t piece(int64_t i) const { return at + (uintptr_t)(i / inner * outer_step + i % inner * inner_step); }
+    uintptr_t end() const { return at + (uintptr_t)((outer - 1) * outer_step + (inner - 1) * inner_step + len); }
+};
+Pieces whole(const void *p, int64_t len) { return {(uintptr_t)p, len, 1, len, 1, len}; }
+// the heads of k or v; what stands without a gap is one piece
+Pieces heads_of(const KvDev &d, const void *p) {
+    const int64_t head = (int64_t)d.cap * d.hd * d.size(), hs = d.hs * d.size(), ss = d.ss * d.size();
+    Pieces x = d.hs < d.ss ? Pieces{(uintptr_t)p, head, d.nkv, hs, d.n_seq, ss} : Pieces{(uintptr_t)p, head, d.n_seq, ss, d.nkv, hs};
+    if (x.inner == 1 || x.inner_step == head) {
+        const int64_t run = head * x.inner;
+        if (x.outer == 1 || x.outer_step == run) return whole(p, run * x.outer);
+        return {x.at, run, 1, run, x.outer, x.outer_step};
+    }
+    return x;
+}
+// Whether any two share a byte.  What lies apart as a whole, and two caches of which one has no gaps, take few steps.
+bool meet(const Pieces &a, const Pieces &b) {
+    if (a.end() <= b.at || b.end() <= a.at) return false;
+    for (int64_t i = 0, j = 0; i < a.count() && j < b.count();) {
+        const uintptr_t x = a.piece(i), y = b.piece(j);
+        if (x + (uintptr_t)a.len <= y) i++;
+        else if (y + (uintptr_t)b.len <= x) j++;
+        else return true;
+    }
+    return false;
 }
 
 // log2(e) times twice the scale stays in single precision: beyond, a score of zero would be no number
@@ -115,11 +139,11 @@ extern "C" int brrr_kv_evict(const brrr_kv *kv, const brrr_kv *dst, int n, const
     if ((recent > 0 && !d_end) || (!d_seq && n > d.n_seq) || off4(d_seq, d_len, d_end, d_map, d_new_len)) return BRRR_ERR_ARG;
     if (dst) {
         if (!view(dst, &to) || !to.weight || !to.pos || to.type != d.type || to.nkv != d.nkv || to.hd != d.hd || to.cap < keep || (!d_seq && n > to.n_seq)) return BRRR_ERR_ARG;
-        const int64_t x = extent(d), y = extent(to), bx = (int64_t)d.n_seq * d.nkv * d.cap * 4, by = (int64_t)to.n_seq * to.nkv * to.cap * 4;
-        const struct { const void *p; int64_t n; } from[4] = {{d.k, x}, {d.v, x}, {d.weight, bx}, {d.pos, bx}}, into[4] = {{to.k, y}, {to.v, y}, {to.weight, by}, {to.pos, by}};
+        const int64_t x = (int64_t)d.n_seq * d.nkv * d.cap * 4, y = (int64_t)to.n_seq * to.nkv * to.cap * 4;
+        const Pieces from[4] = {heads_of(d, d.k), heads_of(d, d.v), whole(d.weight, x), whole(d.pos, x)}, into[4] = {heads_of(to, to.k), heads_of(to, to.v), whole(to.weight, y), whole(to.pos, y)};
         for (auto &f : from)
             for (auto &t : into)
-                if (!apart(f.p, f.n, t.p, t.n)) return BRRR_ERR_ARG;
+                if (meet(f, t)) return BRRR_ERR_ARG;
     }
     if (int rc = on_this_device(d)) return rc;
     if (dst)

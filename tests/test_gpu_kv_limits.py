@@ -163,3 +163,41 @@ def test_a_window_that_hides_nothing_changes_no_bit(brrr, dev, rows, heads, kv, 
             s.view(brrr).weigh(1, rows, s.up(s.lens, np.int32), s.up(s.q), heads, lse, s.scale, mask=s.up(np.array(s.masks, np.uint64)), window=x)
             books.append(s.weight.clone())
         assert torch.equal(*books) and bool(books[0].any())
+
+
+# ---------------------------------------------------------------- destinations between the source's heads
+@pytest.mark.parametrize("layout", ["sequences", "heads", "halves"])
+def test_evict_into_rows_between_the_sources(brrr, dev, layout):
+    """One allocation holds both caches, whose heads alternate: sequences inside a head, heads of a sequence one by one, a source in the first half of every row."""
+    import torch
+    n, nkv, hd, cap, keep = 2, 3, 64, 40, 16
+    rng = np.random.default_rng(4)
+    shape = {"sequences": (nkv, 2 * n, cap * hd), "heads": (n, nkv, 2, cap * hd), "halves": (n, 2 * nkv, cap * hd)}[layout]
+    raw = [torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).to(dev) for _ in range(2)]
+    if layout == "sequences":
+        at, strides = [(0, 0), (0, n)], dict(head_stride=2 * n * cap * hd, seq_stride=cap * hd)
+        rows = lambda x, i: x[:, i * n: (i + 1) * n].transpose(0, 1)  # noqa: E731
+    elif layout == "heads":
+        at, strides = [(0, 0, 0), (0, 0, 1)], dict(head_stride=2 * cap * hd, seq_stride=2 * nkv * cap * hd)
+        rows = lambda x, i: x[:, :, i]  # noqa: E731
+    else:
+        at, strides = [(0, 0), (0, nkv)], dict(head_stride=cap * hd, seq_stride=2 * nkv * cap * hd)
+        rows = lambda x, i: x[:, i * nkv: (i + 1) * nkv]  # noqa: E731
+    weight, pos = torch.rand((2, n, nkv, cap), device=dev), torch.arange(cap, dtype=torch.int32, device=dev).repeat(2, n, nkv, 1)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    src, dst = (brrr.KvCache(raw[0][i], raw[1][i], n, nkv, hd, cap, weight=weight[j], pos=pos[j], err=err, **strides) for j, i in enumerate(at))
+    old, books = [x.clone() for x in raw], weight.clone()
+    lens, kept = [33, 40], torch.zeros((n, nkv, keep), dtype=torch.int32, device=dev)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    src.evict(n, i32(lens), keep, 2, 3, i32(lens), kept, dst=dst)
+    torch.cuda.synchronize()
+    assert int(err) == 0
+    for x, was in zip(raw, old):
+        assert torch.equal(rows(x, 0), rows(was, 0)) and torch.equal(rows(x, 1).unflatten(-1, (cap, hd))[:, :, keep:], rows(was, 1).unflatten(-1, (cap, hd))[:, :, keep:])
+    for b in range(n):
+        for h in range(nkv):
+            want = R.evict(books[0, b, h, : lens[b]].cpu().numpy(), list(range(lens[b])), keep, 2, 3, lens[b])
+            assert kept[b, h].tolist() == want
+            for x, was in zip(raw, old):
+                assert torch.equal(rows(x, 1)[b, h].view(cap, hd)[:keep], rows(was, 0)[b, h].view(cap, hd)[torch.tensor(want, device=dev)])
+            assert torch.equal(weight[1, b, h, :keep], books[0, b, h][torch.tensor(want, device=dev)])

@@ -70,3 +70,39 @@ def test_the_class_reads_no_array_as_another_type(brrr):
     unsigned = dict(length=a(torch.uint32), q=f, out=f, mask=a(torch.uint64))
     with pytest.raises(brrr.BrrrError, match="brrr_attn_tree"):
         calls["attn_tree"][0](**unsigned)
+
+
+def test_a_destination_may_stand_between_the_sources_heads(brrr):
+    """Random layouts of two views over one stretch of memory: refused exactly where two rows share a byte."""
+    import random
+
+    import torch
+    L, rng, seen = brrr.lib(), random.Random(5), {True: 0, False: 0}
+
+    def layout():
+        n_seq, nkv, cap = rng.randint(1, 3), 2, rng.randint(1, 3)
+        head = cap * 64
+        inner = head + rng.choice([0, 0, 64, 200])
+        if rng.random() < 0.5:
+            hs, ss = inner, inner * (nkv - 1) + head + rng.choice([0, 8, 400, 1000])
+        else:
+            hs, ss = inner * (n_seq - 1) + head + rng.choice([0, 8, 400, 1000]), inner
+        if rng.random() < 0.2:
+            hs = ss = 0
+        return dict(n_seq=n_seq, n_head_kv=nkv, cap=cap, head_stride=hs, seq_stride=ss)
+
+    def bytes_of(at, c):
+        head = c["cap"] * 64
+        hs = c["head_stride"] or head
+        ss = c["seq_stride"] or hs * c["n_head_kv"]
+        return {at + 4 * (s * ss + h * hs) + i for s in range(c["n_seq"]) for h in range(c["n_head_kv"]) for i in range(0, 4 * head, 16)}
+    for _ in range(600):
+        a, b = layout(), layout()
+        at, to = P, P + 16 * rng.randint(0, 700)
+        src, dst = view(brrr, **a, k=at, v=2 * P), view(brrr, **b, k=to, v=6 * P, weight=7 * P, pos=8 * P)
+        overlap = bool(bytes_of(at, a) & bytes_of(to, b))
+        got = L.brrr_kv_evict(C.byref(src), C.byref(dst), 1, None, P, 1, 0, 0, None, P, None, 0, None)
+        seen[overlap] += 1
+        assert (got == ARG) == overlap or (not overlap and torch.cuda.is_available()), (a, b, to - at)
+        assert got in (ARG, CUDA)
+    assert min(seen.values()) > 50, seen
