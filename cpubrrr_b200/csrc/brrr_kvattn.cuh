@@ -171,10 +171,12 @@ static cudaError_t launch_cluster(dim3 grid, int threads, int cluster, size_t sm
 }
 
 // CTAs (1..16) that share the steps of one of `jobs` pieces of work, `lanes` steps of a CTA going on at a time: the least time of all waves, where a
-// CTA's start and end cost about as much as `fixed` steps.  How many clusters of a size the GPU holds at once is asked for once per kernel, size and device.
+// CTA's start and end cost about as much as `fixed` steps.  How many clusters of a size the GPU holds at once is asked for once per kernel, size and device; a kernel
+// launched with different amounts of shared memory numbers them (kind), each asked for with the largest that is launched as this kind.
+constexpr int ROOM_KINDS = 17;
 template <auto K, bool CLUSTER = true>
-static int cluster_size(long long jobs, int steps, int lanes, int fixed, int threads, size_t smem, size_t most, cudaError_t *err) {
-    static std::atomic<int> room[64][17];
+static int cluster_size(long long jobs, int steps, int lanes, int fixed, int threads, size_t smem, size_t most, cudaError_t *err, int kind = 0) {
+    static std::atomic<int> rooms[64][ROOM_KINDS][17];
     int dev = 0;
     *err = cudaGetDevice(&dev);
     if (*err == cudaSuccess) *err = allow<K>(most);
@@ -183,7 +185,7 @@ static int cluster_size(long long jobs, int steps, int lanes, int fixed, int thr
     double least = 0.0;
     for (int c = 1; c <= 16; c++) {           // without clusters c CTAs take c of the places for one
         const int c_room = CLUSTER ? c : 1;
-        int held = dev < 64 ? room[dev][c_room].load() : 0;
+        int held = dev < 64 ? rooms[dev][kind][c_room].load() : 0;
         if (!held) {
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3(c_room);
@@ -197,7 +199,7 @@ static int cluster_size(long long jobs, int steps, int lanes, int fixed, int thr
             cfg.numAttrs = 1;
             if (cudaOccupancyMaxActiveClusters(&held, K, &cfg) != cudaSuccess) { (void)cudaGetLastError(); held = 0; }
             held = held > 0 ? held : -1;
-            if (dev < 64) room[dev][c_room].store(held);
+            if (dev < 64) rooms[dev][kind][c_room].store(held);
         }
         if (held < 0) continue;
         const int turns = (steps + c * lanes - 1) / (c * lanes);

@@ -806,13 +806,17 @@ static cudaError_t launch_blocks(const KvDev &kv, int rows, const int32_t *seq, 
     // a tile of eight blocks' scores costs about as much as a step
     const int steps = min(nsel, nb + 1) * (block / STEP) + (nb > nsel ? nb / 8 : 0);
     constexpr size_t room = Room<T, HD, NT>::BYTES + 1024, most = room + 16385 * 4;
+    // the blocks' keys, 4 KB by 4 KB (the last kind: 64 KB and a word)
+    const size_t keys = (size_t)(kv.cap / block + 1) * 4;
+    const int kind = (int)min((keys - 1) / 4096, (size_t)ROOM_KINDS - 1);
+    const size_t keys_most = min((size_t)(kind + 1) * 4096, most - room);
     constexpr auto K = blocks_kernel<T, HD, NT>;
     KvMaps maps;
     cudaError_t e = kv_maps(kv, STEP, &maps);
     if (e != cudaSuccess) return e;
-    const int c = cluster_size<K>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, room + 4096, most, &e);
+    const int c = cluster_size<K>((long long)rows * kv.nkv, steps, AW, 4, AW * 32, room + keys_most, most, &e, kind);
     if (e != cudaSuccess) return e;
-    return launch_cluster<K>(dim3(c, rows, kv.nkv), AW * 32, c, room + (size_t)(kv.cap / block + 1) * 4, most, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
+    return launch_cluster<K>(dim3(c, rows, kv.nkv), AW * 32, c, room + keys, most, st, kv, seq, len, block, means, nsel, first, local, q, nh, scale,
                              sinks, sel, out, lse, maps);
 }
 

@@ -201,3 +201,38 @@ def test_evict_into_rows_between_the_sources(brrr, dev, layout):
             for x, was in zip(raw, old):
                 assert torch.equal(rows(x, 1)[b, h].view(cap, hd)[:keep], rows(was, 0)[b, h].view(cap, hd)[torch.tensor(want, device=dev)])
             assert torch.equal(weight[1, b, h, :keep], books[0, b, h][torch.tensor(want, device=dev)])
+
+
+# ---------------------------------------------------------------- long lists of blocks
+@pytest.mark.parametrize("hd,bf16,heads", [(64, True, 4), (128, False, 16), (128, True, 9)])
+@pytest.mark.parametrize("blocks,nsel,ties", [(1023, 5, False), (1025, 40, True), (5000, 256, False), (5001, 17, True), (16384, 33, True), (16384, 256, False)])
+def test_blocks_of_long_caches(brrr, dev, blocks, nsel, ties, hd, bf16, heads):
+    """Up to the largest number of blocks, full and short sequences in one call: the choice is the restatement's, block by block."""
+    import torch
+    block, rows, kv = 16, 3, 1
+    s = Setup(dev, 29, 1, kv, hd, blocks * block + 3, bf16)
+    lens = [s.cap, blocks * block // 3 + 5, block]
+    means = torch.full((1, kv, blocks, hd), float("nan"), device=dev)
+    view = s.view(brrr)
+    view.means(1, s.up([s.cap], np.int32), block, means)
+    if ties:
+        few = s.up(s.f32(40, hd) / 4)
+        means[0, 0] = few[torch.from_numpy(s.rng.integers(0, 40, blocks)).to(dev)]
+        means[0, 0, 7: blocks: 100] = float("nan")
+    q = s.f32(rows, heads, hd)
+    m = means[0, 0].cpu().numpy()
+    k, v = s.values()
+    chosen = [R.choose(q[r], m, lens[r], block, nsel, 1, 2) for r in range(rows)]
+    for hint in (0, 100):
+        out, lse = torch.zeros((rows, heads * hd), device=dev), torch.zeros((rows, heads), device=dev)
+        sel = torch.full((rows, kv, nsel), 77, dtype=torch.int32, device=dev)
+        view.attn_blocks(rows, s.up([0] * rows, np.int32), s.up(lens, np.int32), block, means, nsel, 1, 2, s.up(q), heads, out, 1 / math.sqrt(hd), sel, len_hint=hint, lse=lse)
+        torch.cuda.synchronize()
+        assert s.ok()
+        for r in range(rows):
+            assert sel[r, 0].tolist() == chosen[r] + [-1] * (nsel - len(chosen[r]))
+            slots = [t for j in chosen[r] for t in range(j * block, min((j + 1) * block, lens[r]))]
+            for h in range(heads):
+                want, z, _ = R.attend(q[r, h].astype(np.float64), k[0, 0], v[0, 0], slots, 1 / math.sqrt(hd))
+                close(out[r].cpu().numpy().reshape(heads, hd)[h], want)
+                close_lse(lse[r, h].cpu().numpy()[None], np.array([z]))
