@@ -236,3 +236,69 @@ def test_blocks_of_long_caches(brrr, dev, blocks, nsel, ties, hd, bf16, heads):
                 want, z, _ = R.attend(q[r, h].astype(np.float64), k[0, 0], v[0, 0], slots, 1 / math.sqrt(hd))
                 close(out[r].cpu().numpy().reshape(heads, hd)[h], want)
                 close_lse(lse[r, h].cpu().numpy()[None], np.array([z]))
+
+
+# ---------------------------------------------------------------- every piece of an operand
+def cut16(x):
+    """x without what a third piece of eight bits would hold."""
+    return (np.ascontiguousarray(x, np.float32).view(np.uint32) & 0xFFFF0000).view(np.float32).astype(np.float64) + \
+        (np.ascontiguousarray(x - (x.view(np.uint32) & 0xFFFF0000).view(np.float32)).view(np.uint32) & 0xFFFF0000).view(np.float32)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("hint", [0, 1])
+def test_no_piece_of_an_operand_is_lost(brrr, dev, hint, hd, bf16):
+    """Rows of one or two slots, where sums hide nothing: hint 0 goes to the kernels of 128-row tiles (three pieces of eight bits), 1 to those of 16 rows (tf32 twice).
+
+    Relative bounds, each from its roundings.  VALUE, a row that sees one slot returns its value: 24 bits in three pieces are exact, two tf32 parts leave out 2^-22 at
+    most, the division and the product 2^-22 + 2^-24: 2^-20.  SCORE, the log-sum of such a row whose query has one dimension is one product: what is left out of a
+    product 2^-21 (mid x lo twice; tf32: 2^-21 as well), three additions that matter, truncated, 3 x 2^-23, five roundings of the scale and the logarithms'
+    factors 5 x 2^-24: 1.2e-6 < 2^-19.  WEIGHT, values 1 and 0 under scores 0 and s with |s| < 3: an exponent of 4.4 off by 3 x 2^-24 of it changes a weight by
+    5.5e-7, the power, the pieces and the division by 2^-22 each: 1.3e-6 < 2^-19.  BOOK, e^s with s < 8: 8 times the bound of a score, 9.6e-6, and the power's 2^-22: 1.2e-5.
+    16 bits of one operand are off by up to 2^-15: each bound is checked to see that."""
+    import torch
+    value, score, weight, book = 2.0**-20, 2.0**-19, 2.0**-19, 1.2e-5
+    rows, heads, kv, cap = 64, 32, 2, 4000
+    per, half = heads // kv, rows // 2
+    s = Setup(dev, 41, 1, kv, hd, cap, bf16)
+    view, out, lse = s.view(brrr), torch.zeros((1, rows, heads * hd), device=dev), torch.zeros((1, rows, heads), device=dev)
+
+    def run(masks, q):
+        view.attn_tree(1, rows, s.up([0], np.int32), s.up(q), heads, out, 0.125, mask=s.up(np.array([masks], np.uint64)), len_hint=hint, lse=lse)
+        torch.cuda.synchronize()
+        assert s.ok()
+        return out.double().cpu().numpy().reshape(rows, heads, hd), lse.double().cpu().numpy()[0]
+
+    def off(got, want):
+        return (np.abs(got - want) / np.abs(want)).max()
+
+    # one slot each: its value, its score
+    k, v = s.values()
+    q = np.zeros((rows, heads, hd), np.float32)
+    i, h = np.meshgrid(np.arange(rows), np.arange(heads), indexing="ij")
+    d = (5 * i + h) % hd
+    key = k[0, h // per, i, d]
+    q[i, h, d] = (s.rng.uniform(32, 64, (rows, heads)) / key).astype(np.float32)          # scaled scores of 4 to 8
+    one = q[i, h, d]
+    o, z = run([1 << i for i in range(rows)], q)
+    assert off(o, v[0, h // per, i]) < value
+    assert off(z, 0.125 * one.astype(np.float64) * key) < score < off(0.125 * cut16(one) * key, 0.125 * one.astype(np.float64) * key)
+    s.weight.zero_()
+    view.weigh(1, rows, s.up([0], np.int32), s.up(q), heads, torch.zeros_like(lse), 0.125, mask=s.up(np.array([[1 << i for i in range(rows)]], np.uint64)))
+    want, less = (np.exp(0.125 * x * key).reshape(rows, kv, per).sum(2).T for x in (one.astype(np.float64), cut16(one)))
+    got = s.weight[0, :, :rows].double().cpu().numpy()
+    assert off(got, want) < book < off(less, want)
+    if not bf16:
+        k32, v32 = key.astype(np.float32), v[0].astype(np.float32)
+        assert score < off(one * cut16(k32), one * key) and value < off(cut16(v32), v[0]) and book < off(np.exp(0.125 * one * cut16(k32)), np.exp(0.125 * one * key))
+    # two slots: row i < 32 sees itself, of key 0 and value 1, and slot 32 + i, whose value is 0
+    s.k[:, :, :half], s.v[:, :, :half], s.v[:, :, half: rows] = 0.0, 1.0, 0.0
+    s.k[:, :, half: rows] = 1.0
+    x = s.rng.uniform(0.5, 3, (rows, heads)).astype(np.float32)
+    q[:] = 0.0
+    q[:, :, 3] = 8 * x
+    o, _ = run([1 << i | 1 << (half + i % half) for i in range(rows)], q)
+    want = 1 / (1 + np.exp(x[:half].astype(np.float64)))
+    p = np.exp(-x[:half].astype(np.float64))
+    assert off(o[:half], want[:, :, None]) < weight < off(cut16(p.astype(np.float32)) / (1 + p), want)
