@@ -100,7 +100,7 @@ cudaError_t launch_kv_append(const KvDev &kv, int n, int rows, const int32_t *se
 cudaError_t launch_kv_commit(const KvDev &kv, int n, int rows, const int32_t *seq, const int32_t *len, const int32_t *path, const int32_t *npath, int32_t *new_len,
                              cudaStream_t st);
 cudaError_t launch_kv_evict(const KvDev &kv, const KvDev *dst, int n, const int32_t *seq, const int32_t *len, int keep, int first, int recent, const int32_t *end,
-                            int32_t *map, int32_t *new_len, int len_hint, cudaStream_t st);
+                            int32_t *map, int32_t *new_len, cudaStream_t st);
 cudaError_t launch_kv_means(const KvDev &kv, int n, const int32_t *seq, const int32_t *since, const int32_t *len, int block, int len_hint, float *means, cudaStream_t st);
 cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, cudaStream_t st);
 cudaError_t launch_tree_tc(const KvDev &kv, const TreeArgs &a, int slots, cudaStream_t st);      // kernels_kvtc.cu; slots: about as many per entry

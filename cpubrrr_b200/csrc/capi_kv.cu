@@ -132,7 +132,7 @@ extern "C" int brrr_kv_weigh(const brrr_kv *kv, int n, int rows, const int32_t *
 }
 
 extern "C" int brrr_kv_evict(const brrr_kv *kv, const brrr_kv *dst, int n, const int32_t *d_seq, const int32_t *d_len, int keep, int first, int recent,
-                             const int32_t *d_end, int32_t *d_map, int32_t *d_new_len, int len_hint, void *stream) {
+                             const int32_t *d_end, int32_t *d_map, int32_t *d_new_len, int /* len_hint */, void *stream) {
     KvDev d, to;
     if (!view(kv, &d) || !d.weight || !d.pos || !d_len || !d_map || d_new_len == d_len) return BRRR_ERR_ARG;
     if (n <= 0 || n > 65535 || keep <= 0 || keep > d.cap || first < 0 || recent < 0 || first > keep || recent > keep - first) return BRRR_ERR_ARG;
@@ -148,7 +148,7 @@ extern "C" int brrr_kv_evict(const brrr_kv *kv, const brrr_kv *dst, int n, const
     if (int rc = on_this_device(d)) return rc;
     if (dst)
         if (int rc = on_this_device(to)) return rc;
-    return done(launch_kv_evict(d, dst ? &to : nullptr, n, d_seq, d_len, keep, first, recent, d_end, d_map, d_new_len, len_hint, (cudaStream_t)stream));
+    return done(launch_kv_evict(d, dst ? &to : nullptr, n, d_seq, d_len, keep, first, recent, d_end, d_map, d_new_len, (cudaStream_t)stream));
 }
 
 extern "C" int brrr_kv_means(const brrr_kv *kv, int n, const int32_t *d_seq, const int32_t *d_since, const int32_t *d_len, int block, int len_hint, float *d_means,

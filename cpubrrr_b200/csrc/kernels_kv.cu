@@ -132,10 +132,11 @@ cudaError_t launch_kv_commit(const KvDev &kv, int n, int rows, const int32_t *se
 
 // ---------------------------------------------------------------- eviction
 // Which entries stay: a CTA per (kv head, entry) finds the key of the last one kept digit by digit, then turns the keys into one bit per slot, and pairs the
-// freed slots below m with the kept entries behind: by a list of these where the keys stood, by searches in the running counts where there is no such room.  Bits and running counts per 32 slots stand in shared memory, and the keys where there is
-// room for a cache's (46,000 slots; above, they are formed from the books again at every pass).  Bound by barriers and dependent reads, not by bytes: 8 heads x
-// 4096 entries 11.9 us alone, 128 heads of 32 caches x 3900 13.8.  A whole eviction from one cache took 19.4 us with sums by walking, 15.2 with five barriers a digit,
-// 12.8 with pairs by two searches, and takes 12.4.  512 threads: 13.8 and 18.9 us in place of 12.9 and 15.1.
+// freed slots below m with the kept entries behind: by a list of these where the keys stood, by searches in the running counts where there is no such room.  Bits
+// and running counts per 32 slots stand in shared memory, and the keys where there is room for a cache's (46,000 slots; above, they are formed from the books again
+// at every pass).  Bound by barriers and dependent reads, not by bytes: launched alone 11.6 us for 8 heads x 4096 entries, 12.1 for 128 heads of 32 caches x 3900.
+// A whole eviction from one cache took 19.4 us with sums by walking, 15.2 with five barriers a digit, 12.8 with pairs by two searches, 12.1 with a list; counting
+// the protected entries takes 0.2 more.  512 threads took 13.8 and 18.9 us for the two cases in an earlier form of this kernel that took 12.9 and 15.1.
 constexpr int EV_THREADS = 1024;
 
 // Protected entries above all weights, NaN below all, -0 as +0.  crowded: more entries are protected than are kept, so these alone are in question, by their
@@ -273,8 +274,8 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(KvDev kv, KvDev ds
 }
 
 // A thread moves 16 bytes of up to MV_BATCH entries' keys and values, all read before the first is written; the books go with an entry's first bytes.
-// Bound by memory: evictions from 32 caches x 4 heads, 2001 entries of 256 bytes, take 54 us with two entries a thread (4.9 TB/s read and written, the
-// selection's 10 us among them), 59 with one, 57 with three, 61 with four, 79 with eight.
+// Bound by memory: evictions from 32 caches x 4 heads, 2001 entries of 256 bytes, took 54 us with two entries a thread, 59 with one, 57 with three, 61 with
+// four, 79 with eight; since the selection reads faster they take 52 (5.1 TB/s read and written; launched alone this kernel takes 40).
 constexpr int MV_BATCH = 2;
 __global__ void __launch_bounds__(256) kv_move_kernel(KvDev kv, KvDev dst, bool inplace, const int32_t *seq, int keep, const int32_t *map) {
     const int kvh = blockIdx.y, b = blockIdx.z, per = kv.hd * kv.size() / 16;       // a power of two
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvDev kv, KvDev dst, bool 
 }
 
 cudaError_t launch_kv_evict(const KvDev &kv, const KvDev *dst, int n, const int32_t *seq, const int32_t *len, int keep, int first, int recent, const int32_t *end,
-                            int32_t *map, int32_t *new_len, int len_hint, cudaStream_t st) {
+                            int32_t *map, int32_t *new_len, cudaStream_t st) {
     const KvDev &to = dst ? *dst : kv;
     const size_t bits = ((size_t)(kv.cap + 31) / 32 * 3 + 1) * 4, all = bits + (size_t)kv.cap * 4, most = 200 * 1024;
     const bool keys = all <= most;

@@ -4,13 +4,13 @@
 // transposed, S^T = K Q^T and O^T = V^T P^T, with mma.sync (m16n8k8, tf32 operands, f32 sums): slots and dimensions are the 16 rows of operand A, and the
 // 8 columns of operand B are the rows above, of which a token has 8 (64 query heads over 8): nothing is padded.  Results are single precision: an f32 operand
 // x is split into hi = x rounded to tf32's 11 bits and the rest lo = x - hi, exact, of which tf32 takes 11 bits again; hi hi + hi lo + lo hi leaves out
-// 2^-22 of a product at most.  bf16 values are tf32 values: for such a cache two products are enough.  The tensor cores' adders truncate, so no long sum is
+// 2^-21 of a product at most (lo lo, and the last bit of each lo).  bf16 values are tf32 values: for such a cache two products are enough.  The tensor cores' adders truncate, so no long sum is
 // left to them: a step's scores take head_dim / 16 additions, a step's share of the output starts at zero and joins the running output by one fused
 // multiply-add that also rescales it to the new running maximum.
 //
 // Every warp has a ring of operands of its own in shared memory, filled by tensor copies of 16 rows several operands ahead, and waits for nobody else.  The
 // copies swizzle the rows: with rows as they are, 16-byte reads of keys met two and of values four to a bank (201 tokens x 8 heads over 24 blocks of 32 f32
-// slots took 159 us in place of 144).  The k index of a product may be any order of the dimensions (slots) that both operands have, so a lane's k = t, t + 4 of
+// slots took 159 us and, swizzled, 144; now, with smaller rings, 118).  The k index of a product may be any order of the dimensions (slots) that both operands have, so a lane's k = t, t + 4 of
 // consecutive products are the consecutive values of one 16-byte read, and the rows of V^T may be any order of the dimensions.  Weights change from the
 // accumulator's place (slot g, rows 2t, 2t + 1 in lane 4 g + t) to operand B's (slots 2t, 2t + 1, row g) by shuffles.  Queries are split once and wait in
 // shared memory in fragment order.
@@ -24,7 +24,7 @@
 
 namespace brrr {
 
-constexpr int AW = 4;                       // warps of an attention CTA; three CTAs on an SM
+constexpr int AW = 4;                       // warps of an attention CTA; two to four CTAs on an SM
 
 // x rounded to tf32's 11 bits; from 0x7F7FF000 on, just below the largest value, to infinity
 __device__ __forceinline__ float tf32_hi(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u); }
@@ -488,8 +488,8 @@ cudaError_t launch_attn_tree(const KvDev &kv, const TreeArgs &a, int len_hint, c
 }
 
 // ---------------------------------------------------------------- book of weights
-// Up to 16 rows per kv head.  A warp owns a step of slots: the scores of its keys, their powers, the sum over the rows.  24 sequences of 3801 f32 slots: 29.8 us, keys at
-// 5 TB/s.  More rows go to kernels_kvtc.cu; 16 take 3.8 us here and 6.1 there over 200 slots of 64 f32 dimensions, 13.2 and 23.4 from 8 sequences of 2500.
+// Up to 16 rows per kv head.  A warp owns a step of slots: the scores of its keys, their powers, the sum over the rows.  24 sequences of 3801 f32 slots: 30.7 us, keys at
+// 4.9 TB/s.  More rows go to kernels_kvtc.cu; 16 take 3.8 us here and 6.1 there over 200 slots of 64 f32 dimensions, 13.2 and 23.4 from 8 sequences of 2500.
 template <class T, int HD, int NT>
 __global__ void __launch_bounds__(AW * 32, 3) weigh_kernel(KvDev kv, TreeArgs a, const uint64_t *picked, const __grid_constant__ KvMaps maps) {
     typedef Ring<T, HD> Rg;
@@ -608,7 +608,7 @@ cudaError_t launch_kv_weigh(const KvDev &kv, const TreeArgs &a, const uint64_t *
 // ---------------------------------------------------------------- chosen blocks
 // A cluster per (kv head, row).  Its CTAs share the blocks' scores: products of f64 (mma m8n8k4, 8 heads by 8 blocks), whose largest over the heads every CTA
 // gets as a 32-bit key in the order of the values.  Then each CTA finds the nsel largest keys and takes its share of the chosen blocks' steps.  201 rows x 8 heads over 282
-// blocks, 24 of 32 f32 slots chosen: 115 us, 632 MB of keys and values out of L2 at 5.5 TB/s, issue slots half full (rings of 12 KB and three CTAs on an SM
+// blocks, 24 of 32 f32 slots chosen: 118 us, 632 MB of keys and values out of L2 at 5.4 TB/s, issue slots half full (rings of 12 KB and three CTAs on an SM
 // took 24 us more).  One row over 954 bf16 blocks of 64: 18.2 us, a sequence of latencies (means, scores, cluster barrier, digits, steps, join).
 __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
     asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));

@@ -1,10 +1,11 @@
-// Attention of drafted trees with more than 16 rows per kv head on the fifth-generation tensor cores (tcgen05.mma, accumulators in tensor memory).
+// Attention of drafted trees with many rows per kv head (wide_rows_pay says from where on), and their book of weights (more than 16), on the fifth-generation
+// tensor cores (tcgen05.mma, accumulators in tensor memory).
 //
 // Rows are (drafted token, query head) pairs, 128 to a CTA, one per lane of tensor memory; a tile is N slots.  Single precision out of bf16 products:
 // an f32 value is cut into three pieces of eight bits (hi: the upper 16 bits of its pattern; mid: those of the rest; lo: what is left - all
 // exact), q into q0 + q1 + q2, weights p into p0 + p1 + p2.  A bf16 cache's values are one piece: three products give the full product.  f32 values have
-// three: the six products down to 2^-16 are formed, what is left out is 2^-22 of the product.  The small ones come first in the accumulator, so that few
-// of its (truncating) additions carry weight; an output tile starts at zero and joins the running output in registers, scaled to the new maximum.
+// three: the six products down to 2^-16 are formed, what is left out is 2^-21 of the product at most (mid lo and lo mid).  The small ones come first in the
+// accumulator, so that few of its (truncating) additions carry weight; an output tile starts at zero and joins the running output in registers, scaled to the new maximum.
 //
 // Warp roles: 0-7 softmax and output (thread = row and half of a tile's slots, then half of the dimensions).  bf16: 13 brings keys and values, tensor copies in
 // operand order, swizzled; 8-11 look at the values of tiles that not every row sees whole; 12 issues.  f32: 17 brings raw rows into a ring, 8-15 cut them

@@ -3,6 +3,7 @@
 `KvCache` is a view of device memory that the caller owns (brrr_kv of include/brrr.h, where every call is described); its
 methods are the C entry points with the optional arguments by name.  Device arrays are given as addresses or as anything
 with data_ptr() (a contiguous torch tensor); `stream` is a cudaStream_t as an integer (None: the default stream).
+What only the device can see - an entry that does not fit - sets the word `err`; without one it is left out silently.
 """
 import ctypes as C
 
@@ -63,7 +64,8 @@ class KvCache:
         return x.data_ptr()
 
     def append(self, n, rows, length, qkv, n_head=0, q=None, at=None, rope=None, n_rope=0, count=None, seq=None, ld=0, stream=None):
-        """Rows of q | k | v into the cache at slots length[b] + i, rotated by their positions; rotated q to `q`."""
+        """Rows of q | k | v into the cache at slots length[b] + i, rotated by their positions `at` (None: the slots' numbers, wrong in a tree and after an
+        eviction in place); rotated q to `q`."""
         p, v = self._at, self.view
         width = (n_head + 2 * v.n_head_kv) * v.head_dim
         check(self._lib.brrr_kv_append(self._ref, n, rows, p(seq, n, INT), p(length, n, INT), p(count, n, INT), p(at, n * rows, INT), p(qkv, (n * rows - 1) * (ld or width) + width), ld, n_head,

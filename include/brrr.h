@@ -297,16 +297,18 @@ int brrr_qwen_cli_main(int argc, char **argv);
  * Operators beside brrr_attn_decode for what a long cache and a draft need.  They work on caches that the caller owns, described by a
  * brrr_kv; everything is enqueued on `stream` of the current device (to which every pointer belongs), nothing is allocated or kept
  * between calls, and every call may be captured into a CUDA graph.  Arithmetic is single precision or better whatever the cache's type,
- * in a fixed order: equal inputs give equal bits.
+ * in a fixed order: equal calls give equal bits.  How the work is split follows from the number of entries and rows, the capacity and len_hint, so a sequence's
+ * last bits may differ with who else is in the call.
  *
  * Lengths, sequences, counts, paths and positions are device arrays.  What the host cannot see is checked by the kernels: an entry of a
  * list whose sequence, length or count does not fit the cache, or that names a sequence which an earlier entry of a writing call (append,
- * commit, weigh, evict, means) has named already, is left out, its outputs stay as they were, and *err (if given) becomes 1.
+ * commit, weigh, evict, means) has named already, is left out, its outputs stay as they were, and *err (if given) becomes 1; so it does where a
+ * copy inside a kernel has not come in time.  Without err nothing tells of either: give one, and read it when the stream is waited for anyway.
  * d_seq [n] names the sequences of a call; NULL: entry b is sequence b.  len_hint: about the largest length among the entries (0: unknown);
- * it steers how work is split, never what is computed.
- * A slot that a row does not see may hold anything, infinities, NaN and the largest finite values included; a row that sees an infinity or NaN, or whose weighted
- * values add up beyond single precision, has no defined result.  A sink may be
- * -infinity (no sink for that head), not +infinity; `scale` is any number up to BRRR_KV_SCALE_MAX in magnitude (scaled scores beyond single precision give no defined result).
+ * it steers how work is split (brrr_kv_evict does not look at it), never what is computed beyond the last bits.
+ * A slot that a row does not see may hold anything, infinities, NaN and the largest finite values included; a row that sees an infinity or NaN, or
+ * whose weighted values add up beyond single precision, has no defined result.  A sink may be -infinity (no sink for that head), not +infinity; `scale` is
+ * any number up to BRRR_KV_SCALE_MAX in magnitude (scaled scores beyond single precision give no defined result).
  * An output overlaps no input, except that d_out may be d_q. */
 enum { BRRR_KV_F32 = 0, BRRR_KV_BF16 = 1 };
 #define BRRR_TREE_MAX 64     /* rows per sequence of brrr_attn_tree, brrr_kv_commit and brrr_kv_weigh */
@@ -314,7 +316,7 @@ enum { BRRR_KV_F32 = 0, BRRR_KV_BF16 = 1 };
 #define BRRR_KV_SCALE_MAX 1e38f
 typedef struct brrr_kv {
     void *k, *v;                      /* [n_seq][n_head_kv][cap][head_dim] values of `type`, keys rotated; 16-byte aligned */
-    int32_t type;                     /* BRRR_KV_F32 (the engines' caches) or BRRR_KV_BF16 */
+    int32_t type;                     /* BRRR_KV_F32 (as the engines keep theirs, which are not reached from here) or BRRR_KV_BF16 */
     int32_t n_seq, n_head_kv;         /* n_head_kv <= 512 */
     int32_t head_dim;                 /* 64 or 128 */
     int32_t cap;                      /* slots per head */
@@ -325,7 +327,8 @@ typedef struct brrr_kv {
 } brrr_kv;
 
 /* Row i < count[b] (d_count NULL: rows) of entry b goes to slot len[b] + i: keys rotated and values, converted to the cache's type; the
- * slot's weight becomes 0 and its position at[b][i] (d_at NULL: the slot's number).  A row of d_qkv is q (n_head heads, may be 0) | k | v,
+ * slot's weight becomes 0 and its position at[b][i] (d_at NULL: the slot's number, which is no position of the sequence once entries have been evicted in place, or
+ * in a tree: there d_at is needed, for the rotation and for what an eviction protects).  A row of d_qkv is q (n_head heads, may be 0) | k | v,
  * ld floats from the next (0: dense), 16-byte aligned, ld % 4 == 0.  d_rope [n_rope][head_dim / 2][2] cosines and sines as brrr_rope_table makes them, pairs
  * (j, j + head_dim / 2); NULL: k and q are taken as they are.  d_q (nullable, no overlap with d_qkv): the rotated q [n][rows][n_head * head_dim].
  * A row whose position the table does not have is left out.  rows <= cap.  Replaces the rotation and the cache write of
@@ -336,7 +339,8 @@ int brrr_kv_append(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, con
 /* Attention of `rows` (1..BRRR_TREE_MAX) drafted tokens per entry over the entry's cache: row i's key and value stand in slot len[b] + i.
  * Row i sees the cached slots t < len[b] and of the drafted ones j < count[b] those whose bit j of mask[b][i] is set: the row itself and its
  * ancestors (d_mask NULL: every j <= i, a chain).  window > 0: with depth(i) the number of rows that i sees other than itself, only slots
- * t >= len[b] + depth(i) + 1 - window and rows with depth(i) - depth(j) < window are seen.  d_q [n][rows][n_head * head_dim], rotated; n_head a
+ * t >= len[b] + depth(i) + 1 - window and rows with depth(i) - depth(j) < window are seen; a window counts slots, so it means positions only where no entry
+ * has been evicted.  d_q [n][rows][n_head * head_dim], rotated; n_head a
  * multiple of n_head_kv, at most 16 times it.  d_sinks [n_head] (nullable): a logit per head that takes weight and adds nothing.
  *   d_out [n][rows][n_head * head_dim] = sum over seen t of exp(scale q.k_t - lse) v_t;  d_lse [n][rows][n_head] (nullable) = log of the sum of exponentials,
  * the sink's included.  A row that sees nothing: zeros, and lse the sink or -infinity.  Rows >= count[b] stay as they were.
@@ -363,7 +367,8 @@ int brrr_kv_weigh(const brrr_kv *kv, int n, int rows, const int32_t *d_seq, cons
  * ascending order, with their weights and positions: attention does not ask for an order, so no more than that moves.  d_map [n][n_head_kv][keep]: the
  * slot that each entry came from, -1 from m on.  dst NULL: in place (what lies behind m is then nobody's); else all kept entries are written to the same sequence of
  * dst, another view of the same type, heads and dimension with cap >= keep whose memory does not overlap.  d_new_len (nullable, not d_len) [n] = m.
- * first + recent <= keep.  Views need both books.  For an entry that is left out: d_map -1, d_new_len len[b]. */
+ * first + recent <= keep.  Views need both books.  For an entry that is left out: d_map -1, d_new_len len[b].  Means of blocks (brrr_kv_means) in which an entry
+ * was replaced are the old ones until they are formed anew, with since 0. */
 int brrr_kv_evict(const brrr_kv *kv, const brrr_kv *dst, int n, const int32_t *d_seq, const int32_t *d_len, int keep, int first, int recent,
                   const int32_t *d_end, int32_t *d_map, int32_t *d_new_len, int len_hint, void *stream);
 
