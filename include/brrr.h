@@ -308,7 +308,7 @@ int brrr_qwen_cli_main(int argc, char **argv);
  * it steers how work is split (brrr_kv_evict does not look at it), never what is computed beyond the last bits.
  * A slot that a row does not see may hold anything, infinities, NaN and the largest finite values included; a row that sees an infinity or NaN, or
  * whose weighted values add up beyond single precision, has no defined result.  A sink may be -infinity (no sink for that head), not +infinity; `scale` is
- * any number up to BRRR_KV_SCALE_MAX in magnitude (scaled scores beyond single precision give no defined result).
+ * any number up to BRRR_KV_SCALE_MAX in magnitude (scores beyond single precision, scaled or not, give no defined result).
  * An output overlaps no input, except that d_out may be d_q. */
 enum { BRRR_KV_F32 = 0, BRRR_KV_BF16 = 1 };
 #define BRRR_TREE_MAX 64     /* rows per sequence of brrr_attn_tree, brrr_kv_commit and brrr_kv_weigh */
